@@ -266,6 +266,99 @@ class AspireClearDumpArgs(ctypes.Structure):
     ]
 
 
+# Element types of the feed-forward operators.
+T_F32 = 0
+T_BF16 = 1
+T_F16 = 2
+
+
+class AspireW4Args(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("codes", ctypes.c_void_p),
+        ("codes_stride", ctypes.c_int64),
+        ("codes_stride_e", ctypes.c_int64),
+        ("scales", ctypes.c_void_p),
+        ("scales_stride", ctypes.c_int64),
+        ("scales_stride_e", ctypes.c_int64),
+        ("zeros", ctypes.c_void_p),
+        ("zeros_stride", ctypes.c_int64),
+        ("zeros_stride_e", ctypes.c_int64),
+        ("residual", ctypes.c_void_p),
+        ("residual_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_stride", ctypes.c_int64),
+        ("n", ctypes.c_int32),
+        ("k", ctypes.c_int32),
+        ("group", ctypes.c_int32),
+        ("type", ctypes.c_int32),
+        ("swiglu", ctypes.c_int32),
+        ("offsets", ctypes.c_void_p),
+        ("experts", ctypes.c_int32),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class AspireMoeRouteArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("logits_type", ctypes.c_int32),
+        ("logits_stride", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("num_experts", ctypes.c_int32),
+        ("top_k", ctypes.c_int32),
+        ("renormalize", ctypes.c_int32),
+        ("weights", ctypes.c_void_p),
+        ("experts", ctypes.c_void_p),
+        ("position", ctypes.c_void_p),
+        ("source", ctypes.c_void_p),
+        ("offsets", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class AspireMoeRouteGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("logits_type", ctypes.c_int32),
+        ("logits_stride", ctypes.c_int64),
+        ("weights", ctypes.c_void_p),
+        ("experts", ctypes.c_void_p),
+        ("grad_weights", ctypes.c_void_p),
+        ("tokens", ctypes.c_int64),
+        ("num_experts", ctypes.c_int32),
+        ("top_k", ctypes.c_int32),
+        ("renormalize", ctypes.c_int32),
+        ("grad_logits", ctypes.c_void_p),
+    ]
+
+
+class AspireMoePermuteArgs(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int32),
+        ("in_", ctypes.c_void_p),
+        ("in_stride", ctypes.c_int64),
+        ("residual", ctypes.c_void_p),
+        ("residual_stride", ctypes.c_int64),
+        ("weights", ctypes.c_void_p),
+        ("position", ctypes.c_void_p),
+        ("offsets", ctypes.c_void_p),
+        ("num_experts", ctypes.c_int32),
+        ("top_k", ctypes.c_int32),
+        ("tokens", ctypes.c_int64),
+        ("width", ctypes.c_int32),
+        ("out", ctypes.c_void_p),
+        ("out_stride", ctypes.c_int64),
+        ("grad", ctypes.c_void_p),
+        ("grad_stride", ctypes.c_int64),
+        ("grad_weights", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
 # Exported symbols and their signatures (must match include/aspire_b200.h).
 _SIGNATURES = {
     "aspire_plan": (
@@ -297,6 +390,13 @@ _SIGNATURES = {
     "aspire_qkv_prologue": (ctypes.c_int, [ctypes.POINTER(AspirePrologueArgs), ctypes.c_void_p]),
     "aspire_draft_page_spill": (ctypes.c_int, [ctypes.POINTER(AspireSpillArgs), ctypes.c_void_p]),
     "aspire_clear_dump_slots": (ctypes.c_int, [ctypes.POINTER(AspireClearDumpArgs), ctypes.c_void_p]),
+    "aspire_w4_linear": (ctypes.c_int, [ctypes.POINTER(AspireW4Args), ctypes.c_void_p]),
+    "aspire_moe_route": (ctypes.c_int, [ctypes.POINTER(AspireMoeRouteArgs), ctypes.c_void_p]),
+    "aspire_moe_route_workspace": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]),
+    "aspire_moe_route_grad": (ctypes.c_int, [ctypes.POINTER(AspireMoeRouteGradArgs), ctypes.c_void_p]),
+    "aspire_moe_dispatch": (ctypes.c_int, [ctypes.POINTER(AspireMoePermuteArgs), ctypes.c_void_p]),
+    "aspire_moe_combine": (ctypes.c_int, [ctypes.POINTER(AspireMoePermuteArgs), ctypes.c_void_p]),
+    "aspire_moe_combine_grad": (ctypes.c_int, [ctypes.POINTER(AspireMoePermuteArgs), ctypes.c_void_p]),
     "aspire_plan_device": (
         ctypes.c_int,
         [c_int32_p, c_int32_p, c_int32_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,

@@ -33,6 +33,10 @@ SOURCES = [
     "noalloc.cu",
     "draft_spill.cu",
     "dump_state.cu",
+    "capi_ffn.cu",
+    "w4_small.cu",
+    "moe_route.cu",
+    "moe_permute.cu",
 ]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -72,6 +76,8 @@ def build(verbose_ptxas: bool = False, force: bool = False) -> Path:
         "-std=c++17",
         *ARCH_FLAGS,
         "-lineinfo",
+        "--threads",
+        "8",
         "-shared",
         "-Xcompiler",
         "-fPIC,-fvisibility=hidden",

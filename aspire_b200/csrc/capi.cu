@@ -9,10 +9,9 @@
 #include <string>
 #include <utility>
 
-#include <cudaTypedefs.h>
-
 #include "kernels.cuh"
 #include "errors.h"
+#include "launch.cuh"
 
 namespace aspire {
 
@@ -33,26 +32,6 @@ int check_cuda(int st, const char* what) {
                                         cudaGetErrorString(static_cast<cudaError_t>(st)));
 }
 
-// Launches `kernel` with a programmatic dependency on the preceding work in
-// the stream (every kernel begins with griddepcontrol.launch_dependents +
-// wait, so it is scheduled early but reads nothing before its predecessor
-// has finished).
-template <typename... KArgs, typename... Args>
-int launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const char* what,
-           Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...), what);
-}
-
 int plan_impl(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_len,
               int32_t batch_size, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
               int32_t page_size, int32_t causal, int32_t num_sms, bool tc_enabled, int32_t tc_min_rows,
@@ -61,61 +40,12 @@ int plan_impl(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t*
 
 namespace {
 
-int current_sm_count(int* out) {
-  int dev = 0;
-  int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
-  if (rc) return rc;
-  return check_cuda(cudaDeviceGetAttribute(out, cudaDevAttrMultiProcessorCount, dev),
-                    "cudaDeviceGetAttribute(SM count)");
-}
-
-// Dynamic shared memory a kernel has been opted in to, per device: the
-// attribute set by cudaFuncSetAttribute applies to the current device only,
-// so a host thread that drives several GPUs sets it once on each.
-constexpr int kMaxDevices = 64;
-struct SmemOptIn {
-  std::atomic<int> bytes[kMaxDevices];
-  SmemOptIn() {
-    for (auto& b : bytes) b.store(48 * 1024);
-  }
-};
-
-// Opt-in to large dynamic shared memory once per (kernel, device, size).
-int ensure_smem(const void* func, size_t bytes, SmemOptIn& cache) {
-  int dev = 0;
-  int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
-  if (rc) return rc;
-  const bool cached = dev >= 0 && dev < kMaxDevices;
-  if (cached && int(bytes) <= cache.bytes[dev].load(std::memory_order_relaxed)) return ASPIRE_OK;
-  rc = check_cuda(cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)),
-                  "cudaFuncSetAttribute(max dynamic smem)");
-  if (rc == ASPIRE_OK && cached) {
-    int cur = cache.bytes[dev].load(std::memory_order_relaxed);
-    while (cur < int(bytes) && !cache.bytes[dev].compare_exchange_weak(cur, int(bytes))) {
-    }
-  }
-  return rc;
-}
-
 SmemOptIn g_gather_smem, g_tc_smem, g_sel_smem;
 
 // Bound of one pipeline wait of the tcgen05 kernel (aspire_set_wait_limit_ns);
 // 0 selects the default.
 constexpr uint64_t kDefaultWaitNs = 1000000000ull;
 std::atomic<uint64_t> g_wait_limit_ns{0};
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no libcuda link).
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  if (!fn) {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-  }
-  return fn;
-}
 
 // 5-D view of the paged cache [pages, 2, 16, Hkv, 128] (innermost first:
 // dim, head, token, K/V, page) with a 64-dim x 16-token box, 128-byte swizzle.
@@ -245,7 +175,9 @@ int aspire_set_wait_limit_ns(uint64_t ns) {
 const char* aspire_kernel_names(void) {
   return "aspire_attn_gather_kernel\naspire_attn_tc_kernel\naspire_attn_merge_kernel\naspire_append_kv_kernel\n"
          "aspire_select_pages_kernel\naspire_page_scores_kernel\naspire_build_indices_kernel\naspire_qkv_prologue_kernel\naspire_plan_device_kernel\n"
-         "aspire_draft_spill_kernel\naspire_clear_dump_kernel\n";
+         "aspire_draft_spill_kernel\naspire_clear_dump_kernel\n"
+         "aspire_w4_small_kernel\naspire_moe_route_kernel\naspire_moe_sort_kernel\naspire_moe_route_grad_kernel\n"
+         "aspire_moe_dispatch_kernel\naspire_moe_combine_kernel\naspire_moe_combine_grad_kernel\n";
 }
 
 int aspire_plan_host_only(const int32_t* qo_indptr, const int32_t* kv_indptr,

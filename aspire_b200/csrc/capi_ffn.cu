@@ -1,0 +1,332 @@
+// extern "C" entry points of the feed-forward operators: 4-bit products and
+// the tokens' way to their experts and back (declared in
+// include/aspire_b200.h).  Argument checking and launch configuration; no
+// entry point allocates device memory or synchronises, and none lets a C++
+// exception out.
+#include <algorithm>
+#include <cstdint>
+#include <string>
+
+#include "errors.h"
+#include "launch.cuh"
+#include "moe.cuh"
+#include "w4.cuh"
+
+namespace aspire {
+namespace {
+
+// Runs an entry point's body; an exception (out of host memory while a message
+// is built) becomes an error code.
+template <typename F>
+int guarded(F&& body) noexcept {
+  try {
+    clear_error();
+    return body();
+  } catch (...) {
+    return ASPIRE_ERR_CAPACITY;
+  }
+}
+
+int invalid(const char* who, const char* what) {
+  return set_error(ASPIRE_ERR_INVALID, std::string(who) + ": " + what);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int ceil32(int v) { return (v + 31) / 32 * 32; }
+
+// Opt-in caches of the small kernel's variants: [type][tokens 8, 16, 32]
+// [groups 1, 2, 4][swiglu].
+SmemOptIn g_w4_small[2][3][3][2];
+
+int index_of(int v) { return v <= 1 ? 0 : (v == 2 ? 1 : 2); }
+
+int w4_launch(W4Kernel kernel, dim3 grid, int cluster, int threads, size_t smem, cudaStream_t stream,
+              const char* what, const W4Params& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), what);
+}
+
+// Upper bound of the token tiles of `rows` rows in `experts` ranges (0: one
+// range), the tail past the last range included.
+int64_t tiles_bound(int64_t rows, int32_t experts, bool grouped, int width) {
+  if (!grouped) return (rows + width - 1) / width;
+  return std::min<int64_t>(rows, experts) + rows / width + 1;
+}
+
+int w4_small(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
+  const bool grouped = a->offsets != nullptr;
+  // Tokens per tile: the fewest columns that hold the rows (an expert's
+  // average share of them), up to 32.
+  const int64_t typical = grouped ? (a->rows + a->experts - 1) / std::max(a->experts, 1) : a->rows;
+  const int tokens = typical <= 8 ? 8 : (typical <= 16 ? 16 : 32);
+  const int groups = a->group == 32 ? 4 : (a->group == 64 ? 2 : 1);
+  const int features = a->swiglu ? w4::kRows / 2 : w4::kRows;
+  const int64_t ny = (int64_t(a->n) + features - 1) / features;
+  const int64_t nz = tiles_bound(a->rows, a->experts, grouped, tokens);
+  if (ny > 65535 || nz > 65535) return invalid("aspire_w4_linear", "n or rows too large");
+  int sms = 0;
+  int rc = current_sm_count(&sms);
+  if (rc) return rc;
+  // Split K over a cluster while the tiles leave half of the CTA slots (two
+  // per SM) empty and every rank has a stage of its own.
+  const int64_t stages = (a->k + 255) / 256;
+  int cluster = 1;
+  while (cluster < 8 && ny * nz * cluster * 2 <= 2 * sms && cluster * 2 <= stages) cluster *= 2;
+  W4Kernel kernel = w4_small_kernel(a->type == ASPIRE_T_BF16, tokens, groups, a->swiglu != 0);
+  const size_t smem = w4_small_smem(tokens, groups);
+  rc = ensure_smem(reinterpret_cast<const void*>(kernel), smem,
+                   g_w4_small[a->type == ASPIRE_T_BF16][tokens == 8 ? 0 : (tokens == 16 ? 1 : 2)][index_of(groups)]
+                             [a->swiglu != 0]);
+  if (rc) return rc;
+  return w4_launch(kernel, dim3(unsigned(cluster), unsigned(ny), unsigned(nz)), cluster, kW4SmallThreads, smem, stream,
+                   "aspire_w4_small_kernel launch", p);
+}
+
+int64_t elem_bytes(int32_t type) { return type == ASPIRE_T_F32 ? 4 : 2; }
+
+bool known_type(int32_t t) { return t == ASPIRE_T_F32 || t == ASPIRE_T_BF16 || t == ASPIRE_T_F16; }
+
+// Slots per block of the sort, and its blocks.
+void route_blocks(int64_t tokens, int32_t top_k, int64_t* block_tokens, int64_t* blocks) {
+  if (tokens * top_k <= kMoeSlotsOne) {
+    *block_tokens = tokens;
+    *blocks = 1;
+  } else {
+    *block_tokens = kMoeSlotsBlock / top_k;
+    *blocks = (tokens + *block_tokens - 1) / *block_tokens;
+  }
+}
+
+int check_permute(const AspireMoePermuteArgs* a, const char* who, bool grad) {
+  if (!a) return invalid(who, "null argument");
+  if (!known_type(a->type)) return invalid(who, "type must be ASPIRE_T_F32, ASPIRE_T_BF16 or ASPIRE_T_F16");
+  if (a->tokens < 0 || a->top_k <= 0 || a->top_k > kMoeMaxTopK) return invalid(who, "bad token count or top_k");
+  if (a->num_experts < 0 || a->width <= 0) return invalid(who, "bad expert count or width");
+  if (a->tokens == 0) return ASPIRE_OK;
+  if (a->tokens > INT32_MAX / a->top_k) return invalid(who, "too many tokens");
+  if (!a->position || !a->offsets) return invalid(who, "null position or offsets");
+  const int64_t vec = 16 / elem_bytes(a->type);
+  if (a->width % vec) return invalid(who, "rows must be a multiple of 16 bytes");
+  if ((a->in && (a->in_stride % vec || a->in_stride < a->width)) ||
+      (a->out && (a->out_stride % vec || a->out_stride < a->width)) ||
+      (a->residual && (a->residual_stride % vec || a->residual_stride < a->width)) ||
+      (a->grad && (a->grad_stride % vec || a->grad_stride < a->width)))
+    return invalid(who, "row strides must be multiples of 16 bytes and at least the width");
+  if (!aligned16(a->in) || !aligned16(a->out) || !aligned16(a->residual) || !aligned16(a->grad))
+    return invalid(who, "tensors must be 16-byte aligned");
+  if (grad) {
+    if (!a->grad) return invalid(who, "null gradient");
+    if (a->grad_weights && !a->in) return invalid(who, "the weights' gradient needs the rows");
+  } else if (!a->in || !a->out) {
+    return invalid(who, "null tensor pointer");
+  }
+  return ASPIRE_OK;
+}
+
+MoePermuteParams permute_params(const AspireMoePermuteArgs* a) {
+  MoePermuteParams p = {};
+  p.in = a->in;
+  p.in_stride = a->in_stride;
+  p.residual = a->residual;
+  p.residual_stride = a->residual_stride;
+  p.weights = a->weights;
+  p.position = a->position;
+  p.offsets = a->offsets;
+  p.num_experts = a->num_experts;
+  p.tokens = int32_t(a->tokens);
+  p.top_k = a->top_k;
+  p.width = a->width;
+  p.out = a->out;
+  p.out_stride = a->out_stride;
+  p.grad = a->grad;
+  p.grad_stride = a->grad_stride;
+  p.grad_weights = a->grad_weights;
+  p.status = a->status;
+  return p;
+}
+
+}  // namespace
+}  // namespace aspire
+
+using namespace aspire;
+
+extern "C" {
+
+int aspire_w4_linear(const AspireW4Args* a, void* stream) {
+  return guarded([&]() -> int {
+    const char* who = "aspire_w4_linear";
+    if (!a) return invalid(who, "null argument");
+    if (a->type != ASPIRE_T_BF16 && a->type != ASPIRE_T_F16)
+      return invalid(who, "type must be ASPIRE_T_BF16 or ASPIRE_T_F16");
+    if (a->rows < 0 || a->rows > INT32_MAX || a->n <= 0 || a->k <= 0) return invalid(who, "bad sizes");
+    if (a->group != 32 && a->group != 64 && (a->group <= 0 || a->group % 128))
+      return invalid(who, "group must be 32, 64 or a multiple of 128");
+    if (a->k % 32 || a->k % a->group) return invalid(who, "k must be a multiple of 32 and of group");
+    if (a->offsets && a->experts <= 0) return invalid(who, "offsets need experts > 0");
+    if (a->swiglu && a->residual) return invalid(who, "the gated form takes no residual");
+    if (a->swiglu && a->n > INT32_MAX / 2) return invalid(who, "bad sizes");
+    if (a->rows == 0) return ASPIRE_OK;
+    if (!a->x || !a->codes || !a->scales || !a->out) return invalid(who, "null tensor pointer");
+    const int64_t groups = a->k / a->group;
+    if (a->x_stride < a->k || a->codes_stride < a->k / 8 || a->scales_stride < groups || a->out_stride < a->n ||
+        (a->zeros && a->zeros_stride < groups) || (a->residual && a->residual_stride < a->n))
+      return invalid(who, "a row stride is shorter than its row");
+    if (!aligned16(a->x) || !aligned16(a->codes)) return invalid(who, "x and codes must be 16-byte aligned");
+    if ((a->x_stride & 7) || (a->codes_stride & 3) || (a->offsets && (a->codes_stride_e & 3)))
+      return invalid(who, "x rows must be multiples of 8 elements and codes rows of 4 words apart");
+    W4Params p = {};
+    p.x = static_cast<const uint16_t*>(a->x);
+    p.x_stride = a->x_stride;
+    p.rows = int32_t(a->rows);
+    p.codes = a->codes;
+    p.codes_stride = a->codes_stride;
+    p.codes_stride_e = a->codes_stride_e;
+    p.scales = static_cast<const uint16_t*>(a->scales);
+    p.scales_stride = a->scales_stride;
+    p.scales_stride_e = a->scales_stride_e;
+    p.zeros = a->zeros;
+    p.zeros_stride = a->zeros_stride;
+    p.zeros_stride_e = a->zeros_stride_e;
+    p.residual = static_cast<const uint16_t*>(a->residual);
+    p.residual_stride = a->residual_stride;
+    p.out = static_cast<uint16_t*>(a->out);
+    p.out_stride = a->out_stride;
+    p.n = a->n;
+    p.k = a->k;
+    p.group = a->group;
+    p.offsets = a->offsets;
+    p.num_experts = a->offsets ? a->experts : 0;
+    p.status = a->status;
+    return w4_small(a, p, static_cast<cudaStream_t>(stream));
+  });
+}
+
+size_t aspire_moe_route_workspace(int64_t tokens, int32_t num_experts, int32_t top_k) {
+  if (tokens <= 0 || top_k <= 0 || top_k > kMoeMaxTopK || num_experts <= 0 || tokens > INT32_MAX / top_k) return 0;
+  int64_t bt, nb;
+  route_blocks(tokens, top_k, &bt, &nb);
+  return nb > 1 ? size_t(nb) * size_t(num_experts) * sizeof(int32_t) : 0;
+}
+
+int aspire_moe_route(const AspireMoeRouteArgs* a, void* stream) {
+  return guarded([&]() -> int {
+    const char* who = "aspire_moe_route";
+    if (!a) return invalid(who, "null argument");
+    if (a->num_experts <= 0 || a->num_experts > kMoeMaxExperts) return invalid(who, "num_experts must be in [1, 512]");
+    if (a->top_k <= 0 || a->top_k > kMoeMaxTopK) return invalid(who, "top_k must be in [1, 32]");
+    if (a->logits && a->top_k > a->num_experts) return invalid(who, "top_k must not exceed num_experts");
+    if (a->tokens < 0 || a->tokens > INT32_MAX / a->top_k) return invalid(who, "bad token count");
+    if (a->logits && !known_type(a->logits_type)) return invalid(who, "bad logits type");
+    if (a->logits && a->tokens > 1 && a->logits_stride < a->num_experts)
+      return invalid(who, "logits rows are shorter than num_experts");
+    if (!a->offsets) return invalid(who, "null offsets");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->tokens == 0)
+      return check_cuda(cudaMemsetAsync(a->offsets, 0, sizeof(int32_t) * (size_t(a->num_experts) + 1), st),
+                        "aspire_moe_route memset");
+    if (!a->experts || !a->position || !a->source || (a->logits && !a->weights)) return invalid(who, "null pointer");
+    int64_t bt, nb;
+    route_blocks(a->tokens, a->top_k, &bt, &nb);
+    if (nb > 1 && (!a->workspace || a->workspace_bytes < aspire_moe_route_workspace(a->tokens, a->num_experts, a->top_k)))
+      return set_error(ASPIRE_ERR_CAPACITY, "aspire_moe_route: workspace too small");
+    MoeRouteParams p = {};
+    p.logits = a->logits;
+    p.logits_type = a->logits_type;
+    p.logits_stride = a->logits_stride;
+    p.tokens = int32_t(a->tokens);
+    p.num_experts = a->num_experts;
+    p.top_k = a->top_k;
+    p.renormalize = a->renormalize ? 1 : 0;
+    p.weights = a->weights;
+    p.experts = a->experts;
+    p.position = a->position;
+    p.source = a->source;
+    p.offsets = a->offsets;
+    p.counts = a->workspace;
+    p.block_tokens = int32_t(bt);
+    int threads = kMoeSlotsBlock;
+    if (nb == 1) {  // a thread per slot and per expert, a warp per token
+      threads = std::max(ceil32(int(a->tokens * a->top_k)), ceil32(a->num_experts));
+      if (a->logits) threads = std::max(threads, 32 * int(std::min<int64_t>(a->tokens, 32)));
+    }
+    int rc = launch(moe_route_kernel(a->logits ? a->num_experts : 0), dim3(unsigned(nb)), dim3(unsigned(threads)), 0,
+                    st, "aspire_moe_route_kernel launch", p);
+    if (rc || nb == 1) return rc;
+    return launch(aspire_moe_sort_kernel, dim3(unsigned(nb)), dim3(kMoeSlotsBlock), 0, st,
+                  "aspire_moe_sort_kernel launch", p);
+  });
+}
+
+int aspire_moe_route_grad(const AspireMoeRouteGradArgs* a, void* stream) {
+  return guarded([&]() -> int {
+    const char* who = "aspire_moe_route_grad";
+    if (!a) return invalid(who, "null argument");
+    if (a->num_experts <= 0 || a->num_experts > kMoeMaxExperts || a->top_k <= 0 || a->top_k > kMoeMaxTopK ||
+        a->top_k > a->num_experts || a->tokens < 0 || a->tokens > INT32_MAX / a->top_k)
+      return invalid(who, "bad sizes");
+    if (!known_type(a->logits_type)) return invalid(who, "bad logits type");
+    if (a->tokens == 0) return ASPIRE_OK;
+    if (!a->weights || !a->experts || !a->grad_weights || !a->grad_logits || (!a->renormalize && !a->logits))
+      return invalid(who, "null pointer");
+    if (!a->renormalize && a->tokens > 1 && a->logits_stride < a->num_experts)
+      return invalid(who, "logits rows are shorter than num_experts");
+    MoeRouteGradParams p = {};
+    p.logits = a->logits;
+    p.logits_type = a->logits_type;
+    p.logits_stride = a->logits_stride;
+    p.weights = a->weights;
+    p.experts = a->experts;
+    p.grad_weights = a->grad_weights;
+    p.tokens = int32_t(a->tokens);
+    p.num_experts = a->num_experts;
+    p.top_k = a->top_k;
+    p.renormalize = a->renormalize ? 1 : 0;
+    p.grad_logits = a->grad_logits;
+    return launch(aspire_moe_route_grad_kernel, dim3(unsigned((a->tokens + 7) / 8)), dim3(256), 0,
+                  static_cast<cudaStream_t>(stream), "aspire_moe_route_grad_kernel launch", p);
+  });
+}
+
+int aspire_moe_dispatch(const AspireMoePermuteArgs* a, void* stream) {
+  return guarded([&]() -> int {
+    int rc = check_permute(a, "aspire_moe_dispatch", false);
+    if (rc || a->tokens == 0) return rc;
+    return launch(moe_dispatch_kernel(a->type), dim3(unsigned(a->tokens)), dim3(kMoeThreads), 0,
+                  static_cast<cudaStream_t>(stream), "aspire_moe_dispatch_kernel launch", permute_params(a));
+  });
+}
+
+int aspire_moe_combine(const AspireMoePermuteArgs* a, void* stream) {
+  return guarded([&]() -> int {
+    int rc = check_permute(a, "aspire_moe_combine", false);
+    if (rc || a->tokens == 0) return rc;
+    return launch(moe_combine_kernel(a->type), dim3(unsigned(a->tokens)), dim3(kMoeThreads), 0,
+                  static_cast<cudaStream_t>(stream), "aspire_moe_combine_kernel launch", permute_params(a));
+  });
+}
+
+int aspire_moe_combine_grad(const AspireMoePermuteArgs* a, void* stream) {
+  return guarded([&]() -> int {
+    int rc = check_permute(a, "aspire_moe_combine_grad", true);
+    if (rc || a->tokens == 0) return rc;
+    if (!a->out && !a->grad_weights) return ASPIRE_OK;
+    return launch(moe_combine_grad_kernel(a->type), dim3(unsigned(a->tokens)), dim3(kMoeThreads), 0,
+                  static_cast<cudaStream_t>(stream), "aspire_moe_combine_grad_kernel launch", permute_params(a));
+  });
+}
+
+}  // extern "C"

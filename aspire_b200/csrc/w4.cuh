@@ -1,0 +1,186 @@
+// Products with 4-bit weights and group scales: parameters, tile lookup and
+// the unpacking shared by the two kernels (w4_small.cu for few tokens,
+// w4_tc.cu for many).
+//
+//   y[t, n] = sum_k x[t, k] (q[n, k] - z[n, k / G]) s[n, k / G]  (+ r[t, n])
+//
+// or, with the activation, rows [0, n) of the matrix are the gate's and rows
+// [n, 2n) the up product's: y = silu(gate) * up.  Sums are in fp32 and each
+// output is rounded once.  A matrix is uint32 words [rows, k / 8]: word j of a
+// row holds weights 8j..8j+7, weight 8j+2i in bits 4i and weight 8j+2i+1 in
+// bits 16+4i, so (word >> 4i) & 0x000F000F is a pair of neighbouring weights
+// in the two halves of a register.
+#pragma once
+
+#include "kernels.cuh"
+
+namespace aspire {
+
+struct W4Params {
+  const uint16_t* x;        // [rows, k] bf16 or fp16
+  int64_t x_stride;
+  int32_t rows;
+  const uint32_t* codes;    // [experts,] [matrix rows, k / 8]
+  int64_t codes_stride, codes_stride_e;    // words
+  const uint16_t* scales;   // [experts,] [matrix rows, k / group], x's type
+  int64_t scales_stride, scales_stride_e;
+  const uint8_t* zeros;     // the same shape, or NULL: 8
+  int64_t zeros_stride, zeros_stride_e;
+  const uint16_t* residual; // [rows, n] or NULL
+  int64_t residual_stride;
+  uint16_t* out;            // [rows, n]
+  int64_t out_stride;
+  int32_t n, k, group;
+  const int32_t* offsets;   // rows of expert e: [offsets[e], offsets[e + 1]); NULL: one matrix for all rows
+  int32_t num_experts;
+  uint32_t* status;
+  uint64_t wait_ns;         // bound of one pipeline wait (tcgen05 kernel)
+};
+
+namespace w4 {
+
+constexpr int kRows = 128;  // matrix rows of a tile
+
+// A CTA's share of the output: `count` rows of x from `row0`, with the matrix
+// of `expert`.  expert -1: the rows belong to none and their outputs are zero.
+// count 0: nothing to do.
+struct Tile {
+  int32_t expert, row0, count;
+};
+
+// Token tile `index` (of `width` rows) among the experts' row ranges, in
+// expert order, followed by the rows past the last expert's.  Run by one
+// whole warp; every lane returns the tile.  Ranges that leave [0, rows) or
+// run backwards are cut to it and reported.
+__device__ __forceinline__ Tile find_tile(const W4Params& p, int index, int width, int lane) {
+  Tile t{0, 0, 0};
+  if (p.offsets == nullptr) {
+    t.row0 = index * width;
+    t.count = min(width, p.rows - t.row0);
+    return t;
+  }
+  // Lane l counts the tiles of experts [l * per, (l + 1) * per).
+  const int per = (p.num_experts + 31) / 32;
+  const int e0 = min(lane * per, p.num_experts), e1 = min(e0 + per, p.num_experts);
+  auto range = [&](int e, int& b, int& c) {
+    const int lo = p.offsets[e], hi = p.offsets[e + 1];
+    b = min(max(lo, 0), p.rows);
+    const int end = min(max(hi, b), p.rows);
+    if (lo != b || hi != end) record_status(p.status, ASPIRE_STATUS_BAD_ROW);
+    c = end - b;
+  };
+  int mine = 0;
+  for (int e = e0; e < e1; ++e) {
+    int b, c;
+    range(e, b, c);
+    mine += (c + width - 1) / width;
+  }
+  int incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += v;
+  }
+  const int total = __shfl_sync(0xffffffffu, incl, 31);
+  if (index >= total) {
+    const int last = min(max(p.offsets[p.num_experts], 0), p.rows);
+    t.expert = -1;
+    t.row0 = min(last + (index - total) * width, p.rows);
+    t.count = min(width, p.rows - t.row0);
+    return t;
+  }
+  int left = index - (incl - mine);
+  const unsigned owner = __ballot_sync(0xffffffffu, left >= 0 && left < mine);
+  if (left >= 0 && left < mine) {
+    for (int e = e0; e < e1; ++e) {
+      int b, c;
+      range(e, b, c);
+      const int n = (c + width - 1) / width;
+      if (left < n) {
+        t.expert = e;
+        t.row0 = b + left * width;
+        t.count = min(width, c - left * width);
+        break;
+      }
+      left -= n;
+    }
+  }
+  const int src = __ffs(owner) - 1;
+  t.expert = __shfl_sync(0xffffffffu, t.expert, src);
+  t.row0 = __shfl_sync(0xffffffffu, t.row0, src);
+  t.count = __shfl_sync(0xffffffffu, t.count, src);
+  return t;
+}
+
+// ------------------------------------------------------------------ numbers
+// The two activation types.  A code q < 16 OR-ed into the low mantissa bits of
+// 128 (bf16, 7 bits) or 1024 (fp16, 10 bits) is that number plus q, exactly;
+// subtracting it plus the zero point gives q - z, exactly.
+template <bool BF16>
+struct Num;
+template <>
+struct Num<true> {
+  static constexpr uint32_t kMagic = 0x43004300u;
+  __device__ static __forceinline__ float to_float(uint16_t v) { return __uint_as_float(uint32_t(v) << 16); }
+  __device__ static __forceinline__ uint16_t from_float(float v) {
+    return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  }
+  __device__ static __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  __device__ static __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+template <>
+struct Num<false> {
+  static constexpr uint32_t kMagic = 0x64006400u;
+  __device__ static __forceinline__ float to_float(uint16_t v) { return __half2float(__ushort_as_half(v)); }
+  __device__ static __forceinline__ uint16_t from_float(float v) { return __half_as_ushort(__float2half_rn(v)); }
+  __device__ static __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+    const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  __device__ static __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+
+// Pair i of a word: (weight 2i, weight 2i + 1) + magic.
+template <bool BF16>
+__device__ __forceinline__ uint32_t magic_pair(uint32_t word, int i) {
+  return ((word >> (4 * i)) & 0x000F000Fu) | Num<BF16>::kMagic;
+}
+
+// A group's scale (bits 16-31) and magic + zero point (bits 0-15) in one word.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_scale(uint16_t scale, uint32_t zero) {
+  // Bit 0 of the mantissa is worth 1 at both magic numbers, so adding the
+  // zero point to the bits adds it to the number (zero points past 15 would
+  // leave the mantissa: they are cut to 4 bits).
+  return (uint32_t(scale) << 16) | ((Num<BF16>::kMagic & 0xFFFFu) + (zero & 15u));
+}
+template <bool BF16>
+__device__ __forceinline__ float scale_of(uint32_t packed) {
+  return Num<BF16>::to_float(uint16_t(packed >> 16));
+}
+__device__ __forceinline__ uint32_t zero_pair(uint32_t packed) { return __byte_perm(packed, 0, 0x1010); }
+__device__ __forceinline__ uint32_t scale_pair(uint32_t packed) { return __byte_perm(packed, 0, 0x3232); }
+
+__device__ __forceinline__ float silu(float v) { return v / (1.0f + __expf(-v)); }
+
+}  // namespace w4
+
+constexpr int kW4SmallThreads = 256;
+// The small kernel's dynamic shared memory, by tokens per tile (8, 16, 32)
+// and groups per 128 weights of a row (1, 2, 4).
+size_t w4_small_smem(int tokens, int groups);
+// The kernel for an activation type, tokens per tile (8, 16, 32), groups per
+// 128 weights (1, 2, 4) and output form.
+using W4Kernel = void (*)(W4Params);
+W4Kernel w4_small_kernel(bool bf16, int tokens, int groups, bool swiglu);
+
+}  // namespace aspire

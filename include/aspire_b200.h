@@ -12,7 +12,10 @@
  *   3. the paged KV append of the step's new tokens, the mixed page-list
  *      build, the draft-page spill insert and the dump-state reset of cleared
  *      slots;
- *   4. planning: on the host, or on the device inside a CUDA graph.
+ *   4. planning: on the host, or on the device inside a CUDA graph;
+ *   5. the feed-forward block around it: products with 4-bit weights (one
+ *      matrix, or one per expert) and the tokens' way to their experts and
+ *      back, with its gradients.
  *
  * Every entry point takes plain pointers, sizes and a CUDA stream handle
  * (passed as void*); no framework types cross this boundary.  Every entry
@@ -542,6 +545,135 @@ typedef struct AspireClearDumpArgs {
  * Capturable; allocates nothing.
  */
 ASPIRE_API int aspire_clear_dump_slots(const AspireClearDumpArgs* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Products with 4-bit weights and group scales (device).                   */
+/* ------------------------------------------------------------------------ */
+
+/* Element types of the feed-forward operators. */
+#define ASPIRE_T_F32 0
+#define ASPIRE_T_BF16 1
+#define ASPIRE_T_F16 2
+
+/*
+ * A 4-bit matrix of R rows and k columns: codes uint32 [R, k / 8], scales
+ * [R, k / group] in the type of x, and optionally zeros uint8 [R, k / group]
+ * (0..15; NULL means 8 everywhere).  Weight (r, j) is (q - zero) * scale.  A
+ * word holds eight consecutive weights of a row: weight 8w + 2i in bits
+ * 4i..4i+3 and weight 8w + 2i + 1 in bits 16+4i..19+4i.
+ */
+typedef struct AspireW4Args {
+  const void* x;             /* [rows, k], bf16 or fp16                                     */
+  int64_t x_stride;          /* elements; a multiple of 8                                   */
+  int64_t rows;
+  const uint32_t* codes;     /* [experts,] [R, k / 8]; R = n, or 2n with swiglu             */
+  int64_t codes_stride;      /* words per row (a multiple of 4) and per expert              */
+  int64_t codes_stride_e;
+  const void* scales;        /* [experts,] [R, k / group]                                   */
+  int64_t scales_stride, scales_stride_e;
+  const uint8_t* zeros;      /* [experts,] [R, k / group] or NULL                           */
+  int64_t zeros_stride, zeros_stride_e;
+  const void* residual;      /* [rows, n] added to the product, or NULL                     */
+  int64_t residual_stride;
+  void* out;                 /* [rows, n]                                                   */
+  int64_t out_stride;
+  int32_t n, k;              /* k a multiple of 32 and of group                             */
+  int32_t group;             /* 32, 64 or a multiple of 128                                 */
+  int32_t type;              /* ASPIRE_T_BF16 or ASPIRE_T_F16                               */
+  int32_t swiglu;            /* 1: rows [0, n) gate, [n, 2n) up; out = silu(gate) * up      */
+  const int32_t* offsets;    /* int32 [experts + 1]: expert e's rows of x; NULL: one matrix */
+  int32_t experts;
+  uint32_t* status;          /* optional device status word                                 */
+} AspireW4Args;
+
+/*
+ * out[t] = x[t] W^T (+ residual[t]), or its gated form, in one launch; with
+ * offsets, rows offsets[e] <= t < offsets[e + 1] use expert e's matrix and
+ * rows past the last expert's become zero.  Sums are in fp32 and every output
+ * is rounded once; with more than 32 rows the weights are rounded to x's type
+ * before the product.  Row ranges that run backwards or leave [0, rows) are
+ * cut and set ASPIRE_STATUS_BAD_ROW.  Capturable; allocates nothing.  No
+ * counterpart in the reference, whose linear layers are bf16.
+ */
+ASPIRE_API int aspire_w4_linear(const AspireW4Args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Tokens to experts and back (device).                                     */
+/* ------------------------------------------------------------------------ */
+
+/* Slots are (token, choice) pairs, numbered token * top_k + choice.  Limits:
+ * 512 experts, top_k <= 32. */
+typedef struct AspireMoeRouteArgs {
+  const void* logits;        /* [tokens, num_experts]; NULL: experts is an input (sort only) */
+  int32_t logits_type;       /* ASPIRE_T_*                                                   */
+  int64_t logits_stride;     /* elements                                                     */
+  int64_t tokens;
+  int32_t num_experts, top_k;
+  int32_t renormalize;       /* 1: weights sum to 1 over the choices                         */
+  float* weights;            /* [tokens, top_k] (unused without logits)                      */
+  int32_t* experts;          /* [tokens, top_k]; -1 = no expert                              */
+  int32_t* position;         /* [tokens, top_k]: the slot's sorted row, -1 = none            */
+  int32_t* source;           /* [tokens * top_k]: the sorted row's slot, -1 past the last    */
+  int32_t* offsets;          /* [num_experts + 1]                                            */
+  int32_t* workspace;        /* aspire_moe_route_workspace() bytes, or NULL when that is 0   */
+  size_t workspace_bytes;
+} AspireMoeRouteArgs;
+
+/*
+ * The top_k largest logits of every token (equal ones: the lowest expert
+ * first; NaN and -inf are never chosen, and missing choices get expert -1 and
+ * weight 0), their weights (softmax over all experts, or over the chosen ones
+ * when renormalised) and the stable sort of the slots by expert.  One launch
+ * up to 1024 slots, two beyond.  Expert ids outside [0, num_experts) count as
+ * none.  Capturable.
+ */
+ASPIRE_API int aspire_moe_route(const AspireMoeRouteArgs* args, void* stream);
+ASPIRE_API size_t aspire_moe_route_workspace(int64_t tokens, int32_t num_experts, int32_t top_k);
+
+typedef struct AspireMoeRouteGradArgs {
+  const void* logits;        /* as in aspire_moe_route (read only without renormalize)       */
+  int32_t logits_type;
+  int64_t logits_stride;
+  const float* weights;      /* aspire_moe_route's results                                   */
+  const int32_t* experts;
+  const float* grad_weights; /* [tokens, top_k]                                              */
+  int64_t tokens;
+  int32_t num_experts, top_k, renormalize;
+  void* grad_logits;         /* [tokens, num_experts], the logits' type                      */
+} AspireMoeRouteGradArgs;
+
+/* Gradient of the weights of aspire_moe_route to the logits. */
+ASPIRE_API int aspire_moe_route_grad(const AspireMoeRouteGradArgs* args, void* stream);
+
+typedef struct AspireMoePermuteArgs {
+  int32_t type;              /* ASPIRE_T_* of in, residual, out and grad                     */
+  const void* in;            /* dispatch: [tokens, width]; else [tokens * top_k, width]      */
+  int64_t in_stride;         /* strides: elements, rows 16-byte aligned                      */
+  const void* residual;      /* combine: [tokens, width] or NULL                             */
+  int64_t residual_stride;
+  const float* weights;      /* [tokens, top_k]; NULL: 1                                     */
+  const int32_t* position;   /* [tokens, top_k]                                              */
+  const int32_t* offsets;    /* [num_experts + 1]                                            */
+  int32_t num_experts, top_k;
+  int64_t tokens;
+  int32_t width;             /* a multiple of 16 bytes                                       */
+  void* out;                 /* dispatch and combine_grad: [tokens * top_k, width]           */
+  int64_t out_stride;
+  const void* grad;          /* combine_grad: [tokens, width] gradient of the outputs        */
+  int64_t grad_stride;
+  float* grad_weights;       /* combine_grad: [tokens, top_k] or NULL                        */
+  uint32_t* status;          /* optional device status word                                  */
+} AspireMoePermuteArgs;
+
+/* out[position[t, j]] = in[t]; rows past offsets[num_experts] become zero. */
+ASPIRE_API int aspire_moe_dispatch(const AspireMoePermuteArgs* args, void* stream);
+/* out[t] = sum_j weights[t, j] in[position[t, j]] (+ residual[t]), fp32 sums.
+ * Without weights it is the gradient of aspire_moe_dispatch. */
+ASPIRE_API int aspire_moe_combine(const AspireMoePermuteArgs* args, void* stream);
+/* Gradients of aspire_moe_combine: out[position[t, j]] = weights[t, j]
+ * grad[t] (rows past the last expert's: zero; out may be NULL) and
+ * grad_weights[t, j] = <grad[t], in[position[t, j]]>. */
+ASPIRE_API int aspire_moe_combine_grad(const AspireMoePermuteArgs* args, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Utilities.                                                               */
