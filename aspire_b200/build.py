@@ -35,6 +35,7 @@ SOURCES = [
     "dump_state.cu",
     "capi_ffn.cu",
     "w4_small.cu",
+    "w4_tc.cu",
     "moe_route.cu",
     "moe_permute.cu",
 ]

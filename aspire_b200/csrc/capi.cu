@@ -42,7 +42,7 @@ namespace {
 
 SmemOptIn g_gather_smem, g_tc_smem, g_sel_smem;
 
-// Bound of one pipeline wait of the tcgen05 kernel (aspire_set_wait_limit_ns);
+// Bound of one pipeline wait of the tcgen05 kernels (aspire_set_wait_limit_ns);
 // 0 selects the default.
 constexpr uint64_t kDefaultWaitNs = 1000000000ull;
 std::atomic<uint64_t> g_wait_limit_ns{0};
@@ -107,6 +107,11 @@ bool tc_env_enabled() {
 }
 
 }  // namespace
+
+uint64_t wait_limit_ns() {
+  const uint64_t v = g_wait_limit_ns.load(std::memory_order_relaxed);
+  return v ? v : kDefaultWaitNs;
+}
 
 int check_attention_args(const AspireAttnArgs* a, const AspirePlanInfo* plan, const char* who) {
   const std::string w(who);
@@ -176,7 +181,7 @@ const char* aspire_kernel_names(void) {
   return "aspire_attn_gather_kernel\naspire_attn_tc_kernel\naspire_attn_merge_kernel\naspire_append_kv_kernel\n"
          "aspire_select_pages_kernel\naspire_page_scores_kernel\naspire_build_indices_kernel\naspire_qkv_prologue_kernel\naspire_plan_device_kernel\n"
          "aspire_draft_spill_kernel\naspire_clear_dump_kernel\n"
-         "aspire_w4_small_kernel\naspire_moe_route_kernel\naspire_moe_sort_kernel\naspire_moe_route_grad_kernel\n"
+         "aspire_w4_small_kernel\naspire_w4_tc_kernel\naspire_moe_route_kernel\naspire_moe_sort_kernel\naspire_moe_route_grad_kernel\n"
          "aspire_moe_dispatch_kernel\naspire_moe_combine_kernel\naspire_moe_combine_grad_kernel\n";
 }
 
@@ -332,8 +337,7 @@ int aspire_mixed_attention(const AspireAttnArgs* a, const AspirePlanInfo* plan, 
   p.plan = reinterpret_cast<const int32_t*>(static_cast<const char*>(a->int_ws) + kStatusBytes);
   p.status = static_cast<uint32_t*>(a->int_ws);
   p.partial_o = static_cast<float*>(a->float_ws);
-  const uint64_t wait_ns = g_wait_limit_ns.load(std::memory_order_relaxed);
-  p.wait_ns = wait_ns ? wait_ns : kDefaultWaitNs;
+  p.wait_ns = wait_limit_ns();
 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Kernels are launched with plan-independent grids: items live in device

@@ -35,14 +35,20 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 int ceil32(int v) { return (v + 31) / 32 * 32; }
 
+// Rows (an expert's average share of them) up to which the kernel for few
+// tokens runs.
+constexpr int64_t kW4SmallRows = 32;
+
 // Opt-in caches of the small kernel's variants: [type][tokens 8, 16, 32]
 // [groups 1, 2, 4][swiglu].
 SmemOptIn g_w4_small[2][3][3][2];
 
 int index_of(int v) { return v <= 1 ? 0 : (v == 2 ? 1 : 2); }
 
-int w4_launch(W4Kernel kernel, dim3 grid, int cluster, int threads, size_t smem, cudaStream_t stream,
-              const char* what, const W4Params& p) {
+// Launch with a programmatic dependency and, for cluster > 1, clusters along x.
+template <typename... KArgs, typename... Args>
+int w4_launch(void (*kernel)(KArgs...), dim3 grid, int cluster, int threads, size_t smem, cudaStream_t stream,
+              const char* what, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -57,7 +63,7 @@ int w4_launch(W4Kernel kernel, dim3 grid, int cluster, int threads, size_t smem,
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), what);
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), what);
 }
 
 // Upper bound of the token tiles of `rows` rows in `experts` ranges (0: one
@@ -67,11 +73,15 @@ int64_t tiles_bound(int64_t rows, int32_t experts, bool grouped, int width) {
   return std::min<int64_t>(rows, experts) + rows / width + 1;
 }
 
+// Rows an ordinary tile has to hold: all of them, or an expert's average share.
+int64_t typical_rows(const AspireW4Args* a) {
+  return a->offsets ? (a->rows + a->experts - 1) / a->experts : a->rows;
+}
+
 int w4_small(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
   const bool grouped = a->offsets != nullptr;
-  // Tokens per tile: the fewest columns that hold the rows (an expert's
-  // average share of them), up to 32.
-  const int64_t typical = grouped ? (a->rows + a->experts - 1) / std::max(a->experts, 1) : a->rows;
+  // Tokens per tile: the fewest columns that hold the rows.
+  const int64_t typical = typical_rows(a);
   const int tokens = typical <= 8 ? 8 : (typical <= 16 ? 16 : 32);
   const int groups = a->group == 32 ? 4 : (a->group == 64 ? 2 : 1);
   const int features = a->swiglu ? w4::kRows / 2 : w4::kRows;
@@ -94,6 +104,67 @@ int w4_small(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
   if (rc) return rc;
   return w4_launch(kernel, dim3(unsigned(cluster), unsigned(ny), unsigned(nz)), cluster, kW4SmallThreads, smem, stream,
                    "aspire_w4_small_kernel launch", p);
+}
+
+int encode_map(CUtensorMap* map, CUtensorMapDataType type, int dims, const void* base, const cuuint64_t* size,
+               const cuuint64_t* strides, const cuuint32_t* box) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (!enc) return set_error(ASPIRE_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  const cuuint32_t ones[3] = {1, 1, 1};
+  const CUresult r = enc(map, type, cuuint32_t(dims), const_cast<void*>(base), size, strides, box, ones,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(ASPIRE_ERR_INVALID,
+                     "aspire_w4_linear: cuTensorMapEncodeTiled failed with code " + std::to_string(int(r)));
+  return ASPIRE_OK;
+}
+
+SmemOptIn g_w4_tc[2][3][3][2];
+
+int w4_tc(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
+  const bool grouped = a->offsets != nullptr;
+  const int64_t typical = typical_rows(a);
+  const int tokens = typical <= 64 ? 64 : (typical <= 128 ? 128 : 256);
+  const int groups = a->group == 32 ? 4 : (a->group == 64 ? 2 : 1);
+  const int features = a->swiglu ? w4::kRows / 2 : w4::kRows;
+  const int64_t ny = (int64_t(a->n) + features - 1) / features;
+  const int64_t nz = tiles_bound(a->rows, a->experts, grouped, tokens);
+  if (ny > 65535 || nz > 65535) return invalid("aspire_w4_linear", "n or rows too large");
+  int sms = 0;
+  int rc = current_sm_count(&sms);
+  if (rc) return rc;
+  const int64_t slots = int64_t(sms) * (tokens == 256 ? 1 : 2);
+  const int64_t stages = (a->k + 255) / 256;
+  int cluster = 1;
+  while (cluster < 8 && ny * nz * cluster * 2 <= slots && cluster * 2 <= stages) cluster *= 2;
+  CUtensorMap codes_map, x_map;
+  const cuuint64_t matrix_rows = cuuint64_t(a->n) * (a->swiglu ? 2 : 1);
+  {
+    const cuuint64_t size[3] = {cuuint64_t(a->k / 8), matrix_rows, cuuint64_t(grouped ? a->experts : 1)};
+    const cuuint64_t strides[2] = {cuuint64_t(a->codes_stride) * 4,
+                                   cuuint64_t(grouped && a->experts > 1 ? a->codes_stride_e : a->codes_stride) * 4};
+    const cuuint32_t box[3] = {32, cuuint32_t(features), 1};
+    rc = encode_map(&codes_map, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, a->codes, size, strides, box);
+    if (rc) return rc;
+  }
+  {
+    const cuuint64_t size[2] = {cuuint64_t(a->k), cuuint64_t(a->rows)};
+    const cuuint64_t strides[1] = {cuuint64_t(a->x_stride) * 2};
+    const cuuint32_t box[2] = {64, cuuint32_t(tokens)};
+    rc = encode_map(&x_map,
+                    a->type == ASPIRE_T_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                    a->x, size, strides, box);
+    if (rc) return rc;
+  }
+  W4TcKernel kernel = w4_tc_kernel(a->type == ASPIRE_T_BF16, tokens, groups, a->swiglu != 0);
+  const size_t smem = w4_tc_smem(tokens);
+  rc = ensure_smem(reinterpret_cast<const void*>(kernel), smem,
+                   g_w4_tc[a->type == ASPIRE_T_BF16][tokens == 64 ? 0 : (tokens == 128 ? 1 : 2)][index_of(groups)]
+                          [a->swiglu != 0]);
+  if (rc) return rc;
+  return w4_launch(kernel, dim3(unsigned(cluster), unsigned(ny), unsigned(nz)), cluster, kW4TcThreads, smem, stream,
+                   "aspire_w4_tc_kernel launch", p, codes_map, x_map);
 }
 
 int64_t elem_bytes(int32_t type) { return type == ASPIRE_T_F32 ? 4 : 2; }
@@ -211,7 +282,9 @@ int aspire_w4_linear(const AspireW4Args* a, void* stream) {
     p.offsets = a->offsets;
     p.num_experts = a->offsets ? a->experts : 0;
     p.status = a->status;
-    return w4_small(a, p, static_cast<cudaStream_t>(stream));
+    p.wait_ns = wait_limit_ns();
+    return typical_rows(a) <= kW4SmallRows ? w4_small(a, p, static_cast<cudaStream_t>(stream))
+                                           : w4_tc(a, p, static_cast<cudaStream_t>(stream));
   });
 }
 

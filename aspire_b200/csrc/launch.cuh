@@ -33,6 +33,9 @@ int launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStr
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...), what);
 }
 
+// Bound of one pipeline wait of the tcgen05 kernels, in nanoseconds.
+uint64_t wait_limit_ns();
+
 inline int current_sm_count(int* out) {
   int dev = 0;
   int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");

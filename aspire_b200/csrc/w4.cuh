@@ -183,4 +183,13 @@ size_t w4_small_smem(int tokens, int groups);
 using W4Kernel = void (*)(W4Params);
 W4Kernel w4_small_kernel(bool bf16, int tokens, int groups, bool swiglu);
 
+// The tcgen05 kernel, by tokens per tile (64, 128, 256).  Its tensor maps:
+// the codes as int32 [experts, rows, k / 8] with boxes of 32 words x 128 rows
+// (64 with the activation), the tokens as [rows, k] with boxes of 64 x tokens,
+// both with the 128-byte swizzle.
+constexpr int kW4TcThreads = 320;
+size_t w4_tc_smem(int tokens);
+using W4TcKernel = void (*)(W4Params, CUtensorMap, CUtensorMap);
+W4TcKernel w4_tc_kernel(bool bf16, int tokens, int groups, bool swiglu);
+
 }  // namespace aspire
