@@ -278,7 +278,15 @@ int aspire_w4_linear(const AspireW4Args* a, void* stream) {
     p.out_stride = a->out_stride;
     p.n = a->n;
     p.k = a->k;
-    p.group = a->group;
+    p.group_blocks = std::max(a->group / 128, 1);
+    p.group_recip = p.group_blocks > 1 ? uint32_t((uint64_t(1) << 32) / uint64_t(p.group_blocks)) + 1u : 0u;
+    // 256 weights have 8, 4 or 2 groups: 16, 8 or 4 bytes of scales, and 8 or 4
+    // of zero points (two groups' are half a word).
+    const uintptr_t sb = a->group == 32 ? 16 : (a->group == 64 ? 8 : 4), zb = a->group == 32 ? 8 : 4;
+    p.scales_vec = a->group <= 128 && (reinterpret_cast<uintptr_t>(a->scales) | uintptr_t(a->scales_stride * 2) |
+                                       uintptr_t(a->offsets ? a->scales_stride_e * 2 : 0)) % sb == 0;
+    p.zeros_vec = a->group <= 128 && (reinterpret_cast<uintptr_t>(a->zeros) | uintptr_t(a->zeros_stride) |
+                                      uintptr_t(a->offsets ? a->zeros_stride_e : 0)) % zb == 0;
     p.offsets = a->offsets;
     p.num_experts = a->offsets ? a->experts : 0;
     p.status = a->status;

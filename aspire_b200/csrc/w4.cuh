@@ -12,6 +12,8 @@
 // in the two halves of a register.
 #pragma once
 
+#include <cooperative_groups.h>
+
 #include "kernels.cuh"
 
 namespace aspire {
@@ -30,7 +32,12 @@ struct W4Params {
   int64_t residual_stride;
   uint16_t* out;            // [rows, n]
   int64_t out_stride;
-  int32_t n, k, group;
+  int32_t n, k;
+  int32_t group_blocks;     // groups of 128 m weights: m; else 1
+  uint32_t group_recip;     // floor(2^32 / m) + 1, or 0 when m is 1
+  // Whether rows are aligned such that the groups of 256 weights load at once
+  // (with one group per 128 weights: that group is 128, and a word holds them).
+  int32_t scales_vec, zeros_vec;
   const int32_t* offsets;   // rows of expert e: [offsets[e], offsets[e + 1]); NULL: one matrix for all rows
   int32_t num_experts;
   uint32_t* status;
@@ -152,7 +159,11 @@ struct Num<false> {
 // Pair i of a word: (weight 2i, weight 2i + 1) + magic.
 template <bool BF16>
 __device__ __forceinline__ uint32_t magic_pair(uint32_t word, int i) {
-  return ((word >> (4 * i)) & 0x000F000Fu) | Num<BF16>::kMagic;
+  // One three-input operation, (a & b) | c: written out, since the compiler
+  // keeps it as two when both constants are immediates.
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(word >> (4 * i)), "r"(0x000F000Fu), "r"(Num<BF16>::kMagic));
+  return r;
 }
 
 // A group's scale (bits 16-31) and magic + zero point (bits 0-15) in one word.
@@ -170,7 +181,100 @@ __device__ __forceinline__ float scale_of(uint32_t packed) {
 __device__ __forceinline__ uint32_t zero_pair(uint32_t packed) { return __byte_perm(packed, 0, 0x1010); }
 __device__ __forceinline__ uint32_t scale_pair(uint32_t packed) { return __byte_perm(packed, 0, 0x3232); }
 
+// One matrix row's packed scales, GROUPS (1, 2, 4) for every block of 128
+// weights; a group of 128 m weights has one for m blocks.
+template <bool BF16, int GROUPS>
+struct ScaleRow {
+  const uint16_t* scale;
+  const uint8_t* zero;  // NULL: 8
+  bool live;
+
+  __device__ __forceinline__ ScaleRow(const W4Params& p, int expert, int64_t row, bool live_)
+      : scale(p.scales + int64_t(expert) * p.scales_stride_e + row * p.scales_stride),
+        zero(p.zeros ? p.zeros + int64_t(expert) * p.zeros_stride_e + row * p.zeros_stride : nullptr),
+        live(live_) {}
+
+  __device__ __forceinline__ static int first_group(const W4Params& p, int block) {
+    if (GROUPS > 1) return block * GROUPS;
+    return p.group_recip ? int(__umulhi(uint32_t(block), p.group_recip)) : block;
+  }
+  // Blocks past the row's end give scale 0.
+  __device__ __forceinline__ void load(const W4Params& p, int block, uint32_t* v) const {
+#pragma unroll
+    for (int e = 0; e < GROUPS; ++e) v[e] = pack_scale<BF16>(0, 8);
+    if (!live || block * 128 >= p.k) return;
+    const int gi = first_group(p, block);
+    alignas(8) uint16_t s[GROUPS];
+    alignas(4) uint8_t z[GROUPS];
+    // A whole block's groups in one load each, where rows are aligned for it.
+    const bool whole = GROUPS > 1 && block * 128 + 128 <= p.k;
+    if (whole && p.scales_vec) {
+      if constexpr (GROUPS == 4) *reinterpret_cast<uint2*>(s) = __ldg(reinterpret_cast<const uint2*>(scale + gi));
+      if constexpr (GROUPS == 2) *reinterpret_cast<uint32_t*>(s) = __ldg(reinterpret_cast<const uint32_t*>(scale + gi));
+    } else {
+#pragma unroll
+      for (int e = 0; e < GROUPS; ++e) s[e] = block * 128 + e * (128 / GROUPS) < p.k ? __ldg(scale + gi + e) : 0;
+    }
+#pragma unroll
+    for (int e = 0; e < GROUPS; ++e) z[e] = 8;
+    if (zero) {
+      if (whole && p.zeros_vec) {
+        if constexpr (GROUPS == 4) *reinterpret_cast<uint32_t*>(z) = __ldg(reinterpret_cast<const uint32_t*>(zero + gi));
+        if constexpr (GROUPS == 2) *reinterpret_cast<uint16_t*>(z) = __ldg(reinterpret_cast<const uint16_t*>(zero + gi));
+      } else {
+#pragma unroll
+        for (int e = 0; e < GROUPS; ++e)
+          if (block * 128 + e * (128 / GROUPS) < p.k) z[e] = __ldg(zero + gi + e);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < GROUPS; ++e) v[e] = pack_scale<BF16>(s[e], z[e]);
+  }
+};
+
 __device__ __forceinline__ float silu(float v) { return v / (1.0f + __expf(-v)); }
+
+// The outputs of a tile from the ranks' fp32 partials `red` [tokens][pitch]
+// (matrix rows along a line), added in rank order: rank r finishes its part
+// of the features.  Threads go along the features, so a token's outputs leave
+// as consecutive elements.
+template <bool BF16, bool SWIGLU>
+__device__ __forceinline__ void finish_tile(const W4Params& p, const Tile& tile, int f0, int rank, int ranks,
+                                            float* red, int pitch, int tid, int threads) {
+  constexpr int FEATURES = SWIGLU ? kRows / 2 : kRows;
+  const int share = FEATURES / ranks;  // a power of two
+  const int shift = 31 - __clz(share);
+  for (int i = tid; i < tile.count * share; i += threads) {
+    const int t = i >> shift, fl = rank * share + (i & (share - 1)), f = f0 + fl;
+    if (f >= p.n) continue;
+    const int at = t * pitch + fl;
+    float a = 0.f, b = 0.f;
+    if (ranks == 1) {
+      a = red[at];
+      if (SWIGLU) b = red[at + FEATURES];
+    } else {
+      float va[8], vb[8];  // all in flight at once
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        va[q] = vb[q] = 0.f;
+        if (q < ranks) {
+          const float* rq = cooperative_groups::this_cluster().map_shared_rank(red, q);
+          va[q] = rq[at];
+          if (SWIGLU) vb[q] = rq[at + FEATURES];
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        a += va[q];
+        if (SWIGLU) b += vb[q];
+      }
+    }
+    const int64_t row = tile.row0 + t;
+    if (SWIGLU) a = silu(a) * b;
+    if (p.residual) a += Num<BF16>::to_float(p.residual[row * p.residual_stride + f]);
+    p.out[row * p.out_stride + f] = Num<BF16>::from_float(a);
+  }
+}
 
 }  // namespace w4
 
@@ -187,7 +291,7 @@ W4Kernel w4_small_kernel(bool bf16, int tokens, int groups, bool swiglu);
 // the codes as int32 [experts, rows, k / 8] with boxes of 32 words x 128 rows
 // (64 with the activation), the tokens as [rows, k] with boxes of 64 x tokens,
 // both with the 128-byte swizzle.
-constexpr int kW4TcThreads = 320;
+constexpr int kW4TcThreads = 352;
 size_t w4_tc_smem(int tokens);
 using W4TcKernel = void (*)(W4Params, CUtensorMap, CUtensorMap);
 W4TcKernel w4_tc_kernel(bool bf16, int tokens, int groups, bool swiglu);

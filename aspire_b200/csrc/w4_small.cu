@@ -4,18 +4,23 @@
 // owns 128 matrix rows (64 gate and 64 up rows with the activation), 8, 16 or
 // 32 tokens and a range of K, and streams the rows' codes through a ring of
 // 256-weight stages in shared memory (asynchronous 16-byte copies, 128
-// contiguous bytes of a row at a time; chunk c of row r sits at slot c ^ (r &
-// 7), so the fragment loads below touch every bank once).
+// contiguous bytes of a row at a time).  The loop is unrolled over the ring,
+// so that its addresses are constants: unpacking a weight takes about 1.5
+// instructions, and every one around it counts.
 //
 // The products run on warp-level matrix instructions with the weights as A
 // (16 rows x 16 k) unpacked in registers and the tokens as B (8 columns): at
 // 8 to 32 tokens the unpacking, not the tensor rate, is what could slow the
 // stream, and unpacked fragments go straight from registers into the
-// instruction.  Lane (g, c) of a warp (g = lane / 4) holds word c of a row's
-// 32-weight chunk, and the sum over k may run in any order, so the
-// instruction's k slots are assigned to the word's weights in place (its
-// first two pairs feed one instruction, the last two the next) and the
-// tokens' fragment is the 16 contiguous bytes x[token g][32 i + 8 c ...].
+// instruction.  The sum over k may run in any order, so the instruction's k
+// slots are assigned to the codes as they lie: of each group's part of a stage
+// lane (g, c) of a warp (g = lane / 4) loads the c-th quarter of row g's codes
+// with one load, and a word's first two pairs of weights feed one instruction,
+// its last two the next.  The tokens' matching 8-element pieces are permuted
+// on their way into shared memory such that a fragment is one conflict-free
+// 16-byte load; the codes' 16-byte chunks are placed at slot chunk ^ reversed
+// bits of (row & 7), which keeps 4-, 8- and 16-byte fragment loads free of
+// conflicts.
 //
 // Codes minus zero points are exact in 16 bits; a group's sum is scaled in
 // fp32 and added to the running sum, so nothing is rounded before the output.
@@ -41,21 +46,38 @@ constexpr int kXPitch = kStageK * 2 + 64;         // bytes; 64 mod 128: conflict
 constexpr int kRedPitch = kRows + 4;              // floats
 constexpr int kSmemBudget = 113 * 1024;           // two CTAs per SM
 
-__host__ __device__ constexpr int stage_bytes(int tokens) { return kCodeBytes + tokens * kXPitch; }
-// Packed scales of a stage: 128 rows x groups of 256 weights, double buffered.
-__host__ __device__ constexpr int scale_bytes(int groups) { return 2 * 2 * groups * kRows * 4; }
+// A stage: codes, tokens, and 128 rows' scales (2 x groups of 2 bytes) and
+// zero points (a byte each; 4 bytes at least, the smallest copy).
+__host__ __device__ constexpr int scale_row_bytes(int groups) { return 4 * groups; }
+__host__ __device__ constexpr int zero_row_bytes(int groups) { return groups == 4 ? 8 : 4; }
+__host__ __device__ constexpr int scale_at(int tokens) { return kCodeBytes + tokens * kXPitch; }
+__host__ __device__ constexpr int zero_at(int tokens, int groups) {
+  return scale_at(tokens) + kRows * scale_row_bytes(groups);
+}
+__host__ __device__ constexpr int stage_bytes(int tokens, int groups) {
+  return zero_at(tokens, groups) + kRows * zero_row_bytes(groups);
+}
 __host__ __device__ constexpr int stages_for(int tokens, int groups) {
-  const int s = (kSmemBudget - scale_bytes(groups)) / stage_bytes(tokens);
+  const int s = kSmemBudget / stage_bytes(tokens, groups);
   return s > 4 ? 4 : s;
 }
 __host__ __device__ constexpr int ring_bytes(int tokens, int groups) {
-  const int ring = stages_for(tokens, groups) * stage_bytes(tokens);
-  const int red = 2 * tokens * kRedPitch * 4;  // the partials reuse the ring
+  const int ring = stages_for(tokens, groups) * stage_bytes(tokens, groups);
+  const int red = tokens * kRedPitch * 4;  // the partials reuse the ring
   return ring > red ? ring : red;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+// Slot of a row's 16-byte chunk: chunk ^ this (f of row 0..7: 0 4 2 6 1 5 3 7).
+__device__ __forceinline__ int slot_mask(int row) { return ((row & 1) << 2) | (row & 2) | ((row >> 2) & 1); }
+
+// 16 bytes, of which `size` (16 or 0) come from src and the rest are zero.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t size) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
+}
+// SIZE bytes (4, 8 or 16), the first `size` of them from src, the rest zero.
+template <int SIZE>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, uint32_t size) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(SIZE), "r"(size) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -87,11 +109,10 @@ __global__ void __launch_bounds__(kW4SmallThreads, 2) aspire_w4_small_kernel(con
   pdl_begin();
   constexpr int NT = TOKENS / 8;
   constexpr int STAGES = stages_for(TOKENS, GROUPS);
-  constexpr int ENTRIES = 2 * GROUPS * kRows / kW4SmallThreads;  // packed scales of a stage per thread
-  constexpr int CHUNKS_PER_GROUP = 4 / GROUPS;
+  constexpr int WORDS = 4 / GROUPS;  // words of a group's part a lane loads
+  constexpr int STAGE = stage_bytes(TOKENS, GROUPS);
   constexpr int FEATURES = SWIGLU ? kRows / 2 : kRows;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint32_t* sc = reinterpret_cast<uint32_t*>(smem + ring_bytes(TOKENS, GROUPS));
   float* red = reinterpret_cast<float*>(smem);
   __shared__ Tile tile_s;
 
@@ -120,8 +141,6 @@ __global__ void __launch_bounds__(kW4SmallThreads, 2) aspire_w4_small_kernel(con
     return;
   }
   const uint32_t* codes = p.codes + int64_t(tile.expert) * p.codes_stride_e;
-  const uint16_t* scales = p.scales + int64_t(tile.expert) * p.scales_stride_e;
-  const uint8_t* zeros = p.zeros ? p.zeros + int64_t(tile.expert) * p.zeros_stride_e : nullptr;
   const uint16_t* x = p.x + int64_t(tile.row0) * p.x_stride;
 
   // Matrix row of tile row r (-1 past the matrix).
@@ -136,53 +155,92 @@ __global__ void __launch_bounds__(kW4SmallThreads, 2) aspire_w4_small_kernel(con
   const int n_stages = (p.k + kStageK - 1) / kStageK;
   const int s_begin = int(int64_t(n_stages) * rank / ranks), s_end = int(int64_t(n_stages) * (rank + 1) / ranks);
 
+  const void* const codes_any = p.codes;  // a readable address for copies of size 0
   // Copies of a stage: thread tid moves 16-byte chunk tid % 8 of rows tid / 8
-  // + 32 i, and its share of the tokens' chunks.
+  // + 32 i and 8-element piece lane of tokens warp + 8 i.  A size of 0 fills
+  // with zeros and reads nothing.
   const int cc = tid & 7;
   const uint32_t* code_src[4];
-  bool code_live[4];
+  uint32_t code_size[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t mr = matrix_row((tid >> 3) + 32 * i);
-    code_live[i] = mr >= 0;
-    code_src[i] = codes + (mr >= 0 ? mr : 0) * p.codes_stride + cc * 4;
+    code_size[i] = mr >= 0 ? 16 : 0;
+    code_src[i] = codes + (mr >= 0 ? mr : 0) * p.codes_stride + int64_t(s_begin) * (kStageK / 8) + cc * 4;
+  }
+  constexpr int XN = TOKENS / 8;
+  const uint16_t* x_src[XN];
+  uint32_t x_size[XN];
+#pragma unroll
+  for (int i = 0; i < XN; ++i) {
+    const int t = warp + i * 8;
+    x_size[i] = t < tile.count ? 16 : 0;
+    x_src[i] = x + (t < tile.count ? t : 0) * p.x_stride + int64_t(s_begin) * kStageK + lane * 8;
   }
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-  auto load_stage = [&](int s) {
+  const uint32_t code_dst = ring + (tid >> 3) * 128 + ((cc ^ slot_mask(tid >> 3)) << 4);
+  // Piece u = WORDS c + i of a group's part goes to place 4 i + c.
+  const int u = lane & (4 * WORDS - 1);
+  const int place = (lane & ~(4 * WORDS - 1)) + (u % WORDS) * 4 + u / WORDS;
+  const uint32_t x_dst = ring + kCodeBytes + warp * kXPitch + place * 16;
+  // Scales and zero points: threads 0-127 copy their row's scales of the
+  // stage, threads 128-255 its zero points.  Rows that are not aligned for
+  // those copies are read element by element when the stage is loaded.
+  constexpr int SB = scale_row_bytes(GROUPS), ZB = zero_row_bytes(GROUPS), PER_STAGE = 2 * GROUPS;
+  const int sr = tid & (kRows - 1);
+  const bool is_zero = tid >= kRows;
+  const int64_t srow = matrix_row(sr);
+  const uint8_t* side_src = nullptr;  // the row's first scale or zero point; NULL: nothing to copy
+  if (srow >= 0) {
+    if (!is_zero)
+      side_src = reinterpret_cast<const uint8_t*>(p.scales + int64_t(tile.expert) * p.scales_stride_e +
+                                                  srow * p.scales_stride);
+    else if (p.zeros)
+      side_src = p.zeros + int64_t(tile.expert) * p.zeros_stride_e + srow * p.zeros_stride;
+  }
+  const bool side_fast = is_zero ? p.zeros_vec : p.scales_vec;
+  const int n_groups = int(int64_t(p.k) * GROUPS / 128);  // of a row, where the copies are used
+  const uint32_t side_dst = ring + (is_zero ? zero_at(TOKENS, GROUPS) + sr * ZB : scale_at(TOKENS) + sr * SB);
+  auto load_side = [&](int s, int slot) {
+    const uint32_t dst = side_dst + slot * STAGE;
+    if (side_fast) {
+      // A stage's zero points with one group per 128 weights are half a word:
+      // the word is copied, the reader picks its half.
+      const int first = s * PER_STAGE & (is_zero ? ~(ZB - 1) : ~0);
+      const int left = max(n_groups - first, 0);
+      if (!is_zero)
+        cp_async_small<SB>(dst, side_src ? side_src + first * 2 : codes_any, side_src ? min(left * 2, SB) : 0);
+      else
+        cp_async_small<ZB>(dst, side_src ? side_src + first : codes_any, side_src ? min(left, ZB) : 0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < PER_STAGE; ++e) {
+        const int block = s * 2 + e / GROUPS;
+        const int gi = ScaleRow<BF16, GROUPS>::first_group(p, block) + e % GROUPS;
+        const bool live = side_src && block * 128 + (e % GROUPS) * (128 / GROUPS) < p.k;
+        if (!is_zero)
+          *reinterpret_cast<uint16_t*>(smem + (dst - ring) + e * 2) =
+              live ? __ldg(reinterpret_cast<const uint16_t*>(side_src) + gi) : 0;
+        else
+          smem[dst - ring + (ZB > PER_STAGE ? (s & 1) * PER_STAGE : 0) + e] = live ? __ldg(side_src + gi) : 8;
+      }
+    }
+  };
+  // Stage s_first + ahead into ring slot `slot`, from sources at stage s_first.
+  auto load_stage = [&](int s_first, int ahead, int slot) {
+    const int s = s_first + ahead;
     if (s < s_end) {
-      const uint32_t base = ring + uint32_t((s - s_begin) % STAGES) * stage_bytes(TOKENS);
-      const int kc = s * kStageK + cc * 32;
+      const bool code_live = s * kStageK + cc * 32 < p.k, x_live = s * kStageK + lane * 8 < p.k;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = (tid >> 3) + 32 * i;
-        const bool live = code_live[i] && kc < p.k;
-        cp_async16(base + r * 128 + ((cc ^ (r & 7)) << 4), live ? code_src[i] + s * (kStageK / 8) : codes, live);
-      }
+      for (int i = 0; i < 4; ++i)
+        cp_async16(code_dst + slot * STAGE + i * 32 * 128, code_src[i] + ahead * (kStageK / 8),
+                   code_live ? code_size[i] : 0);
 #pragma unroll
-      for (int i = 0; i < TOKENS * 32 / kW4SmallThreads; ++i) {
-        const int e = tid + i * kW4SmallThreads, t = e >> 5, ch = e & 31;
-        const int kx = s * kStageK + ch * 8;
-        const bool live = t < tile.count && kx < p.k;
-        cp_async16(base + kCodeBytes + t * kXPitch + ch * 16, live ? x + t * p.x_stride + kx : p.x, live);
-      }
+      for (int i = 0; i < XN; ++i)
+        cp_async16(x_dst + slot * STAGE + i * 8 * kXPitch, x_src[i] + ahead * kStageK, x_live ? x_size[i] : 0);
+      if (!is_zero || p.zeros) load_side(s, slot);
     }
     cp_commit();
-  };
-  // Packed scales of a stage: entry e of row r covers weights [e * 128 /
-  // GROUPS, ...) of the stage; loaded one stage ahead into registers.
-  auto load_scales = [&](int s, uint32_t* v) {
-#pragma unroll
-    for (int i = 0; i < ENTRIES; ++i) {
-      const int r = tid & (kRows - 1), e = (tid >> 7) + 2 * i;
-      const int k0 = s * kStageK + e * (128 / GROUPS);
-      const int64_t mr = matrix_row(r);
-      v[i] = pack_scale<BF16>(0, 8);
-      if (s < s_end && mr >= 0 && k0 < p.k) {
-        const int gi = k0 / p.group;
-        const uint32_t z = zeros ? zeros[mr * p.zeros_stride + gi] : 8u;
-        v[i] = pack_scale<BF16>(scales[mr * p.scales_stride + gi], z);
-      }
-    }
   };
 
   float acc[2][NT][4];
@@ -195,109 +253,133 @@ __global__ void __launch_bounds__(kW4SmallThreads, 2) aspire_w4_small_kernel(con
 
   const int wg = warp >> 2;             // half of the stage
   const int row_w = (warp & 3) * 32;    // the warp's 32 tile rows
-  uint32_t next_sc[ENTRIES];
-  load_scales(s_begin, next_sc);
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) load_stage(s_begin + s);
+  for (int s = 0; s < STAGES - 1; ++s) load_stage(s_begin, s, s);
 
-  for (int s = s_begin; s < s_end; ++s) {
-    uint32_t* sb = sc + ((s - s_begin) & 1) * (2 * GROUPS * kRows);
+  const uint8_t* const scale_src = smem + scale_at(TOKENS) + (row_w + g) * SB + wg * GROUPS * 2;
+  const uint8_t* const zero_src = smem + zero_at(TOKENS, GROUPS) + (row_w + g) * ZB + wg * GROUPS;
+  const bool has_zeros = p.zeros != nullptr;
+  // The lane's codes of each group's part (16, 8 or 4 bytes of the row), and
+  // its piece of the tokens.
+  const uint8_t* code_at[GROUPS];
 #pragma unroll
-    for (int i = 0; i < ENTRIES; ++i) sb[((tid >> 7) + 2 * i) * kRows + (tid & (kRows - 1))] = next_sc[i];
-    cp_wait<STAGES - 2>();
-    __syncthreads();
-    load_stage(s + STAGES - 1);
-    load_scales(s + 1, next_sc);
-    const uint8_t* st = smem + ((s - s_begin) % STAGES) * stage_bytes(TOKENS);
-    const uint8_t* xs = st + kCodeBytes + g * kXPitch + wg * 256 + c * 16;
+  for (int gr = 0; gr < GROUPS; ++gr) {
+    const int byte = wg * 64 + gr * 16 * WORDS + c * 4 * WORDS;
+    code_at[gr] = smem + (row_w + g) * 128 + (((byte >> 4) ^ slot_mask(g)) << 4) + (byte & 15);
+  }
+  const uint8_t* const x_at = smem + kCodeBytes + g * kXPitch + wg * 256 + c * 16;
+
+  for (int s0 = s_begin; s0 < s_end; s0 += STAGES) {
 #pragma unroll
-    for (int gr = 0; gr < GROUPS; ++gr) {
-      uint32_t ps[2][2];
+    for (int u = 0; u < STAGES; ++u) {
+      const int s = s0 + u;
+      if (s >= s_end) break;
+      cp_wait<STAGES - 2>();
+      __syncthreads();
+      load_stage(s0, u + STAGES - 1, (u + STAGES - 1) % STAGES);
+      const uint8_t* const zero_s = zero_src + u * STAGE + (ZB > PER_STAGE ? (s & 1) * PER_STAGE : 0);
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+      for (int gr = 0; gr < GROUPS; ++gr) {
+        uint32_t w[2][2][4];  // row g and g + 8 of both 16-row tiles
 #pragma unroll
-        for (int h = 0; h < 2; ++h) ps[m][h] = sb[(wg * GROUPS + gr) * kRows + row_w + m * 16 + h * 8 + g];
-      float blk[2][NT][4];
+        for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) blk[m][t][i] = 0.f;
-#pragma unroll
-      for (int q = 0; q < CHUNKS_PER_GROUP; ++q) {
-        const int ch = gr * CHUNKS_PER_GROUP + q;  // 32-weight chunk of the half stage
-        uint4 xf[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) xf[t] = *reinterpret_cast<const uint4*>(xs + t * 8 * kXPitch + ch * 64);
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const int r = row_w + m * 16 + g;  // r & 7 == g for this row and the one 8 below
-          const uint8_t* wr = st + r * 128 + (((wg * 4 + ch) ^ g) << 4) + c * 4;
-          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(wr);
-          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(wr + 8 * 128);
-          const uint32_t z0 = zero_pair(ps[m][0]), z1 = zero_pair(ps[m][1]);
-          uint32_t a[2][4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            a[i >> 1][(i & 1) * 2] = Num<BF16>::sub2(magic_pair<BF16>(w0, i), z0);
-            a[i >> 1][(i & 1) * 2 + 1] = Num<BF16>::sub2(magic_pair<BF16>(w1, i), z1);
+          for (int h = 0; h < 2; ++h) {
+            const uint8_t* at = code_at[gr] + u * STAGE + (m * 16 + h * 8) * 128;
+            if constexpr (WORDS == 4) *reinterpret_cast<uint4*>(w[m][h]) = *reinterpret_cast<const uint4*>(at);
+            if constexpr (WORDS == 2) *reinterpret_cast<uint2*>(w[m][h]) = *reinterpret_cast<const uint2*>(at);
+            if constexpr (WORDS == 1) w[m][h][0] = *reinterpret_cast<const uint32_t*>(at);
           }
+        // Scales in fp32, and magic + zero point as a pair (bit 0 of the
+        // mantissa is worth 1 at both magic numbers).
+        float ks[2][2];
+        uint32_t zp[2][2];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            mma16816<BF16>(blk[m][t], a[0], xf[t].x, xf[t].y);
-            mma16816<BF16>(blk[m][t], a[1], xf[t].z, xf[t].w);
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = m * 16 + h * 8;
+            ks[m][h] = Num<BF16>::to_float(
+                *reinterpret_cast<const uint16_t*>(scale_src + u * STAGE + r * SB + gr * 2));
+            zp[m][h] = Num<BF16>::kMagic + 0x00080008u;
+            if (has_zeros) zp[m][h] = Num<BF16>::kMagic + 0x00010001u * (zero_s[r * ZB + gr] & 15u);
+          }
+        float blk[2][NT][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) blk[m][t][i] = 0.f;
+#pragma unroll
+        for (int q = 0; q < WORDS; ++q) {
+          uint4 xf[NT];
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+            xf[t] = *reinterpret_cast<const uint4*>(x_at + u * STAGE + t * 8 * kXPitch + (gr * WORDS + q) * 64);
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const uint32_t z0 = zp[m][0], z1 = zp[m][1];
+            uint32_t a[2][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              a[i >> 1][(i & 1) * 2] = Num<BF16>::sub2(magic_pair<BF16>(w[m][0][q], i), z0);
+              a[i >> 1][(i & 1) * 2 + 1] = Num<BF16>::sub2(magic_pair<BF16>(w[m][1][q], i), z1);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              mma16816<BF16>(blk[m][t], a[0], xf[t].x, xf[t].y);
+              mma16816<BF16>(blk[m][t], a[1], xf[t].z, xf[t].w);
+            }
           }
         }
-      }
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        const float s0 = scale_of<BF16>(ps[m][0]), s1 = scale_of<BF16>(ps[m][1]);
+        for (int m = 0; m < 2; ++m) {
+          const float k0 = ks[m][0], k1 = ks[m][1];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          acc[m][t][0] = fmaf(blk[m][t][0], s0, acc[m][t][0]);
-          acc[m][t][1] = fmaf(blk[m][t][1], s0, acc[m][t][1]);
-          acc[m][t][2] = fmaf(blk[m][t][2], s1, acc[m][t][2]);
-          acc[m][t][3] = fmaf(blk[m][t][3], s1, acc[m][t][3]);
+          for (int t = 0; t < NT; ++t) {
+            acc[m][t][0] = fmaf(blk[m][t][0], k0, acc[m][t][0]);
+            acc[m][t][1] = fmaf(blk[m][t][1], k0, acc[m][t][1]);
+            acc[m][t][2] = fmaf(blk[m][t][2], k1, acc[m][t][2]);
+            acc[m][t][3] = fmaf(blk[m][t][3], k1, acc[m][t][3]);
+          }
         }
       }
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) code_src[i] += STAGES * (kStageK / 8);
+#pragma unroll
+    for (int i = 0; i < XN; ++i) x_src[i] += STAGES * kStageK;
   }
 
-  // The warpgroups' and ranks' partials meet in shared memory.
+  // The second warpgroup's partials join the first's, then the ranks' meet.
   cp_wait<0>();
   __syncthreads();
+  auto red_at = [&](int m, int t, int i) {
+    return (t * 8 + 2 * c + (i & 1)) * kRedPitch + row_w + m * 16 + (i >> 1) * 8 + g;
+  };
+  if (wg == 1) {
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        red[(wg * TOKENS + t * 8 + 2 * c + (i & 1)) * kRedPitch + row_w + m * 16 + (i >> 1) * 8 + g] = acc[m][t][i];
+        for (int i = 0; i < 4; ++i) red[red_at(m, t, i)] = acc[m][t][i];
+  }
+  __syncthreads();
+  if (wg == 0) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) red[red_at(m, t, i)] += acc[m][t][i];
+  }
   if (ranks > 1)
     cg::this_cluster().sync();
   else
     __syncthreads();
-  // Rank r finishes features [r, r + 1) x FEATURES / ranks.
-  const int share = FEATURES / ranks;
-  for (int i = tid; i < tile.count * share; i += kW4SmallThreads) {
-    const int t = i / share, fl = rank * share + i % share, f = f0 + fl;
-    if (f >= p.n) continue;
-    float a = 0.f, b = 0.f;
-    for (int q = 0; q < ranks; ++q) {
-      const float* rq = ranks > 1 ? cg::this_cluster().map_shared_rank(red, q) : red;
-      a += rq[t * kRedPitch + fl];
-      a += rq[(TOKENS + t) * kRedPitch + fl];
-      if (SWIGLU) {
-        b += rq[t * kRedPitch + FEATURES + fl];
-        b += rq[(TOKENS + t) * kRedPitch + FEATURES + fl];
-      }
-    }
-    const int64_t row = tile.row0 + t;
-    if (SWIGLU) a = silu(a) * b;
-    if (p.residual) a += Num<BF16>::to_float(p.residual[row * p.residual_stride + f]);
-    p.out[row * p.out_stride + f] = Num<BF16>::from_float(a);
-  }
+  finish_tile<BF16, SWIGLU>(p, tile, f0, rank, ranks, red, kRedPitch, tid, kW4SmallThreads);
   if (ranks > 1) cg::this_cluster().sync();  // peers read this CTA's partials until here
 }
 
@@ -316,7 +398,7 @@ W4Kernel by_tokens(int tokens, int groups) {
 
 }  // namespace
 
-size_t w4_small_smem(int tokens, int groups) { return size_t(ring_bytes(tokens, groups)) + scale_bytes(groups); }
+size_t w4_small_smem(int tokens, int groups) { return size_t(ring_bytes(tokens, groups)); }
 
 W4Kernel w4_small_kernel(bool bf16, int tokens, int groups, bool swiglu) {
   if (bf16) return swiglu ? by_tokens<true, true>(tokens, groups) : by_tokens<true, false>(tokens, groups);

@@ -13,8 +13,9 @@
 //
 // Roles: warps 0-3 and 4-7 unpack (one warpgroup takes steps 0 and 1 of a
 // 256-weight stage, the other steps 2 and 3; the sum's order is free, so the
-// MMA takes them alternately) and run the epilogue, warp 8 issues the TMA
-// loads, warp 9 the MMAs.  Every wait is bounded; after a timeout the CTA
+// MMA takes them alternately) and run the epilogue, warp 8 loads the tokens,
+// warp 10 the codes (each as far ahead as its own ring allows), warp 9 issues
+// the MMAs.  Every wait is bounded; after a timeout the CTA
 // reports it, lets its copies and MMAs land, frees TMEM and returns.
 //
 // Few tiles: a cluster splits K and adds the partials in distributed shared
@@ -40,7 +41,7 @@ constexpr int kSteps = kStageK / kStepK;
 constexpr uint32_t kCodeBytes = kRows * kStageK / 2;
 constexpr int kRedPitch = kRows + 4;             // floats
 constexpr int kUnpackThreads = 256;
-constexpr int kTmaWarp = 8, kMmaWarp = 9;
+constexpr int kXWarp = 8, kMmaWarp = 9, kCodeWarp = 10;
 
 template <int TOKENS>
 struct Shape {
@@ -134,47 +135,38 @@ __global__ void __launch_bounds__(kW4TcThreads, TOKENS == 256 ? 1 : 2)
   // Step i of the MMA's order: stage i / 4, K sub-block (0, 2, 1, 3)[i % 4].
   auto sub_of = [](int i) { return ((i & 1) << 1) | ((i >> 1) & 1); };
 
-  if (warp == kTmaWarp) {
+  if (warp == kCodeWarp) {
     if (lane == 0) {
       ptx::prefetch_tmap(&codes_map);
-      ptx::prefetch_tmap(&x_map);
-      bool ok = true;
-      int issued_w = 0, issued_x = 0;
-      for (int s = 0; s < stages && ok; ++s) {
+      int s = 0;
+      for (; s < stages; ++s) {
         const int ws = s % SW;
-        if (!wait_bar(sm, sm.w_empty[ws], ((s / SW) & 1) ^ 1, p.status)) {
-          ok = false;
-          break;
-        }
+        if (!wait_bar(sm, sm.w_empty[ws], ((s / SW) & 1) ^ 1, p.status)) break;
         const uint32_t bar = ptx::smem_addr(&sm.w_full[ws]);
         const uint32_t dst = ptx::smem_addr(codes_s + ws * kCodeBytes);
         const int c0 = (s_begin + s) * (kStageK / 8);
         ptx::mbar_arrive_expect_tx(bar, kCodeBytes);
-        if (SWIGLU) {
-          ptx::tma_load_3d(dst, &codes_map, bar, c0, f0, tile.expert);
-          ptx::tma_load_3d(dst + kCodeBytes / 2, &codes_map, bar, c0, p.n + f0, tile.expert);
-        } else {
-          ptx::tma_load_3d(dst, &codes_map, bar, c0, f0, tile.expert);
-        }
-        issued_w = s + 1;
-        for (int q = 0; q < kSteps; ++q) {
-          const int i = s * kSteps + q, xs = i % SX;
-          if (!wait_bar(sm, sm.x_empty[xs], ((i / SX) & 1) ^ 1, p.status)) {
-            ok = false;
-            break;
-          }
-          const uint32_t xbar = ptx::smem_addr(&sm.x_full[xs]);
-          ptx::mbar_arrive_expect_tx(xbar, S::kXBytes);
-          ptx::tma_load_2d(ptx::smem_addr(x_s + xs * S::kXBytes), &x_map, xbar,
-                           (s_begin + s) * kStageK + sub_of(q) * kStepK, tile.row0);
-          issued_x = i + 1;
-        }
+        ptx::tma_load_3d(dst, &codes_map, bar, c0, f0, tile.expert);
+        if (SWIGLU) ptx::tma_load_3d(dst + kCodeBytes / 2, &codes_map, bar, c0, p.n + f0, tile.expert);
       }
-      if (!ok || pipe::aborted(sm)) {
-        // The copies in flight land before the CTA ends.
-        for (int s = max(0, issued_w - SW); s < issued_w; ++s) drain_bar(sm.w_full[s % SW], (s / SW) & 1);
-        for (int i = max(0, issued_x - SX); i < issued_x; ++i) drain_bar(sm.x_full[i % SX], (i / SX) & 1);
+      // After a timeout anywhere the copies in flight land before the CTA ends.
+      if (s < stages || pipe::aborted(sm))
+        for (int i = max(0, s - SW); i < s; ++i) drain_bar(sm.w_full[i % SW], (i / SW) & 1);
+    }
+  } else if (warp == kXWarp) {
+    if (lane == 0) {
+      ptx::prefetch_tmap(&x_map);
+      int i = 0;
+      for (; i < steps; ++i) {
+        const int xs = i % SX;
+        if (!wait_bar(sm, sm.x_empty[xs], ((i / SX) & 1) ^ 1, p.status)) break;
+        const uint32_t bar = ptx::smem_addr(&sm.x_full[xs]);
+        ptx::mbar_arrive_expect_tx(bar, S::kXBytes);
+        ptx::tma_load_2d(ptx::smem_addr(x_s + xs * S::kXBytes), &x_map, bar,
+                         (s_begin + i / kSteps) * kStageK + sub_of(i % kSteps) * kStepK, tile.row0);
       }
+      if (i < steps || pipe::aborted(sm))
+        for (int j = max(0, i - SX); j < i; ++j) drain_bar(sm.x_full[j % SX], (j / SX) & 1);
     }
   } else if (warp == kMmaWarp) {
     constexpr uint32_t idesc =
@@ -201,7 +193,7 @@ __global__ void __launch_bounds__(kW4TcThreads, TOKENS == 256 ? 1 : 2)
     if (lane == 0) ptx::mma_commit(ptx::smem_addr(&sm.d_full));
     __syncwarp();
     drain_bar(sm.d_full, 0);
-  } else {
+  } else if (warp < 8) {
     // -------------------------------------------------------------- unpack
     const int wg = warp >> 2;              // half of a stage
     const int r = tid & (kRows - 1);       // tile row
@@ -209,30 +201,15 @@ __global__ void __launch_bounds__(kW4TcThreads, TOKENS == 256 ? 1 : 2)
     const bool live = mr < p.n;
     if (SWIGLU && r >= FEATURES) mr += p.n;
     if (!live) mr = 0;
-    const uint16_t* sc = p.scales + int64_t(tile.expert) * p.scales_stride_e + mr * p.scales_stride;
-    const uint8_t* zr =
-        p.zeros ? p.zeros + int64_t(tile.expert) * p.zeros_stride_e + mr * p.zeros_stride : nullptr;
-    // Packed scales of this warpgroup's half of stage s, loaded a stage ahead.
-    auto load_scales = [&](int s, uint32_t* v) {
-      const int k0 = (s_begin + s) * kStageK + wg * 128;
-#pragma unroll
-      for (int e = 0; e < GROUPS; ++e) {
-        const int k = k0 + e * (128 / GROUPS);
-        v[e] = pack_scale<BF16>(0, 8);
-        if (s < stages && live && k < p.k) {
-          const int gi = k / p.group;
-          v[e] = pack_scale<BF16>(sc[gi], zr ? zr[gi] : 8u);
-        }
-      }
-    };
+    const ScaleRow<BF16, GROUPS> scales(p, tile.expert, mr, live);
     const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
     uint32_t cur[GROUPS], nxt[GROUPS];
-    load_scales(0, nxt);
+    scales.load(p, s_begin * 2 + wg, nxt);
     bool ok = true;
     for (int s = 0; s < stages && ok; ++s) {
 #pragma unroll
       for (int e = 0; e < GROUPS; ++e) cur[e] = nxt[e];
-      load_scales(s + 1, nxt);
+      if (s + 1 < stages) scales.load(p, (s_begin + s + 1) * 2 + wg, nxt);
       const int ws = s % SW;
       if (!wait_bar(sm, sm.w_full[ws], (s / SW) & 1, p.status)) ok = false;
       if (!__all_sync(0xffffffffu, ok)) break;
@@ -293,21 +270,7 @@ __global__ void __launch_bounds__(kW4TcThreads, TOKENS == 256 ? 1 : 2)
     ptx::tmem_dealloc(tmem, S::kTmemCols);
   }
   if (good) {
-    const int share = FEATURES / ranks;
-    for (int i = tid; i < tile.count * share; i += kW4TcThreads) {
-      const int t = i / share, fl = rank * share + i % share, f = f0 + fl;
-      if (f >= p.n) continue;
-      float a = 0.f, b = 0.f;
-      for (int q = 0; q < ranks; ++q) {
-        const float* rq = ranks > 1 ? cg::this_cluster().map_shared_rank(red, q) : red;
-        a += rq[t * kRedPitch + fl];
-        if (SWIGLU) b += rq[t * kRedPitch + FEATURES + fl];
-      }
-      const int64_t row = tile.row0 + t;
-      if (SWIGLU) a = silu(a) * b;
-      if (p.residual) a += Num<BF16>::to_float(p.residual[row * p.residual_stride + f]);
-      p.out[row * p.out_stride + f] = Num<BF16>::from_float(a);
-    }
+    finish_tile<BF16, SWIGLU>(p, tile, f0, rank, ranks, red, kRedPitch, tid, kW4TcThreads);
   }
   if (ranks > 1) cg::this_cluster().sync();  // peers read this CTA's partials until here
 }
