@@ -37,11 +37,11 @@ int ceil32(int v) { return (v + 31) / 32 * 32; }
 
 // Rows (an expert's average share of them) up to which the kernel for few
 // tokens runs.
-constexpr int64_t kW4SmallRows = 32;
+constexpr int64_t kW4SmallRows = 16;
 
-// Opt-in caches of the small kernel's variants: [type][tokens 8, 16, 32]
+// Opt-in caches of the small kernel's variants: [type][tokens 8, 16]
 // [groups 1, 2, 4][swiglu].
-SmemOptIn g_w4_small[2][3][3][2];
+SmemOptIn g_w4_small[2][2][3][2];
 
 int index_of(int v) { return v <= 1 ? 0 : (v == 2 ? 1 : 2); }
 
@@ -82,7 +82,7 @@ int w4_small(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
   const bool grouped = a->offsets != nullptr;
   // Tokens per tile: the fewest columns that hold the rows.
   const int64_t typical = typical_rows(a);
-  const int tokens = typical <= 8 ? 8 : (typical <= 16 ? 16 : 32);
+  const int tokens = typical <= 8 ? 8 : 16;
   const int groups = a->group == 32 ? 4 : (a->group == 64 ? 2 : 1);
   const int features = a->swiglu ? w4::kRows / 2 : w4::kRows;
   const int64_t ny = (int64_t(a->n) + features - 1) / features;
@@ -99,8 +99,7 @@ int w4_small(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
   W4Kernel kernel = w4_small_kernel(a->type == ASPIRE_T_BF16, tokens, groups, a->swiglu != 0);
   const size_t smem = w4_small_smem(tokens, groups);
   rc = ensure_smem(reinterpret_cast<const void*>(kernel), smem,
-                   g_w4_small[a->type == ASPIRE_T_BF16][tokens == 8 ? 0 : (tokens == 16 ? 1 : 2)][index_of(groups)]
-                             [a->swiglu != 0]);
+                   g_w4_small[a->type == ASPIRE_T_BF16][tokens != 8][index_of(groups)][a->swiglu != 0]);
   if (rc) return rc;
   return w4_launch(kernel, dim3(unsigned(cluster), unsigned(ny), unsigned(nz)), cluster, kW4SmallThreads, smem, stream,
                    "aspire_w4_small_kernel launch", p);

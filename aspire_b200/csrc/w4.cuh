@@ -120,65 +120,87 @@ __device__ __forceinline__ Tile find_tile(const W4Params& p, int index, int widt
 }
 
 // ------------------------------------------------------------------ numbers
-// The two activation types.  A code q < 16 OR-ed into the low mantissa bits of
-// 128 (bf16, 7 bits) or 1024 (fp16, 10 bits) is that number plus q, exactly;
-// subtracting it plus the zero point gives q - z, exactly.
+// The two activation types and how a word of codes becomes numbers: unpack()
+// gives (q - z) / kUnit of its eight weights as four pairs of neighbours, each
+// exactly.  c0 and c1 hold the zero point as that takes it (zero_consts).
+// Pairs whose nibbles sit in the low four bits are OR-ed into the mantissa of
+// 128 (bf16, 7 bits) or 1024 (fp16, 10 bits): the number plus q.  The nibbles
+// above them would need a shift each, but are numbers as they stand: in fp16
+// OR-ed into 1024 they are 1024 + 16 q, and in bf16 the bare bits are q 2^-129
+// (below 8 a subnormal, above it the first binade, which continues it), which
+// one fused operation scales by 2^127.  So a word takes one shift.
 template <bool BF16>
 struct Num;
+
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t or_) {
+  // One three-input operation, written out: the compiler keeps it as two when
+  // both constants are immediates.
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(mask), "r"(or_));
+  return r;
+}
+
 template <>
 struct Num<true> {
-  static constexpr uint32_t kMagic = 0x43004300u;
+  static constexpr float kUnit = 4.0f;
   __device__ static __forceinline__ float to_float(uint16_t v) { return __uint_as_float(uint32_t(v) << 16); }
   __device__ static __forceinline__ uint16_t from_float(float v) {
     return __bfloat16_as_ushort(__float2bfloat16_rn(v));
   }
-  __device__ static __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
+  __device__ static __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
   }
   __device__ static __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
     const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
   }
+  // c0 = -(128 + z) / 4 and c1 = -z / 4, as pairs.
+  __device__ static __forceinline__ void zero_consts(uint32_t z, uint32_t& c0, uint32_t& c1) {
+    c0 = 0xC200C200u + z * 0x00010001u;
+    c1 = fma2(c0, 0x3F803F80u, 0x42004200u);  // + 32
+  }
+  __device__ static __forceinline__ void unpack(uint32_t word, uint32_t c0, uint32_t c1, uint32_t* v) {
+    const uint32_t high = word >> 8;
+    v[0] = fma2(and_or(word, 0x000F000Fu, 0x43004300u), 0x3E803E80u, c0);
+    v[1] = fma2(word & 0x00F000F0u, 0x7F007F00u, c1);
+    v[2] = fma2(and_or(high, 0x000F000Fu, 0x43004300u), 0x3E803E80u, c0);
+    v[3] = fma2(high & 0x00F000F0u, 0x7F007F00u, c1);
+  }
 };
 template <>
 struct Num<false> {
-  static constexpr uint32_t kMagic = 0x64006400u;
+  static constexpr float kUnit = 1.0f;
   __device__ static __forceinline__ float to_float(uint16_t v) { return __half2float(__ushort_as_half(v)); }
   __device__ static __forceinline__ uint16_t from_float(float v) { return __half_as_ushort(__float2half_rn(v)); }
-  __device__ static __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
-    const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
+  __device__ static __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
   }
   __device__ static __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
   }
+  // c0 = -(1024 + z) and c1 = -(64 + z), as pairs.
+  __device__ static __forceinline__ void zero_consts(uint32_t z, uint32_t& c0, uint32_t& c1) {
+    c0 = 0xE400E400u + z * 0x00010001u;
+    c1 = fma2(c0, 0x3C003C00u, 0x63806380u);  // + 960
+  }
+  __device__ static __forceinline__ void unpack(uint32_t word, uint32_t c0, uint32_t c1, uint32_t* v) {
+    const uint32_t high = word >> 8;
+    v[0] = fma2(and_or(word, 0x000F000Fu, 0x64006400u), 0x3C003C00u, c0);
+    v[1] = fma2(and_or(word, 0x00F000F0u, 0x64006400u), 0x2C002C00u, c1);
+    v[2] = fma2(and_or(high, 0x000F000Fu, 0x64006400u), 0x3C003C00u, c0);
+    v[3] = fma2(and_or(high, 0x00F000F0u, 0x64006400u), 0x2C002C00u, c1);
+  }
 };
 
-// Pair i of a word: (weight 2i, weight 2i + 1) + magic.
-template <bool BF16>
-__device__ __forceinline__ uint32_t magic_pair(uint32_t word, int i) {
-  // One three-input operation, (a & b) | c: written out, since the compiler
-  // keeps it as two when both constants are immediates.
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(word >> (4 * i)), "r"(0x000F000Fu), "r"(Num<BF16>::kMagic));
-  return r;
-}
-
-// A group's scale (bits 16-31) and magic + zero point (bits 0-15) in one word.
-template <bool BF16>
+// A group's scale (bits 16-31) and zero point (4 bits: larger ones are cut).
 __device__ __forceinline__ uint32_t pack_scale(uint16_t scale, uint32_t zero) {
-  // Bit 0 of the mantissa is worth 1 at both magic numbers, so adding the
-  // zero point to the bits adds it to the number (zero points past 15 would
-  // leave the mantissa: they are cut to 4 bits).
-  return (uint32_t(scale) << 16) | ((Num<BF16>::kMagic & 0xFFFFu) + (zero & 15u));
+  return (uint32_t(scale) << 16) | (zero & 15u);
 }
-template <bool BF16>
-__device__ __forceinline__ float scale_of(uint32_t packed) {
-  return Num<BF16>::to_float(uint16_t(packed >> 16));
-}
-__device__ __forceinline__ uint32_t zero_pair(uint32_t packed) { return __byte_perm(packed, 0, 0x1010); }
 __device__ __forceinline__ uint32_t scale_pair(uint32_t packed) { return __byte_perm(packed, 0, 0x3232); }
 
 // One matrix row's packed scales, GROUPS (1, 2, 4) for every block of 128
@@ -201,7 +223,7 @@ struct ScaleRow {
   // Blocks past the row's end give scale 0.
   __device__ __forceinline__ void load(const W4Params& p, int block, uint32_t* v) const {
 #pragma unroll
-    for (int e = 0; e < GROUPS; ++e) v[e] = pack_scale<BF16>(0, 8);
+    for (int e = 0; e < GROUPS; ++e) v[e] = pack_scale(0, 8);
     if (!live || block * 128 >= p.k) return;
     const int gi = first_group(p, block);
     alignas(8) uint16_t s[GROUPS];
@@ -228,7 +250,7 @@ struct ScaleRow {
       }
     }
 #pragma unroll
-    for (int e = 0; e < GROUPS; ++e) v[e] = pack_scale<BF16>(s[e], z[e]);
+    for (int e = 0; e < GROUPS; ++e) v[e] = pack_scale(s[e], z[e]);
   }
 };
 
@@ -279,10 +301,10 @@ __device__ __forceinline__ void finish_tile(const W4Params& p, const Tile& tile,
 }  // namespace w4
 
 constexpr int kW4SmallThreads = 256;
-// The small kernel's dynamic shared memory, by tokens per tile (8, 16, 32)
+// The small kernel's dynamic shared memory, by tokens per tile (8, 16)
 // and groups per 128 weights of a row (1, 2, 4).
 size_t w4_small_smem(int tokens, int groups);
-// The kernel for an activation type, tokens per tile (8, 16, 32), groups per
+// The kernel for an activation type, tokens per tile (8, 16), groups per
 // 128 weights (1, 2, 4) and output form.
 using W4Kernel = void (*)(W4Params);
 W4Kernel w4_small_kernel(bool bf16, int tokens, int groups, bool swiglu);

@@ -1,16 +1,16 @@
 // 4-bit products of few tokens (a drafting or verifying row, a decode batch).
 //
 // The weights' bytes bound it: 0.5 byte feeds 2 x tokens operations.  A CTA
-// owns 128 matrix rows (64 gate and 64 up rows with the activation), 8, 16 or
-// 32 tokens and a range of K, and streams the rows' codes through a ring of
+// owns 128 matrix rows (64 gate and 64 up rows with the activation), 8 or 16
+// tokens and a range of K, and streams the rows' codes through a ring of
 // 256-weight stages in shared memory (asynchronous 16-byte copies, 128
 // contiguous bytes of a row at a time).  The loop is unrolled over the ring,
-// so that its addresses are constants: unpacking a weight takes about 1.5
+// so that its addresses are constants: unpacking a weight takes about 1.2
 // instructions, and every one around it counts.
 //
 // The products run on warp-level matrix instructions with the weights as A
 // (16 rows x 16 k) unpacked in registers and the tokens as B (8 columns): at
-// 8 to 32 tokens the unpacking, not the tensor rate, is what could slow the
+// 16 tokens and fewer the unpacking, not the tensor rate, is what could slow the
 // stream, and unpacked fragments go straight from registers into the
 // instruction.  The sum over k may run in any order, so the instruction's k
 // slots are assigned to the codes as they lie: of each group's part of a stage
@@ -101,7 +101,7 @@ __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// TOKENS: tokens of a tile.  GROUPS: scale groups per 128 weights of a row (a
+// TOKENS: tokens of a tile (8, 16).  GROUPS: scale groups per 128 weights of a row (a
 // group of more than 128 counts as one).  Grid: (cluster ranks, row tiles,
 // token tiles).
 template <bool BF16, int TOKENS, int GROUPS, bool SWIGLU>
@@ -290,10 +290,8 @@ __global__ void __launch_bounds__(kW4SmallThreads, 2) aspire_w4_small_kernel(con
             if constexpr (WORDS == 2) *reinterpret_cast<uint2*>(w[m][h]) = *reinterpret_cast<const uint2*>(at);
             if constexpr (WORDS == 1) w[m][h][0] = *reinterpret_cast<const uint32_t*>(at);
           }
-        // Scales in fp32, and magic + zero point as a pair (bit 0 of the
-        // mantissa is worth 1 at both magic numbers).
         float ks[2][2];
-        uint32_t zp[2][2];
+        uint32_t z0[2][2], z1[2][2];
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -301,8 +299,9 @@ __global__ void __launch_bounds__(kW4SmallThreads, 2) aspire_w4_small_kernel(con
             const int r = m * 16 + h * 8;
             ks[m][h] = Num<BF16>::to_float(
                 *reinterpret_cast<const uint16_t*>(scale_src + u * STAGE + r * SB + gr * 2));
-            zp[m][h] = Num<BF16>::kMagic + 0x00080008u;
-            if (has_zeros) zp[m][h] = Num<BF16>::kMagic + 0x00010001u * (zero_s[r * ZB + gr] & 15u);
+            uint32_t z = 8;
+            if (has_zeros) z = zero_s[r * ZB + gr] & 15u;
+            Num<BF16>::zero_consts(z, z0[m][h], z1[m][h]);
           }
         float blk[2][NT][4];
 #pragma unroll
@@ -319,13 +318,10 @@ __global__ void __launch_bounds__(kW4SmallThreads, 2) aspire_w4_small_kernel(con
             xf[t] = *reinterpret_cast<const uint4*>(x_at + u * STAGE + t * 8 * kXPitch + (gr * WORDS + q) * 64);
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
-            const uint32_t z0 = zp[m][0], z1 = zp[m][1];
-            uint32_t a[2][4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              a[i >> 1][(i & 1) * 2] = Num<BF16>::sub2(magic_pair<BF16>(w[m][0][q], i), z0);
-              a[i >> 1][(i & 1) * 2 + 1] = Num<BF16>::sub2(magic_pair<BF16>(w[m][1][q], i), z1);
-            }
+            uint32_t lo[4], hi[4];  // rows g and g + 8
+            Num<BF16>::unpack(w[m][0][q], z0[m][0], z1[m][0], lo);
+            Num<BF16>::unpack(w[m][1][q], z0[m][1], z1[m][1], hi);
+            const uint32_t a[2][4] = {{lo[0], hi[0], lo[1], hi[1]}, {lo[2], hi[2], lo[3], hi[3]}};
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               mma16816<BF16>(blk[m][t], a[0], xf[t].x, xf[t].y);
@@ -364,7 +360,7 @@ __global__ void __launch_bounds__(kW4SmallThreads, 2) aspire_w4_small_kernel(con
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[red_at(m, t, i)] = acc[m][t][i];
+        for (int i = 0; i < 4; ++i) red[red_at(m, t, i)] = acc[m][t][i] * Num<BF16>::kUnit;
   }
   __syncthreads();
   if (wg == 0) {
@@ -373,7 +369,7 @@ __global__ void __launch_bounds__(kW4SmallThreads, 2) aspire_w4_small_kernel(con
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[red_at(m, t, i)] += acc[m][t][i];
+        for (int i = 0; i < 4; ++i) red[red_at(m, t, i)] += acc[m][t][i] * Num<BF16>::kUnit;
   }
   if (ranks > 1)
     cg::this_cluster().sync();
@@ -391,9 +387,7 @@ W4Kernel by_groups(int groups) {
 }
 template <bool BF16, bool SWIGLU>
 W4Kernel by_tokens(int tokens, int groups) {
-  if (tokens == 8) return by_groups<BF16, 8, SWIGLU>(groups);
-  if (tokens == 16) return by_groups<BF16, 16, SWIGLU>(groups);
-  return by_groups<BF16, 32, SWIGLU>(groups);
+  return tokens == 8 ? by_groups<BF16, 8, SWIGLU>(groups) : by_groups<BF16, 16, SWIGLU>(groups);
 }
 
 }  // namespace

@@ -224,10 +224,12 @@ __global__ void __launch_bounds__(kW4TcThreads, TOKENS == 256 ? 1 : 2)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const uint32_t ps = cur[(h * 64 + j * 8) * GROUPS / 128];
-          const uint32_t z = zero_pair(ps), m = scale_pair(ps);
+          const uint32_t m = scale_pair(ps);
+          uint32_t z0, z1;
+          Num<BF16>::zero_consts(ps & 15u, z0, z1);
+          Num<BF16>::unpack(w[j], z0, z1, a + j * 4);
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            a[j * 4 + q] = Num<BF16>::mul2(Num<BF16>::sub2(magic_pair<BF16>(w[j], q), z), m);
+          for (int q = 0; q < 4; ++q) a[j * 4 + q] = Num<BF16>::mul2(a[j * 4 + q], m);
         }
         if (!wait_bar(sm, sm.a_empty[as], ((i / SA) & 1) ^ 1, p.status)) ok = false;
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -257,7 +259,7 @@ __global__ void __launch_bounds__(kW4TcThreads, TOKENS == 256 ? 1 : 2)
       ptx::tmem_ld32(lanes + uint32_t(c), v);
       ptx::tmem_wait_ld();
 #pragma unroll
-      for (int j = 0; j < 32; ++j) red[(c + j) * kRedPitch + r] = v[j];
+      for (int j = 0; j < 32; ++j) red[(c + j) * kRedPitch + r] = v[j] * Num<BF16>::kUnit;
     }
   }
   ptx::tc_fence_before();

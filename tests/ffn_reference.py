@@ -4,7 +4,7 @@ error bounds those follow from.
 Bounds: a product's output is rounded once (half a unit in the last place, u =
 2^-8 bf16 or 2^-11 fp16 relative); its sum runs in fp32, where each of the k
 additions and roundings loses at most 2^-22 of the sum of magnitudes (the
-matrix instructions may truncate); with more than 32 rows the weights are
+matrix instructions may truncate); with more than 16 rows the weights are
 rounded to the activations' type first (u of each weight's magnitude).
 """
 
@@ -43,7 +43,7 @@ def product(x, w, residual=None, swiglu=False, rows=None):
     y = xd @ w.t()
     mag = xd.abs() @ w.abs().t()
     k = w.shape[1]
-    err = mag * (k * 2.0 ** -22 + (u if (rows if rows is not None else x.shape[0]) > 32 else 0.0))
+    err = mag * (k * 2.0 ** -22 + (u if (rows if rows is not None else x.shape[0]) > 16 else 0.0))
     if swiglu:
         n = w.shape[0] // 2
         a, b, ea, eb = y[:, :n], y[:, n:], err[:, :n], err[:, n:]
