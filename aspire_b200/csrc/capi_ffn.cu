@@ -124,26 +124,27 @@ SmemOptIn g_w4_tc[2][3][3][2];
 int w4_tc(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
   const bool grouped = a->offsets != nullptr;
   const int64_t typical = typical_rows(a);
-  const int tokens = typical <= 64 ? 64 : (typical <= 128 ? 128 : 256);
+  const int tokens = typical <= 32 ? 32 : (typical <= 64 ? 64 : 128);
   const int groups = a->group == 32 ? 4 : (a->group == 64 ? 2 : 1);
-  const int features = a->swiglu ? w4::kRows / 2 : w4::kRows;
-  const int64_t ny = (int64_t(a->n) + features - 1) / features;
-  const int64_t nz = tiles_bound(a->rows, a->experts, grouped, tokens);
-  if (ny > 65535 || nz > 65535) return invalid("aspire_w4_linear", "n or rows too large");
+  const int features = a->swiglu ? w4::kRows : 2 * w4::kRows;
+  const int64_t tiles = (int64_t(a->n) + features - 1) / features * tiles_bound(a->rows, a->experts, grouped, tokens);
+  if (tiles > INT32_MAX) return invalid("aspire_w4_linear", "n or rows too large");
   int sms = 0;
   int rc = current_sm_count(&sms);
   if (rc) return rc;
-  const int64_t slots = int64_t(sms) * (tokens == 256 ? 1 : 2);
+  // One CTA per SM; K is split over a cluster while the tiles leave half of
+  // the SMs idle and every rank has a stage of its own.
   const int64_t stages = (a->k + 255) / 256;
   int cluster = 1;
-  while (cluster < 8 && ny * nz * cluster * 2 <= slots && cluster * 2 <= stages) cluster *= 2;
+  while (cluster < 8 && tiles * cluster * 2 <= sms && cluster * 2 <= stages) cluster *= 2;
+  const int64_t ctas = cluster > 1 ? tiles : std::min<int64_t>(tiles, sms);
   CUtensorMap codes_map, x_map;
-  const cuuint64_t matrix_rows = cuuint64_t(a->n) * (a->swiglu ? 2 : 1);
   {
-    const cuuint64_t size[3] = {cuuint64_t(a->k / 8), matrix_rows, cuuint64_t(grouped ? a->experts : 1)};
+    const cuuint64_t size[3] = {cuuint64_t(a->k / 8), cuuint64_t(a->n) * (a->swiglu ? 2 : 1),
+                                cuuint64_t(grouped ? a->experts : 1)};
     const cuuint64_t strides[2] = {cuuint64_t(a->codes_stride) * 4,
                                    cuuint64_t(grouped && a->experts > 1 ? a->codes_stride_e : a->codes_stride) * 4};
-    const cuuint32_t box[3] = {32, cuuint32_t(features), 1};
+    const cuuint32_t box[3] = {32, cuuint32_t(w4::kRows), 1};
     rc = encode_map(&codes_map, CU_TENSOR_MAP_DATA_TYPE_INT32, 3, a->codes, size, strides, box);
     if (rc) return rc;
   }
@@ -159,10 +160,10 @@ int w4_tc(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
   W4TcKernel kernel = w4_tc_kernel(a->type == ASPIRE_T_BF16, tokens, groups, a->swiglu != 0);
   const size_t smem = w4_tc_smem(tokens);
   rc = ensure_smem(reinterpret_cast<const void*>(kernel), smem,
-                   g_w4_tc[a->type == ASPIRE_T_BF16][tokens == 64 ? 0 : (tokens == 128 ? 1 : 2)][index_of(groups)]
+                   g_w4_tc[a->type == ASPIRE_T_BF16][tokens == 32 ? 0 : (tokens == 64 ? 1 : 2)][index_of(groups)]
                           [a->swiglu != 0]);
   if (rc) return rc;
-  return w4_launch(kernel, dim3(unsigned(cluster), unsigned(ny), unsigned(nz)), cluster, kW4TcThreads, smem, stream,
+  return w4_launch(kernel, dim3(unsigned(cluster), unsigned(ctas)), cluster, kW4TcThreads, smem, stream,
                    "aspire_w4_tc_kernel launch", p, codes_map, x_map);
 }
 
@@ -247,6 +248,7 @@ int aspire_w4_linear(const AspireW4Args* a, void* stream) {
       return invalid(who, "group must be 32, 64 or a multiple of 128");
     if (a->k % 32 || a->k % a->group) return invalid(who, "k must be a multiple of 32 and of group");
     if (a->offsets && a->experts <= 0) return invalid(who, "offsets need experts > 0");
+    if (a->offsets && a->experts > kW4MaxExperts) return invalid(who, "at most 1024 experts are supported");
     if (a->swiglu && a->residual) return invalid(who, "the gated form takes no residual");
     if (a->swiglu && a->n > INT32_MAX / 2) return invalid(who, "bad sizes");
     if (a->rows == 0) return ASPIRE_OK;

@@ -46,7 +46,7 @@ struct W4Params {
 
 namespace w4 {
 
-constexpr int kRows = 128;  // matrix rows of a tile
+constexpr int kRows = 128;  // matrix rows of a tile (of each half of one in the tcgen05 kernel)
 
 // A CTA's share of the output: `count` rows of x from `row0`, with the matrix
 // of `expert`.  expert -1: the rows belong to none and their outputs are zero.
@@ -55,67 +55,82 @@ struct Tile {
   int32_t expert, row0, count;
 };
 
-// Token tile `index` (of `width` rows) among the experts' row ranges, in
-// expert order, followed by the rows past the last expert's.  Run by one
-// whole warp; every lane returns the tile.  Ranges that leave [0, rows) or
-// run backwards are cut to it and reported.
-__device__ __forceinline__ Tile find_tile(const W4Params& p, int index, int width, int lane) {
-  Tile t{0, 0, 0};
+// A row range of the offsets, cut to [0, rows); one that leaves it or runs
+// backwards is reported.
+__device__ __forceinline__ void expert_range(const W4Params& p, int e, int& begin, int& count) {
+  const int lo = p.offsets[e], hi = p.offsets[e + 1];
+  begin = min(max(lo, 0), p.rows);
+  const int end = min(max(hi, begin), p.rows);
+  if (lo != begin || hi != end) record_status(p.status, ASPIRE_STATUS_BAD_ROW);
+  count = end - begin;
+}
+
+// For every expert its first row and its first token tile (tiles of `width`
+// rows, numbered in expert order) in first_row / first_tile [experts + 1]; the
+// last entries are the end of the last expert's rows and the number of tiles.
+// Run by one whole warp.
+__device__ __forceinline__ void expert_tiles(const W4Params& p, int width, int lane, int32_t* first_row,
+                                             int32_t* first_tile) {
+  int base = 0;
+  for (int e0 = 0; e0 < p.num_experts; e0 += 32) {
+    const int e = e0 + lane;
+    int begin = 0, count = 0;
+    if (e < p.num_experts) expert_range(p, e, begin, count);
+    const int mine = (count + width - 1) / width;
+    int incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += v;
+    }
+    if (e < p.num_experts) {
+      // With broken offsets ranges may overlap; a tile's rows end with its
+      // expert's range, which the next entry must not move.
+      first_row[e] = begin;
+      first_tile[e] = base + incl - mine;
+    }
+    base += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  if (lane == 0) {
+    first_row[p.num_experts] = min(max(p.offsets[p.num_experts], 0), p.rows);
+    first_tile[p.num_experts] = base;
+  }
+}
+
+// Number of token tiles, the rows past the last expert's included.
+__device__ __forceinline__ int token_tile_count(const W4Params& p, int width, const int32_t* first_row,
+                                                const int32_t* first_tile) {
+  if (p.offsets == nullptr) return (p.rows + width - 1) / width;
+  return first_tile[p.num_experts] + (p.rows - first_row[p.num_experts] + width - 1) / width;
+}
+
+// Token tile `index` of expert_tiles' arrays.
+__device__ __forceinline__ Tile find_tile(const W4Params& p, int index, int width, const int32_t* first_row,
+                                          const int32_t* first_tile) {
+  Tile t;
   if (p.offsets == nullptr) {
+    t.expert = 0;
     t.row0 = index * width;
     t.count = min(width, p.rows - t.row0);
     return t;
   }
-  // Lane l counts the tiles of experts [l * per, (l + 1) * per).
-  const int per = (p.num_experts + 31) / 32;
-  const int e0 = min(lane * per, p.num_experts), e1 = min(e0 + per, p.num_experts);
-  auto range = [&](int e, int& b, int& c) {
-    const int lo = p.offsets[e], hi = p.offsets[e + 1];
-    b = min(max(lo, 0), p.rows);
-    const int end = min(max(hi, b), p.rows);
-    if (lo != b || hi != end) record_status(p.status, ASPIRE_STATUS_BAD_ROW);
-    c = end - b;
-  };
-  int mine = 0;
-  for (int e = e0; e < e1; ++e) {
-    int b, c;
-    range(e, b, c);
-    mine += (c + width - 1) / width;
-  }
-  int incl = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += v;
-  }
-  const int total = __shfl_sync(0xffffffffu, incl, 31);
-  if (index >= total) {
-    const int last = min(max(p.offsets[p.num_experts], 0), p.rows);
+  const int E = p.num_experts;
+  if (index >= first_tile[E]) {
     t.expert = -1;
-    t.row0 = min(last + (index - total) * width, p.rows);
+    t.row0 = first_row[E] + (index - first_tile[E]) * width;
     t.count = min(width, p.rows - t.row0);
     return t;
   }
-  int left = index - (incl - mine);
-  const unsigned owner = __ballot_sync(0xffffffffu, left >= 0 && left < mine);
-  if (left >= 0 && left < mine) {
-    for (int e = e0; e < e1; ++e) {
-      int b, c;
-      range(e, b, c);
-      const int n = (c + width - 1) / width;
-      if (left < n) {
-        t.expert = e;
-        t.row0 = b + left * width;
-        t.count = min(width, c - left * width);
-        break;
-      }
-      left -= n;
-    }
+  int lo = 0, hi = E;  // the last expert whose first tile is at or before the index
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first_tile[mid] <= index) lo = mid; else hi = mid;
   }
-  const int src = __ffs(owner) - 1;
-  t.expert = __shfl_sync(0xffffffffu, t.expert, src);
-  t.row0 = __shfl_sync(0xffffffffu, t.row0, src);
-  t.count = __shfl_sync(0xffffffffu, t.count, src);
+  int begin, count;
+  expert_range(p, lo, begin, count);
+  t.expert = lo;
+  t.row0 = begin + (index - first_tile[lo]) * width;
+  t.count = min(width, begin + count - t.row0);
   return t;
 }
 
@@ -220,50 +235,72 @@ struct ScaleRow {
     if (GROUPS > 1) return block * GROUPS;
     return p.group_recip ? int(__umulhi(uint32_t(block), p.group_recip)) : block;
   }
+  // What load() reads: the groups' scales and zero points as they lie in
+  // memory.  Nothing is computed from them before packed() asks, so that the
+  // loads stay in flight.
+  struct Raw {
+    uint32_t scale[(GROUPS + 1) / 2];
+    uint32_t zero;
+  };
   // Blocks past the row's end give scale 0.
-  __device__ __forceinline__ void load(const W4Params& p, int block, uint32_t* v) const {
+  __device__ __forceinline__ Raw load(const W4Params& p, int block) const {
+    Raw v;
 #pragma unroll
-    for (int e = 0; e < GROUPS; ++e) v[e] = pack_scale(0, 8);
-    if (!live || block * 128 >= p.k) return;
+    for (int e = 0; e < (GROUPS + 1) / 2; ++e) v.scale[e] = 0;
+    v.zero = 0x08080808u;
+    if (!live || block * 128 >= p.k) return v;
     const int gi = first_group(p, block);
-    alignas(8) uint16_t s[GROUPS];
-    alignas(4) uint8_t z[GROUPS];
-    // A whole block's groups in one load each, where rows are aligned for it.
-    const bool whole = GROUPS > 1 && block * 128 + 128 <= p.k;
-    if (whole && p.scales_vec) {
-      if constexpr (GROUPS == 4) *reinterpret_cast<uint2*>(s) = __ldg(reinterpret_cast<const uint2*>(scale + gi));
-      if constexpr (GROUPS == 2) *reinterpret_cast<uint32_t*>(s) = __ldg(reinterpret_cast<const uint32_t*>(scale + gi));
+    if constexpr (GROUPS == 1) {
+      v.scale[0] = __ldg(scale + gi);
+      if (zero) v.zero = __ldg(zero + gi);
     } else {
-#pragma unroll
-      for (int e = 0; e < GROUPS; ++e) s[e] = block * 128 + e * (128 / GROUPS) < p.k ? __ldg(scale + gi + e) : 0;
-    }
-#pragma unroll
-    for (int e = 0; e < GROUPS; ++e) z[e] = 8;
-    if (zero) {
-      if (whole && p.zeros_vec) {
-        if constexpr (GROUPS == 4) *reinterpret_cast<uint32_t*>(z) = __ldg(reinterpret_cast<const uint32_t*>(zero + gi));
-        if constexpr (GROUPS == 2) *reinterpret_cast<uint16_t*>(z) = __ldg(reinterpret_cast<const uint16_t*>(zero + gi));
+      // A whole block's groups in one load each, where rows are aligned for it.
+      const bool whole = block * 128 + 128 <= p.k;
+      if (whole && p.scales_vec) {
+        if constexpr (GROUPS == 4) {
+          const uint2 u = __ldg(reinterpret_cast<const uint2*>(scale + gi));
+          v.scale[0] = u.x;
+          v.scale[1] = u.y;
+        } else {
+          v.scale[0] = __ldg(reinterpret_cast<const uint32_t*>(scale + gi));
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < GROUPS; ++e)
-          if (block * 128 + e * (128 / GROUPS) < p.k) z[e] = __ldg(zero + gi + e);
+          if (block * 128 + e * (128 / GROUPS) < p.k) v.scale[e / 2] |= uint32_t(__ldg(scale + gi + e)) << (16 * (e & 1));
+      }
+      if (zero) {
+        if (whole && p.zeros_vec) {
+          if constexpr (GROUPS == 4)
+            v.zero = __ldg(reinterpret_cast<const uint32_t*>(zero + gi));
+          else
+            v.zero = __ldg(reinterpret_cast<const uint16_t*>(zero + gi));
+        } else {
+          v.zero = 0;
+#pragma unroll
+          for (int e = 0; e < GROUPS; ++e)
+            if (block * 128 + e * (128 / GROUPS) < p.k) v.zero |= uint32_t(__ldg(zero + gi + e)) << (8 * e);
+        }
       }
     }
-#pragma unroll
-    for (int e = 0; e < GROUPS; ++e) v[e] = pack_scale(s[e], z[e]);
+    return v;
+  }
+  // Group e's scale and zero point in one word (pack_scale).
+  __device__ __forceinline__ static uint32_t packed(const Raw& v, int e) {
+    return pack_scale(uint16_t(v.scale[e / 2] >> (16 * (e & 1))), v.zero >> (8 * e));
   }
 };
 
 __device__ __forceinline__ float silu(float v) { return v / (1.0f + __expf(-v)); }
 
-// The outputs of a tile from the ranks' fp32 partials `red` [tokens][pitch]
-// (matrix rows along a line), added in rank order: rank r finishes its part
-// of the features.  Threads go along the features, so a token's outputs leave
-// as consecutive elements.
-template <bool BF16, bool SWIGLU>
+// The outputs of a tile of ROWS matrix rows from the ranks' fp32 partials `red`
+// [tokens][pitch] (matrix rows along a line), added in rank order: rank r
+// finishes its part of the features.  Threads go along the features, so a
+// token's outputs leave as consecutive elements.
+template <bool BF16, bool SWIGLU, int ROWS>
 __device__ __forceinline__ void finish_tile(const W4Params& p, const Tile& tile, int f0, int rank, int ranks,
                                             float* red, int pitch, int tid, int threads) {
-  constexpr int FEATURES = SWIGLU ? kRows / 2 : kRows;
+  constexpr int FEATURES = SWIGLU ? ROWS / 2 : ROWS;
   const int share = FEATURES / ranks;  // a power of two
   const int shift = 31 - __clz(share);
   for (int i = tid; i < tile.count * share; i += threads) {
@@ -309,11 +346,12 @@ size_t w4_small_smem(int tokens, int groups);
 using W4Kernel = void (*)(W4Params);
 W4Kernel w4_small_kernel(bool bf16, int tokens, int groups, bool swiglu);
 
-// The tcgen05 kernel, by tokens per tile (64, 128, 256).  Its tensor maps:
-// the codes as int32 [experts, rows, k / 8] with boxes of 32 words x 128 rows
-// (64 with the activation), the tokens as [rows, k] with boxes of 64 x tokens,
-// both with the 128-byte swizzle.
-constexpr int kW4TcThreads = 352;
+// The tcgen05 kernel, by tokens per tile (32, 64, 128).  Its tensor maps:
+// the codes as int32 [experts, rows, k / 8] with boxes of 32 words x 128 rows,
+// the tokens as [rows, k] with boxes of 64 x tokens, both with the 128-byte
+// swizzle.
+constexpr int kW4TcThreads = 640;
+constexpr int kW4MaxExperts = 1024;
 size_t w4_tc_smem(int tokens);
 using W4TcKernel = void (*)(W4Params, CUtensorMap, CUtensorMap);
 W4TcKernel w4_tc_kernel(bool bf16, int tokens, int groups, bool swiglu);

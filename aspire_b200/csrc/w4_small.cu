@@ -120,16 +120,21 @@ __global__ void __launch_bounds__(kW4SmallThreads, 2) aspire_w4_small_kernel(con
   const int g = lane >> 2, c = lane & 3;
   const int rank = blockIdx.x, ranks = gridDim.x;
   const int f0 = blockIdx.y * FEATURES;
-  if (p.offsets != nullptr) {
-    if (warp == 0) {
-      const Tile t = find_tile(p, blockIdx.z, TOKENS, lane);
-      if (lane == 0) tile_s = t;
+  if (warp == 0) {
+    // (The ring's memory is free until the first copies.)
+    int32_t* const first_row = reinterpret_cast<int32_t*>(smem);
+    int32_t* const first_tile = first_row + kW4MaxExperts + 1;
+    if (p.offsets != nullptr) {
+      expert_tiles(p, TOKENS, lane, first_row, first_tile);
+      __syncwarp();
     }
-    __syncthreads();
-  } else if (tid == 0) {
-    tile_s = find_tile(p, blockIdx.z, TOKENS, 0);
+    if (lane == 0) {
+      tile_s = Tile{0, 0, 0};
+      if (int(blockIdx.z) < token_tile_count(p, TOKENS, first_row, first_tile))
+        tile_s = find_tile(p, blockIdx.z, TOKENS, first_row, first_tile);
+    }
   }
-  if (p.offsets == nullptr) __syncthreads();
+  __syncthreads();
   const Tile tile = tile_s;
   if (tile.count <= 0) return;  // the whole cluster: its CTAs share the tile
   if (tile.expert < 0) {
@@ -375,7 +380,7 @@ __global__ void __launch_bounds__(kW4SmallThreads, 2) aspire_w4_small_kernel(con
     cg::this_cluster().sync();
   else
     __syncthreads();
-  finish_tile<BF16, SWIGLU>(p, tile, f0, rank, ranks, red, kRedPitch, tid, kW4SmallThreads);
+  finish_tile<BF16, SWIGLU, kRows>(p, tile, f0, rank, ranks, red, kRedPitch, tid, kW4SmallThreads);
   if (ranks > 1) cg::this_cluster().sync();  // peers read this CTA's partials until here
 }
 

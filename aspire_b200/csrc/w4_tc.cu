@@ -1,25 +1,35 @@
 // 4-bit products of many tokens (a decode batch, a prefill chunk) on tcgen05.
 //
-// A CTA owns 128 matrix rows (64 gate and 64 up rows with the activation) as
-// the MMA's M dimension, TOKENS tokens as its N, and a range of K.  The
-// weights' way is HBM -> shared memory (TMA, 128 rows x 256 weights a stage)
-// -> registers -> TMEM: thread r of a warpgroup unpacks row r's 64 weights of
-// a step, (q - z) exactly and times the scale with one rounding to the
+// One CTA per SM walks over tiles of 256 matrix rows x 32, 64 or 128 tokens.
+// A tile's two halves of 128 rows (gate and up rows with the activation) are
+// the M dimension of two MMAs that share every tile of tokens.  The weights'
+// way is HBM -> shared memory (TMA, 256 rows x 256 weights a stage) ->
+// registers -> TMEM: thread r of a warpgroup unpacks row r's 128 weights of a
+// step, (q - z) exactly and times the scale with one rounding to the
 // activations' type, and stores them as the MMA's A operand in TMEM, lane r.
-// The tokens come by TMA as the K-major B operand, 64 of K a stage, and the
+// The tokens come by TMA as the K-major B operand, 128 of K a step, and the
 // fp32 sums stay in TMEM until the epilogue.  So the unpacked weights never
 // take shared-memory bandwidth, which the B operand needs, and every thread
 // meets one row's scales only.
 //
-// Roles: warps 0-3 and 4-7 unpack (one warpgroup takes steps 0 and 1 of a
-// 256-weight stage, the other steps 2 and 3; the sum's order is free, so the
-// MMA takes them alternately) and run the epilogue, warp 8 loads the tokens,
-// warp 10 the codes (each as far ahead as its own ring allows), warp 9 issues
-// the MMAs.  Every wait is bounded; after a timeout the CTA
+// An MMA of 128 rows x 16 k takes 64 cycles up to 128 tokens, and the thread
+// that issues it spends 100 to 200 more on every wait and commit.  So each
+// half has its own issuing warp, a step is 8 MMAs between one wait and one
+// commit, and the rest is the unpacking warps' business: they see to it that
+// the tokens are there before they report a step as unpacked, and release the
+// tokens' stage when they find a step's operand free again.
+//
+// Roles: warps 0-15 unpack (warpgroup q takes half q & 1 of every other step)
+// and run the epilogue, warp 16 loads the tokens, warp 17 the codes (each as
+// far ahead as its own ring allows, into the next tiles too), warps 18 and 19
+// issue the halves' MMAs.  Every wait is bounded; after a timeout the CTA
 // reports it, lets its copies and MMAs land, frees TMEM and returns.
 //
-// Few tiles: a cluster splits K and adds the partials in distributed shared
-// memory in rank order, as in the kernel for few tokens.
+// The epilogue goes from TMEM to global memory: a lane holds one row, so a
+// warp's store is 32 neighbouring outputs of a token; gate and up sums of an
+// output are in the same lane.  Few tiles: a cluster splits K and adds the
+// partials in distributed shared memory in rank order, as in the kernel for
+// few tokens.
 #include <cooperative_groups.h>
 
 #include "tc_pipeline.cuh"
@@ -35,246 +45,345 @@ using namespace w4;
 using pipe::drain_bar;
 using pipe::wait_bar;
 
+constexpr int kTileRows = 2 * kRows;
 constexpr int kStageK = 256;                     // weights of a row per code stage
-constexpr int kStepK = 64;                       // K of one A / B stage
+constexpr int kStepK = 128;                      // K of one A / B stage
 constexpr int kSteps = kStageK / kStepK;
-constexpr uint32_t kCodeBytes = kRows * kStageK / 2;
-constexpr int kRedPitch = kRows + 4;             // floats
-constexpr int kUnpackThreads = 256;
-constexpr int kXWarp = 8, kMmaWarp = 9, kCodeWarp = 10;
+constexpr uint32_t kHalfCodes = kRows * kStageK / 2;
+constexpr uint32_t kCodeBytes = 2 * kHalfCodes;
+constexpr int kRedPitch = kTileRows + 4;         // floats
+constexpr int kUnpackWarps = 16;
+constexpr int kXWarp = 16, kCodeWarp = 17, kMmaWarp = 18;  // and 19: the second half's
+constexpr uint32_t kTmemCols = 512;
+// Room for the experts' first rows and tiles.
+constexpr size_t kExpertBytes = 2 * 4 * (kW4MaxExperts + 1);
 
 template <int TOKENS>
 struct Shape {
-  static constexpr int kCodeStages = TOKENS == 128 ? 2 : 3;  // two CTAs per SM below 256 tokens
-  static constexpr int kXStages = TOKENS == 64 ? 6 : 4;
-  static constexpr uint32_t kXBytes = uint32_t(TOKENS) * kStepK * 2;
-  static constexpr uint32_t kTmemCols = TOKENS == 256 ? 512 : 256;
-  static constexpr int kAStages = (int(kTmemCols) - TOKENS) / 32 > 4 ? ((int(kTmemCols) - TOKENS) / 32 >= 8 ? 8 : 6) : 4;
+  static constexpr uint32_t kBox = uint32_t(TOKENS) * 128;   // 64 of K
+  static constexpr uint32_t kXBytes = 2 * kBox;
+  static constexpr int kXStages = 4;
+  static constexpr int kCodeStages = TOKENS == 128 ? 2 : (TOKENS == 64 ? 4 : 5);
+  // TMEM: the halves' sums, then the A stages (64 columns a half).
+  static constexpr uint32_t kColA = 2 * TOKENS;
+  static constexpr int kAStages = int(kTmemCols - kColA) / 128;
   static constexpr size_t kRing = size_t(kCodeStages) * kCodeBytes + size_t(kXStages) * kXBytes;
   static constexpr size_t kRed = size_t(TOKENS) * kRedPitch * 4;
-  static constexpr size_t kBytes = (kRing > kRed ? kRing : kRed) + 1024;  // 1 KiB to align the swizzled tiles
-  static_assert(TOKENS + 32 * kAStages <= int(kTmemCols), "TMEM columns");
+  static_assert(kRed <= kRing, "the partials reuse the rings");
+  static_assert(kAStages >= 2 && kAStages <= 3, "both parities of steps are in flight");
+  static constexpr size_t kBytes = kRing + kExpertBytes + 1024;  // 1 KiB to align the swizzled tiles
 };
 
 struct Control {
-  uint64_t w_full[3], w_empty[3];
-  uint64_t x_full[6], x_empty[6];
-  uint64_t a_full[8], a_empty[8];
-  uint64_t d_full;
+  uint64_t w_full[5], w_empty[5];
+  uint64_t x_full[4], x_empty[4];
+  uint64_t a_full[3][2], a_empty[3][2];  // by half
+  uint64_t d_full, d_empty, done;
   uint64_t wait_ns;
   uint32_t tmem_base;
   int abort_flag;
-  Tile tile;
 };
 
+// TOKENS: tokens of a tile (32, 64, 128).  GROUPS: scale groups per 128
+// weights of a row (a group of more than 128 counts as one).  Grid: (cluster
+// ranks, CTAs or clusters); with more than one rank a cluster has one tile at
+// most.
 template <bool BF16, int TOKENS, int GROUPS, bool SWIGLU>
-__global__ void __launch_bounds__(kW4TcThreads, TOKENS == 256 ? 1 : 2)
+__global__ void __launch_bounds__(kW4TcThreads, 1)
     aspire_w4_tc_kernel(const __grid_constant__ W4Params p, const __grid_constant__ CUtensorMap codes_map,
                         const __grid_constant__ CUtensorMap x_map) {
   pdl_begin();
   using S = Shape<TOKENS>;
-  constexpr int FEATURES = SWIGLU ? kRows / 2 : kRows;
+  constexpr int FEATURES = SWIGLU ? kRows : kTileRows;
   constexpr int SW = S::kCodeStages, SX = S::kXStages, SA = S::kAStages;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Control sm;
-  uint8_t* smem = smem_raw + ((1024 - (ptx::smem_addr(smem_raw) & 1023)) & 1023);
-  uint8_t* codes_s = smem;
-  uint8_t* x_s = smem + SW * kCodeBytes;
-  float* red = reinterpret_cast<float*>(smem);
+  uint8_t* const codes_s = smem_raw + ((1024 - (ptx::smem_addr(smem_raw) & 1023)) & 1023);
+  uint8_t* const x_s = codes_s + SW * kCodeBytes;
+  float* const red = reinterpret_cast<float*>(codes_s);
+  int32_t* const expert_row = reinterpret_cast<int32_t*>(codes_s + S::kRing);
+  int32_t* const expert_tile = expert_row + kW4MaxExperts + 1;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x, ranks = gridDim.x;
-  const int f0 = blockIdx.y * FEATURES;
   if (warp == 0) {
-    const Tile t = find_tile(p, blockIdx.z, TOKENS, lane);
     if (lane == 0) {
-      sm.tile = t;
       sm.abort_flag = 0;
       sm.wait_ns = p.wait_ns;
       for (int i = 0; i < SW; ++i) {
         ptx::mbar_init(ptx::smem_addr(&sm.w_full[i]), 1);
-        ptx::mbar_init(ptx::smem_addr(&sm.w_empty[i]), kUnpackThreads / 32);
+        ptx::mbar_init(ptx::smem_addr(&sm.w_empty[i]), kUnpackWarps);
       }
       for (int i = 0; i < SX; ++i) {
         ptx::mbar_init(ptx::smem_addr(&sm.x_full[i]), 1);
-        ptx::mbar_init(ptx::smem_addr(&sm.x_empty[i]), 1);
+        ptx::mbar_init(ptx::smem_addr(&sm.x_empty[i]), 2);
       }
-      for (int i = 0; i < SA; ++i) {
-        ptx::mbar_init(ptx::smem_addr(&sm.a_full[i]), 4);
-        ptx::mbar_init(ptx::smem_addr(&sm.a_empty[i]), 1);
-      }
-      ptx::mbar_init(ptx::smem_addr(&sm.d_full), 1);
+      for (int i = 0; i < SA; ++i)
+        for (int h = 0; h < 2; ++h) {
+          ptx::mbar_init(ptx::smem_addr(&sm.a_full[i][h]), 4);
+          ptx::mbar_init(ptx::smem_addr(&sm.a_empty[i][h]), 1);
+        }
+      ptx::mbar_init(ptx::smem_addr(&sm.d_full), 2);
+      ptx::mbar_init(ptx::smem_addr(&sm.done), 2);
+      ptx::mbar_init(ptx::smem_addr(&sm.d_empty), kUnpackWarps);
       ptx::mbar_fence_init();
     }
-  }
-  __syncthreads();
-  const Tile tile = sm.tile;
-  if (tile.count <= 0) return;  // the whole cluster: its CTAs share the tile
-  if (tile.expert < 0) {
-    if (rank == 0)
-      for (int i = tid; i < tile.count * FEATURES; i += kW4TcThreads) {
-        const int t = i / FEATURES, f = f0 + i % FEATURES;
-        if (f < p.n) p.out[int64_t(tile.row0 + t) * p.out_stride + f] = 0;
-      }
-    return;
+    if (p.offsets != nullptr) expert_tiles(p, TOKENS, lane, expert_row, expert_tile);
   }
   if (warp == kMmaWarp) {
-    ptx::tmem_alloc(ptx::smem_addr(&sm.tmem_base), S::kTmemCols);
+    ptx::tmem_alloc(ptx::smem_addr(&sm.tmem_base), kTmemCols);
     ptx::tmem_relinquish();
   }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
-  const uint32_t a_col = TOKENS;  // A stages follow the sums
-
+  const int row_tiles = (p.n + FEATURES - 1) / FEATURES;
+  const int n_tiles = row_tiles * token_tile_count(p, TOKENS, expert_row, expert_tile);
   const int n_stages = (p.k + kStageK - 1) / kStageK;
   const int s_begin = int(int64_t(n_stages) * rank / ranks), s_end = int(int64_t(n_stages) * (rank + 1) / ranks);
-  const int stages = s_end - s_begin;
-  const int steps = stages * kSteps;
-  // Step i of the MMA's order: stage i / 4, K sub-block (0, 2, 1, 3)[i % 4].
-  auto sub_of = [](int i) { return ((i & 1) << 1) | ((i >> 1) & 1); };
+  const int stages = s_end - s_begin, steps = stages * kSteps;
+  const int first_tile = blockIdx.y, tile_step = gridDim.y;
+  auto tile_of = [&](int i) { return find_tile(p, i / row_tiles, TOKENS, expert_row, expert_tile); };
 
   if (warp == kCodeWarp) {
     if (lane == 0) {
       ptx::prefetch_tmap(&codes_map);
-      int s = 0;
-      for (; s < stages; ++s) {
-        const int ws = s % SW;
-        if (!wait_bar(sm, sm.w_empty[ws], ((s / SW) & 1) ^ 1, p.status)) break;
-        const uint32_t bar = ptx::smem_addr(&sm.w_full[ws]);
-        const uint32_t dst = ptx::smem_addr(codes_s + ws * kCodeBytes);
-        const int c0 = (s_begin + s) * (kStageK / 8);
-        ptx::mbar_arrive_expect_tx(bar, kCodeBytes);
-        ptx::tma_load_3d(dst, &codes_map, bar, c0, f0, tile.expert);
-        if (SWIGLU) ptx::tma_load_3d(dst + kCodeBytes / 2, &codes_map, bar, c0, p.n + f0, tile.expert);
+      int n = 0;  // stages so far, over all tiles
+      bool ok = true;
+      for (int i = first_tile; i < n_tiles && ok; i += tile_step) {
+        const Tile tile = tile_of(i);
+        if (tile.expert < 0) continue;
+        const int f0 = (i % row_tiles) * FEATURES;
+        for (int s = s_begin; s < s_end; ++s, ++n) {
+          const int ws = n % SW;
+          if (!wait_bar(sm, sm.w_empty[ws], ((n / SW) & 1) ^ 1, p.status)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = ptx::smem_addr(&sm.w_full[ws]);
+          const uint32_t dst = ptx::smem_addr(codes_s + ws * kCodeBytes);
+          ptx::mbar_arrive_expect_tx(bar, kCodeBytes);
+          ptx::tma_load_3d(dst, &codes_map, bar, s * (kStageK / 8), f0, tile.expert);
+          // (Past the matrix's last row the copy fills with zeros.)
+          ptx::tma_load_3d(dst + kHalfCodes, &codes_map, bar, s * (kStageK / 8), SWIGLU ? p.n + f0 : f0 + kRows,
+                           tile.expert);
+        }
       }
       // After a timeout anywhere the copies in flight land before the CTA ends.
-      if (s < stages || pipe::aborted(sm))
-        for (int i = max(0, s - SW); i < s; ++i) drain_bar(sm.w_full[i % SW], (i / SW) & 1);
+      if (!ok || pipe::aborted(sm))
+        for (int j = max(0, n - SW); j < n; ++j) drain_bar(sm.w_full[j % SW], (j / SW) & 1);
     }
   } else if (warp == kXWarp) {
     if (lane == 0) {
       ptx::prefetch_tmap(&x_map);
-      int i = 0;
-      for (; i < steps; ++i) {
-        const int xs = i % SX;
-        if (!wait_bar(sm, sm.x_empty[xs], ((i / SX) & 1) ^ 1, p.status)) break;
-        const uint32_t bar = ptx::smem_addr(&sm.x_full[xs]);
-        ptx::mbar_arrive_expect_tx(bar, S::kXBytes);
-        ptx::tma_load_2d(ptx::smem_addr(x_s + xs * S::kXBytes), &x_map, bar,
-                         (s_begin + i / kSteps) * kStageK + sub_of(i % kSteps) * kStepK, tile.row0);
+      int n = 0;  // steps so far
+      bool ok = true;
+      for (int i = first_tile; i < n_tiles && ok; i += tile_step) {
+        const Tile tile = tile_of(i);
+        if (tile.expert < 0) continue;
+        for (int j = 0; j < steps; ++j, ++n) {
+          const int xs = n % SX;
+          if (!wait_bar(sm, sm.x_empty[xs], ((n / SX) & 1) ^ 1, p.status)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = ptx::smem_addr(&sm.x_full[xs]);
+          ptx::mbar_arrive_expect_tx(bar, S::kXBytes);
+          const uint32_t dst = ptx::smem_addr(x_s + xs * S::kXBytes);
+          const int k = s_begin * kStageK + j * kStepK;
+          ptx::tma_load_2d(dst, &x_map, bar, k, tile.row0);
+          ptx::tma_load_2d(dst + S::kBox, &x_map, bar, k + 64, tile.row0);
+        }
       }
-      if (i < steps || pipe::aborted(sm))
-        for (int j = max(0, i - SX); j < i; ++j) drain_bar(sm.x_full[j % SX], (j / SX) & 1);
+      if (!ok || pipe::aborted(sm))
+        for (int j = max(0, n - SX); j < n; ++j) drain_bar(sm.x_full[j % SX], (j / SX) & 1);
     }
-  } else if (warp == kMmaWarp) {
+  } else if (warp >= kMmaWarp) {
     constexpr uint32_t idesc =
         BF16 ? ptx::idesc_bf16(kRows, TOKENS, false, false) : ptx::idesc_f16(kRows, TOKENS, false, false);
+    const int half = warp - kMmaWarp;
+    const uint32_t d = tmem + half * TOKENS, a0 = tmem + S::kColA + half * 64;
+    int n = 0, tiles = 0;
     bool ok = true;
-    for (int i = 0; i < steps; ++i) {
-      const int as = i % SA, xs = i % SX;
-      if (!wait_bar(sm, sm.x_full[xs], (i / SX) & 1, p.status) || !wait_bar(sm, sm.a_full[as], (i / SA) & 1, p.status))
-        ok = false;
-      if (!__all_sync(0xffffffffu, ok)) break;
-      ptx::tc_fence_after();
-      if (lane == 0) {
-        const uint64_t b = ptx::smem_desc(ptx::smem_addr(x_s + xs * S::kXBytes), 16, 1024, ptx::kLayoutSw128);
+    for (int i = first_tile; i < n_tiles && ok; i += tile_step) {
+      if (tile_of(i).expert < 0) continue;
+      // The previous tile's sums have been read.
+      if (tiles > 0 && !wait_bar(sm, sm.d_empty, (tiles - 1) & 1, p.status)) ok = false;
+      for (int j = 0; j < steps && ok; ++j, ++n) {
+        const int as = n % SA, xs = n % SX;
+        // (Of a step whose tokens have arrived as well.)
+        ok = wait_bar(sm, sm.a_full[as][half], (n / SA) & 1, p.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        if (lane == 0) {
+          const uint64_t b = ptx::smem_desc(ptx::smem_addr(x_s + xs * S::kXBytes), 16, 1024, ptx::kLayoutSw128);
 #pragma unroll
-        for (int kk = 0; kk < kStepK / 16; ++kk)
-          ptx::mma_bf16_ts(tmem, tmem + a_col + uint32_t(as) * 32 + uint32_t(kk) * 8, b + uint64_t(kk * 32 >> 4), idesc,
-                           (i > 0 || kk > 0) ? 1u : 0u);
-        ptx::mma_commit(ptx::smem_addr(&sm.a_empty[as]));
-        ptx::mma_commit(ptx::smem_addr(&sm.x_empty[xs]));
+          for (int kk = 0; kk < kStepK / 16; ++kk)
+            ptx::mma_bf16_ts(d, a0 + uint32_t(as) * 128 + kk * 8, b + (((kk / 4) * S::kBox + (kk % 4) * 32) >> 4), idesc,
+                             (j > 0 || kk > 0) ? 1u : 0u);
+          ptx::mma_commit(ptx::smem_addr(&sm.a_empty[as][half]));
+          if (j == steps - 1) ptx::mma_commit(ptx::smem_addr(&sm.d_full));
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      ++tiles;
     }
     // Fires once every MMA issued so far has completed, after a timeout too.
-    if (lane == 0) ptx::mma_commit(ptx::smem_addr(&sm.d_full));
+    if (lane == 0) ptx::mma_commit(ptx::smem_addr(&sm.done));
     __syncwarp();
-    drain_bar(sm.d_full, 0);
-  } else if (warp < 8) {
+    drain_bar(sm.done, 0);
+  } else {
     // -------------------------------------------------------------- unpack
-    const int wg = warp >> 2;              // half of a stage
-    const int r = tid & (kRows - 1);       // tile row
-    int64_t mr = SWIGLU ? f0 + (r & (FEATURES - 1)) : f0 + r;
-    const bool live = mr < p.n;
-    if (SWIGLU && r >= FEATURES) mr += p.n;
-    if (!live) mr = 0;
-    const ScaleRow<BF16, GROUPS> scales(p, tile.expert, mr, live);
+    const int half = (warp >> 2) & 1, parity = warp >> 3;
+    const int r = tid & (kRows - 1);       // row of the half
     const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
-    uint32_t cur[GROUPS], nxt[GROUPS];
-    scales.load(p, s_begin * 2 + wg, nxt);
+    const uint32_t a_lanes = lanes + S::kColA + half * 64;
+    uint32_t row_at[4];                    // the warp's 16-byte chunks of a stage: block `parity` of 128 weights
+#pragma unroll
+    for (int q = 0; q < 4; ++q) row_at[q] = half * kHalfCodes + r * 128 + (((parity * 4 + q) ^ (r & 7)) << 4);
+    int n = 0, tiles = 0;                  // stages and tiles so far
     bool ok = true;
-    for (int s = 0; s < stages && ok; ++s) {
+    for (int i = first_tile; i < n_tiles && ok; i += tile_step) {
+      const Tile tile = tile_of(i);
+      const int f0 = (i % row_tiles) * FEATURES;
+      if (tile.expert < 0) {
+        if (rank == 0)
+          for (int j = tid; j < tile.count * FEATURES; j += kUnpackWarps * 32) {
+            const int t = j / FEATURES, f = f0 + j % FEATURES;
+            if (f < p.n) p.out[int64_t(tile.row0 + t) * p.out_stride + f] = 0;
+          }
+        continue;
+      }
+      const int f = SWIGLU ? f0 + r : f0 + half * kRows + r;
+      const bool live = f < p.n;
+      const ScaleRow<BF16, GROUPS> scales(p, tile.expert, live ? (SWIGLU && half ? int64_t(p.n) + f : f) : 0, live);
+      // The block's scales, loaded a stage ahead.
+      typename ScaleRow<BF16, GROUPS>::Raw nxt = scales.load(p, s_begin * 2 + parity);
+      for (int s = 0; s < stages && ok; ++s) {
+        uint32_t sc[GROUPS];
 #pragma unroll
-      for (int e = 0; e < GROUPS; ++e) cur[e] = nxt[e];
-      if (s + 1 < stages) scales.load(p, (s_begin + s + 1) * 2 + wg, nxt);
-      const int ws = s % SW;
-      if (!wait_bar(sm, sm.w_full[ws], (s / SW) & 1, p.status)) ok = false;
-      if (!__all_sync(0xffffffffu, ok)) break;
-      const uint8_t* row = codes_s + ws * kCodeBytes + r * 128;
+        for (int e = 0; e < GROUPS; ++e) sc[e] = ScaleRow<BF16, GROUPS>::packed(nxt, e);
+        if (s + 1 < stages) nxt = scales.load(p, (s_begin + s + 1) * 2 + parity);
+        const int ws = (n + s) % SW;
+        ok = wait_bar(sm, sm.w_full[ws], ((n + s) / SW) & 1, p.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint8_t* const st = codes_s + ws * kCodeBytes;
+        const int j = (n + s) * kSteps + parity, as = j % SA;
+        uint32_t w[16];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int i = s * kSteps + h * 2 + wg, as = i % SA;
-        uint32_t w[8];
-        *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(row + (((wg * 4 + h * 2) ^ (r & 7)) << 4));
-        *reinterpret_cast<uint4*>(w + 4) = *reinterpret_cast<const uint4*>(row + (((wg * 4 + h * 2 + 1) ^ (r & 7)) << 4));
-        uint32_t a[32];
+        for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(w + q * 4) = *reinterpret_cast<const uint4*>(st + row_at[q]);
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.w_empty[ws]));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t ps = cur[(h * 64 + j * 8) * GROUPS / 128];
-          const uint32_t m = scale_pair(ps);
-          uint32_t z0, z1;
-          Num<BF16>::zero_consts(ps & 15u, z0, z1);
-          Num<BF16>::unpack(w[j], z0, z1, a + j * 4);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t a[32];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) a[j * 4 + q] = Num<BF16>::mul2(a[j * 4 + q], m);
+          for (int q = 0; q < 8; ++q) {
+            const uint32_t ps = sc[(h * 8 + q) * GROUPS / 16], m = scale_pair(ps);
+            uint32_t z0, z1;
+            Num<BF16>::zero_consts(ps & 15u, z0, z1);
+            Num<BF16>::unpack(w[h * 8 + q], z0, z1, a + q * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[q * 4 + e] = Num<BF16>::mul2(a[q * 4 + e], m);
+          }
+          if (h == 0) {
+            // The stage's previous step is through the tensor core, and with it
+            // its tokens.
+            ok = wait_bar(sm, sm.a_empty[as][half], ((j / SA) & 1) ^ 1, p.status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            if (j >= SA && (warp & 3) == 0 && lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.x_empty[(j - SA) % SX]));
+          }
+          ptx::tmem_st32(a_lanes + uint32_t(as) * 128 + h * 32, a);
         }
-        if (!wait_bar(sm, sm.a_empty[as], ((i / SA) & 1) ^ 1, p.status)) ok = false;
-        if (!__all_sync(0xffffffffu, ok)) break;
-        ptx::tc_fence_after();
-        ptx::tmem_st32(lanes + a_col + uint32_t(as) * 32, a);
+        if (!ok) break;
         ptx::tmem_wait_st();
+        if ((warp & 3) == 0) {
+          ok = wait_bar(sm, sm.x_full[j % SX], (j / SX) & 1, p.status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.a_full[as]));
+        if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.a_full[as][half]));
       }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.w_empty[ws]));
-    }
-    // The sums, once every MMA has completed (and with it every read of the
-    // rings, whose memory the partials take).
-    if (ok && !wait_bar(sm, sm.d_full, 0, p.status)) ok = false;
-  }
-  __syncthreads();
-  ptx::tc_fence_after();
-  const bool good = !pipe::aborted(sm);
-  if (good && warp < 8) {
-    const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
-    const int r = tid & (kRows - 1);
+      n += stages;
+      // ---------------------------------------------------------- epilogue
+      if (ok) ok = wait_bar(sm, sm.d_full, tiles & 1, p.status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      ++tiles;
+      ptx::tc_fence_after();
+      if (ranks > 1) {
+        // (The rings are idle: their memory takes the partials.)
 #pragma unroll 1
-    for (int c = (warp >> 2) * (TOKENS / 2); c < ((warp >> 2) + 1) * (TOKENS / 2); c += 32) {
-      float v[32];
-      ptx::tmem_ld32(lanes + uint32_t(c), v);
-      ptx::tmem_wait_ld();
+        for (int c = parity * (TOKENS / 2); c < (parity + 1) * (TOKENS / 2); c += 16) {
+          float v[16];
+          ptx::tmem_ld16(lanes + half * TOKENS + uint32_t(c), v);
+          ptx::tmem_wait_ld();
 #pragma unroll
-      for (int j = 0; j < 32; ++j) red[(c + j) * kRedPitch + r] = v[j] * Num<BF16>::kUnit;
+          for (int e = 0; e < 16; ++e) red[(c + e) * kRedPitch + half * kRows + r] = v[e] * Num<BF16>::kUnit;
+        }
+      } else {
+        // Without the activation a warp writes its half's rows; with it, both
+        // halves' warps share the tokens and read gate and up sums.
+        constexpr int SHARE = SWIGLU ? TOKENS / 4 : TOKENS / 2;
+        constexpr int AT_ONCE = SHARE < 16 ? SHARE : 16;
+        const int c0 = SWIGLU ? (parity * 2 + half) * SHARE : parity * SHARE;
+#pragma unroll 1
+        for (int c = c0; c < c0 + SHARE; c += AT_ONCE) {
+          const int left = tile.count - c;
+          if (left <= 0) break;
+          float v[AT_ONCE], u[AT_ONCE];
+#pragma unroll
+          for (int e = 0; e < AT_ONCE; e += 8) {
+            ptx::tmem_ld8(lanes + (SWIGLU ? 0 : half * TOKENS) + uint32_t(c + e), v + e);
+            if (SWIGLU) ptx::tmem_ld8(lanes + TOKENS + uint32_t(c + e), u + e);
+          }
+          ptx::tmem_wait_ld();
+          const int64_t row = tile.row0 + c;
+          uint16_t* const out = p.out + row * p.out_stride + f;
+          const uint16_t* const res = p.residual ? p.residual + row * p.residual_stride + f : nullptr;
+          const int64_t out_stride = p.out_stride, res_stride = p.residual_stride;
+          float add[AT_ONCE];
+#pragma unroll
+          for (int e = 0; e < AT_ONCE; ++e)
+            add[e] = res && live && e < left ? Num<BF16>::to_float(res[e * res_stride]) : 0.f;
+#pragma unroll
+          for (int e = 0; e < AT_ONCE; ++e) {
+            float y = v[e] * Num<BF16>::kUnit;
+            if (SWIGLU) y = silu(y) * (u[e] * Num<BF16>::kUnit);
+            if (res) y += add[e];
+            if (live && e < left) out[e * out_stride] = Num<BF16>::from_float(y);
+          }
+        }
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.d_empty));
     }
   }
   ptx::tc_fence_before();
-  if (ranks > 1)
-    cg::this_cluster().sync();
-  else
-    __syncthreads();
+  __syncthreads();
   if (warp == kMmaWarp) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem, S::kTmemCols);
+    ptx::tmem_dealloc(tmem, kTmemCols);
   }
-  if (good) {
-    finish_tile<BF16, SWIGLU>(p, tile, f0, rank, ranks, red, kRedPitch, tid, kW4TcThreads);
+  if (ranks > 1) {
+    // One tile per cluster: its CTAs' partials meet, added in rank order.
+    cg::this_cluster().sync();
+    if (first_tile < n_tiles) {
+      const Tile tile = tile_of(first_tile);
+      if (tile.expert >= 0 && !pipe::aborted(sm))
+        finish_tile<BF16, SWIGLU, kTileRows>(p, tile, (first_tile % row_tiles) * FEATURES, rank, ranks, red, kRedPitch,
+                                             tid, kW4TcThreads);
+    }
+    cg::this_cluster().sync();  // peers read this CTA's partials until here
   }
-  if (ranks > 1) cg::this_cluster().sync();  // peers read this CTA's partials until here
 }
 
 template <bool BF16, int TOKENS, bool SWIGLU>
@@ -285,15 +394,15 @@ W4TcKernel by_groups(int groups) {
 }
 template <bool BF16, bool SWIGLU>
 W4TcKernel by_tokens(int tokens, int groups) {
+  if (tokens == 32) return by_groups<BF16, 32, SWIGLU>(groups);
   if (tokens == 64) return by_groups<BF16, 64, SWIGLU>(groups);
-  if (tokens == 128) return by_groups<BF16, 128, SWIGLU>(groups);
-  return by_groups<BF16, 256, SWIGLU>(groups);
+  return by_groups<BF16, 128, SWIGLU>(groups);
 }
 
 }  // namespace
 
 size_t w4_tc_smem(int tokens) {
-  return tokens == 64 ? Shape<64>::kBytes : (tokens == 128 ? Shape<128>::kBytes : Shape<256>::kBytes);
+  return tokens == 32 ? Shape<32>::kBytes : (tokens == 64 ? Shape<64>::kBytes : Shape<128>::kBytes);
 }
 
 W4TcKernel w4_tc_kernel(bool bf16, int tokens, int groups, bool swiglu) {

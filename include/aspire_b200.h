@@ -582,7 +582,7 @@ typedef struct AspireW4Args {
   int32_t type;              /* ASPIRE_T_BF16 or ASPIRE_T_F16                               */
   int32_t swiglu;            /* 1: rows [0, n) gate, [n, 2n) up; out = silu(gate) * up      */
   const int32_t* offsets;    /* int32 [experts + 1]: expert e's rows of x; NULL: one matrix */
-  int32_t experts;
+  int32_t experts;           /* at most 1024                                                */
   uint32_t* status;          /* optional device status word                                 */
 } AspireW4Args;
 
