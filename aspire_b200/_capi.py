@@ -418,6 +418,8 @@ _lock = threading.Lock()
 def load_library(path: os.PathLike | str | None = None) -> ctypes.CDLL:
     """Loads libaspire_b200.so once and binds the exported signatures."""
     global _lib
+    if _lib is not None and path is None:
+        return _lib
     with _lock:
         if _lib is not None and path is None:
             return _lib
@@ -448,6 +450,22 @@ def check(rc: int, what: str) -> None:
     if rc == ASPIRE_ERR_INVALID:
         raise ValueError(f"{what}: {msg}")
     raise RuntimeError(f"{what} failed ({rc}): {msg}")
+
+
+def call(name: str, args: ctypes.Structure, device) -> None:
+    """Calls entry point ``name(args, stream)`` on the current stream of a CUDA
+    device, which is made current for the call."""
+    import torch
+
+    index = device.index
+    fn = getattr(load_library(), name)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != ASPIRE_OK:
+        check(rc, name)
 
 
 def status_offset() -> int:

@@ -21,7 +21,6 @@ gradient.
 
 from __future__ import annotations
 
-import ctypes
 from dataclasses import dataclass
 
 import torch
@@ -91,68 +90,68 @@ def dequantize_w4(w: W4Weight) -> torch.Tensor:
 
 
 def _product(x, codes, scales, zeros, residual, out, swiglu, offsets, status):
-    lead = 1 if offsets is not None else 0
-    if x.dim() != 2 or codes.dim() != 2 + lead or scales.dim() != 2 + lead:
+    # Every attribute is read once: a small call is bound by the host.
+    lead = 0 if offsets is None else 1
+    shape, cshape, sshape = x.shape, codes.shape, scales.shape
+    if len(shape) != 2 or len(cshape) != 2 + lead or len(sshape) != 2 + lead:
         raise ValueError("x must be [rows, k] and codes / scales [n, ...], with a leading expert dimension for experts")
-    kind = _TYPES.get(x.dtype)
-    if kind is None or scales.dtype != x.dtype:
+    dtype, dev = x.dtype, x.device
+    kind = _TYPES.get(dtype)
+    if kind is None or scales.dtype != dtype:
         raise ValueError("x and scales must both be bfloat16 or both float16")
     if codes.dtype != torch.int32:
         raise ValueError("codes must be int32")
-    dev = x.device
     if dev.type != "cuda" or codes.device != dev or scales.device != dev:
         raise ValueError("x, codes and scales must be on one CUDA device")
-    rows, k = x.shape
-    r = codes.shape[lead]
-    if codes.shape[-1] * 8 != k:
+    rows, k = shape
+    r, groups = cshape[lead], sshape[-1]
+    if cshape[-1] * 8 != k:
         raise ValueError("codes and x disagree on k")
-    if scales.shape[:-1] != codes.shape[:-1] or scales.shape[-1] == 0 or k % scales.shape[-1]:
+    if sshape[:-1] != cshape[:-1] or groups == 0 or k % groups:
         raise ValueError("scales must be [..., n, k / group]")
-    group = k // scales.shape[-1]
+    group = k // groups
     _check_group(k, group)
     if swiglu and r % 2:
         raise ValueError("the gated form needs as many gate as up rows")
     n = r // 2 if swiglu else r
-    if (rows and x.stride(1) != 1) or codes.stride(-1) != 1 or (scales.shape[-1] > 1 and scales.stride(-1) != 1):
+    xs, cs, ss, zs = x.stride(), codes.stride(), scales.stride(), None
+    if (rows and xs[1] != 1) or cs[-1] != 1 or (groups > 1 and ss[-1] != 1):
         raise ValueError("x, codes and scales need contiguous rows")
     if zeros is not None:
-        if zeros.dtype != torch.uint8 or zeros.shape != scales.shape or zeros.device != dev:
+        if zeros.dtype != torch.uint8 or zeros.shape != sshape or zeros.device != dev:
             raise ValueError("zeros must be uint8 of the scales' shape on their device")
-        if zeros.shape[-1] > 1 and zeros.stride(-1) != 1:
+        zs = zeros.stride()
+        if groups > 1 and zs[-1] != 1:
             raise ValueError("zeros need contiguous rows")
     if offsets is not None and (offsets.dtype != torch.int32 or offsets.device != dev or not offsets.is_contiguous()
-                                or offsets.shape != (codes.shape[0] + 1,)):
+                                or offsets.shape != (cshape[0] + 1,)):
         raise ValueError("offsets must be contiguous int32 [experts + 1] on x's device")
+    if residual is not None:
+        rs = _check_output("residual", residual, dtype, rows, n, dev)
     if out is None:
-        out = torch.empty(rows, n, dtype=x.dtype, device=dev)
-    for name, t in (("out", out), ("residual", residual)):
-        if t is not None and (t.dtype != x.dtype or t.shape != (rows, n) or t.device != dev
-                              or (n > 1 and rows and t.stride(1) != 1)):
-            raise ValueError(f"{name} must be [rows, n] of x's type with contiguous rows on x's device")
+        out, os = torch.empty(rows, n, dtype=dtype, device=dev), n
+    else:
+        os = _check_output("out", out, dtype, rows, n, dev)
     if rows == 0 or n == 0:
         return out
-    a = _capi.AspireW4Args()
-    a.x, a.x_stride, a.rows = x.data_ptr(), x.stride(0) if rows > 1 else k, rows
-    a.codes, a.codes_stride = codes.data_ptr(), codes.stride(lead)
-    a.scales, a.scales_stride = scales.data_ptr(), scales.stride(lead)
-    if zeros is not None:
-        a.zeros, a.zeros_stride = zeros.data_ptr(), zeros.stride(lead)
-    if residual is not None:
-        a.residual, a.residual_stride = residual.data_ptr(), residual.stride(0) if rows > 1 else n
-    a.out, a.out_stride = out.data_ptr(), out.stride(0) if rows > 1 else n
-    a.n, a.k, a.group, a.type, a.swiglu = n, k, group, kind, int(swiglu)
-    if offsets is not None:
-        a.offsets, a.experts = offsets.data_ptr(), codes.shape[0]
-        a.codes_stride_e, a.scales_stride_e = codes.stride(0), scales.stride(0)
-        if zeros is not None:
-            a.zeros_stride_e = zeros.stride(0)
-    if status is not None:
-        a.status = status.data_ptr()
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    with torch.cuda.device(dev):
-        rc = _capi.load_library().aspire_w4_linear(ctypes.byref(a), ctypes.c_void_p(stream))
-    _capi.check(rc, "aspire_w4_linear")
+    _capi.call("aspire_w4_linear", _capi.AspireW4Args(
+        x.data_ptr(), xs[0] if rows > 1 else k, rows,
+        codes.data_ptr(), cs[lead], cs[0] if lead else 0,
+        scales.data_ptr(), ss[lead], ss[0] if lead else 0,
+        None if zeros is None else zeros.data_ptr(), 0 if zs is None else zs[lead], zs[0] if zs and lead else 0,
+        None if residual is None else residual.data_ptr(), 0 if residual is None else rs,
+        out.data_ptr(), os, n, k, group, kind, swiglu,
+        None if offsets is None else offsets.data_ptr(), cshape[0] if lead else 0,
+        None if status is None else status.data_ptr()), dev)
     return out
+
+
+def _check_output(name, t, dtype, rows, n, dev):
+    """The row stride of an output or residual."""
+    st = t.stride()
+    if t.dtype != dtype or t.shape != (rows, n) or t.device != dev or (n > 1 and rows and st[1] != 1):
+        raise ValueError(f"{name} must be [rows, n] of x's type with contiguous rows on x's device")
+    return st[0] if rows > 1 else n
 
 
 def w4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
