@@ -1,8 +1,10 @@
 // Router top-k and the sort of the tokens by expert.
 //
-// One warp per token.  Lane l holds the logits of experts l, l + 32, ... as
-// order-preserving integers; each of the top_k rounds takes the warp's
-// maximum and, among equals, the lowest expert index.  A NaN or -inf logit is
+// One warp per token, two tokens at a time (a round's latency is that of two
+// warp reductions, and the second token's fill it).  Lane l holds the logits of
+// experts l, l + 32, ... as order-preserving integers, sorted; each of the
+// top_k rounds takes the maximum of the lanes' heads and, among equals, the
+// lowest expert index.  A NaN or -inf logit is
 // never chosen: a token with fewer than top_k others gets expert -1 and
 // weight 0 for the rest.  The weights are the softmax over all experts at the
 // chosen ones or, renormalised, the softmax over the chosen ones.
@@ -41,16 +43,34 @@ __device__ __forceinline__ float exp_below(float v, float m) { return v == m ? 1
 struct SortShared {
   uint16_t count[32][kMoeMaxExperts];  // per warp: slots of the expert, then the warps before it
   int32_t base[kMoeMaxExperts];        // the block's first row of the expert
+  int32_t part[2][kMoeSlotsBlock];     // several blocks: sums of a share of their counts (all, earlier)
   int32_t scan[32];
+  int16_t ids[kMoeSlotsOne];           // the block's choices
 };
 
-// Sorts the block's slots (thread = slot, expert id or -1).  earlier[e] /
-// total[e]: slots of expert e in earlier blocks / all blocks; with one block
-// they are 0 and the block's own counts.
-__device__ void sort_block(const MoeRouteParams& p, SortShared& sh, int32_t id, int64_t slot, bool live, bool one) {
+// Sorts the block's slots (thread = slot, expert id or -1).
+template <bool ONE>
+__device__ void sort_block(const MoeRouteParams& p, SortShared& sh, int32_t id, int64_t slot, bool live) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int warps = blockDim.x >> 5, E = p.num_experts;
-  for (int i = tid; i < warps * E; i += blockDim.x) sh.count[i / E][i % E] = 0;
+  for (int w = warp; w < 32; w += warps)  // (all 32: the sums below are unrolled)
+    for (int e = lane; e < E; e += 32) sh.count[w][e] = 0;
+  if constexpr (!ONE) {
+    // The blocks' counts, a share of the blocks for every blockDim / E threads.
+    const int shares = blockDim.x / E, share = tid / E, e = tid - share * E;
+    int32_t all = 0, earlier = 0;
+    if (share < shares) {
+      const int blocks = gridDim.x, self = blockIdx.x;
+#pragma unroll 8
+      for (int b = share; b < blocks; b += shares) {
+        const int32_t n = p.counts[int64_t(b) * E + e];
+        all += n;
+        earlier += b < self ? n : 0;
+      }
+    }
+    sh.part[0][tid] = all;
+    sh.part[1][tid] = earlier;
+  }
   __syncthreads();
   const unsigned peers = __match_any_sync(0xffffffffu, id);
   const int rank = __popc(peers & ((1u << lane) - 1));
@@ -60,20 +80,19 @@ __device__ void sort_block(const MoeRouteParams& p, SortShared& sh, int32_t id, 
   // experts' totals are scanned over all threads (E <= blockDim).
   int32_t total = 0, earlier = 0;
   if (tid < E) {
-    int32_t run = 0;
-    for (int w = 0; w < warps; ++w) {
-      const int32_t n = sh.count[w][tid];
-      sh.count[w][tid] = uint16_t(run);
-      run += n;
+    uint16_t n[32];
+#pragma unroll
+    for (int w = 0; w < 32; ++w) n[w] = sh.count[w][tid];
+#pragma unroll
+    for (int w = 0; w < 32; ++w) {
+      sh.count[w][tid] = uint16_t(total);
+      total += n[w];
     }
-    if (one) {
-      total = run;
-    } else {
-      const int blocks = gridDim.x, self = blockIdx.x;
-      for (int b = 0; b < blocks; ++b) {
-        const int32_t n = p.counts[int64_t(b) * E + tid];
-        total += n;
-        earlier += b < self ? n : 0;
+    if constexpr (!ONE) {
+      total = 0;
+      for (int i = tid; i < int(blockDim.x) / E * E; i += E) {
+        total += sh.part[0][i];
+        earlier += sh.part[1][i];
       }
     }
   }
@@ -85,11 +104,16 @@ __device__ void sort_block(const MoeRouteParams& p, SortShared& sh, int32_t id, 
   }
   if (lane == 31) sh.scan[warp] = incl;
   __syncthreads();
-  int32_t before = 0, all = 0;
-  for (int w = 0; w < warps; ++w) {
-    before += w < warp ? sh.scan[w] : 0;
-    all += sh.scan[w];
+  // Every warp scans the warps' sums.
+  const int32_t mine = lane < warps ? sh.scan[lane] : 0;
+  int32_t sums = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int32_t v = __shfl_up_sync(0xffffffffu, sums, d);
+    if (lane >= d) sums += v;
   }
+  const int32_t all = __shfl_sync(0xffffffffu, sums, 31);
+  const int32_t before = __shfl_sync(0xffffffffu, sums - mine, warp);
   if (tid < E) {
     sh.base[tid] = before + incl - total + earlier;
     if (blockIdx.x == 0) {
@@ -109,59 +133,95 @@ __device__ void sort_block(const MoeRouteParams& p, SortShared& sh, int32_t id, 
   }
 }
 
-// Routes one token with the calling warp.
-template <int EPL>
-__device__ __forceinline__ void route_token(const MoeRouteParams& p, int64_t token, int lane) {
-  uint32_t o[EPL];
+// Routes N tokens (token + i * step, those below `end`) with the calling warp.
+// The choices also go to `ids` (the block's, from its first token on).
+template <int EPL, int N>
+__device__ __forceinline__ void route_tokens(const MoeRouteParams& p, int64_t token, int64_t step, int64_t end,
+                                             int lane, int16_t* ids, int64_t first) {
+  uint32_t o[N][EPL];  // sorted, largest first; equal ones by expert
+  uint8_t at[N][EPL];  // expert = lane + 32 at
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane + 32 * i;
-    o[i] = e < p.num_experts ? order_of(load_logit(p.logits, p.logits_type, token * p.logits_stride + e)) : 0u;
-  }
-  uint32_t top = 0;  // the row's maximum
-  float all = 0.f;   // softmax denominator over all experts
-  uint32_t mine_o = 0;
-  int32_t mine_e = -1;  // lane j keeps choice j
-  for (int j = 0; j < p.top_k; ++j) {
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const int e = lane + 32 * i;
+      at[n][i] = uint8_t(i);
+      o[n][i] = 0u;
+      if (token + n * step < end && e < p.num_experts)
+        o[n][i] = order_of(load_logit(p.logits, p.logits_type, (token + n * step) * p.logits_stride + e));
+    }
+  float all[N];  // softmax denominator over all experts
+  uint32_t top[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    all[n] = 0.f;
     uint32_t best = 0;
-    int at = 0;
 #pragma unroll
-    for (int i = EPL - 1; i >= 0; --i)
-      if (o[i] >= best) {
-        best = o[i];
-        at = i;
+    for (int i = 0; i < EPL; ++i) best = max(best, o[n][i]);
+    top[n] = __reduce_max_sync(0xffffffffu, best);
+    if (!p.renormalize && top[n] != 0) {
+      const float mv = value_of(top[n]);
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (o[n][i] != 0) all[n] += exp_below(value_of(o[n][i]), mv);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) all[n] += __shfl_xor_sync(0xffffffffu, all[n], d);
+    }
+    // Insertion sort; strict comparisons keep equal ones in order.
+#pragma unroll
+    for (int i = 1; i < EPL; ++i)
+#pragma unroll
+      for (int j = i; j > 0; --j)
+        if (o[n][j] > o[n][j - 1]) {
+          const uint32_t t = o[n][j];
+          o[n][j] = o[n][j - 1];
+          o[n][j - 1] = t;
+          const uint8_t u = at[n][j];
+          at[n][j] = at[n][j - 1];
+          at[n][j - 1] = u;
+        }
+  }
+  uint32_t mine_o[N];
+  int32_t mine_e[N];  // lane j keeps choice j
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    mine_o[n] = 0;
+    mine_e[n] = -1;
+  }
+  for (int j = 0; j < p.top_k; ++j) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const uint32_t m = __reduce_max_sync(0xffffffffu, o[n][0]);
+      const uint32_t own = o[n][0] == m ? uint32_t(lane) + 32u * at[n][0] : 0xffffffffu;
+      const uint32_t e = __reduce_min_sync(0xffffffffu, own);
+      if (lane == j && m != 0) {  // 0: nothing left to choose
+        mine_o[n] = m;
+        mine_e[n] = int32_t(e);
       }
-    const uint32_t m = __reduce_max_sync(0xffffffffu, best);
-    if (j == 0) {
-      top = m;
-      if (!p.renormalize && m != 0) {
-        const float mv = value_of(m);
+      if (own == e) {
 #pragma unroll
-        for (int i = 0; i < EPL; ++i)
-          if (o[i] != 0) all += exp_below(value_of(o[i]), mv);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+        for (int i = 0; i + 1 < EPL; ++i) {
+          o[n][i] = o[n][i + 1];
+          at[n][i] = at[n][i + 1];
+        }
+        o[n][EPL - 1] = 0;
       }
     }
-    if (m == 0) break;  // nothing left to choose
-    const uint32_t e = __reduce_min_sync(0xffffffffu, best == m ? uint32_t(lane + 32 * at) : 0xffffffffu);
-    if (lane == j) {
-      mine_o = m;
-      mine_e = int32_t(e);
+  }
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    float w = mine_e[n] >= 0 ? exp_below(value_of(mine_o[n]), value_of(top[n])) : 0.f;
+    if (p.renormalize) {
+      all[n] = w;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) all[n] += __shfl_xor_sync(0xffffffffu, all[n], d);
     }
-#pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (uint32_t(lane + 32 * i) == e) o[i] = 0;
-  }
-  float w = mine_e >= 0 ? exp_below(value_of(mine_o), value_of(top)) : 0.f;
-  if (p.renormalize) {
-    all = w;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
-  }
-  if (lane < p.top_k) {
-    p.weights[token * p.top_k + lane] = mine_e >= 0 ? w / all : 0.f;
-    p.experts[token * p.top_k + lane] = mine_e;
+    const int64_t t = token + n * step;
+    if (t < end && lane < p.top_k) {
+      p.weights[t * p.top_k + lane] = mine_e[n] >= 0 ? w / all[n] : 0.f;
+      p.experts[t * p.top_k + lane] = mine_e[n];
+      ids[(t - first) * p.top_k + lane] = int16_t(mine_e[n]);
+    }
   }
 }
 
@@ -174,15 +234,17 @@ __global__ void __launch_bounds__(kMoeSlotsOne) aspire_moe_route_kernel(MoeRoute
   const int64_t t0 = int64_t(blockIdx.x) * p.block_tokens;
   const int nt = int(min(int64_t(p.block_tokens), p.tokens - t0));
   if constexpr (EPL > 0) {
-    for (int t = warp; t < nt; t += blockDim.x >> 5) route_token<EPL>(p, t0 + t, lane);
-    __syncthreads();  // the block reads its own choices back
+    const int warps = blockDim.x >> 5;
+    constexpr int N = EPL <= 4 ? 2 : 1;
+    for (int t = warp; t < nt; t += N * warps) route_tokens<EPL, N>(p, t0 + t, warps, t0 + nt, lane, sh.ids, t0);
+    __syncthreads();
   }
   const bool live = tid < nt * p.top_k;
   const int64_t slot = t0 * p.top_k + tid;
-  int32_t id = live ? p.experts[slot] : -1;
+  int32_t id = live ? (EPL > 0 ? int32_t(sh.ids[tid]) : p.experts[slot]) : -1;
   if (id >= p.num_experts || id < 0) id = -1;
   if (gridDim.x == 1) {
-    sort_block(p, sh, id, slot, live, true);
+    sort_block<true>(p, sh, id, slot, live);
     return;
   }
   int32_t* count = sh.base;
@@ -205,7 +267,7 @@ __global__ void __launch_bounds__(kMoeSlotsBlock) aspire_moe_sort_kernel(MoeRout
   const int64_t slot = t0 * p.top_k + threadIdx.x;
   int32_t id = live ? p.experts[slot] : -1;
   if (id >= p.num_experts || id < 0) id = -1;
-  sort_block(p, sh, id, slot, live, false);
+  sort_block<false>(p, sh, id, slot, live);
 }
 
 MoeRouteKernel moe_route_kernel(int32_t num_experts) {
