@@ -47,7 +47,7 @@ int index_of(int v) { return v <= 1 ? 0 : (v == 2 ? 1 : 2); }
 
 // Launch with a programmatic dependency and, for cluster > 1, clusters along x.
 template <typename... KArgs, typename... Args>
-int w4_launch(void (*kernel)(KArgs...), dim3 grid, int cluster, int threads, size_t smem, cudaStream_t stream,
+int cluster_launch(void (*kernel)(KArgs...), dim3 grid, int cluster, int threads, size_t smem, cudaStream_t stream,
               const char* what, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
@@ -101,7 +101,7 @@ int w4_small(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
   rc = ensure_smem(reinterpret_cast<const void*>(kernel), smem,
                    g_w4_small[a->type == ASPIRE_T_BF16][tokens != 8][index_of(groups)][a->swiglu != 0]);
   if (rc) return rc;
-  return w4_launch(kernel, dim3(unsigned(cluster), unsigned(ny), unsigned(nz)), cluster, kW4SmallThreads, smem, stream,
+  return cluster_launch(kernel, dim3(unsigned(cluster), unsigned(ny), unsigned(nz)), cluster, kW4SmallThreads, smem, stream,
                    "aspire_w4_small_kernel launch", p);
 }
 
@@ -163,7 +163,7 @@ int w4_tc(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
                    g_w4_tc[a->type == ASPIRE_T_BF16][tokens == 32 ? 0 : (tokens == 64 ? 1 : 2)][index_of(groups)]
                           [a->swiglu != 0]);
   if (rc) return rc;
-  return w4_launch(kernel, dim3(unsigned(cluster), unsigned(ctas)), cluster, kW4TcThreads, smem, stream,
+  return cluster_launch(kernel, dim3(unsigned(cluster), unsigned(ctas)), cluster, kW4TcThreads, smem, stream,
                    "aspire_w4_tc_kernel launch", p, codes_map, x_map);
 }
 
@@ -171,11 +171,15 @@ int64_t elem_bytes(int32_t type) { return type == ASPIRE_T_F32 ? 4 : 2; }
 
 bool known_type(int32_t t) { return t == ASPIRE_T_F32 || t == ASPIRE_T_BF16 || t == ASPIRE_T_F16; }
 
-// Slots per block of the sort, and its blocks.
-void route_blocks(int64_t tokens, int32_t top_k, int64_t* block_tokens, int64_t* blocks) {
-  if (tokens * top_k <= kMoeSlotsOne) {
-    *block_tokens = tokens;
+// Tokens per block of the sort, its blocks, and whether they are one cluster.
+// A cluster takes a block per 8 tokens, so that its warps have one or two each
+// (72 tokens of 128 experts: 9.9 us in one block, 5.7 in eight).
+void route_blocks(int64_t tokens, int32_t top_k, int64_t* block_tokens, int64_t* blocks, bool* one) {
+  *one = tokens <= int64_t(kMoeCluster) * (kMoeSlotsOne / top_k);
+  if (*one) {
     *blocks = 1;
+    while (*blocks < kMoeCluster && *blocks * 8 < tokens) *blocks *= 2;
+    *block_tokens = (tokens + *blocks - 1) / *blocks;
   } else {
     *block_tokens = kMoeSlotsBlock / top_k;
     *blocks = (tokens + *block_tokens - 1) / *block_tokens;
@@ -300,8 +304,9 @@ int aspire_w4_linear(const AspireW4Args* a, void* stream) {
 size_t aspire_moe_route_workspace(int64_t tokens, int32_t num_experts, int32_t top_k) {
   if (tokens <= 0 || top_k <= 0 || top_k > kMoeMaxTopK || num_experts <= 0 || tokens > INT32_MAX / top_k) return 0;
   int64_t bt, nb;
-  route_blocks(tokens, top_k, &bt, &nb);
-  return nb > 1 ? size_t(nb) * size_t(num_experts) * sizeof(int32_t) : 0;
+  bool one;
+  route_blocks(tokens, top_k, &bt, &nb, &one);
+  return one ? 0 : size_t(nb) * size_t(num_experts) * sizeof(int32_t);
 }
 
 int aspire_moe_route(const AspireMoeRouteArgs* a, void* stream) {
@@ -322,8 +327,9 @@ int aspire_moe_route(const AspireMoeRouteArgs* a, void* stream) {
                         "aspire_moe_route memset");
     if (!a->experts || !a->position || !a->source || (a->logits && !a->weights)) return invalid(who, "null pointer");
     int64_t bt, nb;
-    route_blocks(a->tokens, a->top_k, &bt, &nb);
-    if (nb > 1 && (!a->workspace || a->workspace_bytes < aspire_moe_route_workspace(a->tokens, a->num_experts, a->top_k)))
+    bool one;
+    route_blocks(a->tokens, a->top_k, &bt, &nb, &one);
+    if (!one && (!a->workspace || a->workspace_bytes < aspire_moe_route_workspace(a->tokens, a->num_experts, a->top_k)))
       return set_error(ASPIRE_ERR_CAPACITY, "aspire_moe_route: workspace too small");
     MoeRouteParams p = {};
     p.logits = a->logits;
@@ -338,16 +344,17 @@ int aspire_moe_route(const AspireMoeRouteArgs* a, void* stream) {
     p.position = a->position;
     p.source = a->source;
     p.offsets = a->offsets;
-    p.counts = a->workspace;
+    p.counts = one ? nullptr : a->workspace;
     p.block_tokens = int32_t(bt);
-    int threads = kMoeSlotsBlock;
-    if (nb == 1) {  // a thread per slot and per expert, a warp per token
-      threads = std::max(ceil32(int(a->tokens * a->top_k)), ceil32(a->num_experts));
-      if (a->logits) threads = std::max(threads, 32 * int(std::min<int64_t>(a->tokens, 32)));
+    if (one) {  // a thread per slot and per expert, a warp per token
+      int threads = std::max(ceil32(int(bt * a->top_k)), ceil32(a->num_experts));
+      if (a->logits) threads = std::max(threads, 32 * int(std::min<int64_t>(bt, 32)));
+      return cluster_launch(moe_route_kernel(a->logits ? a->num_experts : 0), dim3(unsigned(nb)), int(nb), threads, 0,
+                            st, "aspire_moe_route_kernel launch", p);
     }
-    int rc = launch(moe_route_kernel(a->logits ? a->num_experts : 0), dim3(unsigned(nb)), dim3(unsigned(threads)), 0,
-                    st, "aspire_moe_route_kernel launch", p);
-    if (rc || nb == 1) return rc;
+    int rc = launch(moe_route_kernel(a->logits ? a->num_experts : 0), dim3(unsigned(nb)), dim3(kMoeSlotsBlock), 0, st,
+                    "aspire_moe_route_kernel launch", p);
+    if (rc) return rc;
     return launch(aspire_moe_sort_kernel, dim3(unsigned(nb)), dim3(kMoeSlotsBlock), 0, st,
                   "aspire_moe_sort_kernel launch", p);
   });

@@ -13,8 +13,9 @@ namespace aspire {
 
 constexpr int kMoeMaxExperts = 512;
 constexpr int kMoeMaxTopK = 32;
-// Slots of one sorting block.  One block of 1024 sorts everything when the
-// slots fit (a decode step: one launch); more slots go in blocks of 512.
+// One launch routes and sorts up to 8 x 1024 slots: a cluster of up to 8 blocks
+// of up to 1024.  More slots go in blocks of 512 and take two launches.
+constexpr int kMoeCluster = 8;
 constexpr int kMoeSlotsOne = 1024;
 constexpr int kMoeSlotsBlock = 512;
 
@@ -29,10 +30,11 @@ struct MoeRouteParams {
   int32_t* position;       // [tokens * top_k]
   int32_t* source;         // [tokens * top_k]
   int32_t* offsets;        // [num_experts + 1]
-  int32_t* counts;         // [blocks, num_experts] when there is more than one block
+  int32_t* counts;         // [blocks, num_experts] with two launches, else NULL
   int32_t block_tokens;    // tokens of a block
 };
-// Top-k and the block's expert counts; with one block also the sort.
+// Top-k and, with `counts`, the block's expert counts; without it the sort of
+// the one cluster's slots.
 using MoeRouteKernel = void (*)(MoeRouteParams);
 MoeRouteKernel moe_route_kernel(int32_t num_experts);
 // Sort of one block's slots, from every block's counts.

@@ -12,14 +12,20 @@
 // The sort counts: within a block of slots each warp ranks its 32 slots among
 // those of the same expert (a warp match), per-warp counts are summed over
 // the block's warps and the earlier blocks' counts, so the order is stable
-// and no atomic decides it.  One block sorts a decode step in the launch that
-// routes it; more tokens take a second launch after every block's counts are
-// known.  Both are bound by latency: the bytes are a few megabytes at most.
+// and no atomic decides it.  A cluster of up to 8 blocks routes a decode step
+// and sorts it in the same launch, its counts exchanged in distributed shared
+// memory; more than 8 x 1024 slots take a second launch after every block's
+// counts are known.  Both are bound by latency: the bytes are a few megabytes
+// at most.
+#include <cooperative_groups.h>
+
 #include "moe.cuh"
 
 namespace aspire {
 
 namespace {
+
+namespace cg = cooperative_groups;
 
 __device__ __forceinline__ float load_logit(const void* p, int32_t type, int64_t i) {
   if (type == ASPIRE_T_F32) return static_cast<const float*>(p)[i];
@@ -49,6 +55,7 @@ struct SortShared {
 };
 
 // Sorts the block's slots (thread = slot, expert id or -1).
+// ONE: the blocks are one cluster; otherwise their counts are in p.counts.
 template <bool ONE>
 __device__ void sort_block(const MoeRouteParams& p, SortShared& sh, int32_t id, int64_t slot, bool live) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -88,11 +95,33 @@ __device__ void sort_block(const MoeRouteParams& p, SortShared& sh, int32_t id, 
       sh.count[w][tid] = uint16_t(total);
       total += n[w];
     }
-    if constexpr (!ONE) {
+    if constexpr (ONE) {
+      sh.base[tid] = total;
+    } else {
       total = 0;
       for (int i = tid; i < int(blockDim.x) / E * E; i += E) {
         total += sh.part[0][i];
         earlier += sh.part[1][i];
+      }
+    }
+  }
+  if constexpr (ONE) {
+    const int blocks = gridDim.x;
+    if (blocks > 1) {
+      cg::cluster_group cluster = cg::this_cluster();
+      cluster.sync();
+      int32_t n[kMoeCluster] = {};
+      if (tid < E) {
+#pragma unroll
+        for (int b = 0; b < kMoeCluster; ++b)
+          if (b < blocks) n[b] = cluster.map_shared_rank(sh.base, b)[tid];
+      }
+      cluster.sync();  // before the totals make way for the bases
+      total = 0;
+#pragma unroll
+      for (int b = 0; b < kMoeCluster; ++b) {
+        total += n[b];
+        earlier += b < int(blockIdx.x) ? n[b] : 0;
       }
     }
   }
@@ -243,7 +272,7 @@ __global__ void __launch_bounds__(kMoeSlotsOne) aspire_moe_route_kernel(MoeRoute
   const int64_t slot = t0 * p.top_k + tid;
   int32_t id = live ? (EPL > 0 ? int32_t(sh.ids[tid]) : p.experts[slot]) : -1;
   if (id >= p.num_experts || id < 0) id = -1;
-  if (gridDim.x == 1) {
+  if (p.counts == nullptr) {
     sort_block<true>(p, sh, id, slot, live);
     return;
   }

@@ -24,7 +24,6 @@ import torch
 
 from . import _capi
 
-_SORT_ONE = 1024  # slots that one launch sorts; more need a workspace
 _TYPES = {torch.float32: _capi.T_F32, torch.bfloat16: _capi.T_BF16, torch.float16: _capi.T_F16}
 
 
@@ -53,9 +52,9 @@ def _run_route(logits, experts, num_experts, top_k, renormalize):
     source = torch.empty(tokens * top_k, **i32)
     offsets = torch.empty(num_experts + 1, **i32)
     ws, need = None, 0
-    if tokens * top_k > _SORT_ONE:
+    if tokens * top_k > 4096:  # fewer never need one
         need = _capi.load_library().aspire_moe_route_workspace(tokens, num_experts, top_k)
-        ws = torch.empty(need // 4, **i32)
+        ws = torch.empty(need // 4, **i32) if need else None
     _capi.call("aspire_moe_route", _capi.AspireMoeRouteArgs(
         None if logits is None else logits.data_ptr(), 0 if logits is None else _TYPES[logits.dtype],
         0 if logits is None else logits.stride(0), tokens, num_experts, top_k, renormalize,

@@ -625,7 +625,7 @@ typedef struct AspireMoeRouteArgs {
  * first; NaN and -inf are never chosen, and missing choices get expert -1 and
  * weight 0), their weights (softmax over all experts, or over the chosen ones
  * when renormalised) and the stable sort of the slots by expert.  One launch
- * up to 1024 slots, two beyond.  Expert ids outside [0, num_experts) count as
+ * up to about 8000 slots, two (and a workspace) beyond.  Expert ids outside [0, num_experts) count as
  * none.  Capturable.
  */
 ASPIRE_API int aspire_moe_route(const AspireMoeRouteArgs* args, void* stream);

@@ -99,9 +99,9 @@ def test_route_abi_refusals(built_library, bad):
 
 def test_route_workspace(built_library):
     need = built_library.aspire_moe_route_workspace
-    assert need(128, 64, 8) == 0 and need(0, 64, 8) == 0
-    assert need(129, 64, 8) == 3 * 64 * 4
-    a = _set(_capi.AspireMoeRouteArgs(), dict(logits=1 << 20, logits_stride=64, tokens=129, num_experts=64, top_k=8,
+    assert need(1024, 64, 8) == 0 and need(0, 64, 8) == 0
+    assert need(1025, 64, 8) == 17 * 64 * 4  # blocks of 512 slots
+    a = _set(_capi.AspireMoeRouteArgs(), dict(logits=1 << 20, logits_stride=64, tokens=1025, num_experts=64, top_k=8,
                                               weights=1 << 20, experts=1 << 20, position=1 << 20, source=1 << 20,
                                               offsets=1 << 20), {})
     assert built_library.aspire_moe_route(ctypes.byref(a), None) == _capi.ASPIRE_ERR_CAPACITY
