@@ -281,6 +281,7 @@ int aspire_w4_linear(const AspireW4Args* a, void* stream) {
     p.residual_stride = a->residual_stride;
     p.out = static_cast<uint16_t*>(a->out);
     p.out_stride = a->out_stride;
+    p.out_quads = ((reinterpret_cast<uintptr_t>(a->out) & 7) | uintptr_t(a->out_stride & 3) | uintptr_t(a->n & 3)) == 0;
     p.n = a->n;
     p.k = a->k;
     p.group_blocks = std::max(a->group / 128, 1);

@@ -32,6 +32,7 @@ struct W4Params {
   int64_t residual_stride;
   uint16_t* out;            // [rows, n]
   int64_t out_stride;
+  int32_t out_quads;        // every four neighbouring outputs of a token are 8-byte aligned, and n a multiple of 4
   int32_t n, k;
   int32_t group_blocks;     // groups of 128 m weights: m; else 1
   uint32_t group_recip;     // floor(2^32 / m) + 1, or 0 when m is 1
@@ -162,6 +163,10 @@ struct Num<true> {
   __device__ static __forceinline__ uint16_t from_float(float v) {
     return __bfloat16_as_ushort(__float2bfloat16_rn(v));
   }
+  __device__ static __forceinline__ uint32_t pack2(float lo, float hi) {
+    const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
   __device__ static __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t d;
     asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
@@ -189,6 +194,10 @@ struct Num<false> {
   static constexpr float kUnit = 1.0f;
   __device__ static __forceinline__ float to_float(uint16_t v) { return __half2float(__ushort_as_half(v)); }
   __device__ static __forceinline__ uint16_t from_float(float v) { return __half_as_ushort(__float2half_rn(v)); }
+  __device__ static __forceinline__ uint32_t pack2(float lo, float hi) {
+    const __half2 r = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
   __device__ static __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t d;
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));

@@ -26,8 +26,8 @@
 // reports it, lets its copies and MMAs land, frees TMEM and returns.
 //
 // The epilogue goes from TMEM to global memory: a lane holds one row, so a
-// warp's store is 32 neighbouring outputs of a token; gate and up sums of an
-// output are in the same lane.  Few tiles: a cluster splits K and adds the
+// warp's stores are 32 neighbouring outputs of four tokens; gate and up sums of
+// an output are in the same lane.  Few tiles: a cluster splits K and adds the
 // partials in distributed shared memory in rank order, as in the kernel for
 // few tokens.
 #include <cooperative_groups.h>
@@ -355,10 +355,30 @@ __global__ void __launch_bounds__(kW4TcThreads, 1)
             add[e] = res && live && e < left ? Num<BF16>::to_float(res[e * res_stride]) : 0.f;
 #pragma unroll
           for (int e = 0; e < AT_ONCE; ++e) {
-            float y = v[e] * Num<BF16>::kUnit;
-            if (SWIGLU) y = silu(y) * (u[e] * Num<BF16>::kUnit);
-            if (res) y += add[e];
-            if (live && e < left) out[e * out_stride] = Num<BF16>::from_float(y);
+            v[e] *= Num<BF16>::kUnit;
+            if (SWIGLU) v[e] = silu(v[e]) * (u[e] * Num<BF16>::kUnit);
+            if (res) v[e] += add[e];
+          }
+          if (p.out_quads) {
+            // Four lanes' rows of four tokens change places, so that a lane
+            // stores four rows of one token (8 bytes, a quarter of the stores).
+            const int quad = lane & 3;
+#pragma unroll
+            for (int e = 0; e < AT_ONCE; e += 4) {
+              const uint32_t t01 = Num<BF16>::pack2(v[e], v[e + 1]), t23 = Num<BF16>::pack2(v[e + 2], v[e + 3]);
+              const bool odd = quad & 1, high = quad & 2;
+              const uint32_t got = __shfl_xor_sync(0xffffffffu, __byte_perm(t01, t23, odd ? 0x5410 : 0x7632), 1);
+              const uint32_t ra = __byte_perm(t01, got, odd ? 0x3254 : 0x5410);  // token 0 or 1, two rows
+              const uint32_t rb = __byte_perm(t23, got, odd ? 0x3276 : 0x7610);  // token 2 or 3
+              const uint32_t other = __shfl_xor_sync(0xffffffffu, high ? ra : rb, 2);
+              if (live && e + quad < left)
+                *reinterpret_cast<uint2*>(out - quad + (e + quad) * out_stride) =
+                    high ? make_uint2(other, rb) : make_uint2(ra, other);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < AT_ONCE; ++e)
+              if (live && e < left) out[e * out_stride] = Num<BF16>::from_float(v[e]);
           }
         }
       }
