@@ -235,6 +235,8 @@ struct ScaleRow {
   const uint8_t* zero;  // NULL: 8
   bool live;
 
+  __device__ __forceinline__ ScaleRow(const uint16_t* scale_, const uint8_t* zero_, bool live_)
+      : scale(scale_), zero(zero_), live(live_) {}
   __device__ __forceinline__ ScaleRow(const W4Params& p, int expert, int64_t row, bool live_)
       : scale(p.scales + int64_t(expert) * p.scales_stride_e + row * p.scales_stride),
         zero(p.zeros ? p.zeros + int64_t(expert) * p.zeros_stride_e + row * p.zeros_stride : nullptr),

@@ -25,7 +25,8 @@
 // issue the halves' MMAs.  Every wait is bounded; after a timeout the CTA
 // reports it, lets its copies and MMAs land, frees TMEM and returns.
 //
-// The epilogue goes from TMEM to global memory: a lane holds one row, so a
+// The epilogue goes from TMEM by registers to global memory, while the MMAs of
+// the next tile's first steps (unpacked before it) run: a lane holds one row, so a
 // warp's stores are 32 neighbouring outputs of four tokens; gate and up sums of
 // an output are in the same lane.  Few tiles: a cluster splits K and adds the
 // partials in distributed shared memory in rank order, as in the kernel for
@@ -243,78 +244,91 @@ __global__ void __launch_bounds__(kW4TcThreads, 1)
     uint32_t row_at[4];                    // the warp's 16-byte chunks of a stage: block `parity` of 128 weights
 #pragma unroll
     for (int q = 0; q < 4; ++q) row_at[q] = half * kHalfCodes + r * 128 + (((parity * 4 + q) ^ (r & 7)) << 4);
-    int n = 0, tiles = 0;                  // stages and tiles so far
+    int n = 0, tiles = 0;                  // stages unpacked and tiles finished so far
     bool ok = true;
-    for (int i = first_tile; i < n_tiles && ok; i += tile_step) {
-      const Tile tile = tile_of(i);
+    // The tile being unpacked: its thread's output, and the block's scales,
+    // loaded a stage ahead.
+    int f = 0;
+    bool live = false;
+    ScaleRow<BF16, GROUPS> scales(nullptr, nullptr, false);
+    typename ScaleRow<BF16, GROUPS>::Raw nxt;
+    auto enter = [&](const Tile& tile, int i) {
       const int f0 = (i % row_tiles) * FEATURES;
-      if (tile.expert < 0) {
-        if (rank == 0)
-          for (int j = tid; j < tile.count * FEATURES; j += kUnpackWarps * 32) {
-            const int t = j / FEATURES, f = f0 + j % FEATURES;
-            if (f < p.n) p.out[int64_t(tile.row0 + t) * p.out_stride + f] = 0;
-          }
-        continue;
-      }
-      const int f = SWIGLU ? f0 + r : f0 + half * kRows + r;
-      const bool live = f < p.n;
-      const ScaleRow<BF16, GROUPS> scales(p, tile.expert, live ? (SWIGLU && half ? int64_t(p.n) + f : f) : 0, live);
-      // The block's scales, loaded a stage ahead.
-      typename ScaleRow<BF16, GROUPS>::Raw nxt = scales.load(p, s_begin * 2 + parity);
-      for (int s = 0; s < stages && ok; ++s) {
-        uint32_t sc[GROUPS];
+      f = SWIGLU ? f0 + r : f0 + half * kRows + r;
+      live = f < p.n;
+      scales = ScaleRow<BF16, GROUPS>(p, tile.expert, live ? (SWIGLU && half ? int64_t(p.n) + f : f) : 0, live);
+      nxt = scales.load(p, s_begin * 2 + parity);
+    };
+    auto unpack_stage = [&](int s) -> bool {
+      uint32_t sc[GROUPS];
 #pragma unroll
-        for (int e = 0; e < GROUPS; ++e) sc[e] = ScaleRow<BF16, GROUPS>::packed(nxt, e);
-        if (s + 1 < stages) nxt = scales.load(p, (s_begin + s + 1) * 2 + parity);
-        const int ws = (n + s) % SW;
-        ok = wait_bar(sm, sm.w_full[ws], ((n + s) / SW) & 1, p.status);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint8_t* const st = codes_s + ws * kCodeBytes;
-        const int j = (n + s) * kSteps + parity, as = j % SA;
-        uint32_t w[16];
+      for (int e = 0; e < GROUPS; ++e) sc[e] = ScaleRow<BF16, GROUPS>::packed(nxt, e);
+      if (s + 1 < stages) nxt = scales.load(p, (s_begin + s + 1) * 2 + parity);
+      const int ws = n % SW;
+      if (!__all_sync(0xffffffffu, wait_bar(sm, sm.w_full[ws], (n / SW) & 1, p.status))) return false;
+      const uint8_t* const st = codes_s + ws * kCodeBytes;
+      const int j = n * kSteps + parity, as = j % SA;
+      ++n;
+      uint32_t w[16];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(w + q * 4) = *reinterpret_cast<const uint4*>(st + row_at[q]);
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.w_empty[ws]));
+      for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(w + q * 4) = *reinterpret_cast<const uint4*>(st + row_at[q]);
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.w_empty[ws]));
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t a[32];
+      for (int h = 0; h < 2; ++h) {
+        uint32_t a[32];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const uint32_t ps = sc[(h * 8 + q) * GROUPS / 16], m = scale_pair(ps);
-            uint32_t z0, z1;
-            Num<BF16>::zero_consts(ps & 15u, z0, z1);
-            Num<BF16>::unpack(w[h * 8 + q], z0, z1, a + q * 4);
+        for (int q = 0; q < 8; ++q) {
+          const uint32_t ps = sc[(h * 8 + q) * GROUPS / 16], m = scale_pair(ps);
+          uint32_t z0, z1;
+          Num<BF16>::zero_consts(ps & 15u, z0, z1);
+          Num<BF16>::unpack(w[h * 8 + q], z0, z1, a + q * 4);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) a[q * 4 + e] = Num<BF16>::mul2(a[q * 4 + e], m);
-          }
-          if (h == 0) {
-            // The stage's previous step is through the tensor core, and with it
-            // its tokens.
-            ok = wait_bar(sm, sm.a_empty[as][half], ((j / SA) & 1) ^ 1, p.status);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            ptx::tc_fence_after();
-            if (j >= SA && (warp & 3) == 0 && lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.x_empty[(j - SA) % SX]));
-          }
-          ptx::tmem_st32(a_lanes + uint32_t(as) * 128 + h * 32, a);
+          for (int e = 0; e < 4; ++e) a[q * 4 + e] = Num<BF16>::mul2(a[q * 4 + e], m);
         }
-        if (!ok) break;
-        ptx::tmem_wait_st();
-        if ((warp & 3) == 0) {
-          ok = wait_bar(sm, sm.x_full[j % SX], (j / SX) & 1, p.status);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
+        if (h == 0) {
+          // The A stage's previous step is through the tensor core, and with it
+          // its tokens.
+          if (!__all_sync(0xffffffffu, wait_bar(sm, sm.a_empty[as][half], ((j / SA) & 1) ^ 1, p.status))) return false;
+          ptx::tc_fence_after();
+          if (j >= SA && (warp & 3) == 0 && lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.x_empty[(j - SA) % SX]));
         }
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.a_full[as][half]));
+        ptx::tmem_st32(a_lanes + uint32_t(as) * 128 + h * 32, a);
       }
-      n += stages;
+      ptx::tmem_wait_st();
+      if ((warp & 3) == 0 &&
+          !__all_sync(0xffffffffu, wait_bar(sm, sm.x_full[j % SX], (j / SX) & 1, p.status)))
+        return false;
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.a_full[as][half]));
+      return true;
+    };
+
+    int i = first_tile;
+    Tile tile{-1, 0, 0};
+    if (i < n_tiles) tile = tile_of(i);
+    int ahead = 0;  // stages of the tile that were unpacked before its turn
+    if (tile.expert >= 0) enter(tile, i);
+    while (i < n_tiles && tile.expert >= 0) {
+      for (int s = ahead; s < stages && ok; ++s) ok = unpack_stage(s);
+      // The next tile's first stage is unpacked before this one's epilogue, so
+      // that its MMAs start as soon as the sums have been read.
+      const Tile done = tile;
+      const int done_f = f;
+      const bool done_live = live;
+      i += tile_step;
+      ahead = 0;
+      if (i < n_tiles) {
+        tile = tile_of(i);
+        if (tile.expert >= 0 && ok) {
+          enter(tile, i);
+          ok = unpack_stage(0);
+          ahead = 1;
+        }
+      }
       // ---------------------------------------------------------- epilogue
-      if (ok) ok = wait_bar(sm, sm.d_full, tiles & 1, p.status);
-      ok = __all_sync(0xffffffffu, ok);
+      if (ok) ok = __all_sync(0xffffffffu, wait_bar(sm, sm.d_full, tiles & 1, p.status));
       if (!ok) break;
       ++tiles;
       ptx::tc_fence_after();
@@ -328,63 +342,78 @@ __global__ void __launch_bounds__(kW4TcThreads, 1)
 #pragma unroll
           for (int e = 0; e < 16; ++e) red[(c + e) * kRedPitch + half * kRows + r] = v[e] * Num<BF16>::kUnit;
         }
-      } else {
-        // Without the activation a warp writes its half's rows; with it, both
-        // halves' warps share the tokens and read gate and up sums.
-        constexpr int SHARE = SWIGLU ? TOKENS / 4 : TOKENS / 2;
-        constexpr int AT_ONCE = SHARE < 16 ? SHARE : 16;
-        const int c0 = SWIGLU ? (parity * 2 + half) * SHARE : parity * SHARE;
-#pragma unroll 1
-        for (int c = c0; c < c0 + SHARE; c += AT_ONCE) {
-          const int left = tile.count - c;
-          if (left <= 0) break;
-          float v[AT_ONCE], u[AT_ONCE];
-#pragma unroll
-          for (int e = 0; e < AT_ONCE; e += 8) {
-            ptx::tmem_ld8(lanes + (SWIGLU ? 0 : half * TOKENS) + uint32_t(c + e), v + e);
-            if (SWIGLU) ptx::tmem_ld8(lanes + TOKENS + uint32_t(c + e), u + e);
-          }
-          ptx::tmem_wait_ld();
-          const int64_t row = tile.row0 + c;
-          uint16_t* const out = p.out + row * p.out_stride + f;
-          const uint16_t* const res = p.residual ? p.residual + row * p.residual_stride + f : nullptr;
-          const int64_t out_stride = p.out_stride, res_stride = p.residual_stride;
-          float add[AT_ONCE];
-#pragma unroll
-          for (int e = 0; e < AT_ONCE; ++e)
-            add[e] = res && live && e < left ? Num<BF16>::to_float(res[e * res_stride]) : 0.f;
-#pragma unroll
-          for (int e = 0; e < AT_ONCE; ++e) {
-            v[e] *= Num<BF16>::kUnit;
-            if (SWIGLU) v[e] = silu(v[e]) * (u[e] * Num<BF16>::kUnit);
-            if (res) v[e] += add[e];
-          }
-          if (p.out_quads) {
-            // Four lanes' rows of four tokens change places, so that a lane
-            // stores four rows of one token (8 bytes, a quarter of the stores).
-            const int quad = lane & 3;
-#pragma unroll
-            for (int e = 0; e < AT_ONCE; e += 4) {
-              const uint32_t t01 = Num<BF16>::pack2(v[e], v[e + 1]), t23 = Num<BF16>::pack2(v[e + 2], v[e + 3]);
-              const bool odd = quad & 1, high = quad & 2;
-              const uint32_t got = __shfl_xor_sync(0xffffffffu, __byte_perm(t01, t23, odd ? 0x5410 : 0x7632), 1);
-              const uint32_t ra = __byte_perm(t01, got, odd ? 0x3254 : 0x5410);  // token 0 or 1, two rows
-              const uint32_t rb = __byte_perm(t23, got, odd ? 0x3276 : 0x7610);  // token 2 or 3
-              const uint32_t other = __shfl_xor_sync(0xffffffffu, high ? ra : rb, 2);
-              if (live && e + quad < left)
-                *reinterpret_cast<uint2*>(out - quad + (e + quad) * out_stride) =
-                    high ? make_uint2(other, rb) : make_uint2(ra, other);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < AT_ONCE; ++e)
-              if (live && e < left) out[e * out_stride] = Num<BF16>::from_float(v[e]);
-          }
-        }
+        continue;
       }
+      // Without the activation a warp writes its half's rows; with it, both
+      // halves' warps share the tokens and read gate and up sums.  All sums go
+      // to registers first: the next tile's MMAs run during the rest.
+      constexpr int SHARE = SWIGLU ? TOKENS / 4 : TOKENS / 2;
+      constexpr int AT_ONCE = SHARE < 16 ? SHARE : 16;
+      const int c0 = SWIGLU ? (parity * 2 + half) * SHARE : parity * SHARE;
+      float v[SHARE], u[SWIGLU ? SHARE : 1];
+#pragma unroll
+      for (int e = 0; e < SHARE; e += 8) {
+        ptx::tmem_ld8(lanes + (SWIGLU ? 0 : half * TOKENS) + uint32_t(c0 + e), v + e);
+        if constexpr (SWIGLU) ptx::tmem_ld8(lanes + TOKENS + uint32_t(c0 + e), u + e);
+      }
+      ptx::tmem_wait_ld();
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.d_empty));
+      const int64_t out_stride = p.out_stride, res_stride = p.residual_stride;
+#pragma unroll
+      for (int c = 0; c < SHARE; c += AT_ONCE) {
+        const int left = done.count - c0 - c;
+        if (left <= 0) break;
+        const int64_t row = done.row0 + c0 + c;
+        uint16_t* const out = p.out + row * out_stride + done_f;
+        if (p.residual) {
+          const uint16_t* const res = p.residual + row * res_stride + done_f;
+          uint16_t add[AT_ONCE];
+#pragma unroll
+          for (int e = 0; e < AT_ONCE; ++e) add[e] = done_live && e < left ? res[e * res_stride] : 0;
+#pragma unroll
+          for (int e = 0; e < AT_ONCE; ++e) v[c + e] = fmaf(v[c + e], Num<BF16>::kUnit, Num<BF16>::to_float(add[e]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < AT_ONCE; ++e) {
+            v[c + e] *= Num<BF16>::kUnit;
+            if constexpr (SWIGLU) v[c + e] = silu(v[c + e]) * (u[c + e] * Num<BF16>::kUnit);
+          }
+        }
+        if (p.out_quads) {
+          // Four lanes' rows of four tokens change places, so that a lane
+          // stores four rows of one token (8 bytes, a quarter of the stores).
+          const int quad = lane & 3;
+          const bool odd = quad & 1, high = quad & 2;
+          uint16_t* to = out - quad + quad * out_stride;
+#pragma unroll
+          for (int e = 0; e < AT_ONCE; e += 4, to += 4 * out_stride) {
+            const uint32_t t01 = Num<BF16>::pack2(v[c + e], v[c + e + 1]);
+            const uint32_t t23 = Num<BF16>::pack2(v[c + e + 2], v[c + e + 3]);
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, __byte_perm(t01, t23, odd ? 0x5410 : 0x7632), 1);
+            const uint32_t ra = __byte_perm(t01, got, odd ? 0x3254 : 0x5410);  // token 0 or 1, two rows
+            const uint32_t rb = __byte_perm(t23, got, odd ? 0x3276 : 0x7610);  // token 2 or 3
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, high ? ra : rb, 2);
+            if (done_live && e + quad < left)
+              *reinterpret_cast<uint2*>(to) = high ? make_uint2(other, rb) : make_uint2(ra, other);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < AT_ONCE; ++e)
+            if (done_live && e < left) out[e * out_stride] = Num<BF16>::from_float(v[c + e]);
+        }
+      }
+    }
+    // Rows of no expert: the last tiles.
+    for (; ok && i < n_tiles; i += tile_step) {
+      const Tile rest = tile_of(i);
+      const int f0 = (i % row_tiles) * FEATURES;
+      if (rest.expert >= 0 || rank != 0) continue;
+      for (int j = tid; j < rest.count * FEATURES; j += kUnpackWarps * 32) {
+        const int t = j / FEATURES, at = f0 + j % FEATURES;
+        if (at < p.n) p.out[int64_t(rest.row0 + t) * p.out_stride + at] = 0;
+      }
     }
   }
   ptx::tc_fence_before();
