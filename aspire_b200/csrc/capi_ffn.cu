@@ -4,6 +4,7 @@
 // entry point allocates device memory or synchronises, and none lets a C++
 // exception out.
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <string>
 
@@ -66,6 +67,70 @@ int cluster_launch(void (*kernel)(KArgs...), dim3 grid, int cluster, int threads
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), what);
 }
 
+// Clusters of 2, 4 and 8 CTAs that are resident at once (index log2 - 1), per
+// device; 0: not asked yet.  (A GPC's SMs are no multiple of 8: 15 clusters of
+// 8 CTAs with an SM each fit on 148 SMs, 33 of 4, 74 of 2.)
+struct ClusterCounts {
+  std::atomic<int> n[kMaxDevices][3];
+  ClusterCounts() {
+    for (auto& d : n)
+      for (auto& c : d) c.store(0);
+  }
+};
+
+template <typename Kernel>
+int cluster_count(Kernel kernel, int threads, size_t smem, int cluster, ClusterCounts& cache, int* out) {
+  int dev = 0;
+  int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+  if (rc) return rc;
+  const int at = cluster == 2 ? 0 : (cluster == 4 ? 1 : 2);
+  const bool cached = dev >= 0 && dev < kMaxDevices;
+  int n = cached ? cache.n[dev][at].load(std::memory_order_relaxed) : 0;
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(cluster));
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(cluster);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    rc = check_cuda(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg), "cudaOccupancyMaxActiveClusters");
+    if (rc) return rc;
+    if (cached) cache.n[dev][at].store(n, std::memory_order_relaxed);
+  }
+  *out = n;
+  return ASPIRE_OK;
+}
+
+ClusterCounts g_w4_small_clusters;
+
+// CTAs that split a tile's K: the size whose waves of tiles take the fewest
+// stages one after the other, a join of partials counted as `join` tenths of a
+// stage.  `slots`: CTAs resident at once without clusters.
+template <typename Kernel>
+int pick_cluster(Kernel kernel, int threads, size_t smem, int64_t tiles, int64_t stages, int64_t slots, int64_t join,
+                 ClusterCounts& cache, int* out) {
+  *out = 1;
+  if (2 * tiles > slots) return ASPIRE_OK;  // the rest would not hold a second wave
+  int64_t best = (tiles + slots - 1) / slots * stages * 10;
+  for (int c = 2; c <= 8 && c <= stages; c *= 2) {
+    int n = 0;
+    const int rc = cluster_count(kernel, threads, smem, c, cache, &n);
+    if (rc) return rc;
+    if (n <= 0) break;
+    const int64_t cost = (tiles + n - 1) / n * ((stages + c - 1) / c * 10 + join);
+    if (cost < best) {
+      best = cost;
+      *out = c;
+    }
+  }
+  return ASPIRE_OK;
+}
+
 // Upper bound of the token tiles of `rows` rows in `experts` ranges (0: one
 // range), the tail past the last range included.
 int64_t tiles_bound(int64_t rows, int32_t experts, bool grouped, int width) {
@@ -91,15 +156,15 @@ int w4_small(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
   int sms = 0;
   int rc = current_sm_count(&sms);
   if (rc) return rc;
-  // Split K over a cluster while the tiles leave half of the CTA slots (two
-  // per SM) empty and every rank has a stage of its own.
-  const int64_t stages = (a->k + 255) / 256;
-  int cluster = 1;
-  while (cluster < 8 && ny * nz * cluster * 2 <= 2 * sms && cluster * 2 <= stages) cluster *= 2;
   W4Kernel kernel = w4_small_kernel(a->type == ASPIRE_T_BF16, tokens, groups, a->swiglu != 0);
   const size_t smem = w4_small_smem(tokens, groups);
   rc = ensure_smem(reinterpret_cast<const void*>(kernel), smem,
                    g_w4_small[a->type == ASPIRE_T_BF16][tokens != 8][index_of(groups)][a->swiglu != 0]);
+  if (rc) return rc;
+  // Two CTAs per SM; a join takes about 1.5 us, a stage 0.6.
+  int cluster = 1;
+  rc = pick_cluster(kernel, kW4SmallThreads, smem, ny * nz, (a->k + 255) / 256, 2 * sms, 25, g_w4_small_clusters,
+                    &cluster);
   if (rc) return rc;
   return cluster_launch(kernel, dim3(unsigned(cluster), unsigned(ny), unsigned(nz)), cluster, kW4SmallThreads, smem, stream,
                    "aspire_w4_small_kernel launch", p);
@@ -120,6 +185,7 @@ int encode_map(CUtensorMap* map, CUtensorMapDataType type, int dims, const void*
 }
 
 SmemOptIn g_w4_tc[2][3][3][2];
+ClusterCounts g_w4_tc_clusters;
 
 int w4_tc(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
   const bool grouped = a->offsets != nullptr;
@@ -132,11 +198,16 @@ int w4_tc(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
   int sms = 0;
   int rc = current_sm_count(&sms);
   if (rc) return rc;
-  // One CTA per SM; K is split over a cluster while the tiles leave half of
-  // the SMs idle and every rank has a stage of its own.
-  const int64_t stages = (a->k + 255) / 256;
+  W4TcKernel kernel = w4_tc_kernel(a->type == ASPIRE_T_BF16, tokens, groups, a->swiglu != 0);
+  const size_t smem = w4_tc_smem(tokens);
+  rc = ensure_smem(reinterpret_cast<const void*>(kernel), smem,
+                   g_w4_tc[a->type == ASPIRE_T_BF16][tokens == 32 ? 0 : (tokens == 64 ? 1 : 2)][index_of(groups)]
+                          [a->swiglu != 0]);
+  if (rc) return rc;
+  // One CTA per SM; a join takes about 3 us, a stage 1.1.
   int cluster = 1;
-  while (cluster < 8 && tiles * cluster * 2 <= sms && cluster * 2 <= stages) cluster *= 2;
+  rc = pick_cluster(kernel, kW4TcThreads, smem, tiles, (a->k + 255) / 256, sms, 30, g_w4_tc_clusters, &cluster);
+  if (rc) return rc;
   const int64_t ctas = cluster > 1 ? tiles : std::min<int64_t>(tiles, sms);
   CUtensorMap codes_map, x_map;
   {
@@ -157,12 +228,6 @@ int w4_tc(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
                     a->x, size, strides, box);
     if (rc) return rc;
   }
-  W4TcKernel kernel = w4_tc_kernel(a->type == ASPIRE_T_BF16, tokens, groups, a->swiglu != 0);
-  const size_t smem = w4_tc_smem(tokens);
-  rc = ensure_smem(reinterpret_cast<const void*>(kernel), smem,
-                   g_w4_tc[a->type == ASPIRE_T_BF16][tokens == 32 ? 0 : (tokens == 64 ? 1 : 2)][index_of(groups)]
-                          [a->swiglu != 0]);
-  if (rc) return rc;
   return cluster_launch(kernel, dim3(unsigned(cluster), unsigned(ctas)), cluster, kW4TcThreads, smem, stream,
                    "aspire_w4_tc_kernel launch", p, codes_map, x_map);
 }

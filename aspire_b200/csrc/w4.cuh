@@ -45,6 +45,8 @@ struct W4Params {
   uint64_t wait_ns;         // bound of one pipeline wait (tcgen05 kernel)
 };
 
+constexpr int kW4MaxExperts = 1024;
+
 namespace w4 {
 
 constexpr int kRows = 128;  // matrix rows of a tile (of each half of one in the tcgen05 kernel)
@@ -56,83 +58,87 @@ struct Tile {
   int32_t expert, row0, count;
 };
 
-// A row range of the offsets, cut to [0, rows); one that leaves it or runs
-// backwards is reported.
-__device__ __forceinline__ void expert_range(const W4Params& p, int e, int& begin, int& count) {
-  const int lo = p.offsets[e], hi = p.offsets[e + 1];
+// A row range [lo, hi) cut to [0, rows); one that leaves it or runs backwards is
+// reported.
+__device__ __forceinline__ void cut_range(const W4Params& p, int lo, int hi, int& begin, int& count) {
   begin = min(max(lo, 0), p.rows);
   const int end = min(max(hi, begin), p.rows);
   if (lo != begin || hi != end) record_status(p.status, ASPIRE_STATUS_BAD_ROW);
   count = end - begin;
 }
 
-// For every expert its first row and its first token tile (tiles of `width`
-// rows, numbered in expert order) in first_row / first_tile [experts + 1]; the
-// last entries are the end of the last expert's rows and the number of tiles.
-// Run by one whole warp.
-__device__ __forceinline__ void expert_tiles(const W4Params& p, int width, int lane, int32_t* first_row,
-                                             int32_t* first_tile) {
+// For every expert its rows and its first token tile (tiles of `width` rows,
+// numbered in expert order); the last entries are the end of the last expert's
+// rows and the number of tiles.
+struct ExpertTiles {
+  int32_t begin[kW4MaxExperts + 1];
+  int32_t end[kW4MaxExperts + 1];
+  int32_t tile[kW4MaxExperts + 1];
+};
+
+// Fills them; run by one whole warp, whose loads for 128 experts are in flight
+// together.
+__device__ __forceinline__ void expert_tiles(const W4Params& p, int width, int lane, ExpertTiles& t) {
   int base = 0;
-  for (int e0 = 0; e0 < p.num_experts; e0 += 32) {
-    const int e = e0 + lane;
-    int begin = 0, count = 0;
-    if (e < p.num_experts) expert_range(p, e, begin, count);
-    const int mine = (count + width - 1) / width;
-    int incl = mine;
+  const int last = p.offsets[p.num_experts];
+  for (int e0 = 0; e0 < p.num_experts; e0 += 128) {
+    int lo[4], hi[4];
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += v;
+    for (int i = 0; i < 4; ++i) {
+      const int e = e0 + i * 32 + lane;
+      lo[i] = hi[i] = 0;
+      if (e < p.num_experts) {
+        lo[i] = p.offsets[e];
+        hi[i] = p.offsets[e + 1];
+      }
     }
-    if (e < p.num_experts) {
-      // With broken offsets ranges may overlap; a tile's rows end with its
-      // expert's range, which the next entry must not move.
-      first_row[e] = begin;
-      first_tile[e] = base + incl - mine;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = e0 + i * 32 + lane;
+      int begin, count;
+      cut_range(p, lo[i], hi[i], begin, count);
+      const int mine = (count + width - 1) / width;
+      int incl = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += v;
+      }
+      if (e < p.num_experts) {
+        t.begin[e] = begin;
+        t.end[e] = begin + count;
+        t.tile[e] = base + incl - mine;
+      }
+      base += __shfl_sync(0xffffffffu, incl, 31);
     }
-    base += __shfl_sync(0xffffffffu, incl, 31);
   }
   if (lane == 0) {
-    first_row[p.num_experts] = min(max(p.offsets[p.num_experts], 0), p.rows);
-    first_tile[p.num_experts] = base;
+    t.begin[p.num_experts] = min(max(last, 0), p.rows);
+    t.tile[p.num_experts] = base;
   }
 }
 
 // Number of token tiles, the rows past the last expert's included.
-__device__ __forceinline__ int token_tile_count(const W4Params& p, int width, const int32_t* first_row,
-                                                const int32_t* first_tile) {
+__device__ __forceinline__ int token_tile_count(const W4Params& p, int width, const ExpertTiles& t) {
   if (p.offsets == nullptr) return (p.rows + width - 1) / width;
-  return first_tile[p.num_experts] + (p.rows - first_row[p.num_experts] + width - 1) / width;
+  return t.tile[p.num_experts] + (p.rows - t.begin[p.num_experts] + width - 1) / width;
 }
 
-// Token tile `index` of expert_tiles' arrays.
-__device__ __forceinline__ Tile find_tile(const W4Params& p, int index, int width, const int32_t* first_row,
-                                          const int32_t* first_tile) {
-  Tile t;
-  if (p.offsets == nullptr) {
-    t.expert = 0;
-    t.row0 = index * width;
-    t.count = min(width, p.rows - t.row0);
-    return t;
-  }
+// Token tile `index`.
+__device__ __forceinline__ Tile find_tile(const W4Params& p, int index, int width, const ExpertTiles& t) {
+  if (p.offsets == nullptr) return Tile{0, index * width, min(width, p.rows - index * width)};
   const int E = p.num_experts;
-  if (index >= first_tile[E]) {
-    t.expert = -1;
-    t.row0 = first_row[E] + (index - first_tile[E]) * width;
-    t.count = min(width, p.rows - t.row0);
-    return t;
+  if (index >= t.tile[E]) {
+    const int row0 = t.begin[E] + (index - t.tile[E]) * width;
+    return Tile{-1, row0, min(width, p.rows - row0)};
   }
   int lo = 0, hi = E;  // the last expert whose first tile is at or before the index
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (first_tile[mid] <= index) lo = mid; else hi = mid;
+    if (t.tile[mid] <= index) lo = mid; else hi = mid;
   }
-  int begin, count;
-  expert_range(p, lo, begin, count);
-  t.expert = lo;
-  t.row0 = begin + (index - first_tile[lo]) * width;
-  t.count = min(width, begin + count - t.row0);
-  return t;
+  const int row0 = t.begin[lo] + (index - t.tile[lo]) * width;
+  return Tile{lo, row0, min(width, t.end[lo] - row0)};
 }
 
 // ------------------------------------------------------------------ numbers
@@ -362,7 +368,6 @@ W4Kernel w4_small_kernel(bool bf16, int tokens, int groups, bool swiglu);
 // the tokens as [rows, k] with boxes of 64 x tokens, both with the 128-byte
 // swizzle.
 constexpr int kW4TcThreads = 640;
-constexpr int kW4MaxExperts = 1024;
 size_t w4_tc_smem(int tokens);
 using W4TcKernel = void (*)(W4Params, CUtensorMap, CUtensorMap);
 W4TcKernel w4_tc_kernel(bool bf16, int tokens, int groups, bool swiglu);

@@ -66,6 +66,7 @@ __host__ __device__ constexpr int ring_bytes(int tokens, int groups) {
   const int red = tokens * kRedPitch * 4;  // the partials reuse the ring
   return ring > red ? ring : red;
 }
+static_assert(sizeof(ExpertTiles) <= ring_bytes(8, 1), "the experts' tiles use the ring before it starts");
 
 // Slot of a row's 16-byte chunk: chunk ^ this (f of row 0..7: 0 4 2 6 1 5 3 7).
 __device__ __forceinline__ int slot_mask(int row) { return ((row & 1) << 2) | (row & 2) | ((row >> 2) & 1); }
@@ -106,7 +107,9 @@ __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b
 // token tiles).
 template <bool BF16, int TOKENS, int GROUPS, bool SWIGLU>
 __global__ void __launch_bounds__(kW4SmallThreads, 2) aspire_w4_small_kernel(const __grid_constant__ W4Params p) {
-  pdl_begin();
+  // The next launch may start, and this one's addresses are worked out while the
+  // last one ends; nothing is read before pdl_wait.
+  pdl_launch_dependents();
   constexpr int NT = TOKENS / 8;
   constexpr int STAGES = stages_for(TOKENS, GROUPS);
   constexpr int WORDS = 4 / GROUPS;  // words of a group's part a lane loads
@@ -122,22 +125,22 @@ __global__ void __launch_bounds__(kW4SmallThreads, 2) aspire_w4_small_kernel(con
   const int f0 = blockIdx.y * FEATURES;
   if (warp == 0) {
     // (The ring's memory is free until the first copies.)
-    int32_t* const first_row = reinterpret_cast<int32_t*>(smem);
-    int32_t* const first_tile = first_row + kW4MaxExperts + 1;
+    ExpertTiles& tiles = *reinterpret_cast<ExpertTiles*>(smem);
     if (p.offsets != nullptr) {
-      expert_tiles(p, TOKENS, lane, first_row, first_tile);
+      pdl_wait();
+      expert_tiles(p, TOKENS, lane, tiles);
       __syncwarp();
     }
     if (lane == 0) {
       tile_s = Tile{0, 0, 0};
-      if (int(blockIdx.z) < token_tile_count(p, TOKENS, first_row, first_tile))
-        tile_s = find_tile(p, blockIdx.z, TOKENS, first_row, first_tile);
+      if (int(blockIdx.z) < token_tile_count(p, TOKENS, tiles)) tile_s = find_tile(p, blockIdx.z, TOKENS, tiles);
     }
   }
   __syncthreads();
   const Tile tile = tile_s;
   if (tile.count <= 0) return;  // the whole cluster: its CTAs share the tile
   if (tile.expert < 0) {
+    pdl_wait();
     if (rank == 0)
       for (int i = tid; i < tile.count * FEATURES; i += kW4SmallThreads) {
         const int t = i / FEATURES, f = f0 + i % FEATURES;
@@ -258,6 +261,7 @@ __global__ void __launch_bounds__(kW4SmallThreads, 2) aspire_w4_small_kernel(con
 
   const int wg = warp >> 2;             // half of the stage
   const int row_w = (warp & 3) * 32;    // the warp's 32 tile rows
+  pdl_wait();
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load_stage(s_begin, s, s);
 

@@ -56,8 +56,6 @@ constexpr int kRedPitch = kTileRows + 4;         // floats
 constexpr int kUnpackWarps = 16;
 constexpr int kXWarp = 16, kCodeWarp = 17, kMmaWarp = 18;  // and 19: the second half's
 constexpr uint32_t kTmemCols = 512;
-// Room for the experts' first rows and tiles.
-constexpr size_t kExpertBytes = 2 * 4 * (kW4MaxExperts + 1);
 
 template <int TOKENS>
 struct Shape {
@@ -72,7 +70,7 @@ struct Shape {
   static constexpr size_t kRed = size_t(TOKENS) * kRedPitch * 4;
   static_assert(kRed <= kRing, "the partials reuse the rings");
   static_assert(kAStages >= 2 && kAStages <= 3, "both parities of steps are in flight");
-  static constexpr size_t kBytes = kRing + kExpertBytes + 1024;  // 1 KiB to align the swizzled tiles
+  static constexpr size_t kBytes = kRing + sizeof(ExpertTiles) + 1024;  // 1 KiB to align the swizzled tiles
 };
 
 struct Control {
@@ -102,8 +100,7 @@ __global__ void __launch_bounds__(kW4TcThreads, 1)
   uint8_t* const codes_s = smem_raw + ((1024 - (ptx::smem_addr(smem_raw) & 1023)) & 1023);
   uint8_t* const x_s = codes_s + SW * kCodeBytes;
   float* const red = reinterpret_cast<float*>(codes_s);
-  int32_t* const expert_row = reinterpret_cast<int32_t*>(codes_s + S::kRing);
-  int32_t* const expert_tile = expert_row + kW4MaxExperts + 1;
+  ExpertTiles& experts = *reinterpret_cast<ExpertTiles*>(codes_s + S::kRing);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x, ranks = gridDim.x;
@@ -129,7 +126,7 @@ __global__ void __launch_bounds__(kW4TcThreads, 1)
       ptx::mbar_init(ptx::smem_addr(&sm.d_empty), kUnpackWarps);
       ptx::mbar_fence_init();
     }
-    if (p.offsets != nullptr) expert_tiles(p, TOKENS, lane, expert_row, expert_tile);
+    if (p.offsets != nullptr) expert_tiles(p, TOKENS, lane, experts);
   }
   if (warp == kMmaWarp) {
     ptx::tmem_alloc(ptx::smem_addr(&sm.tmem_base), kTmemCols);
@@ -140,12 +137,12 @@ __global__ void __launch_bounds__(kW4TcThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
   const int row_tiles = (p.n + FEATURES - 1) / FEATURES;
-  const int n_tiles = row_tiles * token_tile_count(p, TOKENS, expert_row, expert_tile);
+  const int n_tiles = row_tiles * token_tile_count(p, TOKENS, experts);
   const int n_stages = (p.k + kStageK - 1) / kStageK;
   const int s_begin = int(int64_t(n_stages) * rank / ranks), s_end = int(int64_t(n_stages) * (rank + 1) / ranks);
   const int stages = s_end - s_begin, steps = stages * kSteps;
   const int first_tile = blockIdx.y, tile_step = gridDim.y;
-  auto tile_of = [&](int i) { return find_tile(p, i / row_tiles, TOKENS, expert_row, expert_tile); };
+  auto tile_of = [&](int i) { return find_tile(p, i / row_tiles, TOKENS, experts); };
 
   if (warp == kCodeWarp) {
     if (lane == 0) {
