@@ -31,7 +31,14 @@ is in the one mixed forward.  The KV cache uses the engine's layout
 (``[pages, 2, 16, Hkv, 128]`` per layer, row r owning pages
 [r * pps, (r + 1) * pps)), page size 16.
 
-Everything outside the path (GEMMs, norms, SwiGLU, embedding, argmax,
+With ``weight_bits=4`` the model's products run on 4-bit weights
+(``aspire_b200.quant``), the gate and up products with their activation in one
+launch, and with ``n_expert`` the feed-forward layers route every token to
+``top_k`` experts (``aspire_b200.moe``): a draft or verify step reads the
+weights for a few tokens per row, so outside attention their bytes are its
+time.
+
+Everything else outside the path (GEMMs, norms, SwiGLU, embedding, argmax,
 NCCL all-reduces of the tensor-parallel model) is plain torch; the mixed
 forward of each step shape is replayed as one CUDA graph, as the reference
 runs it.  Under torch.distributed each rank holds its tensor-parallel shard
@@ -60,7 +67,9 @@ import torch.nn.functional as F
 
 from .attention import HolisticAttentionWrapper, first_last_dump_jit_args
 from .kv_ops import draft_page_spill, qkv_prologue
+from .moe import moe_combine, moe_dispatch, moe_route
 from .page_selector import PageSelectorFirstLastAvg
+from .quant import W4Weight, quantize_w4, w4_expert_linear, w4_expert_swiglu, w4_linear, w4_swiglu
 from .tp import tp_heads
 
 PAGE = 16
@@ -81,6 +90,8 @@ class ModelConfig:
     norm_eps: float = 1e-6
     rope_scale: float = 1.0
     llama31: Optional[tuple] = None  # (low_freq_factor, high_freq_factor, old_context_len)
+    n_expert: int = 0  # experts of a sparse feed-forward layer (0: dense); `intermediate` is one expert's
+    top_k: int = 0     # experts of a token
 
 
 PRESETS = {
@@ -105,9 +116,17 @@ def _dist():
 
 
 class DenseModel:
-    """Random-init decoder of a preset's shapes, holding this rank's shard."""
+    """Random-init decoder of a preset's shapes, holding this rank's shard.
+    ``weight_bits=4`` rounds every matrix but the embedding to 4 bits in groups
+    of ``group`` weights (the router of a sparse layer stays bf16); a sparse
+    model (``cfg.n_expert``) needs it."""
 
-    def __init__(self, cfg: ModelConfig, device: torch.device, *, seed: int = 0, n_layer: Optional[int] = None):
+    def __init__(self, cfg: ModelConfig, device: torch.device, *, seed: int = 0, n_layer: Optional[int] = None,
+                 weight_bits: int = 16, group: int = 128):
+        if weight_bits not in (4, 16):
+            raise ValueError("weight_bits must be 4 or 16")
+        if cfg.n_expert and weight_bits != 4:
+            raise ValueError("the experts' products run on 4-bit weights: give weight_bits=4")
         self.cfg = cfg
         self.device = device
         d = _dist()
@@ -133,7 +152,11 @@ class DenseModel:
 
         D, I, Hq, Hkv = cfg.dim, cfg.intermediate, cfg.n_head, cfg.n_kv_head
         self.emb = randn((cfg.vocab, D), 1)
-        self.w_out = randn((D, cfg.vocab), 2)[:, voc.start:voc.stop].contiguous()
+
+        def pack(w):  # [..., in, out], the layout of a bf16 product, or its 4-bit matrix
+            return w.contiguous() if weight_bits == 16 else quantize_w4(w.transpose(-1, -2), group)
+
+        self.w_out = pack(randn((D, cfg.vocab), 2)[:, voc.start:voc.stop])
         ones = lambda n: torch.ones(n, dtype=torch.bfloat16, device=device)  # noqa: E731
         self.final_norm = ones(D)
         self.layers = []
@@ -143,12 +166,14 @@ class DenseModel:
             wk = randn((D, Hkv * HEAD_DIM), s + 1)[:, kvcols]
             wv = randn((D, Hkv * HEAD_DIM), s + 2)[:, kvcols]
             wo = randn((Hq * HEAD_DIM, D), s + 3)[qcols, :]
-            w1 = randn((D, I), s + 4)[:, inter.start:inter.stop]
-            w3 = randn((D, I), s + 5)[:, inter.start:inter.stop]
-            w2 = randn((I, D), s + 6)[inter.start:inter.stop, :]
+            E = (cfg.n_expert,) if cfg.n_expert else ()
+            w1 = randn((*E, D, I), s + 4)[..., inter.start:inter.stop]
+            w3 = randn((*E, D, I), s + 5)[..., inter.start:inter.stop]
+            w2 = randn((*E, I, D), s + 6)[..., inter.start:inter.stop, :]
             self.layers.append(dict(
-                wqkv=torch.cat([wq, wk, wv], dim=1).contiguous(), wo=wo.contiguous(),
-                w13=torch.cat([w1, w3], dim=1).contiguous(), w2=w2.contiguous(),
+                wqkv=pack(torch.cat([wq, wk, wv], dim=1)), wo=pack(wo),
+                w13=pack(torch.cat([w1, w3], dim=-1)), w2=pack(w2),
+                router=randn((D, cfg.n_expert), s + 7) if cfg.n_expert else None,
                 attn_norm=ones(D), ffn_norm=ones(D),
                 q_norm=ones(HEAD_DIM) if cfg.qk_norm else None, k_norm=ones(HEAD_DIM) if cfg.qk_norm else None))
             del wq, wk, wv, wo, w1, w3, w2
@@ -159,6 +184,31 @@ class DenseModel:
             d.all_reduce(t)
         return t
 
+    @staticmethod
+    def _product(x: torch.Tensor, w, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x W (+ residual, in the product's epilogue)."""
+        if isinstance(w, W4Weight):
+            return w4_linear(x, w.codes, w.scales, w.zeros, residual=residual)
+        return x @ w if residual is None else torch.addmm(residual, x, w)
+
+    def _feed_forward(self, x: torch.Tensor, h: torch.Tensor, w: dict) -> torch.Tensor:
+        """x plus the layer's feed-forward output for the normalised h.  With
+        shards the partial products are summed before the residual is added."""
+        w13, w2 = w["w13"], w["w2"]
+        alone = self.world == 1
+        if self.cfg.n_expert:
+            weights, _, order = moe_route(h @ w["router"], self.cfg.top_k)
+            a = w4_expert_swiglu(moe_dispatch(h, order), order.offsets, w13.codes, w13.scales, w13.zeros)
+            y = w4_expert_linear(a, order.offsets, w2.codes, w2.scales, w2.zeros)
+            return moe_combine(y, weights, order, residual=x) if alone else x + self._all_reduce(
+                moe_combine(y, weights, order))
+        if isinstance(w13, W4Weight):
+            a = w4_swiglu(h, w13.codes, w13.scales, w13.zeros)
+        else:
+            gu = h @ w13
+            a = F.silu(gu[:, :self.inter_local]).mul_(gu[:, self.inter_local:])
+        return self._product(a, w2, x) if alone else x + self._all_reduce(self._product(a, w2))
+
     def forward(self, tokens: torch.Tensor, attn) -> torch.Tensor:
         """Hidden states after the final norm; `attn(layer, q, k, v)` returns
         the attention output [T, hq, 128] (and does the prologue / append)."""
@@ -168,25 +218,23 @@ class DenseModel:
         x = F.embedding(tokens, self.emb)
         for l, w in enumerate(self.layers):
             h = rms_norm(x, w["attn_norm"], cfg.norm_eps)
-            qkv = h @ w["wqkv"]
+            qkv = self._product(h, w["wqkv"])
             q = qkv[:, :hq * HEAD_DIM].view(T, hq, HEAD_DIM)
             k = qkv[:, hq * HEAD_DIM:(hq + hkv) * HEAD_DIM].view(T, hkv, HEAD_DIM)
             v = qkv[:, (hq + hkv) * HEAD_DIM:].view(T, hkv, HEAD_DIM)
             o = attn(l, q, k, v).reshape(T, hq * HEAD_DIM)
             # One GEMM with the residual add in its epilogue on one GPU; with
             # shards the partial products are summed first.
-            x = torch.addmm(x, o, w["wo"]) if self.world == 1 else x + self._all_reduce(o @ w["wo"])
-            h = rms_norm(x, w["ffn_norm"], cfg.norm_eps)
-            gu = h @ w["w13"]
-            a = F.silu(gu[:, :self.inter_local]).mul_(gu[:, self.inter_local:])
-            x = torch.addmm(x, a, w["w2"]) if self.world == 1 else x + self._all_reduce(a @ w["w2"])
+            x = (self._product(o, w["wo"], x) if self.world == 1
+                 else x + self._all_reduce(self._product(o, w["wo"])))
+            x = self._feed_forward(x, rms_norm(x, w["ffn_norm"], cfg.norm_eps), w)
         return rms_norm(x, self.final_norm, cfg.norm_eps)
 
     def greedy(self, x: torch.Tensor) -> torch.Tensor:
         """Greedy ids [T] over the whole vocabulary: a local max per rank,
         then the rank with the largest value (lowest rank on ties), as
         sparse_draft_transformer.py:268-281 merges the shards."""
-        logits = x @ self.w_out
+        logits = self._product(x, self.w_out)
         vals, ids = logits.max(dim=-1)
         ids = ids + self.vocab_start
         if self.world == 1:
@@ -204,7 +252,7 @@ class DenseModel:
     def token_logit_stats(self, x: torch.Tensor, emitted: torch.Tensor):
         """(top-1 id, top-1 logit, top-2 logit, logit of `emitted`) per row of
         x, over the whole vocabulary (fp32; shards merged by all-reduce)."""
-        logits = (x @ self.w_out).float()
+        logits = self._product(x, self.w_out).float()
         top = logits.topk(2, dim=-1)
         T = x.shape[0]
         vals = torch.zeros(T, self.world, 2, device=x.device)
