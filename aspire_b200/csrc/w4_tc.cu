@@ -269,8 +269,6 @@ __global__ void __launch_bounds__(kW4TcThreads, 1)
       uint32_t w[16];
 #pragma unroll
       for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(w + q * 4) = *reinterpret_cast<const uint4*>(st + row_at[q]);
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.w_empty[ws]));
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t a[32];
@@ -282,6 +280,12 @@ __global__ void __launch_bounds__(kW4TcThreads, 1)
           Num<BF16>::unpack(w[h * 8 + q], z0, z1, a + q * 4);
 #pragma unroll
           for (int e = 0; e < 4; ++e) a[q * 4 + e] = Num<BF16>::mul2(a[q * 4 + e], m);
+        }
+        if (h == 1) {
+          // The stage is released only now that every code has been used: an
+          // arrival does not wait for loads that are still on their way.
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.w_empty[ws]));
         }
         if (h == 0) {
           // The A stage's previous step is through the tensor core, and with it

@@ -180,3 +180,45 @@ def test_quantized_weights_through_the_product(cuda_device, symmetric):
     x = _x(4, 512, BF16, cuda_device, 6)
     ref, bound = product(x, w)
     check(quant.w4_linear(x, q.codes, q.scales, q.zeros), ref, bound)
+
+
+@pytest.mark.parametrize("rows,n,k,group,zeros,dtype,swiglu", [
+    (1500, 3000, 4096, 32, True, BF16, False),
+    (1500, 3000, 4096, 32, True, F16, False),
+    (700, 2048, 2048, 64, True, BF16, True),
+    (48, 12000, 4096, 128, False, BF16, True),
+    (16, 20000, 4096, 64, True, BF16, False),
+])
+def test_large_products_repeat_bit_by_bit(cuda_device, rows, n, k, group, zeros, dtype, swiglu):
+    """Many tiles per CTA in a row: a stage that is released or read a moment
+    too early shows in some of the runs."""
+    codes, scales, z, w = random_w4((2 * n if swiglu else n,), k, group, zeros, dtype, cuda_device, seed=n)
+    x = _x(rows, k, dtype, cuda_device, 3)
+    call = quant.w4_swiglu if swiglu else quant.w4_linear
+    first = call(x, codes, scales, z)
+    for _ in range(15):
+        assert torch.equal(call(x, codes, scales, z), first)
+    some = list(range(0, rows, max(1, rows // 40)))  # every tile of tokens
+    ref, bound = product(x[some], w, swiglu=swiglu, rows=rows)
+    check(first[some], ref, bound)
+
+
+@pytest.mark.parametrize("rows,n,k,expires", [(300, 2048, 1024, True), (40, 512, 4096, False)])
+def test_expired_waits_are_reported_and_leave_the_device_usable(cuda_device, built_library, rows, n, k, expires):
+    """With a wait limit of 1 ns the tcgen05 kernel stops at its first wait that
+    a poll finds unfinished: it reports a timeout, and the next call gives the
+    same result as before.  (In the second case, a cluster with few stages, a
+    poll may outlast every wait; then the result has to be right.)"""
+    codes, scales, z, w = random_w4((n,), k, 64, True, BF16, cuda_device, seed=2)
+    x = _x(rows, k, BF16, cuda_device, 3)
+    want = quant.w4_linear(x, codes, scales, z)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    built_library.aspire_set_wait_limit_ns(1)
+    try:
+        got = quant.w4_linear(x, codes, scales, z, status=status)
+        torch.cuda.synchronize()
+    finally:
+        built_library.aspire_set_wait_limit_ns(0)
+    timed_out = bool(int(status) & 8)
+    assert timed_out or (not expires and torch.equal(got, want))
+    assert torch.equal(quant.w4_linear(x, codes, scales, z), want)
