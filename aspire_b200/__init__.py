@@ -9,6 +9,10 @@ Public surface (drop-in for the reference's Python interfaces):
   ``torch.ops.aspire_b200.update_kv_padded`` - paged KV append.
 * ``aspire_b200.page_selector.PageSelectorFirstLastAvg`` - fused page
   scoring + top-k re-selection, optionally written in place.
+* ``aspire_b200.quant`` - products with 4-bit weights and group scales
+  (``w4_linear``, ``w4_swiglu`` and their per-expert forms).
+* ``aspire_b200.moe`` - router top-k with the sort of tokens by expert,
+  dispatch and combine, with gradients.
 
 All of it runs through libaspire_b200.so (C ABI in include/aspire_b200.h).
 There is no CPU fallback: a missing library or GPU raises.
