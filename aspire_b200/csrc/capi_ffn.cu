@@ -315,14 +315,14 @@ int aspire_w4_linear(const AspireW4Args* a, void* stream) {
     if (!a) return invalid(who, "null argument");
     if (a->type != ASPIRE_T_BF16 && a->type != ASPIRE_T_F16)
       return invalid(who, "type must be ASPIRE_T_BF16 or ASPIRE_T_F16");
-    if (a->rows < 0 || a->rows > INT32_MAX || a->n <= 0 || a->k <= 0) return invalid(who, "bad sizes");
+    if (a->rows < 0 || a->rows > INT32_MAX || a->n <= 0 || a->k <= 0 || a->n > (1 << 29) || a->k > (1 << 29))
+      return invalid(who, "bad sizes");
     if (a->group != 32 && a->group != 64 && (a->group <= 0 || a->group % 128))
       return invalid(who, "group must be 32, 64 or a multiple of 128");
     if (a->k % 32 || a->k % a->group) return invalid(who, "k must be a multiple of 32 and of group");
     if (a->offsets && a->experts <= 0) return invalid(who, "offsets need experts > 0");
     if (a->offsets && a->experts > kW4MaxExperts) return invalid(who, "at most 1024 experts are supported");
     if (a->swiglu && a->residual) return invalid(who, "the gated form takes no residual");
-    if (a->swiglu && a->n > INT32_MAX / 2) return invalid(who, "bad sizes");
     if (a->rows == 0) return ASPIRE_OK;
     if (!a->x || !a->codes || !a->scales || !a->out) return invalid(who, "null tensor pointer");
     const int64_t groups = a->k / a->group;

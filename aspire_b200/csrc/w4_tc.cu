@@ -31,6 +31,9 @@
 // an output are in the same lane.  Few tiles: a cluster splits K and adds the
 // partials in distributed shared memory in rank order, as in the kernel for
 // few tokens.
+//
+// 4099 tokens 4096 -> 12288, bf16, groups of 128: 356 us (1.17 PFLOP/s), bound by
+// the issue of the MMAs between waits; 64 tokens 4096 -> 2 x 12288: 31 us.
 #include <cooperative_groups.h>
 
 #include "tc_pipeline.cuh"

@@ -21,6 +21,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _capi
 
@@ -78,6 +79,7 @@ class _RouteWeights(torch.autograd.Function):
         return weights
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_weights):
         weights, experts, *rest = ctx.saved_tensors
         grad = torch.empty(ctx.shape, dtype=ctx.logits_dtype, device=weights.device)
@@ -216,6 +218,7 @@ class _Dispatch(torch.autograd.Function):
         return _run_dispatch(x, src, position, offsets, sizes, status)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         position, offsets = ctx.saved_tensors
         g, src = _grad_rows(grad)
@@ -231,6 +234,7 @@ class _Combine(torch.autograd.Function):
         return _run_combine(rows, src, weights, position, offsets, sizes, res, None, status)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         rows, weights, position, offsets = ctx.saved_tensors
         need_rows, need_weights, need_residual = ctx.needs_input_grad[:3]

@@ -132,6 +132,8 @@ def _product(x, codes, scales, zeros, residual, out, swiglu, offsets, status):
         out, os = torch.empty(rows, n, dtype=dtype, device=dev), n
     else:
         os = _check_output("out", out, dtype, rows, n, dev)
+        if rows and out.data_ptr() == x.data_ptr():
+            raise ValueError("out must not be x")
     if rows == 0 or n == 0:
         return out
     _capi.call("aspire_w4_linear", _capi.AspireW4Args(
