@@ -452,20 +452,30 @@ def check(rc: int, what: str) -> None:
     raise RuntimeError(f"{what} failed ({rc}): {msg}")
 
 
-def call(name: str, args: ctypes.Structure, device) -> None:
-    """Calls entry point ``name(args, stream)`` on the current stream of a CUDA
-    device, which is made current for the call."""
-    import torch
+_BOUND = ("aspire_last_error", "aspire_w4_linear", "aspire_moe_route", "aspire_moe_route_workspace",
+          "aspire_moe_route_grad", "aspire_moe_dispatch", "aspire_moe_combine", "aspire_moe_combine_grad")
+_ops = None
 
-    index = device.index
-    fn = getattr(load_library(), name)
-    if index == torch._C._cuda_getDevice():
-        rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
-    if rc != ASPIRE_OK:
-        check(rc, name)
+
+def ops():
+    """The compiled calls of the feed-forward operators (csrc/torch_binding.cpp),
+    on the entry points of the loaded library."""
+    global _ops
+    if _ops is None:
+        import torch
+
+        lib = load_library()
+        try:
+            from . import _torch_binding as binding
+        except ImportError as e:
+            raise RuntimeError(
+                "_torch_binding.so is missing or of another torch: build it with `python -m aspire_b200.build`") from e
+        if torch.__version__.split("+")[0] != binding.torch_version:
+            raise RuntimeError(
+                f"_torch_binding.so was built for torch {binding.torch_version}, not {torch.__version__}")
+        binding.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _BOUND))
+        _ops = binding
+    return _ops
 
 
 def status_offset() -> int:

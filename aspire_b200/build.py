@@ -1,7 +1,8 @@
-"""Builds libaspire_b200.so in-tree with nvcc for sm_100a.
+"""Builds libaspire_b200.so in-tree with nvcc for sm_100a, and _torch_binding.so
+(the feed-forward operators' Python calls) with the host compiler.
 
-Usage: ``python -m aspire_b200.build [--verbose-ptxas]``.  The library is
-written next to this file so that it travels with the source tree.
+Usage: ``python -m aspire_b200.build [--verbose-ptxas]``.  Both are written next
+to this file so that they travel with the source tree.
 """
 
 from __future__ import annotations
@@ -11,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -18,6 +20,8 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = PKG_DIR.parent / "include"
 LIB_NAME = "libaspire_b200.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+BINDING_PATH = PKG_DIR / "_torch_binding.so"
+BINDING_SOURCE = CSRC / "torch_binding.cpp"
 
 SOURCES = [
     "capi.cu",
@@ -59,16 +63,58 @@ def _inputs() -> list[Path]:
     return files
 
 
-def is_stale() -> bool:
-    if not LIB_PATH.exists():
+def _older(path: Path, inputs: list[Path]) -> bool:
+    if not path.exists():
         return True
-    lib_mtime = LIB_PATH.stat().st_mtime
-    return any(f.exists() and f.stat().st_mtime > lib_mtime for f in _inputs())
+    mtime = path.stat().st_mtime
+    return any(f.exists() and f.stat().st_mtime > mtime for f in inputs)
+
+
+def _binding_stale() -> bool:
+    return _older(BINDING_PATH, [BINDING_SOURCE, INCLUDE / "aspire_b200.h"])
+
+
+def is_stale() -> bool:
+    return _older(LIB_PATH, _inputs()) or _binding_stale()
+
+
+def _build_binding() -> None:
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    nvcc = Path(nvcc_path()).resolve()
+    includes = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+                Path(sysconfig.get_paths()["include"]), nvcc.parent.parent / "include"]
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    cmd = [
+        os.environ.get("CXX", "g++"),
+        "-O2",
+        "-std=c++17",
+        "-shared",
+        "-fPIC",
+        "-fvisibility=hidden",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        "-I",
+        str(INCLUDE),
+        *[a for i in includes for a in ("-isystem", str(i))],
+        "-o",
+        str(tmp),
+        str(BINDING_SOURCE),
+        f"-L{root / 'lib'}",
+        *["-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"],
+    ]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError("building _torch_binding.so failed:\n" + " ".join(cmd) + "\n" + proc.stdout + proc.stderr)
+    os.replace(tmp, BINDING_PATH)
 
 
 def build(verbose_ptxas: bool = False, force: bool = False) -> Path:
-    """Compiles every CUDA/C++ source of the library into one shared object."""
-    if not force and not is_stale():
+    """Compiles every CUDA/C++ source of the library into one shared object, and
+    the binding."""
+    if force or _binding_stale():
+        _build_binding()
+    if not force and not _older(LIB_PATH, _inputs()):
         return LIB_PATH
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [

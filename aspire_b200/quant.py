@@ -27,7 +27,7 @@ import torch
 
 from . import _capi
 
-_TYPES = {torch.bfloat16: _capi.T_BF16, torch.float16: _capi.T_F16}
+_TYPES = (torch.bfloat16, torch.float16)
 _NIBBLE = (0, 16, 4, 20, 8, 24, 12, 28)  # bit of each of a word's eight weights
 
 
@@ -89,86 +89,19 @@ def dequantize_w4(w: W4Weight) -> torch.Tensor:
     return ((q - z) * w.scales.float()[..., None]).flatten(-2)
 
 
-def _product(x, codes, scales, zeros, residual, out, swiglu, offsets, status):
-    # Every attribute is read once: a small call is bound by the host.
-    lead = 0 if offsets is None else 1
-    shape, cshape, sshape = x.shape, codes.shape, scales.shape
-    if len(shape) != 2 or len(cshape) != 2 + lead or len(sshape) != 2 + lead:
-        raise ValueError("x must be [rows, k] and codes / scales [n, ...], with a leading expert dimension for experts")
-    dtype, dev = x.dtype, x.device
-    kind = _TYPES.get(dtype)
-    if kind is None or scales.dtype != dtype:
-        raise ValueError("x and scales must both be bfloat16 or both float16")
-    if codes.dtype != torch.int32:
-        raise ValueError("codes must be int32")
-    if dev.type != "cuda" or codes.device != dev or scales.device != dev:
-        raise ValueError("x, codes and scales must be on one CUDA device")
-    rows, k = shape
-    r, groups = cshape[lead], sshape[-1]
-    if cshape[-1] * 8 != k:
-        raise ValueError("codes and x disagree on k")
-    if sshape[:-1] != cshape[:-1] or groups == 0 or k % groups:
-        raise ValueError("scales must be [..., n, k / group]")
-    group = k // groups
-    _check_group(k, group)
-    if swiglu and r % 2:
-        raise ValueError("the gated form needs as many gate as up rows")
-    n = r // 2 if swiglu else r
-    xs, cs, ss, zs = x.stride(), codes.stride(), scales.stride(), None
-    if (rows and xs[1] != 1) or cs[-1] != 1 or (groups > 1 and ss[-1] != 1):
-        raise ValueError("x, codes and scales need contiguous rows")
-    if zeros is not None:
-        if zeros.dtype != torch.uint8 or zeros.shape != sshape or zeros.device != dev:
-            raise ValueError("zeros must be uint8 of the scales' shape on their device")
-        zs = zeros.stride()
-        if groups > 1 and zs[-1] != 1:
-            raise ValueError("zeros need contiguous rows")
-    if offsets is not None and (offsets.dtype != torch.int32 or offsets.device != dev or not offsets.is_contiguous()
-                                or offsets.shape != (cshape[0] + 1,)):
-        raise ValueError("offsets must be contiguous int32 [experts + 1] on x's device")
-    if residual is not None:
-        rs = _check_output("residual", residual, dtype, rows, n, dev)
-    if out is None:
-        out, os = torch.empty(rows, n, dtype=dtype, device=dev), n
-    else:
-        os = _check_output("out", out, dtype, rows, n, dev)
-        if rows and out.data_ptr() == x.data_ptr():
-            raise ValueError("out must not be x")
-    if rows == 0 or n == 0:
-        return out
-    _capi.call("aspire_w4_linear", _capi.AspireW4Args(
-        x.data_ptr(), xs[0] if rows > 1 else k, rows,
-        codes.data_ptr(), cs[lead], cs[0] if lead else 0,
-        scales.data_ptr(), ss[lead], ss[0] if lead else 0,
-        None if zeros is None else zeros.data_ptr(), 0 if zs is None else zs[lead], zs[0] if zs and lead else 0,
-        None if residual is None else residual.data_ptr(), 0 if residual is None else rs,
-        out.data_ptr(), os, n, k, group, kind, swiglu,
-        None if offsets is None else offsets.data_ptr(), cshape[0] if lead else 0,
-        None if status is None else status.data_ptr()), dev)
-    return out
-
-
-def _check_output(name, t, dtype, rows, n, dev):
-    """The row stride of an output or residual."""
-    st = t.stride()
-    if t.dtype != dtype or t.shape != (rows, n) or t.device != dev or (n > 1 and rows and st[1] != 1):
-        raise ValueError(f"{name} must be [rows, n] of x's type with contiguous rows on x's device")
-    return st[0] if rows > 1 else n
-
-
 def w4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
               residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
               status: torch.Tensor | None = None) -> torch.Tensor:
     """``x [rows, k] @ W^T`` (``+ residual``) -> ``[rows, n]``, for one token up
     to a prefill chunk.  ``out`` may be ``residual`` itself."""
-    return _product(x, codes, scales, zeros, residual, out, False, None, status)
+    return _capi.ops().w4(x, codes, scales, zeros, residual, out, False, None, status)
 
 
 def w4_swiglu(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
               out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """``silu(x G^T) * (x U^T)`` -> ``[rows, n]`` with the matrix's rows
     ``[0, n)`` the gate's and ``[n, 2n)`` the up product's."""
-    return _product(x, codes, scales, zeros, None, out, True, None, status)
+    return _capi.ops().w4(x, codes, scales, zeros, None, out, True, None, status)
 
 
 def w4_expert_linear(x: torch.Tensor, offsets: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
@@ -178,7 +111,7 @@ def w4_expert_linear(x: torch.Tensor, offsets: torch.Tensor, codes: torch.Tensor
     ``offsets[e] .. offsets[e + 1]`` of ``x`` (sorted by expert, as
     :func:`aspire_b200.moe.moe_dispatch` leaves them) use matrix ``e``; rows
     past the last expert's give zero."""
-    return _product(x, codes, scales, zeros, None, out, False, offsets, status)
+    return _capi.ops().w4(x, codes, scales, zeros, None, out, False, offsets, status)
 
 
 def w4_expert_swiglu(x: torch.Tensor, offsets: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
@@ -186,4 +119,4 @@ def w4_expert_swiglu(x: torch.Tensor, offsets: torch.Tensor, codes: torch.Tensor
                      status: torch.Tensor | None = None) -> torch.Tensor:
     """The gated form of :func:`w4_expert_linear` (each expert's matrix holds
     its gate rows, then its up rows)."""
-    return _product(x, codes, scales, zeros, None, out, True, offsets, status)
+    return _capi.ops().w4(x, codes, scales, zeros, None, out, True, offsets, status)

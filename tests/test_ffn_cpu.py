@@ -6,7 +6,7 @@ import ctypes
 import pytest
 import torch
 
-from aspire_b200 import _capi, quant
+from aspire_b200 import _capi, moe, quant
 
 
 @pytest.mark.parametrize("symmetric", [True, False])
@@ -120,3 +120,12 @@ def test_permute_abi_refusals(built_library, bad):
         assert getattr(built_library, name)(ctypes.byref(a), None) == _capi.ASPIRE_ERR_INVALID
     a = _set(_capi.AspireMoePermuteArgs(), base, {})
     assert built_library.aspire_moe_combine_grad(ctypes.byref(a), None) == _capi.ASPIRE_ERR_INVALID  # no gradient
+
+
+def test_calls_refuse_what_is_not_a_tensor(built_library):
+    with pytest.raises(ValueError, match="tensor"):
+        quant.w4_linear([1.0], None, None)
+    with pytest.raises(ValueError, match="tensor"):
+        moe.moe_sort([[0, 1]], 2)
+    with pytest.raises(ValueError, match="integer"):
+        moe.moe_route(torch.zeros(2, 4), 1.5)

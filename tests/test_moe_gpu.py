@@ -284,3 +284,20 @@ def test_refusals(cuda_device):
     ):
         with pytest.raises(ValueError):
             call()
+
+
+def test_gradients_of_any_layout(cuda_device):
+    # Autograd hands over whatever the consumer made: broadcast, transposed, off a 16-byte boundary.
+    tokens, experts, top_k, width = 5, 4, 2, 64
+    order, _ = _order(tokens, experts, top_k, cuda_device, 3)
+    x = _randn(tokens, width, seed=1).to(cuda_device).requires_grad_()
+    rows = _randn(tokens * top_k, width, seed=2).to(cuda_device).requires_grad_()
+    weights = _randn(tokens, top_k, seed=3).to(cuda_device).requires_grad_()
+    for n, y, wrt in ((tokens * top_k, moe.moe_dispatch(x, order), (x,)),
+                      (tokens, moe.moe_combine(rows, weights, order), (rows, weights))):
+        off = torch.empty(n * width + 1, device=cuda_device)[1:].view(n, width)
+        off.copy_(_randn(n, width, seed=4))
+        for g in (off, _randn(width, n, seed=5).to(cuda_device).t(), torch.ones(1, 1, device=cuda_device).expand(n, width)):
+            got = torch.autograd.grad(y, wrt, g, retain_graph=True)
+            want = torch.autograd.grad(y, wrt, torch.empty(n, width, device=cuda_device).copy_(g), retain_graph=True)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
