@@ -209,8 +209,9 @@ __global__ void __launch_bounds__(kW4TcThreads, 1)
     bool ok = true;
     for (int i = first_tile; i < n_tiles && ok; i += tile_step) {
       if (tile_of(i).expert < 0) continue;
-      // The previous tile's sums have been read.
-      if (tiles > 0 && !wait_bar(sm, sm.d_empty, (tiles - 1) & 1, p.status)) ok = false;
+      // The previous tile's sums have been read.  (The warp decides as one: around
+      // a timeout some lanes may find the phase complete and others the abort.)
+      if (tiles > 0) ok = __all_sync(0xffffffffu, wait_bar(sm, sm.d_empty, (tiles - 1) & 1, p.status));
       for (int j = 0; j < steps && ok; ++j, ++n) {
         const int as = n % SA, xs = n % SX;
         // (Of a step whose tokens have arrived as well.)

@@ -1,0 +1,55 @@
+"""GPU tests of the tcgen05 products' bounded waits and of the hand-over of
+their stages."""
+
+import pytest
+import torch
+
+from aspire_b200 import quant
+from ffn_reference import random_w4
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def _x(rows, k, dtype, device, seed):
+    g = torch.Generator(device="cpu")
+    g.manual_seed(seed)
+    return torch.randn(rows, k, generator=g).to(dtype).to(device)
+
+
+@pytest.fixture
+def short_waits(built_library):
+    """Sets the limit of a wait in nanoseconds; the default comes back at the end."""
+    yield built_library.aspire_set_wait_limit_ns
+    built_library.aspire_set_wait_limit_ns(0)
+
+
+@pytest.mark.parametrize("limit", [1, 2000, 5000, 10000])
+@pytest.mark.parametrize("experts", [0, 16])
+def test_expired_waits_with_many_tiles_per_cta(cuda_device, short_waits, experts, limit):
+    """Each CTA has several tiles, so that the wait for the previous tile's sums
+    is among those that can expire, at different places by the limit.  Every
+    call ends; one that reports no timeout is right, and so is the next call
+    with the default limit."""
+    n, k, rows = 3000 if experts else 9000, 512, 2400
+    codes, scales, z, _ = random_w4((experts, n) if experts else (n,), k, 64, True, BF16, cuda_device, seed=limit)
+    x = _x(rows, k, BF16, cuda_device, 3)
+    offsets = (torch.arange(experts + 1) * (rows // max(experts, 1))).to(torch.int32).to(cuda_device)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+
+    def call():
+        if experts:
+            return quant.w4_expert_linear(x, offsets, codes, scales, z, status=status)
+        return quant.w4_linear(x, codes, scales, z, status=status)
+    want = call()
+    assert int(status) == 0
+    for _ in range(4):
+        status.zero_()
+        short_waits(limit)
+        got = call()
+        torch.cuda.synchronize()
+        short_waits(0)
+        assert int(status) == 8 or (int(status) == 0 and torch.equal(got, want))
+        status.zero_()
+        assert torch.equal(call(), want) and int(status) == 0
