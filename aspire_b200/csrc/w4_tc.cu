@@ -171,9 +171,9 @@ __global__ void __launch_bounds__(kW4TcThreads, 1)
                            tile.expert);
         }
       }
-      // After a timeout anywhere the copies in flight land before the CTA ends.
-      if (!ok || pipe::aborted(sm))
-        for (int j = max(0, n - SW); j < n; ++j) drain_bar(sm.w_full[j % SW], (j / SW) & 1);
+      // The last copies land before the CTA ends, whatever stops the other roles:
+      // a timeout may come after this warp has issued everything.
+      for (int j = max(0, n - SW); j < n; ++j) drain_bar(sm.w_full[j % SW], (j / SW) & 1);
     }
   } else if (warp == kXWarp) {
     if (lane == 0) {
@@ -197,8 +197,7 @@ __global__ void __launch_bounds__(kW4TcThreads, 1)
           ptx::tma_load_2d(dst + S::kBox, &x_map, bar, k + 64, tile.row0);
         }
       }
-      if (!ok || pipe::aborted(sm))
-        for (int j = max(0, n - SX); j < n; ++j) drain_bar(sm.x_full[j % SX], (j / SX) & 1);
+      for (int j = max(0, n - SX); j < n; ++j) drain_bar(sm.x_full[j % SX], (j / SX) & 1);
     }
   } else if (warp >= kMmaWarp) {
     constexpr uint32_t idesc =

@@ -53,3 +53,27 @@ def test_expired_waits_with_many_tiles_per_cta(cuda_device, short_waits, experts
         assert int(status) == 8 or (int(status) == 0 and torch.equal(got, want))
         status.zero_()
         assert torch.equal(call(), want) and int(status) == 0
+
+
+@pytest.mark.parametrize("rows,n,k", [(40, 512, 4096), (300, 256, 1024), (64, 1024, 512)])
+def test_expired_waits_leave_no_copy_behind(cuda_device, short_waits, rows, n, k):
+    """The producers of these calls (few stages per CTA, clusters) issue all their
+    copies without a wait, and another role stops the CTA after that.  The next
+    launches take the same shared memory at once: a copy that landed late would
+    change their results."""
+    codes, scales, z, _ = random_w4((n,), k, 64, True, BF16, cuda_device, seed=4)
+    x = _x(rows, k, BF16, cuda_device, 5)
+    other_codes, other_scales, other_z, _ = random_w4((1024,), 2048, 64, True, BF16, cuda_device, seed=6)
+    other_x = _x(96, 2048, BF16, cuda_device, 7)
+    want = quant.w4_linear(other_x, other_codes, other_scales, other_z)
+    mine = quant.w4_linear(x, codes, scales, z)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    for _ in range(25):
+        status.zero_()
+        short_waits(1)
+        got = quant.w4_linear(x, codes, scales, z, status=status)
+        short_waits(0)
+        after = [quant.w4_linear(other_x, other_codes, other_scales, other_z) for _ in range(2)]
+        assert int(status) == 8 or torch.equal(got, mine)
+        assert all(torch.equal(a, want) for a in after)
+    assert torch.equal(quant.w4_linear(x, codes, scales, z), mine)
