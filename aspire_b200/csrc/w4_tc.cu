@@ -284,12 +284,6 @@ __global__ void __launch_bounds__(kW4TcThreads, 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) a[q * 4 + e] = Num<BF16>::mul2(a[q * 4 + e], m);
         }
-        if (h == 1) {
-          // The stage is released only now that every code has been used: an
-          // arrival does not wait for loads that are still on their way.
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.w_empty[ws]));
-        }
         if (h == 0) {
           // The A stage's previous step is through the tensor core, and with it
           // its tokens.
@@ -299,6 +293,11 @@ __global__ void __launch_bounds__(kW4TcThreads, 1)
         }
         ptx::tmem_st32(a_lanes + uint32_t(as) * 128 + h * 32, a);
       }
+      // The stage is released only after the stores that take what was unpacked
+      // from its last codes: an arrival does not wait for loads that are still on
+      // their way, and only the stores (as volatile as the arrival) hold the order.
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&sm.w_empty[ws]));
       ptx::tmem_wait_st();
       if ((warp & 3) == 0 &&
           !__all_sync(0xffffffffu, wait_bar(sm, sm.x_full[j % SX], (j / SX) & 1, p.status)))

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from aspire_b200 import quant
-from ffn_reference import random_w4
+from ffn_reference import check, product, random_w4
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,29 @@ def test_expired_waits_leave_no_copy_behind(cuda_device, short_waits, rows, n, k
         assert int(status) == 8 or torch.equal(got, mine)
         assert all(torch.equal(a, want) for a in after)
     assert torch.equal(quant.w4_linear(x, codes, scales, z), mine)
+
+
+@pytest.mark.parametrize("rows", [32, 64, 300])
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_every_variant_repeats_bit_by_bit(cuda_device, rows, swiglu, group, dtype):
+    """All 36 forms of the kernel with two tiles and more per CTA: a stage that is
+    released before its codes have been read shows in some of the runs."""
+    R, k = 80000, 1024
+    g = torch.Generator(device=cuda_device)
+    g.manual_seed(group + rows)
+    codes = torch.randint(-2 ** 31, 2 ** 31, (R, k // 8), generator=g, device=cuda_device).to(torch.int32)
+    scales = ((torch.rand(R, k // group, generator=g, device=cuda_device) + 0.25) * 0.01).to(dtype)
+    z = torch.randint(0, 16, (R, k // group), generator=g, device=cuda_device).to(torch.uint8)
+    x = _x(rows, k, dtype, cuda_device, 3)
+    call = quant.w4_swiglu if swiglu else quant.w4_linear
+    first = call(x, codes, scales, z)
+    for _ in range(15):
+        assert torch.equal(call(x, codes, scales, z), first)
+    n = first.shape[1]
+    some = torch.arange(0, n, n // 300 + 1, device=cuda_device)  # features of every tile
+    pick = torch.cat([some, some + n]) if swiglu else some
+    w = quant.dequantize_w4(quant.W4Weight(codes[pick], scales[pick], z[pick])).double().cpu()
+    ref, bound = product(x, w, swiglu=swiglu)
+    check(first[:, some], ref, bound)
