@@ -18,6 +18,7 @@
 #include <utility>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -75,7 +76,10 @@ int type_of(const Tensor& t) {
 
 const Tensor& tensor(PyObject* o) {
   if (!THPVariable_Check(o)) throw Invalid("a tensor is required");
-  return THPVariable_Unpack(o);
+  const Tensor& t = THPVariable_Unpack(o);
+  // A tangent would be dropped, not carried through.
+  require(!t._fw_grad(0).defined(), "the feed-forward operators have no forward-mode derivative");
+  return t;
 }
 // NULL for None.
 const Tensor* optional(PyObject* o) { return o == Py_None ? nullptr : &tensor(o); }
@@ -107,6 +111,10 @@ int64_t output_stride(const Tensor& t, const Tensor& x, int64_t rows, int64_t n)
 Tensor w4(const Tensor& x, const Tensor& codes, const Tensor& scales, const Tensor* zeros, const Tensor* residual,
           const Tensor* out_given, bool swiglu, const Tensor* offsets, const Tensor* status) {
   const int lead = offsets ? 1 : 0;
+  // The result has no history, so a gradient would stop here without a word.
+  require(!at::GradMode::is_enabled() ||
+              !(x.requires_grad() || scales.requires_grad() || (residual && residual->requires_grad())),
+          "the 4-bit products have no gradient: detach the operands or call them under torch.no_grad()");
   require(x.dim() == 2 && codes.dim() == 2 + lead && scales.dim() == 2 + lead,
           "x must be [rows, k] and codes / scales [n, ...], with a leading expert dimension for experts");
   const int type = type_of(x);

@@ -15,8 +15,8 @@ A matrix ``[n, k]`` is three tensors (:class:`W4Weight`):
 
 Weight ``(r, j)`` is ``(q - zero) * scale``.  ``group`` is 32, 64 or a multiple
 of 128.  The experts of a sparse layer are one such matrix each, stacked in a
-leading dimension.  The weights are constants: no operator here has a
-gradient.
+leading dimension.  The products have no gradient, of the weights or of ``x``:
+with gradients enabled they refuse operands that require one.
 """
 
 from __future__ import annotations
