@@ -99,6 +99,54 @@ uint32_t* status_word(const Tensor* s, const Tensor& like) {
   return static_cast<uint32_t*>(s->data_ptr());
 }
 
+// ------------------------------------------------------------------- outputs
+// Rows of `bytes` bytes each, `pitch` (at least as many) bytes apart.
+struct Block {
+  uintptr_t at;
+  int64_t rows, bytes, pitch;
+};
+
+Block block_of(const Tensor& t, int64_t stride) {
+  const int64_t size = t.element_size();
+  return {reinterpret_cast<uintptr_t>(t.data_ptr()), t.size(0), t.size(1) * size, stride * size};
+}
+
+// Whether two blocks have a byte in common.  Blocks whose address ranges cross
+// may lie between one another's rows (columns of one buffer): their rows are
+// then compared in order of address.
+bool share(const Block& a, const Block& b) {
+  if (a.rows == 0 || b.rows == 0 || a.bytes == 0 || b.bytes == 0) return false;
+  const auto end = [](const Block& v) { return v.at + uintptr_t((v.rows - 1) * v.pitch + v.bytes); };
+  if (end(a) <= b.at || end(b) <= a.at) return false;
+  if (a.pitch < a.bytes || b.pitch < b.bytes) return true;
+  for (int64_t i = 0, j = 0; i < a.rows && j < b.rows;) {
+    const uintptr_t pa = a.at + uintptr_t(i * a.pitch), pb = b.at + uintptr_t(j * b.pitch);
+    if (pa + uintptr_t(a.bytes) <= pb)
+      ++i;
+    else if (pb + uintptr_t(b.bytes) <= pa)
+      ++j;
+    else
+      return true;
+  }
+  return false;
+}
+
+// A given output: apart from what is read, except the residual as a whole
+// (each of its elements is read before it is written, by the same thread or
+// warp).  Autograd learns of the write by the tensor's version.
+void check_out(const Tensor& out, int64_t stride, const Tensor& in, int64_t in_stride, const Tensor* residual,
+               int64_t res_stride) {
+  require(!(at::GradMode::is_enabled() && out.requires_grad()), "out requires a gradient: give another, or use torch.no_grad()");
+  const Block o = block_of(out, stride);
+  require(!share(o, block_of(in, in_stride)), "out must not overlap the operator's input");
+  if (residual) {
+    const Block r = block_of(*residual, res_stride);
+    require((r.at == o.at && (r.pitch == o.pitch || o.rows <= 1)) || !share(o, r),
+            "out may be the residual itself, but must not overlap it otherwise");
+  }
+  out.unsafeGetTensorImpl()->bump_version();
+}
+
 // ------------------------------------------------------------ 4-bit products
 // Row stride of an output or residual.
 int64_t output_stride(const Tensor& t, const Tensor& x, int64_t rows, int64_t n) {
@@ -147,7 +195,7 @@ Tensor w4(const Tensor& x, const Tensor& codes, const Tensor& scales, const Tens
   if (out_given) {
     out = *out_given;
     out_stride = output_stride(out, x, rows, n);
-    require(rows == 0 || out.data_ptr() != x.data_ptr(), "out must not be x");
+    check_out(out, out_stride, x, rows > 1 ? x.stride(0) : k, residual, res_stride);
   } else {
     out = at::empty({rows, n}, x.options());
   }
@@ -350,6 +398,7 @@ Tensor combine(const Tensor& rows, const Tensor* weights, const Order& o, const 
   if (residual) res = rows_of("residual", *residual, o.tokens, &rows);
   Tensor out = out_given ? *out_given : empty_rows(rows, o.tokens);
   const Rows to = out_given ? rows_of("out", out, o.tokens, &rows) : Rows{out.data_ptr(), rows.size(1)};
+  if (out_given) check_out(out, to.stride, rows, in.stride, residual, res.stride);
   if (o.tokens == 0) return out;
   AspireMoePermuteArgs a = o.args(rows, status);
   a.in = in.ptr;

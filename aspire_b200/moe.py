@@ -131,7 +131,8 @@ def moe_combine(rows: torch.Tensor, weights: torch.Tensor, order: ExpertOrder, *
                 status: torch.Tensor | None = None) -> torch.Tensor:
     """``y[t] = sum_j weights[t, j] * rows[order.position[t, j]]``
     (``+ residual[t]``), summed in fp32 (C ABI ``aspire_moe_combine``).  ``out``
-    may be ``residual`` itself; it takes no part in a gradient."""
+    may be ``residual`` itself, otherwise it must not overlap what the call reads;
+    it takes no part in a gradient."""
     if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad
                                     or (residual is not None and residual.requires_grad)):
         if out is not None:

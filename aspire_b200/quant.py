@@ -93,7 +93,8 @@ def w4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros:
               residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
               status: torch.Tensor | None = None) -> torch.Tensor:
     """``x [rows, k] @ W^T`` (``+ residual``) -> ``[rows, n]``, for one token up
-    to a prefill chunk.  ``out`` may be ``residual`` itself."""
+    to a prefill chunk.  ``out`` may be ``residual`` itself; otherwise it must not
+    overlap what the call reads."""
     return _capi.ops().w4(x, codes, scales, zeros, residual, out, False, None, status)
 
 

@@ -575,7 +575,8 @@ typedef struct AspireW4Args {
   int64_t zeros_stride, zeros_stride_e;
   const void* residual;      /* [rows, n] added to the product, or NULL                     */
   int64_t residual_stride;
-  void* out;                 /* [rows, n]                                                   */
+  void* out;                 /* [rows, n]; may be residual (same stride), else apart from   */
+                             /* everything read                                             */
   int64_t out_stride;
   int32_t n, k;              /* k a multiple of 32 and of group                             */
   int32_t group;             /* 32, 64 or a multiple of 128                                 */
@@ -657,7 +658,9 @@ typedef struct AspireMoePermuteArgs {
   int32_t num_experts, top_k;
   int64_t tokens;
   int32_t width;             /* a multiple of 16 bytes                                       */
-  void* out;                 /* dispatch and combine_grad: [tokens * top_k, width]           */
+  void* out;                 /* dispatch and combine_grad: [tokens * top_k, width], combine: */
+                             /* [tokens, width], may be residual (same stride); else apart   */
+                             /* from everything read                                         */
   int64_t out_stride;
   const void* grad;          /* combine_grad: [tokens, width] gradient of the outputs        */
   int64_t grad_stride;
