@@ -134,11 +134,12 @@ int pick_cluster(Kernel kernel, int threads, size_t smem, int64_t tiles, int64_t
   return ASPIRE_OK;
 }
 
-// Upper bound of the token tiles of `rows` rows in `experts` ranges (0: one
-// range), the tail past the last range included.
+// Upper bound of the token tiles of `rows` rows in `experts` ranges, those of the
+// rows before the first and past the last range included: a range of c rows has
+// at most 1 + (c - 1) / width, and there are no more ranges than rows.
 int64_t tiles_bound(int64_t rows, int32_t experts, bool grouped, int width) {
   if (!grouped) return (rows + width - 1) / width;
-  return std::min<int64_t>(rows, experts) + rows / width + 1;
+  return std::min<int64_t>(rows, int64_t(experts) + 2) + rows / width;
 }
 
 // Rows an ordinary tile has to hold: all of them, or an expert's average share.

@@ -69,7 +69,8 @@ __device__ __forceinline__ void cut_range(const W4Params& p, int lo, int hi, int
 
 // For every expert its rows and its first token tile (tiles of `width` rows,
 // numbered in expert order); the last entries are the end of the last expert's
-// rows and the number of tiles.
+// rows and the number of tiles.  The tiles of the rows of no expert, before the
+// first's and past the last's, follow.
 struct ExpertTiles {
   int32_t begin[kW4MaxExperts + 1];
   int32_t end[kW4MaxExperts + 1];
@@ -118,10 +119,11 @@ __device__ __forceinline__ void expert_tiles(const W4Params& p, int width, int l
   }
 }
 
-// Number of token tiles, the rows past the last expert's included.
+// Number of token tiles, those of the rows of no expert included.
 __device__ __forceinline__ int token_tile_count(const W4Params& p, int width, const ExpertTiles& t) {
   if (p.offsets == nullptr) return (p.rows + width - 1) / width;
-  return t.tile[p.num_experts] + (p.rows - t.begin[p.num_experts] + width - 1) / width;
+  return t.tile[p.num_experts] + (t.begin[0] + width - 1) / width +
+         (p.rows - t.begin[p.num_experts] + width - 1) / width;
 }
 
 // Token tile `index`.
@@ -129,7 +131,9 @@ __device__ __forceinline__ Tile find_tile(const W4Params& p, int index, int widt
   if (p.offsets == nullptr) return Tile{0, index * width, min(width, p.rows - index * width)};
   const int E = p.num_experts;
   if (index >= t.tile[E]) {
-    const int row0 = t.begin[E] + (index - t.tile[E]) * width;
+    const int first = t.begin[0], i = index - t.tile[E], before = (first + width - 1) / width;
+    if (i < before) return Tile{-1, i * width, min(width, first - i * width)};
+    const int row0 = t.begin[E] + (i - before) * width;
     return Tile{-1, row0, min(width, p.rows - row0)};
   }
   int lo = 0, hi = E;  // the last expert whose first tile is at or before the index

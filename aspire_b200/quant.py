@@ -111,7 +111,8 @@ def w4_expert_linear(x: torch.Tensor, offsets: torch.Tensor, codes: torch.Tensor
     """Every row's product with its expert's matrix: rows
     ``offsets[e] .. offsets[e + 1]`` of ``x`` (sorted by expert, as
     :func:`aspire_b200.moe.moe_dispatch` leaves them) use matrix ``e``; rows
-    past the last expert's give zero."""
+    before the first expert's and past the last one's give zero, so that the
+    offsets may be those of a share of the experts."""
     return _capi.ops().w4(x, codes, scales, zeros, None, out, False, offsets, status)
 
 

@@ -590,7 +590,7 @@ typedef struct AspireW4Args {
 /*
  * out[t] = x[t] W^T (+ residual[t]), or its gated form, in one launch; with
  * offsets, rows offsets[e] <= t < offsets[e + 1] use expert e's matrix and
- * rows past the last expert's become zero.  Sums are in fp32 and every output
+ * rows of no expert (before the first's or past the last's) become zero.  Sums are in fp32 and every output
  * is rounded once; with more than 16 rows (8 on average for experts) the weights
  * are rounded to x's type before the product.  Row ranges that run backwards or leave [0, rows) are
  * cut and set ASPIRE_STATUS_BAD_ROW.  Capturable; allocates nothing.  No

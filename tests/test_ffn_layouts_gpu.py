@@ -1,5 +1,6 @@
 """GPU tests of where the feed-forward operators' operands and outputs lie:
-outputs that overlap inputs, tensors' versions."""
+outputs that overlap inputs, tensors' versions, row ranges that do not begin at
+the first row."""
 
 import pytest
 import torch
@@ -83,3 +84,29 @@ def test_written_outputs_change_their_version(cuda_device):
             write(leaf)
         with torch.no_grad():
             write(leaf)
+
+
+# ---------------------------------------------------------------- row ranges
+@pytest.mark.parametrize("head,counts,tail", [
+    (1, [2, 0, 3], 0), (9, [1, 7, 0], 4), (40, [3], 0), (12, [0, 0], 0),                    # few rows per expert
+    (3, [60, 0, 20], 0), (200, [30, 1], 5), (131, [0, 140], 70), (290, [0], 0)])            # many
+@pytest.mark.parametrize("n,k,group,zeros,dtype,swiglu", [
+    (72, 288, 32, True, BF16, False), (296, 640, 128, False, BF16, True), (130, 2048, 64, True, F16, False)])
+def test_rows_before_the_first_expert_give_zero(cuda_device, head, counts, tail, n, k, group, zeros, dtype, swiglu):
+    """Offsets of a share of the experts, as a rank that holds only those has
+    them: the rows before belong to none of them, like the rows past the last."""
+    E, rows = len(counts), head + sum(counts) + tail
+    codes, scales, z, w = random_w4((E, 2 * n if swiglu else n), k, group, zeros, dtype, cuda_device, seed=E + n)
+    x = _randn(rows, k, dtype=dtype, device=cuda_device, seed=5)
+    offsets = (torch.tensor([0] + counts).cumsum(0) + head).to(torch.int32).to(cuda_device)
+    call = quant.w4_expert_swiglu if swiglu else quant.w4_expert_linear
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    y = call(x, offsets, codes, scales, z, out=torch.full((rows, n), float("nan"), dtype=dtype, device=cuda_device),
+             status=status)
+    assert bool((y[:head] == 0).all()) and bool((y[rows - tail:] == 0).all())
+    at = head
+    for e, c in enumerate(counts):
+        ref, bound = product(x[at:at + c], w[e], swiglu=swiglu, rows=rows if -(-rows // E) > 8 else 1)
+        check(y[at:at + c], ref, bound, f"expert {e}")
+        at += c
+    assert int(status) == 0
