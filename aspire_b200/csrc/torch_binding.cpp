@@ -206,12 +206,13 @@ Tensor w4(const Tensor& x, const Tensor& codes, const Tensor& scales, const Tens
   a.x_stride = rows > 1 ? x.stride(0) : k;
   a.rows = rows;
   a.codes = static_cast<const uint32_t*>(codes.data_ptr());
-  a.codes_stride = codes.stride(lead);
+  // (The stride of a dimension of size one says nothing.)
+  a.codes_stride = r > 1 ? codes.stride(lead) : k / 8;
   a.scales = scales.data_ptr();
-  a.scales_stride = scales.stride(lead);
+  a.scales_stride = r > 1 ? scales.stride(lead) : groups;
   if (zeros) {
     a.zeros = static_cast<const uint8_t*>(zeros->data_ptr());
-    a.zeros_stride = zeros->stride(lead);
+    a.zeros_stride = r > 1 ? zeros->stride(lead) : groups;
   }
   if (residual) {
     a.residual = residual->data_ptr();
@@ -227,9 +228,11 @@ Tensor w4(const Tensor& x, const Tensor& codes, const Tensor& scales, const Tens
   if (lead) {
     a.offsets = static_cast<const int32_t*>(offsets->data_ptr());
     a.experts = int32_t(codes.size(0));
-    a.codes_stride_e = codes.stride(0);
-    a.scales_stride_e = scales.stride(0);
-    if (zeros) a.zeros_stride_e = zeros->stride(0);
+    if (a.experts > 1) {
+      a.codes_stride_e = codes.stride(0);
+      a.scales_stride_e = scales.stride(0);
+      if (zeros) a.zeros_stride_e = zeros->stride(0);
+    }
   }
   a.status = status_word(status, x);
   on_device(x, [&](void* stream) { check(abi.w4_linear(&a, stream), "aspire_w4_linear"); });

@@ -1,6 +1,6 @@
 """GPU tests of where the feed-forward operators' operands and outputs lie:
 outputs that overlap inputs, tensors' versions, row ranges that do not begin at
-the first row."""
+the first row, strides of broadcast and of size-one dimensions."""
 
 import pytest
 import torch
@@ -110,3 +110,32 @@ def test_rows_before_the_first_expert_give_zero(cuda_device, head, counts, tail,
         check(y[at:at + c], ref, bound, f"expert {e}")
         at += c
     assert int(status) == 0
+
+
+# ------------------------------------------------------------------- strides
+@pytest.mark.parametrize("rows", [6, 100])
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_one_matrix_for_all_experts(cuda_device, rows, swiglu):
+    """An expert stride of 0, whatever the row count."""
+    E, n, k = 3, 96, 512
+    codes, scales, z, _ = random_w4((2 * n if swiglu else n,), k, 64, True, BF16, cuda_device, seed=1)
+    many = [t[None].expand(E, *t.shape) for t in (codes, scales, z)]
+    assert many[0].stride(0) == 0
+    x = _randn(rows, k, dtype=BF16, device=cuda_device, seed=2)
+    offsets = torch.tensor([0, rows // 3, rows // 2, rows], dtype=torch.int32, device=cuda_device)
+    call = quant.w4_expert_swiglu if swiglu else quant.w4_expert_linear
+    assert torch.equal(call(x, offsets, *many), call(x, offsets, *(t.contiguous() for t in many)))
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_strides_of_size_one_dimensions_do_not_matter(cuda_device, rows):
+    k, group = 256, 64
+    codes, scales, z, _ = random_w4((1,), k, group, True, BF16, cuda_device, seed=3)
+    x = _randn(rows, k, dtype=BF16, device=cuda_device, seed=4)
+    want = quant.w4_linear(x, codes, scales, z)
+    odd = [t.as_strided(t.shape, (3, 1)) for t in (codes, scales, z)]
+    assert torch.equal(quant.w4_linear(x, *odd), want)
+    offsets = torch.tensor([0, rows], dtype=torch.int32, device=cuda_device)
+    one = [t.as_strided((1, *t.shape), (1, 3, 1)) for t in (codes, scales, z)]
+    assert torch.equal(quant.w4_expert_linear(x, offsets, *one),
+                       quant.w4_expert_linear(x, offsets, codes[None], scales[None], z[None]))
