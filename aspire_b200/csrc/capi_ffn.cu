@@ -42,6 +42,7 @@ int ceil32(int v) { return (v + 31) / 32 * 32; }
 // experts 2048 -> 2 x 768: 90 and 117 us against 72 and 80; 4: 55 us).
 constexpr int64_t kW4SmallRows = 16;
 constexpr int64_t kW4SmallExpertRows = 8;
+constexpr int64_t kMaxTileTokens = 128;
 
 // Opt-in caches of the small kernel's variants: [type][tokens 8, 16]
 // [groups 1, 2, 4][swiglu].
@@ -198,7 +199,9 @@ int w4_tc(const AspireW4Args* a, const W4Params& p, cudaStream_t stream) {
   const int groups = a->group == 32 ? 4 : (a->group == 64 ? 2 : 1);
   const int features = a->swiglu ? w4::kRows : 2 * w4::kRows;
   const int64_t tiles = (int64_t(a->n) + features - 1) / features * tiles_bound(a->rows, a->experts, grouped, tokens);
-  if (tiles > INT32_MAX) return invalid("aspire_w4_linear", "n or rows too large");
+  // (The second: ranges that overlap, which the kernel reports, count more tiles.)
+  if (tiles > INT32_MAX || (grouped && a->experts * ((a->rows + tokens - 1) / tokens) > INT32_MAX))
+    return invalid("aspire_w4_linear", "n or rows too large");
   int sms = 0;
   int rc = current_sm_count(&sms);
   if (rc) return rc;
@@ -316,11 +319,14 @@ int aspire_w4_linear(const AspireW4Args* a, void* stream) {
     if (!a) return invalid(who, "null argument");
     if (a->type != ASPIRE_T_BF16 && a->type != ASPIRE_T_F16)
       return invalid(who, "type must be ASPIRE_T_BF16 or ASPIRE_T_F16");
-    if (a->rows < 0 || a->rows > INT32_MAX || a->n <= 0 || a->k <= 0 || a->n > (1 << 29) || a->k > (1 << 29))
+    // (Row counts are rounded up to tiles in 32 bits.)
+    if (a->rows < 0 || a->rows > INT32_MAX - kMaxTileTokens || a->n <= 0 || a->k <= 0 || a->n > (1 << 29) || a->k > (1 << 29))
       return invalid(who, "bad sizes");
     if (a->group != 32 && a->group != 64 && (a->group <= 0 || a->group % 128))
       return invalid(who, "group must be 32, 64 or a multiple of 128");
     if (a->k % 32 || a->k % a->group) return invalid(who, "k must be a multiple of 32 and of group");
+    // Up to here the group of a block is exact (group_recip).
+    if (int64_t(a->k / 128) * (a->group / 128) > int64_t(1) << 32) return invalid(who, "k times group past 2^46");
     if (a->offsets && a->experts <= 0) return invalid(who, "offsets need experts > 0");
     if (a->offsets && a->experts > kW4MaxExperts) return invalid(who, "at most 1024 experts are supported");
     if (a->swiglu && a->residual) return invalid(who, "the gated form takes no residual");

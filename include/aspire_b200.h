@@ -579,7 +579,7 @@ typedef struct AspireW4Args {
                              /* everything read                                             */
   int64_t out_stride;
   int32_t n, k;              /* k a multiple of 32 and of group                             */
-  int32_t group;             /* 32, 64 or a multiple of 128                                 */
+  int32_t group;             /* 32, 64 or a multiple of 128; k * group at most 2^46         */
   int32_t type;              /* ASPIRE_T_BF16 or ASPIRE_T_F16                               */
   int32_t swiglu;            /* 1: rows [0, n) gate, [n, 2n) up; out = silu(gate) * up      */
   const int32_t* offsets;    /* int32 [experts + 1]: expert e's rows of x; NULL: one matrix */
