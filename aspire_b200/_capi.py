@@ -462,17 +462,15 @@ def ops():
     on the entry points of the loaded library."""
     global _ops
     if _ops is None:
-        import torch
+        from . import build
 
         lib = load_library()
-        try:
-            from . import _torch_binding as binding
-        except ImportError as e:
-            raise RuntimeError(
-                "_torch_binding.so is missing or of another torch: build it with `python -m aspire_b200.build`") from e
-        if torch.__version__.split("+")[0] != binding.torch_version:
-            raise RuntimeError(
-                f"_torch_binding.so was built for torch {binding.torch_version}, not {torch.__version__}")
+        has, wants = build.binding_has(), build.binding_wants()
+        if has != wants:
+            raise RuntimeError(("_torch_binding.so is missing" if has is None else
+                                f"_torch_binding.so was built for {has}, and this is {wants}")
+                               + ": build it with `python -m aspire_b200.build`")
+        from . import _torch_binding as binding
         binding.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _BOUND))
         _ops = binding
     return _ops

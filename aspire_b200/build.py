@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import argparse
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -70,8 +71,25 @@ def _older(path: Path, inputs: list[Path]) -> bool:
     return any(f.exists() and f.stat().st_mtime > mtime for f in inputs)
 
 
+def binding_wants() -> str:
+    """What a binding built now is for: it works with no other torch or Python."""
+    import torch
+
+    return f"torch {torch.__version__}, {sys.implementation.cache_tag}"
+
+
+def binding_has(path: Path | None = None) -> str | None:
+    """What the built binding is for, read from the file (a module of another
+    Python cannot be asked); None without one."""
+    path = path or BINDING_PATH
+    if not path.exists():
+        return None
+    found = re.search(rb"aspire binding for \[([^\]]*)\]", path.read_bytes())
+    return found.group(1).decode() if found else None
+
+
 def _binding_stale() -> bool:
-    return _older(BINDING_PATH, [BINDING_SOURCE, INCLUDE / "aspire_b200.h"])
+    return _older(BINDING_PATH, [BINDING_SOURCE, INCLUDE / "aspire_b200.h"]) or binding_has() != binding_wants()
 
 
 def is_stale() -> bool:
@@ -94,6 +112,7 @@ def _build_binding() -> None:
         "-fPIC",
         "-fvisibility=hidden",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        f'-DASPIRE_BUILT_FOR="{binding_wants()}"',
         "-I",
         str(INCLUDE),
         *[a for i in includes for a in ("-isystem", str(i))],

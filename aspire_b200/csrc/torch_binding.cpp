@@ -22,7 +22,6 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
-#include <torch/version.h>
 
 #include "aspire_b200.h"
 
@@ -606,6 +605,7 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_binding", nullptr, -1, kMe
 
 PyMODINIT_FUNC PyInit__torch_binding(void) {
   PyObject* m = PyModule_Create(&kModule);
-  if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION) < 0) Py_CLEAR(m);
+  // The torch and the Python it was built for, as build.py finds them in the file.
+  if (m && PyModule_AddStringConstant(m, "built_for", "aspire binding for [" ASPIRE_BUILT_FOR "]") < 0) Py_CLEAR(m);
   return m;
 }
