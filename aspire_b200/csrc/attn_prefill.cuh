@@ -182,20 +182,20 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
     const bool active = h < nh;
     // (The second warp waits too: it releases the query buffer only after
     // this item's rows have landed.)
-    if (!wait_bar(sm, b.q_full, items_done & 1, p.status)) {
+    if (!wait_bar_warp(sm, b.q_full, items_done & 1, p.status)) {
       ok = false;
       break;
     }
     q_pending = false;
     // Scores of the first tile's two sub-tiles, once each S buffer is free
     // (the previous item's last PV on it has completed).
-    if (!wait_bar(sm, b.k_full[g % kKStages], (g / kKStages) & 1, p.status)) {
+    if (!wait_bar_warp(sm, b.k_full[g % kKStages], (g / kKStages) & 1, p.status)) {
       ok = false;
       break;
     }
     if (active) {
       for (int j = 0; j < 2 && ok; ++j) {
-        if (nth > 0 && !wait_bar(sm, b.pv_done[h][j], (nth - 1) & 1, p.status)) {
+        if (nth > 0 && !wait_bar_warp(sm, b.pv_done[h][j], (nth - 1) & 1, p.status)) {
           ok = false;
           break;
         }
@@ -209,7 +209,7 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
     for (int t = 0; t < nt && ok; ++t) {
       const uint32_t gt = g + uint32_t(t);
       const int vs = gt % kVStages;
-      if (!wait_bar(sm, b.v_full[vs], (gt / kVStages) & 1, p.status)) {
+      if (!wait_bar_warp(sm, b.v_full[vs], (gt / kVStages) & 1, p.status)) {
         ok = false;
         break;
       }
@@ -220,7 +220,7 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
         __syncwarp();
         if (tail && nh > 1 && lane == 0) ptx::mbar_arrive(ptx::smem_addr(&b.v_ready[vs]));
       } else if (tail && active) {
-        if (!wait_bar(sm, b.v_ready[vs], (vs ? ntail1 : ntail0) & 1, p.status)) {
+        if (!wait_bar_warp(sm, b.v_ready[vs], (vs ? ntail1 : ntail0) & 1, p.status)) {
           ok = false;
           break;
         }
@@ -231,11 +231,11 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
         for (int bj = 0; bj < 2 && ok; ++bj) {
           const int j = 2 * t + bj;
           // The item's first PV overwrites O_h: the previous item's epilogue has read it.
-          if (j == 0 && nit > 0 && !wait_bar(sm, b.o_free[h], (nit - 1) & 1, p.status)) {
+          if (j == 0 && nit > 0 && !wait_bar_warp(sm, b.o_free[h], (nit - 1) & 1, p.status)) {
             ok = false;
             break;
           }
-          if (!wait_bar(sm, b.p_full[h][bj], th & 1, p.status)) {
+          if (!wait_bar_warp(sm, b.p_full[h][bj], th & 1, p.status)) {
             ok = false;
             break;
           }
@@ -253,11 +253,11 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
           if (t + 1 < nt) {
             // Sub-tile j + 2 (tile t + 1) reuses S buffer bj once PV(j) has read P from it.
             const uint32_t gt2 = gt + 1;
-            if (bj == 0 && !wait_bar(sm, b.k_full[gt2 % kKStages], (gt2 / kKStages) & 1, p.status)) {
+            if (bj == 0 && !wait_bar_warp(sm, b.k_full[gt2 % kKStages], (gt2 / kKStages) & 1, p.status)) {
               ok = false;
               break;
             }
-            if (!wait_bar(sm, b.pv_done[h][bj], th & 1, p.status)) {
+            if (!wait_bar_warp(sm, b.pv_done[h][bj], th & 1, p.status)) {
               ok = false;
               break;
             }
@@ -273,7 +273,7 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
         // The second warp on a single-half item releases the slots unused.
         if (t + 1 < nt) {
           const uint32_t gt2 = gt + 1;
-          if (!wait_bar(sm, b.k_full[gt2 % kKStages], (gt2 / kKStages) & 1, p.status)) {
+          if (!wait_bar_warp(sm, b.k_full[gt2 % kKStages], (gt2 / kKStages) & 1, p.status)) {
             ok = false;
             break;
           }
@@ -296,7 +296,7 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
       break;
     }
     if (nxt >= 0 && leader) {
-      if (!wait_bar(sm, b.q_empty, items_done & 1, p.status)) {
+      if (!wait_bar_warp(sm, b.q_empty, items_done & 1, p.status)) {
         ok = false;
         break;
       }
@@ -393,7 +393,7 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
   for (int j = 0; j < nj; ++j) {
     const int bj = j & 1;
     const uint32_t th = gt + uint32_t(j >> 1);
-    if (!wait_bar(sm, b.s_full[h][bj], th & 1, p.status)) return false;
+    if (!wait_bar_warp(sm, b.s_full[h][bj], th & 1, p.status)) return false;
     ptx::tc_fence_after();
     const int sub0 = it.tok_begin + j * kSub;
     const uint32_t s_addr = tmem_lane + col_s(h, bj);
@@ -424,7 +424,7 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
       // Rescale this row of O_h once the previous sub-tile's PV has landed
       // (tcgen05.ld/st are warp-collective, hence the warp vote).
       const uint32_t tp = gt + uint32_t((j - 1) >> 1);
-      if (!wait_bar(sm, b.pv_done[h][bj ^ 1], tp & 1, p.status)) return false;
+      if (!wait_bar_warp(sm, b.pv_done[h][bj ^ 1], tp & 1, p.status)) return false;
       ptx::tc_fence_after();
 #pragma unroll 1
       for (int c = 0; c < kHeadDim; c += 16) {
@@ -459,7 +459,7 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
 
   // Final O_h row once the item's last PV (buffer 1 of its last tile, issued
   // after every other) has completed, 32 dims at a time; then O_h is free.
-  if (!wait_bar(sm, b.pv_done[h][1], (gt - 1) & 1, p.status)) return false;
+  if (!wait_bar_warp(sm, b.pv_done[h][1], (gt - 1) & 1, p.status)) return false;
   ptx::tc_fence_after();
   const float inv = l > 0.f ? 1.f / l : 0.f;
   const float lse = l > 0.f ? m_ref + lg2(l) : -INFINITY;
@@ -513,7 +513,7 @@ __device__ void consume_items(const AttnParams& p, Sh& sm, bool causal, int h, i
   const uint32_t tmem_lane = sm.tmem_base + (uint32_t(quarter * 32) << 16);
   uint32_t gt = 0;
   for (;;) {
-    if (aborted(sm)) return;
+    if (__any_sync(0xffffffffu, aborted(sm))) return;
     const int ii = seq_read(sm, k, lane, p.status);
     if (ii < 0) return;
     const WorkItem it = load_item(p.plan, ii);

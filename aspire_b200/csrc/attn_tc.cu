@@ -125,7 +125,7 @@ __device__ __forceinline__ bool group_sync(TcShared& sm, uint64_t& grp, uint32_t
   ptx::mbar_arrive(ptx::smem_addr(&grp));
   const uint32_t parity = uses & 1;
   ++uses;
-  return wait_bar(sm, grp, parity, status);
+  return wait_bar_warp(sm, grp, parity, status);
 }
 
 // ------------------------------------------------------------------ MMA issuers
@@ -162,15 +162,15 @@ __device__ void run_qk(const AttnParams& p, const CUtensorMap* qmap, TcShared& s
     const int nt = n_tiles_of(it);
     const uint32_t N = uint32_t(item_columns(it, use_cols));
     const uint32_t idesc_qk = ptx::idesc_bf16(128, N, false, false);
-    if (!wait_bar(sm, sm.q_full, items_done & 1, p.status)) {
+    if (!wait_bar_warp(sm, sm.q_full, items_done & 1, p.status)) {
       ok = false;
       break;
     }
     q_pending = false;
     for (int t = 0; t < nt && ok; ++t, ++g) {
       const int ks = g % kKStages, sb = g % 2;
-      if (!wait_bar(sm, sm.k_full[ks], (g / kKStages) & 1, p.status) ||
-          !wait_bar(sm, sm.s_empty[sb], ((g / 2) & 1) ^ 1, p.status)) {
+      if (!wait_bar_warp(sm, sm.k_full[ks], (g / kKStages) & 1, p.status) ||
+          !wait_bar_warp(sm, sm.s_empty[sb], ((g / 2) & 1) ^ 1, p.status)) {
         ok = false;
         break;
       }
@@ -197,7 +197,7 @@ __device__ void run_qk(const AttnParams& p, const CUtensorMap* qmap, TcShared& s
       break;
     }
     if (nxt >= 0) {
-      if (!wait_bar(sm, sm.q_empty, items_done & 1, p.status)) {
+      if (!wait_bar_warp(sm, sm.q_empty, items_done & 1, p.status)) {
         ok = false;
         break;
       }
@@ -233,14 +233,14 @@ __device__ void run_pv(const AttnParams& p, TcShared& sm, int lane, uint32_t& k,
     for (int t = 0; t < nt && ok; ++t, ++g) {
       const uint32_t vs = g % kVStages, pb = g % 2;
       // The item's first PV overwrites O: the previous item's epilogue has read it.
-      if ((t == 0 && !wait_bar(sm, sm.o_free, (items_done & 1) ^ 1, p.status)) ||
-          !wait_bar(sm, sm.v_full[vs], (g / kVStages) & 1, p.status)) {
+      if ((t == 0 && !wait_bar_warp(sm, sm.o_free, (items_done & 1) ^ 1, p.status)) ||
+          !wait_bar_warp(sm, sm.v_full[vs], (g / kVStages) & 1, p.status)) {
         ok = false;
         break;
       }
       clear_v_tail(sm.v[vs], it.tok_end - (it.tok_begin + t * kTile), lane);
       __syncwarp();
-      if (!wait_bar(sm, sm.p_full[pb], (g / 2) & 1, p.status)) {
+      if (!wait_bar_warp(sm, sm.p_full[pb], (g / 2) & 1, p.status)) {
         ok = false;
         break;
       }
@@ -431,7 +431,7 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
     const uint32_t gt = g0 + t;
     const int b = gt % 2;
     const uint32_t ph = (gt / 2) & 1;
-    if (!wait_bar(sm, sm.s_full[b], ph, p.status)) return false;
+    if (!wait_bar_warp(sm, sm.s_full[b], ph, p.status)) return false;
     ptx::tc_fence_after();
     const int tile0 = it.tok_begin + t * kTile;
     const int tok = tile0 + r;
@@ -528,7 +528,7 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
         // whose phases this thread waits on in order (so the parity test is
         // unambiguous).
         const uint32_t prev = gt - 1;
-        if (!wait_bar(sm, sm.p_empty[prev % 2], (prev / 2) & 1, p.status)) return false;
+        if (!wait_bar_warp(sm, sm.p_empty[prev % 2], (prev / 2) & 1, p.status)) return false;
         ptx::tc_fence_after();
         float ov[NH];
         tmem_load_cols<NH>(tmem_lane + kColO + c0, ov);
@@ -555,7 +555,7 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
       }
     }
     // P^T as bf16, MN-major without swizzle: 8 queries x 16 B per token, token-major.
-    if (!wait_bar(sm, sm.p_empty[b], ph ^ 1, p.status)) return false;
+    if (!wait_bar_warp(sm, sm.p_empty[b], ph ^ 1, p.status)) return false;
     uint8_t* pbuf = sm.p[b] + (c0 / 8) * (kTile * 16);
 #pragma unroll
     for (int c = 0; c < NH / 8; ++c) {
@@ -577,7 +577,7 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
 
   // Final O: wait for the item's last PV (on its P buffer's empty barrier),
   // read this lane (dim r) of the group's columns, free the accumulator.
-  if (!wait_bar(sm, sm.p_empty[(g - 1) % 2], ((g - 1) / 2) & 1, p.status)) return false;
+  if (!wait_bar_warp(sm, sm.p_empty[(g - 1) % 2], ((g - 1) / 2) & 1, p.status)) return false;
   ptx::tc_fence_after();
   float o_fin[NH];
   tmem_load_cols<NH>(tmem_lane + kColO + c0, o_fin);
@@ -658,7 +658,7 @@ __device__ void consume_items(const AttnParams& p, TcShared& sm, bool causal, in
   const int ctid = (warp - kFirstSoftmaxWarp - 4 * wg) * 32 + lane;  // 0..127 within the group
   uint32_t g = 0, grp_uses = 0;
   for (;;) {
-    if (aborted(sm)) return;
+    if (__any_sync(0xffffffffu, aborted(sm))) return;
     const int ii = seq_read(sm, k, lane, p.status);
     if (ii < 0) return;
     const WorkItem it = load_item(p.plan, ii);
@@ -809,7 +809,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
-    if (!aborted(sm)) {
+    if (!__any_sync(0xffffffffu, aborted(sm))) {
       if (warp == 0) {
         run_producer<pf::kKStages>(p, &tmap, sm, pbuf.k, sm.pf.k_full, sm.pf.k_empty, 0, true, pf_first, n_pf,
                                    kHdrPfClaim, kPfMaxRows, lane, k);

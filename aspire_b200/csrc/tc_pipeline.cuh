@@ -53,6 +53,14 @@ __device__ __forceinline__ bool wait_bar(Sh& sm, uint64_t& bar, uint32_t parity,
   return false;
 }
 
+// The same wait by a whole warp, decided as one: around a timeout some lanes may
+// find the phase complete and others the abort, and lanes that part here would
+// meet at different warp or CTA barriers, which no limit bounds.
+template <class Sh>
+__device__ __forceinline__ bool wait_bar_warp(Sh& sm, uint64_t& bar, uint32_t parity, uint32_t* status) {
+  return __all_sync(0xffffffffu, wait_bar(sm, bar, parity, status)) != 0;
+}
+
 // Wait used while draining after an abort: ignores the abort flag and keeps
 // the fixed 1 s bound whatever the launch's wait limit, so that copies and
 // MMAs already issued (which always complete) land before the CTA releases
@@ -213,7 +221,7 @@ __device__ bool run_producer(const AttnParams& p, const CUtensorMap* tmap, Sh& s
         append_new_tokens(p, it, kv_sel, lane);
         appended = true;
       }
-      if (!wait_bar(sm, empty[s], ph ^ 1, p.status)) {
+      if (!wait_bar_warp(sm, empty[s], ph ^ 1, p.status)) {
         ok = false;
         break;
       }
