@@ -245,14 +245,12 @@ __device__ bool run_producer(const AttnParams& p, const CUtensorMap* tmap, Sh& s
       __syncwarp();
     }
   }
-  if (!ok || aborted(sm)) {
-    // Let this CTA's own copies land before the CTA releases its shared memory.
+  // This CTA's own copies land before it releases its shared memory, whatever
+  // stops the other roles: a timeout may come after everything has been issued.
 #pragma unroll
-    for (int s = 0; s < STAGES; ++s)
-      if (last_issue[s] >= 0) drain_bar(full[s], uint32_t(last_issue[s] / STAGES) & 1);
-    return false;
-  }
-  return true;
+  for (int s = 0; s < STAGES; ++s)
+    if (last_issue[s] >= 0) drain_bar(full[s], uint32_t(last_issue[s] / STAGES) & 1);
+  return ok && !aborted(sm);
 }
 
 // A tile's tokens past the item's last one ([valid, 128)) that share a page

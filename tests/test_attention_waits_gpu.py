@@ -50,3 +50,33 @@ def test_waits_that_expire_at_different_places(cuda_device, built_library, kind)
             assert status == 0
             assert_attention_close(out, lse, ref_out, ref_lse)
     assert expired
+
+
+def test_expired_waits_leave_no_copy_behind(cuda_device, built_library):
+    """Short items, whose producers issue all their copies without a wait, stopped
+    by expired waits and followed at once by a launch on the same shared memory."""
+    dev = cuda_device
+    short = rows_layout([1, 3, 5] * 20, [200, 130, 250] * 20, 32, 8, seed=85)
+    other = make_layout(batch=16, ctx=4096, num_qo_heads=32, num_kv_heads=8, draft_fraction=0.5, budget_pages=64, seed=86)
+    run = []
+    for lay in (short, other):
+        q, kv = fill_tensors(lay, device=dev, seed=87)
+        w = HolisticAttentionWrapper(torch.empty(1, device=dev))
+        w.plan_host(torch.from_numpy(lay.qo_indptr), torch.from_numpy(lay.kv_indptr), torch.from_numpy(lay.kv_lens),
+                    torch.from_numpy(lay.kv_indices).to(dev), lay.num_qo_heads, lay.num_kv_heads, 128, 16, causal=True)
+        run.append((w, q, kv, lay))
+    (w, q, kv, _), (w2, q2, kv2, lay2) = run
+    ref_out, ref_lse, _ = oracle_attention(lay2, q2, kv2)
+    for _ in range(10):
+        _capi.check(built_library.aspire_set_wait_limit_ns(1), "aspire_set_wait_limit_ns")
+        try:
+            w.run(q, kv)
+        finally:
+            _capi.check(built_library.aspire_set_wait_limit_ns(0), "aspire_set_wait_limit_ns")
+        w2.clear_device_status()
+        w2.plan_host(torch.from_numpy(lay2.qo_indptr), torch.from_numpy(lay2.kv_indptr), torch.from_numpy(lay2.kv_lens),
+                     torch.from_numpy(lay2.kv_indices).to(dev), lay2.num_qo_heads, lay2.num_kv_heads, 128, 16, causal=True)
+        out, lse = w2.run(q2, kv2, return_lse=True)
+        torch.cuda.synchronize()
+        assert w2.device_status() == 0
+        assert_attention_close(out, lse, ref_out, ref_lse)
