@@ -138,9 +138,10 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
   uint32_t ntail0 = 0, ntail1 = 0;  // tail clears waited for, per V stage (warp 1)
   bool ok = true, q_pending = false;
 
-  // QK_h of sub-tile j of the item (its K tile in stage ks).
-  auto issue_qk = [&](int j, int ks) {
-    if (lane == 0) {
+  // QK_h of sub-tile j of the item (its K tile in stage ks).  The warp goes on or
+  // stops as one, by all lanes' `ready`.
+  auto issue_qk = [&](int j, int ks, bool ready) -> bool {
+    if (lane == 0 && ready) {
       const uint64_t kdesc0 = ptx::smem_desc(k0 + uint32_t(ks) * kSlotBytes + uint32_t(j & 1) * (kSub * 128), 16,
                                              1024, ptx::kLayoutSw128);
 #pragma unroll
@@ -151,7 +152,7 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
       }
       ptx::mma_commit(ptx::smem_addr(&b.s_full[h][j & 1]));
     }
-    __syncwarp();
+    return __all_sync(0xffffffffu, ready) != 0;
   };
   // This warp's release of K stage ks (and of the query rows after the item's
   // last tile): a commit after its MMAs, or a plain arrival.
@@ -195,12 +196,9 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
     }
     if (active) {
       for (int j = 0; j < 2 && ok; ++j) {
-        if (nth > 0 && !wait_bar_warp(sm, b.pv_done[h][j], (nth - 1) & 1, p.status)) {
-          ok = false;
-          break;
-        }
+        const bool ready = nth == 0 || wait_bar(sm, b.pv_done[h][j], (nth - 1) & 1, p.status);
         ptx::tc_fence_after();
-        issue_qk(j, g % kKStages);
+        ok = issue_qk(j, g % kKStages, ready);
       }
       if (!ok) break;
     }
@@ -209,21 +207,17 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
     for (int t = 0; t < nt && ok; ++t) {
       const uint32_t gt = g + uint32_t(t);
       const int vs = gt % kVStages;
-      if (!wait_bar_warp(sm, b.v_full[vs], (gt / kVStages) & 1, p.status)) {
-        ok = false;
-        break;
-      }
+      bool ready = wait_bar(sm, b.v_full[vs], (gt / kVStages) & 1, p.status);
       const int valid = it.tok_end - (it.tok_begin + t * kTile);
       const bool tail = valid < kTile && (valid & (kPageSize - 1)) != 0;
       if (leader) {
-        clear_v_tail(buf.v[vs], valid, lane);
-        __syncwarp();
+        if (ready) clear_v_tail(buf.v[vs], valid, lane);
+        // (Every lane's part of the tail is cleared before lane 0 goes on.)
+        ok = __all_sync(0xffffffffu, ready);
+        if (!ok) break;
         if (tail && nh > 1 && lane == 0) ptx::mbar_arrive(ptx::smem_addr(&b.v_ready[vs]));
       } else if (tail && active) {
-        if (!wait_bar_warp(sm, b.v_ready[vs], (vs ? ntail1 : ntail0) & 1, p.status)) {
-          ok = false;
-          break;
-        }
+        ready = ready && wait_bar(sm, b.v_ready[vs], (vs ? ntail1 : ntail0) & 1, p.status);
         if (vs) ++ntail1; else ++ntail0;
       }
       if (active) {
@@ -231,16 +225,10 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
         for (int bj = 0; bj < 2 && ok; ++bj) {
           const int j = 2 * t + bj;
           // The item's first PV overwrites O_h: the previous item's epilogue has read it.
-          if (j == 0 && nit > 0 && !wait_bar_warp(sm, b.o_free[h], (nit - 1) & 1, p.status)) {
-            ok = false;
-            break;
-          }
-          if (!wait_bar_warp(sm, b.p_full[h][bj], th & 1, p.status)) {
-            ok = false;
-            break;
-          }
+          if (j == 0 && nit > 0) ready = ready && wait_bar(sm, b.o_free[h], (nit - 1) & 1, p.status);
+          ready = ready && wait_bar(sm, b.p_full[h][bj], th & 1, p.status);
           ptx::tc_fence_after();
-          if (lane == 0) {
+          if (lane == 0 && ready) {
             const uint64_t vdesc0 = ptx::smem_desc(v0 + uint32_t(vs) * kSlotBytes + uint32_t(bj) * (kSub / 16) * 2048,
                                                    kHalfBytes, 1024, ptx::kLayoutSw128);
 #pragma unroll
@@ -249,20 +237,16 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
                                vdesc0 + uint64_t(kk * 2048 >> 4), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
             ptx::mma_commit(ptx::smem_addr(&b.pv_done[h][bj]));
           }
-          __syncwarp();
+          ok = __all_sync(0xffffffffu, ready);
+          if (!ok) break;
           if (t + 1 < nt) {
             // Sub-tile j + 2 (tile t + 1) reuses S buffer bj once PV(j) has read P from it.
             const uint32_t gt2 = gt + 1;
-            if (bj == 0 && !wait_bar_warp(sm, b.k_full[gt2 % kKStages], (gt2 / kKStages) & 1, p.status)) {
-              ok = false;
-              break;
-            }
-            if (!wait_bar_warp(sm, b.pv_done[h][bj], th & 1, p.status)) {
-              ok = false;
-              break;
-            }
+            if (bj == 0) ready = wait_bar(sm, b.k_full[gt2 % kKStages], (gt2 / kKStages) & 1, p.status);
+            ready = ready && wait_bar(sm, b.pv_done[h][bj], th & 1, p.status);
             ptx::tc_fence_after();
-            issue_qk(j + 2, gt2 % kKStages);
+            ok = issue_qk(j + 2, gt2 % kKStages, ready);
+            if (!ok) break;
             if (bj == 1) release_k(gt2 % kKStages, t + 1 == nt - 1, true);
           }
         }
@@ -271,6 +255,8 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
         __syncwarp();
       } else {
         // The second warp on a single-half item releases the slots unused.
+        ok = __all_sync(0xffffffffu, ready);
+        if (!ok) break;
         if (t + 1 < nt) {
           const uint32_t gt2 = gt + 1;
           if (!wait_bar_warp(sm, b.k_full[gt2 % kKStages], (gt2 / kKStages) & 1, p.status)) {
@@ -389,11 +375,15 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
   const uint32_t o_addr = tmem_lane + col_o(h);
   float m_ref = -INFINITY;  // reference row max x scale (log2 domain)
   float l = 0.f;
+  // A lane whose wait failed goes on with whatever is there until its warp's
+  // next vote, so that no lane leaves alone.  After a failure no output counts
+  // (ASPIRE_STATUS_TIMEOUT).
+  bool failed = false;
 
   for (int j = 0; j < nj; ++j) {
     const int bj = j & 1;
     const uint32_t th = gt + uint32_t(j >> 1);
-    if (!wait_bar_warp(sm, b.s_full[h][bj], th & 1, p.status)) return false;
+    failed |= !wait_bar(sm, b.s_full[h][bj], th & 1, p.status);
     ptx::tc_fence_after();
     const int sub0 = it.tok_begin + j * kSub;
     const uint32_t s_addr = tmem_lane + col_s(h, bj);
@@ -401,7 +391,7 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
     ptx::tmem_ld32(s_addr, s);
     ptx::tmem_ld32(s_addr + 32, s + 32);
     ptx::tmem_wait_ld();
-    if (warp_dumps && dump_at >= 0) {
+    if (warp_dumps && dump_at >= 0 && !failed) {
 #pragma unroll
       for (int c = 0; c < kSub; ++c)
         if (sub0 + c < dump_end) dump_store(p, dump_at + sub0 + c, s[c]);
@@ -420,7 +410,8 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
       l *= alpha;
       m_ref = ms;
     }
-    if (j > 0 && __any_sync(0xffffffffu, need)) {
+    if (j > 0 && __any_sync(0xffffffffu, need || failed)) {
+      if (__any_sync(0xffffffffu, failed)) return false;
       // Rescale this row of O_h once the previous sub-tile's PV has landed
       // (tcgen05.ld/st are warp-collective, hence the warp vote).
       const uint32_t tp = gt + uint32_t((j - 1) >> 1);
@@ -459,7 +450,8 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
 
   // Final O_h row once the item's last PV (buffer 1 of its last tile, issued
   // after every other) has completed, 32 dims at a time; then O_h is free.
-  if (!wait_bar_warp(sm, b.pv_done[h][1], (gt - 1) & 1, p.status)) return false;
+  failed |= !wait_bar(sm, b.pv_done[h][1], (gt - 1) & 1, p.status);
+  if (__any_sync(0xffffffffu, failed)) return false;
   ptx::tc_fence_after();
   const float inv = l > 0.f ? 1.f / l : 0.f;
   const float lse = l > 0.f ? m_ref + lg2(l) : -INFINITY;

@@ -88,7 +88,7 @@ struct TcShared {
   float alpha[2][kNMax];
   float inv_l[kNMax];     // 1 / column sum of the finished item
   float mref[2][kNMax];   // column reference max x scale (log2 domain), double buffered
-  int flags[2][2][4];     // per softmax group: per-warp exceed votes, double buffered
+  int flags[2][3][4];     // per softmax group: some lane of the warp exceeds, by tile modulo 3
   int grew[2][2];         // per softmax group: some column reference grew (exceed path)
   uint64_t k_full[kKStages], k_empty[kKStages];
   uint64_t v_full[kVStages], v_empty[kVStages];
@@ -119,13 +119,17 @@ __device__ __forceinline__ int item_columns(const WorkItem& it, bool use_cols) {
   return use_cols && it.cols > exact && it.cols <= kNMax && it.cols % 16 == 0 ? it.cols : exact;
 }
 
-// Barrier of one softmax warpgroup's 128 threads on an mbarrier (bounded, so that a thread
-// that stopped on a timeout cannot leave the others blocked).
+// Barrier of one softmax warpgroup's 128 threads on an mbarrier (bounded, so that a warp
+// that stopped on a timeout cannot leave the others blocked).  The result is the
+// lane's own; group_sync_warp's is the warp's.
 __device__ __forceinline__ bool group_sync(TcShared& sm, uint64_t& grp, uint32_t& uses, uint32_t* status) {
   ptx::mbar_arrive(ptx::smem_addr(&grp));
   const uint32_t parity = uses & 1;
   ++uses;
-  return wait_bar_warp(sm, grp, parity, status);
+  return wait_bar(sm, grp, parity, status);
+}
+__device__ __forceinline__ bool group_sync_warp(TcShared& sm, uint64_t& grp, uint32_t& uses, uint32_t* status) {
+  return __all_sync(0xffffffffu, group_sync(sm, grp, uses, status)) != 0;
 }
 
 // ------------------------------------------------------------------ MMA issuers
@@ -169,13 +173,10 @@ __device__ void run_qk(const AttnParams& p, const CUtensorMap* qmap, TcShared& s
     q_pending = false;
     for (int t = 0; t < nt && ok; ++t, ++g) {
       const int ks = g % kKStages, sb = g % 2;
-      if (!wait_bar_warp(sm, sm.k_full[ks], (g / kKStages) & 1, p.status) ||
-          !wait_bar_warp(sm, sm.s_empty[sb], ((g / 2) & 1) ^ 1, p.status)) {
-        ok = false;
-        break;
-      }
+      const bool ready = wait_bar(sm, sm.k_full[ks], (g / kKStages) & 1, p.status) &&
+                         wait_bar(sm, sm.s_empty[sb], ((g / 2) & 1) ^ 1, p.status);
       ptx::tc_fence_after();
-      if (lane == 0) {
+      if (lane == 0 && ready) {
         const uint64_t kdesc0 = ptx::smem_desc(k0 + uint32_t(ks) * kSlotBytes, 16, 1024, ptx::kLayoutSw128);
 #pragma unroll
         for (int kk = 0; kk < 128 / 16; ++kk) {
@@ -187,7 +188,7 @@ __device__ void run_qk(const AttnParams& p, const CUtensorMap* qmap, TcShared& s
         ptx::mma_commit(ptx::smem_addr(&sm.k_empty[ks]));
         if (t == nt - 1) ptx::mma_commit(ptx::smem_addr(&sm.q_empty));
       }
-      __syncwarp();
+      ok = __all_sync(0xffffffffu, ready);  // the warp goes on or stops as one
     }
     if (!ok) break;
     // The next item's query tile loads while this item's last PV and epilogue run.
@@ -233,19 +234,15 @@ __device__ void run_pv(const AttnParams& p, TcShared& sm, int lane, uint32_t& k,
     for (int t = 0; t < nt && ok; ++t, ++g) {
       const uint32_t vs = g % kVStages, pb = g % 2;
       // The item's first PV overwrites O: the previous item's epilogue has read it.
-      if ((t == 0 && !wait_bar_warp(sm, sm.o_free, (items_done & 1) ^ 1, p.status)) ||
-          !wait_bar_warp(sm, sm.v_full[vs], (g / kVStages) & 1, p.status)) {
-        ok = false;
-        break;
-      }
-      clear_v_tail(sm.v[vs], it.tok_end - (it.tok_begin + t * kTile), lane);
-      __syncwarp();
-      if (!wait_bar_warp(sm, sm.p_full[pb], (g / 2) & 1, p.status)) {
-        ok = false;
-        break;
-      }
+      bool ready = (t > 0 || wait_bar(sm, sm.o_free, (items_done & 1) ^ 1, p.status)) &&
+                   wait_bar(sm, sm.v_full[vs], (g / kVStages) & 1, p.status);
+      if (ready) clear_v_tail(sm.v[vs], it.tok_end - (it.tok_begin + t * kTile), lane);
+      // (Every lane's part of the tail is cleared before lane 0 goes on.)
+      ok = __all_sync(0xffffffffu, ready);
+      if (!ok) break;
+      ready = wait_bar(sm, sm.p_full[pb], (g / 2) & 1, p.status);
       ptx::tc_fence_after();
-      if (lane == 0) {
+      if (lane == 0 && ready) {
         const uint64_t vdesc0 = ptx::smem_desc(v0 + vs * kSlotBytes, kHalfBytes, 1024, ptx::kLayoutSw128);
         const uint64_t pdesc0 = ptx::smem_desc(p0 + pb * kPBufBytes, 128, kTile * 16, ptx::kLayoutNone);
 #pragma unroll
@@ -255,7 +252,7 @@ __device__ void run_pv(const AttnParams& p, TcShared& sm, int lane, uint32_t& k,
         ptx::mma_commit(ptx::smem_addr(&sm.v_empty[vs]));
         ptx::mma_commit(ptx::smem_addr(&sm.p_empty[pb]));
       }
-      __syncwarp();
+      ok = __all_sync(0xffffffffu, ready);
     }
     if (!ok) break;
     ++items_done;
@@ -426,12 +423,17 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
   for (int j = 0; j < NH; ++j) l[j] = 0.f;
   int cur = 0;
   const uint32_t g0 = g;
+  // A lane whose wait failed goes on with whatever is there until its warp's
+  // next vote, so that no lane leaves alone; a vote after every wait would cost
+  // the tile loop 4 %.  After a failure no output counts (ASPIRE_STATUS_TIMEOUT).
+  bool failed = false;
+  int flag = 0;  // the first tile sets its flags whatever they hold
 
   for (int t = 0; t < nt; ++t) {
     const uint32_t gt = g0 + t;
     const int b = gt % 2;
     const uint32_t ph = (gt / 2) & 1;
-    if (!wait_bar_warp(sm, sm.s_full[b], ph, p.status)) return false;
+    failed |= !wait_bar(sm, sm.s_full[b], ph, p.status);
     ptx::tc_fence_after();
     const int tile0 = it.tok_begin + t * kTile;
     const int tok = tile0 + r;
@@ -473,7 +475,7 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
       if (d0_lo < d0_hi) ptx::tmem_ld8(tmem_lane + col_s(b) + d0_lo, dv0);
       if (d1_lo < d1_hi) ptx::tmem_ld8(tmem_lane + col_s(b) + d1_lo, dv1);
       ptx::tmem_wait_ld();
-      const bool store = in_chunk && tok < p.dump_kv_stride;
+      const bool store = in_chunk && tok < p.dump_kv_stride && !failed;
       if (d0_lo < d0_hi)
         dump_columns(p, d0_lo, d0_hi, dump_base0, 0, dump_col_stride, tok, store, tmem_lane + col_s(b), dv0);
       if (d1_lo < d1_hi)
@@ -490,18 +492,23 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
 #pragma unroll
       for (int j = 0; j < NH; ++j) exceed |= fmaf(sv[j], scale, -mr[j]) > kLazyLog2;
     }
-    const bool warp_exceed = __any_sync(0xffffffffu, exceed);
-    if (lane == 0) flags[t & 1][wq] = warp_exceed ? 1 : 0;
-    if (!group_sync(sm, grp, grp_uses, p.status)) return false;
-    const bool any_exceed = (flags[t & 1][0] | flags[t & 1][1] | flags[t & 1][2] | flags[t & 1][3]) != 0;
-    if (any_exceed) {
+    // (The next tile's flag was read two tiles ago, before this thread passed the
+    // last barrier: it is free to be cleared.)
+    const int next_flag = flag == 2 ? 0 : flag + 1;
+    if (exceed) flags[flag][wq] = 1;
+    if (lane == 0) flags[next_flag][wq] = 0;
+    failed |= !group_sync(sm, grp, grp_uses, p.status);
+    const bool any_exceed = (flags[flag][0] | flags[flag][1] | flags[flag][2] | flags[flag][3]) != 0;
+    flag = next_flag;
+    if (__any_sync(0xffffffffu, any_exceed || failed)) {
+      if (__any_sync(0xffffffffu, failed)) return false;
       // Exact column maxima of the tile (reduced in place; S is read again from
       // TMEM afterwards).  Thread j < NH then updates column c0 + j's reference
       // (mref[cur ^ 1]) and its rescale factor alpha; the per-column work is
       // spread over threads so that this once-per-item path stays short.
       warp_columns<NH, true>(sv, sm.red[t & 1][wq] + c0, lane);
       if (ctid == 0) grew[t & 1] = 0;
-      if (!group_sync(sm, grp, grp_uses, p.status)) return false;
+      if (!group_sync_warp(sm, grp, grp_uses, p.status)) return false;
       if (ctid < NH) {
         const int c = c0 + ctid;
         const float mo = t > 0 ? sm.mref[cur][c] : -INFINITY;
@@ -517,7 +524,7 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
       ptx::tc_fence_before();
       ptx::mbar_arrive(ptx::smem_addr(&sm.s_empty[b]));
       // New references and alphas visible to every thread (uniform branch).
-      if (!group_sync(sm, grp, grp_uses, p.status)) return false;
+      if (!group_sync_warp(sm, grp, grp_uses, p.status)) return false;
       cur ^= 1;
       if (t > 0 && grew[t & 1]) {
         const float* alpha_s = sm.alpha[t & 1] + c0;
@@ -555,7 +562,7 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
       }
     }
     // P^T as bf16, MN-major without swizzle: 8 queries x 16 B per token, token-major.
-    if (!wait_bar_warp(sm, sm.p_empty[b], ph ^ 1, p.status)) return false;
+    failed |= !wait_bar(sm, sm.p_empty[b], ph ^ 1, p.status);
     uint8_t* pbuf = sm.p[b] + (c0 / 8) * (kTile * 16);
 #pragma unroll
     for (int c = 0; c < NH / 8; ++c) {
@@ -577,7 +584,8 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
 
   // Final O: wait for the item's last PV (on its P buffer's empty barrier),
   // read this lane (dim r) of the group's columns, free the accumulator.
-  if (!wait_bar_warp(sm, sm.p_empty[(g - 1) % 2], ((g - 1) / 2) & 1, p.status)) return false;
+  failed |= !wait_bar(sm, sm.p_empty[(g - 1) % 2], ((g - 1) / 2) & 1, p.status);
+  if (__any_sync(0xffffffffu, failed)) return false;
   ptx::tc_fence_after();
   float o_fin[NH];
   tmem_load_cols<NH>(tmem_lane + kColO + c0, o_fin);
@@ -588,7 +596,7 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
   // Column sums of l across the group's 128 threads; thread j < NH then turns
   // column c0 + j into its reciprocal and LSE once.
   warp_columns<NH, false>(l, sm.red_l[wq] + c0, lane);
-  if (!group_sync(sm, grp, grp_uses, p.status)) return false;
+  if (!group_sync_warp(sm, grp, grp_uses, p.status)) return false;
   float my_lse = -INFINITY;  // LSE of column c0 + ctid
   if (ctid < NH) {
     const int c = c0 + ctid;
@@ -599,7 +607,7 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
   // The previous item's bulk stores (issued by this group's thread 0) have
   // read the group's staging rows before anyone rewrites them.
   if (ctid == 0) ptx::bulk_wait_read();
-  if (!group_sync(sm, grp, grp_uses, p.status)) return false;
+  if (!group_sync_warp(sm, grp, grp_uses, p.status)) return false;
 
   // Normalised rows are staged in shared memory and leave by bulk stores, so
   // the threads move on to the next item at once.
@@ -626,7 +634,7 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
       partial_lse_ptr(p)[int64_t(it.partial_base) + int64_t(it.chunk) * nrows + c0 + ctid] = my_lse;
   }
   ptx::fence_proxy_async_smem();
-  if (!group_sync(sm, grp, grp_uses, p.status)) return false;
+  if (!group_sync_warp(sm, grp, grp_uses, p.status)) return false;
   if (ctid == 0 && c0 < row_end) {
     if (final_rows) {
       const uint32_t src = ptx::smem_addr(stage);

@@ -221,13 +221,11 @@ __device__ bool run_producer(const AttnParams& p, const CUtensorMap* tmap, Sh& s
         append_new_tokens(p, it, kv_sel, lane);
         appended = true;
       }
-      if (!wait_bar_warp(sm, empty[s], ph ^ 1, p.status)) {
-        ok = false;
-        break;
-      }
+      const bool ready = wait_bar(sm, empty[s], ph ^ 1, p.status);
       const uint32_t fb = ptx::smem_addr(&full[s]);
-      if (lane == 0) ptx::mbar_arrive_expect_tx(fb, kSlotBytes);
-      __syncwarp();
+      if (lane == 0 && ready) ptx::mbar_arrive_expect_tx(fb, kSlotBytes);
+      ok = __all_sync(0xffffffffu, ready);  // the warp goes on or stops as one
+      if (!ok) break;
       if (lane < kPagesPerTile) {
         int page = static_cast<int>(p.num_pages_total);  // out of range: TMA fills zeros
         const int lp = first_page + t * kPagesPerTile + lane;
