@@ -7,9 +7,10 @@
 //              d w[t, j] = <dy[t], rows[position[t, j]]>
 //
 // Bound by the bytes.  Every kernel goes by token: a block of 128 threads
-// owns one, reads x[t] or dy[t] once whatever top_k is, and moves 16 bytes per
-// thread and row; sums are in fp32 in the order of the choices, so nothing
-// depends on which block runs first.  8192 tokens x 8 rows of 2048 bf16:
+// owns one, takes x[t] or dy[t] from memory once whatever top_k is (the combine's
+// gradient goes over the row once for every four choices, the later times in the
+// caches), and moves 16 bytes per thread and row; sums are in fp32 in the order of
+// the choices, so nothing depends on which block runs first.  8192 tokens x 8 rows of 2048 bf16:
 // dispatch 51 us and its gradient 46 us (91 % of the copy rate); 4099 x 4 rows
 // of 4096: combine 29 us, its gradients 47 us.
 #include "moe.cuh"
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(kMoeThreads) aspire_moe_combine_kernel(MoePerm
   const uint4* res =
       p.residual ? reinterpret_cast<const uint4*>(static_cast<const T*>(p.residual) + token * p.residual_stride) : nullptr;
   load_slots(p, token, row, weight);
-  for (int c = blockIdx.y * kMoeThreads + threadIdx.x; c < vecs; c += kMoeThreads * gridDim.y) {
+  for (int c = threadIdx.x; c < vecs; c += kMoeThreads) {
     float acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = 0.f;
