@@ -1,6 +1,8 @@
 // 4-bit products of few tokens (a drafting or verifying row, a decode batch).
 //
-// The weights' bytes bound it: 0.5 byte feeds 2 x tokens operations.  A CTA
+// The weights' bytes are its floor: 0.5 byte feeds 2 x tokens operations.  What
+// it spends beyond them is waiting where stages are handed over (one row 4096 ->
+// 151936: 57 % of the issue slots used, no pipe above 46 %).  A CTA
 // owns 128 matrix rows (64 gate and 64 up rows with the activation), 8 or 16
 // tokens and a range of K, and streams the rows' codes through a ring of
 // 256-weight stages in shared memory (asynchronous 16-byte copies, 128
@@ -10,8 +12,8 @@
 //
 // The products run on warp-level matrix instructions with the weights as A
 // (16 rows x 16 k) unpacked in registers and the tokens as B (8 columns): at
-// 16 tokens and fewer the unpacking, not the tensor rate, is what could slow the
-// stream, and unpacked fragments go straight from registers into the
+// 16 tokens and fewer the tensor rate does not limit the stream (26 % of that
+// pipe), and unpacked fragments go straight from registers into the
 // instruction.  The sum over k may run in any order, so the instruction's k
 // slots are assigned to the codes as they lie: of each group's part of a stage
 // lane (g, c) of a warp (g = lane / 4) loads the c-th quarter of row g's codes
@@ -29,7 +31,7 @@
 // are fewer tiles than SMs, a cluster of 2, 4 or 8 CTAs splits K; the
 // partials meet in distributed shared memory in rank order (no atomics, no
 // workspace, the same bits every time).  One row 4096 -> 151936, groups of 128:
-// 73 us (4.4 TB/s); 64 tokens over 128 experts 2048 -> 2 x 768: 54 us.
+// 74 us (4.4 TB/s); 64 tokens over 128 experts 2048 -> 2 x 768: 55 us.
 #include <cooperative_groups.h>
 
 #include "w4.cuh"

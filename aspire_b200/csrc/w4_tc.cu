@@ -32,8 +32,9 @@
 // partials in distributed shared memory in rank order, as in the kernel for
 // few tokens.
 //
-// 4099 tokens 4096 -> 12288, bf16, groups of 128: 356 us (1.17 PFLOP/s), bound by
-// the issue of the MMAs between waits; 64 tokens 4096 -> 2 x 12288: 31 us.
+// 4099 tokens 4096 -> 12288, bf16, groups of 128: 358 us (1.15 PFLOP/s), bound by
+// the issue of the MMAs between waits; 64 tokens 4096 -> 2 x 12288: 31 us.  The
+// 128-token forms spill 40 to 252 bytes a thread around the epilogue.
 #include <cooperative_groups.h>
 
 #include "tc_pipeline.cuh"
