@@ -13,6 +13,10 @@ Public surface (drop-in for the reference's Python interfaces):
   (``w4_linear``, ``w4_swiglu`` and their per-expert forms).
 * ``aspire_b200.moe`` - router top-k with the sort of tokens by expert,
   dispatch and combine, with gradients.
+* A step of tree speculation: ``aspire_b200.kv_ops.build_step_tables`` (block
+  tables and slot maps from lengths), ``HolisticAttentionWrapper.run(...,
+  tree_mask=)``, ``aspire_b200.logits`` (penalties, biases and grammar masks)
+  and ``aspire_b200.tree.accept_tree``.
 
 All of it runs through libaspire_b200.so (C ABI in include/aspire_b200.h).
 There is no CPU fallback: a missing library or GPU raises.

@@ -28,6 +28,9 @@ STATUS_BAD_PAGE = 1
 STATUS_BAD_PLAN = 2
 STATUS_BAD_ROW = 4
 STATUS_TIMEOUT = 8
+STATUS_NO_PAGES = 16
+MAX_CACHES = 128
+MAX_PATH = 64
 DUMP_FIRST_LAST = 0
 DUMP_LAST_TOKEN = 1
 DUMP_F16 = 0
@@ -359,6 +362,94 @@ class AspireMoePermuteArgs(ctypes.Structure):
     ]
 
 
+class AspireStepTablesArgs(ctypes.Structure):
+    _fields_ = [
+        ("lengths", ctypes.c_void_p),
+        ("new_tokens", ctypes.c_void_p),
+        ("rows", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int64),
+        ("block_table_cols", ctypes.c_int32),
+        ("held", ctypes.c_void_p),
+        ("free_pages", ctypes.c_void_p),
+        ("free_count", ctypes.c_void_p),
+        ("free_capacity", ctypes.c_int64),
+        ("parents", ctypes.c_void_p),
+        ("tree_mask_words", ctypes.c_int32),
+        ("tokens", ctypes.c_int64),
+        ("qo_indptr", ctypes.c_void_p),
+        ("kv_indptr", ctypes.c_void_p),
+        ("kv_len", ctypes.c_void_p),
+        ("last_page_len", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("tree_mask", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class AspireLogitsArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("logits_stride", ctypes.c_int64),
+        ("type", ctypes.c_int32),
+        ("tokens", ctypes.c_int64),
+        ("vocab", ctypes.c_int32),
+        ("rows", ctypes.c_int32),
+        ("indptr", ctypes.c_void_p),
+        ("history", ctypes.c_void_p),
+        ("history_stride", ctypes.c_int64),
+        ("history_cols", ctypes.c_int32),
+        ("history_len", ctypes.c_void_p),
+        ("prompt_len", ctypes.c_void_p),
+        ("step_tokens", ctypes.c_void_p),
+        ("tree_mask", ctypes.c_void_p),
+        ("tree_mask_words", ctypes.c_int32),
+        ("repetition", ctypes.c_void_p),
+        ("frequency", ctypes.c_void_p),
+        ("presence", ctypes.c_void_p),
+        ("bias_indptr", ctypes.c_void_p),
+        ("bias_ids", ctypes.c_void_p),
+        ("bias_values", ctypes.c_void_p),
+        ("bias_entries", ctypes.c_int64),
+        ("allowed", ctypes.c_void_p),
+        ("allowed_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_stride", ctypes.c_int64),
+        ("ids", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class AspireTreeAcceptArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_void_p),
+        ("parents", ctypes.c_void_p),
+        ("targets", ctypes.c_void_p),
+        ("indptr", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("total", ctypes.c_int64),
+        ("rows", ctypes.c_int32),
+        ("max_path", ctypes.c_int32),
+        ("count", ctypes.c_void_p),
+        ("path", ctypes.c_void_p),
+        ("out_tokens", ctypes.c_void_p),
+        ("new_lengths", ctypes.c_void_p),
+        ("caches", ctypes.POINTER(ctypes.c_void_p)),
+        ("num_caches", ctypes.c_int32),
+        ("pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int32),
+        ("token_bytes", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int64),
+        ("block_table_cols", ctypes.c_int32),
+        ("status", ctypes.c_void_p),
+    ]
+
+
 # Exported symbols and their signatures (must match include/aspire_b200.h).
 _SIGNATURES = {
     "aspire_plan": (
@@ -388,6 +479,16 @@ _SIGNATURES = {
     "aspire_select_pages": (ctypes.c_int, [ctypes.POINTER(AspireSelectArgs), ctypes.c_void_p]),
     "aspire_build_unified_indices": (ctypes.c_int, [ctypes.POINTER(AspireIndicesArgs), ctypes.c_void_p]),
     "aspire_qkv_prologue": (ctypes.c_int, [ctypes.POINTER(AspirePrologueArgs), ctypes.c_void_p]),
+    "aspire_qkv_prologue_at": (ctypes.c_int, [ctypes.POINTER(AspirePrologueArgs), ctypes.c_void_p, ctypes.c_void_p]),
+    "aspire_tree_attention": (
+        ctypes.c_int,
+        [ctypes.POINTER(AspireAttnArgs), ctypes.c_void_p, ctypes.c_int32, ctypes.POINTER(AspirePlanInfo),
+         ctypes.c_void_p],
+    ),
+    "aspire_step_tables": (ctypes.c_int, [ctypes.POINTER(AspireStepTablesArgs), ctypes.c_void_p]),
+    "aspire_logits_workspace": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
+    "aspire_adjust_logits": (ctypes.c_int, [ctypes.POINTER(AspireLogitsArgs), ctypes.c_void_p]),
+    "aspire_tree_accept": (ctypes.c_int, [ctypes.POINTER(AspireTreeAcceptArgs), ctypes.c_void_p]),
     "aspire_draft_page_spill": (ctypes.c_int, [ctypes.POINTER(AspireSpillArgs), ctypes.c_void_p]),
     "aspire_clear_dump_slots": (ctypes.c_int, [ctypes.POINTER(AspireClearDumpArgs), ctypes.c_void_p]),
     "aspire_w4_linear": (ctypes.c_int, [ctypes.POINTER(AspireW4Args), ctypes.c_void_p]),
@@ -453,13 +554,15 @@ def check(rc: int, what: str) -> None:
 
 
 _BOUND = ("aspire_last_error", "aspire_w4_linear", "aspire_moe_route", "aspire_moe_route_workspace",
-          "aspire_moe_route_grad", "aspire_moe_dispatch", "aspire_moe_combine", "aspire_moe_combine_grad")
+          "aspire_moe_route_grad", "aspire_moe_dispatch", "aspire_moe_combine", "aspire_moe_combine_grad",
+          "aspire_step_tables", "aspire_logits_workspace", "aspire_adjust_logits", "aspire_tree_accept",
+          "aspire_tree_attention")
 _ops = None
 
 
 def ops():
-    """The compiled calls of the feed-forward operators (csrc/torch_binding.cpp),
-    on the entry points of the loaded library."""
+    """The compiled calls of the feed-forward and tree-step operators
+    (csrc/torch_binding.cpp), on the entry points of the loaded library."""
     global _ops
     if _ops is None:
         from . import build

@@ -319,13 +319,22 @@ class HolisticAttentionWrapper:
         return_lse: bool = False,
         lse: Optional[torch.Tensor] = None,
         append: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+        tree_mask: Optional[torch.Tensor] = None,
         **kwargs,
     ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
         """Runs the planned program.  ``append=(k_new, v_new)`` (bf16
         [tokens, num_kv_heads, 128], the queries' own keys and values) also
         writes each row's new tokens into the cache before the row's keys are
         read, as ``append_kv`` with the same qo_indptr and page source would
-        (one launch instead of two); host plans of tcgen05 decode rows only."""
+        (one launch instead of two); host plans of tcgen05 decode rows only.
+
+        ``tree_mask`` (int32 [tokens, words], contiguous) attends trees of
+        drafted tokens (C ABI ``aspire_tree_attention``): a row's last q_len
+        keys are its queries' own, every query sees all keys before those and,
+        of those, key j iff bit j % 32 of word j / 32 of its mask is set, as
+        ``build_step_tables`` makes it.  A query that sees no key gets zeros
+        and an LSE of -inf.  Keys and values that some query does not see must
+        be finite.  The plan must be made with ``causal=False``; no dump."""
         if self._plan_info is None:
             raise RuntimeError("run() before plan()/plan_host()")
         kv = _unpack_paged_kv_cache(paged_kv_cache, self._kv_layout)
@@ -380,6 +389,14 @@ class HolisticAttentionWrapper:
                                            or dump_flags.numel() < self._plan_rows):
                 raise ValueError("mode_flags must be a contiguous int32 tensor with one entry per row")
 
+        if tree_mask is not None:
+            if tree_mask.dtype != torch.int32 or tree_mask.dim() != 2 or not tree_mask.is_contiguous() or \
+                    tree_mask.device != q.device or tree_mask.shape[0] < q.shape[0] or tree_mask.shape[1] < 1:
+                raise ValueError("tree_mask must be a contiguous int32 [tokens, words] tensor on q's device")
+            if self._causal:
+                raise ValueError("tree_mask needs a plan made with causal=False")
+            if dump is not None:
+                raise ValueError("a dump variant takes no tree_mask")
         sm_scale = self._sm_scale if self._sm_scale is not None else 1.0 / math.sqrt(q.shape[2])
         a = _capi.AspireAttnArgs()
         a.q = q.data_ptr()
@@ -430,9 +447,15 @@ class HolisticAttentionWrapper:
         a.float_ws = self._float_workspace.data_ptr()
         a.float_ws_bytes = self._float_workspace.numel()
         stream = torch.cuda.current_stream(q.device).cuda_stream
-        rc = self._lib.aspire_mixed_attention(ctypes.byref(a), ctypes.byref(self._plan_info),
-                                              ctypes.c_void_p(stream))
-        _capi.check(rc, "aspire_mixed_attention")
+        if tree_mask is not None:
+            rc = self._lib.aspire_tree_attention(ctypes.byref(a), ctypes.c_void_p(tree_mask.data_ptr()),
+                                                 tree_mask.shape[1], ctypes.byref(self._plan_info),
+                                                 ctypes.c_void_p(stream))
+            _capi.check(rc, "aspire_tree_attention")
+        else:
+            rc = self._lib.aspire_mixed_attention(ctypes.byref(a), ctypes.byref(self._plan_info),
+                                                  ctypes.c_void_p(stream))
+            _capi.check(rc, "aspire_mixed_attention")
         if return_lse:
             return out, lse
         return out

@@ -43,6 +43,10 @@ SOURCES = [
     "w4_tc.cu",
     "moe_route.cu",
     "moe_permute.cu",
+    "capi_tree.cu",
+    "step_tables.cu",
+    "logits.cu",
+    "tree_accept.cu",
 ]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

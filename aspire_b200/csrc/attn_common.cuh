@@ -39,6 +39,9 @@ struct AttnParams {
   const __nv_bfloat16* k_new;
   const __nv_bfloat16* v_new;
   int64_t k_new_stride_n, k_new_stride_h, v_new_stride_n, v_new_stride_h;
+  // Tree mask (the tree kernel only): which of its row's last q_len keys a query sees.
+  const int32_t* tree_mask;
+  int32_t tree_words;
 };
 
 // Page id of logical page lp of a row: from the flat page list at the row's
@@ -123,6 +126,11 @@ __device__ __forceinline__ float* partial_lse_ptr(const AttnParams& p) {
 
 __device__ __forceinline__ void record_status(uint32_t* status, uint32_t bits) {
   if (status) atomicOr(status, bits);
+}
+
+// Word w of a query's tree mask (q: its row in the step); 0 past the mask.
+__device__ __forceinline__ uint32_t tree_word(const AttnParams& p, int64_t q, int w) {
+  return w >= 0 && w < p.tree_words && q < p.q_rows ? uint32_t(__ldg(p.tree_mask + q * p.tree_words + w)) : 0u;
 }
 
 // Location of packed query row `pq` of an item: token row and query head.

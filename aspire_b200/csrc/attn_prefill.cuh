@@ -342,9 +342,19 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// Which of the row's last q_len keys, from node `node0` on (0 at the first of
+// them, negative before it), 64 consecutive keys, query row q sees.
+__device__ __forceinline__ uint64_t tree_keys(const AttnParams& p, int64_t q, int node0) {
+  const int from = max(node0, 0), w = from >> 5, s = from & 31;
+  uint64_t seen = uint64_t(tree_word(p, q, w)) | (uint64_t(tree_word(p, q, w + 1)) << 32);
+  if (s) seen = (seen >> s) | (uint64_t(tree_word(p, q, w + 2)) << (64 - s));
+  // (Keys before the nodes are seen by every query; at least one of the 64 is not before them.)
+  return node0 < 0 ? (seen << -node0) | ((uint64_t(1) << -node0) - 1) : seen;
+}
+
 // One item for softmax warpgroup h (thread = packed row r of half h).  `gt`
 // counts the K/V tiles this warpgroup has consumed (its barrier phases).
-template <class Sh>
+template <bool kTree, class Sh>
 __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bool causal, int h, int r,
                              uint32_t tmem_lane, uint32_t& gt) {
   Barriers& b = sm.pf;
@@ -359,11 +369,11 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
   // Keys [tok_begin, vis_end) of the item are visible to this row (bottom-right
   // causal mask); padding rows see none.
   int vis_end = it.tok_begin;
-  if (valid) vis_end = causal ? min(it.tok_end, it.kv_len - it.q_len + q_idx + 1) : it.tok_end;
+  if (valid) vis_end = !kTree && causal ? min(it.tok_end, it.kv_len - it.q_len + q_idx + 1) : it.tok_end;
   // Logit dump (raw q.k before scale and mask, dump_index): query 0 to the
   // first slot, query q_len-1 to the last one, as the dump kind has them.
   int64_t dump_at = -1;
-  if (valid && dump_row_on(p, it.row)) {
+  if (!kTree && valid && dump_row_on(p, it.row)) {
     const bool first = dump_has_first(p) && q_idx == 0;
     const bool last = !first && dump_has_last(p, it.q_len) && q_idx == it.q_len - 1;
     if (first || last) dump_at = dump_index(p, it.row, head, last);
@@ -401,6 +411,15 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
 #pragma unroll
       for (int c = 0; c < kSub; ++c)
         if (c >= nvis) s[c] = -INFINITY;
+    }
+    if constexpr (kTree) {
+      const int node0 = sub0 - (it.kv_len - it.q_len);
+      if (node0 + kSub > 0 && valid) {
+        const uint64_t seen = tree_keys(p, int64_t(it.q_start) + q_idx, node0);
+#pragma unroll
+        for (int c = 0; c < kSub; ++c)
+          if (!((seen >> c) & 1)) s[c] = -INFINITY;
+      }
     }
     const float ms = max64(s) * scale;
     const bool need = ms > m_ref + kLazyLog2;
@@ -499,7 +518,7 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
 
 // Softmax warpgroup h's share of the item sequence: both halves of two-half
 // items, half 0 of the others.  `quarter` is the warp's TMEM lane quarter.
-template <class Sh>
+template <bool kTree, class Sh>
 __device__ void consume_items(const AttnParams& p, Sh& sm, bool causal, int h, int quarter, int lane, uint32_t& k) {
   const int r = quarter * 32 + lane;
   const uint32_t tmem_lane = sm.tmem_base + (uint32_t(quarter * 32) << 16);
@@ -520,7 +539,7 @@ __device__ void consume_items(const AttnParams& p, Sh& sm, bool causal, int h, i
       continue;
     }
     if (h >= halves_of(p, it)) continue;
-    if (!consume_item(p, sm, it, causal, h, r, tmem_lane, gt)) return;
+    if (!consume_item<kTree>(p, sm, it, causal, h, r, tmem_lane, gt)) return;
   }
 }
 

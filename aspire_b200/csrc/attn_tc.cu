@@ -376,7 +376,27 @@ __device__ __noinline__ void dump_columns(const AttnParams& p, int lo, int hi, i
 // column's running statistics (reference max, sum, rescale factor) live with
 // its owner, so the two groups never wait for each other; they meet only on
 // the S / P / O barriers shared with the MMA warp.
-template <int NH, bool kDump>
+// Which of the columns [c0, c0 + NH) see the item's key `tok` under the tree
+// mask, bit j for column c0 + j: all of them a key before the row's nodes, else
+// the columns of the queries whose mask names the node.
+template <int NH>
+__device__ __forceinline__ uint32_t tree_columns(const AttnParams& p, const WorkItem& it, int tok, int c0, int nrows) {
+  if (tok >= it.tok_end) return 0;
+  const int node = tok - (it.kv_len - it.q_len);
+  if (node < 0) return 0xffffffffu;
+  uint32_t seen = 0;
+  const int end = min(nrows, c0 + NH);
+  int q = (it.pq_begin + c0) / p.group;
+  for (int c = c0; c < end; ++q) {
+    const int next = min(end, (q + 1) * p.group - it.pq_begin);
+    if ((tree_word(p, int64_t(it.q_start) + q, node >> 5) >> (node & 31)) & 1)
+      seen |= ((1u << (next - c0)) - 1u) & ~((1u << (c - c0)) - 1u);
+    c = next;
+  }
+  return seen;
+}
+
+template <int NH, bool kDump, bool kTree>
 __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& it, bool causal, int r,
                              int ctid, int wg, int wq, int lane, uint32_t& g, uint32_t& grp_uses) {
   constexpr int N = 2 * NH;
@@ -438,7 +458,8 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
     const int tile0 = it.tok_begin + t * kTile;
     const int tok = tile0 + r;
     const bool in_chunk = tok < it.tok_end;
-    const int limit_min = causal ? (it.kv_len - it.q_len + q_idx0 + 1) : it.kv_len;
+    const int limit_min =
+        kTree ? it.kv_len - it.q_len : causal ? (it.kv_len - it.q_len + q_idx0 + 1) : it.kv_len;
     // Padded columns (j >= nrows) only feed ignored O columns: they need no mask.
     const bool full_tile = tile0 + kTile <= it.tok_end && tile0 + kTile <= limit_min;
     const uint32_t s_cols = tmem_lane + col_s(b) + c0;
@@ -450,7 +471,10 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
     // under the bottom-right causal mask, q_idx(j) >= tok - (kv_len - q_len),
     // i.e. j >= jmin: one threshold per thread instead of a division per column.
     int jmin = 0;
-    if (!full_tile) {
+    uint32_t seen = 0xffffffffu;  // (tree: the columns that see `tok`)
+    if constexpr (kTree) {
+      if (!full_tile) seen = tree_columns<NH>(p, it, tok, c0, nrows);
+    } else if (!full_tile) {
       if (!in_chunk || tok >= it.kv_len) {
         jmin = N;
       } else if (causal) {
@@ -462,7 +486,7 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
       if (!full_tile) {
 #pragma unroll
         for (int j = 0; j < NH; ++j)
-          if (c0 + j < jmin) sv[j] = -INFINITY;
+          if (kTree ? !((seen >> j) & 1) : c0 + j < jmin) sv[j] = -INFINITY;
       }
     };
     float sv[NH];
@@ -658,6 +682,7 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
   return true;
 }
 
+template <bool kTree>
 __device__ void consume_items(const AttnParams& p, TcShared& sm, bool causal, int warp, int lane, uint32_t& k,
                               bool use_cols) {
   const int wq = warp & 3;
@@ -684,42 +709,44 @@ __device__ void consume_items(const AttnParams& p, TcShared& sm, bool causal, in
     // Items whose columns include dumped rows (query 0 or the last query, as
     // the dump kind and the row's flag have it) take the instantiation that
     // carries the dump path.
-    const bool dump_item = dump_row_on(p, it.row) &&
+    const bool dump_item = !kTree && dump_row_on(p, it.row) &&
                            ((dump_has_first(p) && it.pq_begin < p.group) ||
                             (dump_has_last(p, it.q_len) && (it.q_len - 1) * p.group < it.pq_end));
     bool ok;
     if (dump_item) {
-      if (N == 16)
-        ok = consume_item<8, true>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
-      else if (N == 32)
-        ok = consume_item<16, true>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
-      else
-        ok = consume_item<24, true>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+      if constexpr (kTree) {
+        ok = false;
+      } else if (N == 16) {
+        ok = consume_item<8, true, false>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+      } else if (N == 32) {
+        ok = consume_item<16, true, false>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+      } else {
+        ok = consume_item<24, true, false>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+      }
     } else {
       if (N == 16)
-        ok = consume_item<8, false>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+        ok = consume_item<8, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
       else if (N == 32)
-        ok = consume_item<16, false>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+        ok = consume_item<16, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
       else
-        ok = consume_item<24, false>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+        ok = consume_item<24, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
     }
     if (!ok) return;
   }
 }
 
+template <bool kTree>
 __device__ void run_consumer(const AttnParams& p, TcShared& sm, bool causal, int warp, int lane, uint32_t& k,
                              bool use_cols) {
-  consume_items(p, sm, causal, warp, lane, k, use_cols);
+  consume_items<kTree>(p, sm, causal, warp, lane, k, use_cols);
   // The bulk stores of each group's last item (issued by its thread 0) finish
   // before the CTA exits.
   if (lane == 0 && (warp - kFirstSoftmaxWarp) % 4 == 0) ptx::bulk_wait_all();
 }
 
-}  // namespace
-
-__global__ void __launch_bounds__(kTcThreads, 1)
-    aspire_attn_tc_kernel(AttnParams p, const __grid_constant__ CUtensorMap tmap,
-                          const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap qmap_pf) {
+template <bool kTree>
+__device__ __forceinline__ void attn_tc(const AttnParams& p, const CUtensorMap& tmap, const CUtensorMap& qmap,
+                                        const CUtensorMap& qmap_pf) {
   pdl_launch_dependents();
   extern __shared__ __align__(1024) uint8_t tc_smem_raw[];
   const uint32_t raw = ptx::smem_addr(tc_smem_raw);
@@ -806,7 +833,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     } else if (warp == kPvWarp) {
       run_pv(p, sm, lane, k, use_cols);
     } else {
-      run_consumer(p, sm, causal, warp, lane, k, use_cols);
+      run_consumer<kTree>(p, sm, causal, warp, lane, k, use_cols);
     }
   }
   // Phase 2: the prefill list, in the same shared memory and TMEM.  Every
@@ -828,7 +855,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // One MMA-issuing warp per item half.
         pf::run_mma(p, &qmap_pf, sm, pbuf, warp == 1 ? 0 : 1, lane, k);
       } else {
-        pf::consume_items(p, sm, causal, (warp - kFirstSoftmaxWarp) / 4, warp & 3, lane, k);
+        pf::consume_items<kTree>(p, sm, causal, (warp - kFirstSoftmaxWarp) / 4, warp & 3, lane, k);
       }
     }
   }
@@ -837,6 +864,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __syncthreads();
   ptx::tc_fence_after();
   if (warp == 1) ptx::tmem_dealloc(sm.tmem_base, kTmemCols);
+}
+
+}  // namespace
+
+__global__ void __launch_bounds__(kTcThreads, 1)
+    aspire_attn_tc_kernel(AttnParams p, const __grid_constant__ CUtensorMap tmap,
+                          const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap qmap_pf) {
+  attn_tc<false>(p, tmap, qmap, qmap_pf);
+}
+
+// The same under a tree mask (AttnParams::tree_mask), without the dump.  Its
+// mask costs the tiles that hold the row's last q_len keys alone: one or two
+// words a query and key there, a comparison per tile elsewhere.
+__global__ void __launch_bounds__(kTcThreads, 1)
+    aspire_attn_tree_kernel(AttnParams p, const __grid_constant__ CUtensorMap tmap,
+                            const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap qmap_pf) {
+  attn_tc<true>(p, tmap, qmap, qmap_pf);
 }
 
 size_t tc_smem_bytes() { return sizeof(TcShared) + 1024; }

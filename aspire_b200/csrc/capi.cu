@@ -40,7 +40,7 @@ int plan_impl(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t*
 
 namespace {
 
-SmemOptIn g_gather_smem, g_tc_smem, g_sel_smem;
+SmemOptIn g_gather_smem, g_tc_smem, g_tree_smem, g_sel_smem;
 
 // Bound of one pipeline wait of the tcgen05 kernels (aspire_set_wait_limit_ns);
 // 0 selects the default.
@@ -104,6 +104,13 @@ int32_t tc_min_kv() {
 bool tc_env_enabled() {
   const char* e = std::getenv("ASPIRE_B200_DISABLE_TC");
   return !(e && e[0] == '1');
+}
+
+// Whether the routing thresholds send every row to the tcgen05 kernel; read
+// from the environment once per process.
+bool all_rows_tc() {
+  static const bool v = tc_min_rows() <= 1;
+  return v;
 }
 
 }  // namespace
@@ -182,7 +189,9 @@ const char* aspire_kernel_names(void) {
          "aspire_select_pages_kernel\naspire_page_scores_kernel\naspire_build_indices_kernel\naspire_qkv_prologue_kernel\naspire_plan_device_kernel\n"
          "aspire_draft_spill_kernel\naspire_clear_dump_kernel\n"
          "aspire_w4_small_kernel\naspire_w4_tc_kernel\naspire_moe_route_kernel\naspire_moe_sort_kernel\naspire_moe_route_grad_kernel\n"
-         "aspire_moe_dispatch_kernel\naspire_moe_combine_kernel\naspire_moe_combine_grad_kernel\n";
+         "aspire_moe_dispatch_kernel\naspire_moe_combine_kernel\naspire_moe_combine_grad_kernel\n"
+         "aspire_attn_tree_kernel\naspire_step_tables_kernel\naspire_step_tokens_kernel\naspire_logits_kernel\n"
+         "aspire_pick_kernel\naspire_tree_accept_kernel\n";
 }
 
 int aspire_plan_host_only(const int32_t* qo_indptr, const int32_t* kv_indptr,
@@ -283,17 +292,23 @@ int aspire_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_
                     "aspire_plan: cudaMemcpyAsync(plan upload)");
 }
 
-int aspire_mixed_attention(const AspireAttnArgs* a, const AspirePlanInfo* plan, void* stream) {
-  clear_error();
-  int rc = check_attention_args(a, plan, "aspire_mixed_attention");
+}  // extern "C"
+
+namespace {
+
+// The planned attention; under a tree mask when tree_mask is set.
+int run_attention(const AspireAttnArgs* a, const int32_t* tree_mask, int32_t mask_words, const AspirePlanInfo* plan,
+                  void* stream, const char* who) {
+  const std::string w(who);
+  int rc = check_attention_args(a, plan, who);
   if (rc) return rc;
-  if (!a->int_ws) return set_error(ASPIRE_ERR_INVALID, "aspire_mixed_attention: null int workspace");
+  if (!a->int_ws) return set_error(ASPIRE_ERR_INVALID, w + ": null int workspace");
   if (size_t(plan->int_bytes) + kStatusBytes > a->int_ws_bytes)
-    return set_error(ASPIRE_ERR_CAPACITY, "aspire_mixed_attention: int workspace smaller than plan");
+    return set_error(ASPIRE_ERR_CAPACITY, w + ": int workspace smaller than plan");
   if (size_t(plan->float_bytes) > a->float_ws_bytes)
-    return set_error(ASPIRE_ERR_CAPACITY, "aspire_mixed_attention: float workspace smaller than plan");
+    return set_error(ASPIRE_ERR_CAPACITY, w + ": float workspace smaller than plan");
   if (plan->num_merge > 0 && !a->float_ws)
-    return set_error(ASPIRE_ERR_INVALID, "aspire_mixed_attention: split-KV needs a float workspace");
+    return set_error(ASPIRE_ERR_INVALID, w + ": split-KV needs a float workspace");
   const int group = a->num_qo_heads / a->num_kv_heads;
   // The tcgen05 kernel takes rows only when a whole query position fits its tile.
   const bool run_tc = plan->tc_enabled && group <= kTcQTile;
@@ -338,15 +353,15 @@ int aspire_mixed_attention(const AspireAttnArgs* a, const AspirePlanInfo* plan, 
   p.status = static_cast<uint32_t*>(a->int_ws);
   p.partial_o = static_cast<float*>(a->float_ws);
   p.wait_ns = wait_limit_ns();
+  p.tree_mask = tree_mask;
+  p.tree_words = mask_words;
 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // Kernels are launched with plan-independent grids: items live in device
   // memory, so a captured graph stays valid across re-plans.  The CUDA-core
   // kernel is left out only when the routing thresholds send every row to
-  // the tcgen05 kernel (no plan can then hold a CUDA-core item); the
-  // thresholds are read from the environment once per process.
-  static const bool all_rows_tc = tc_min_rows() <= 1;
-  if (!(run_tc && all_rows_tc)) {
+  // the tcgen05 kernel (no plan can then hold a CUDA-core item).
+  if (!(run_tc && all_rows_tc())) {
     const size_t smem = gather_smem_bytes();
     rc = ensure_smem(reinterpret_cast<const void*>(&aspire_attn_gather_kernel), smem, g_gather_smem);
     if (rc) return rc;
@@ -356,7 +371,8 @@ int aspire_mixed_attention(const AspireAttnArgs* a, const AspirePlanInfo* plan, 
   }
   if (run_tc) {
     const size_t smem = tc_smem_bytes();
-    rc = ensure_smem(reinterpret_cast<const void*>(&aspire_attn_tc_kernel), smem, g_tc_smem);
+    const auto kernel = tree_mask ? &aspire_attn_tree_kernel : &aspire_attn_tc_kernel;
+    rc = ensure_smem(reinterpret_cast<const void*>(kernel), smem, tree_mask ? g_tree_smem : g_tc_smem);
     if (rc) return rc;
     alignas(64) CUtensorMap tmap;
     rc = encode_kv_tensor_map(&tmap, a->kv_cache, a->num_pages_total, a->num_kv_heads);
@@ -369,13 +385,37 @@ int aspire_mixed_attention(const AspireAttnArgs* a, const AspirePlanInfo* plan, 
     rc = encode_q_tensor_map(&qmap_pf, a->q, a->q_rows, a->num_qo_heads, a->q_stride_n, a->q_stride_h, group,
                              p.pf_box_tokens);
     if (rc) return rc;
-    rc = launch(aspire_attn_tc_kernel, dim3(plan->num_ctas * kTcCtasPerSm), dim3(tc_threads()), smem, st,
-                "aspire_attn_tc_kernel launch", p, tmap, qmap, qmap_pf);
+    rc = launch(kernel, dim3(plan->num_ctas * kTcCtasPerSm), dim3(tc_threads()), smem, st,
+                tree_mask ? "aspire_attn_tree_kernel launch" : "aspire_attn_tc_kernel launch", p, tmap, qmap, qmap_pf);
     if (rc) return rc;
   }
   // Split-KV merge (exits at once when the current plan split nothing).
   return launch(aspire_attn_merge_kernel, dim3(plan->num_ctas * kMergeCtasPerSm), dim3(kMergeThreads), 0, st,
                 "aspire_attn_merge_kernel launch", p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int aspire_mixed_attention(const AspireAttnArgs* a, const AspirePlanInfo* plan, void* stream) {
+  clear_error();
+  return run_attention(a, nullptr, 0, plan, stream, "aspire_mixed_attention");
+}
+
+int aspire_tree_attention(const AspireAttnArgs* a, const int32_t* tree_mask, int32_t mask_words,
+                          const AspirePlanInfo* plan, void* stream) {
+  clear_error();
+  if (!a || !plan || !tree_mask) return set_error(ASPIRE_ERR_INVALID, "aspire_tree_attention: null argument");
+  if (mask_words <= 0) return set_error(ASPIRE_ERR_INVALID, "aspire_tree_attention: mask_words must be > 0");
+  if (plan->causal) return set_error(ASPIRE_ERR_INVALID, "aspire_tree_attention: the plan must be made with causal 0");
+  if (a->dump) return set_error(ASPIRE_ERR_INVALID, "aspire_tree_attention: no dump under a tree mask");
+  if (a->num_kv_heads <= 0 || !plan->tc_enabled || a->num_qo_heads / a->num_kv_heads > kTcQTile || !all_rows_tc())
+    return set_error(ASPIRE_ERR_INVALID,
+                     "aspire_tree_attention: needs the default routing and at most 48 query heads per KV head");
+  if (!plan->on_device && int64_t(plan->max_q_len) > int64_t(32) * mask_words)
+    return set_error(ASPIRE_ERR_INVALID, "aspire_tree_attention: a row has more queries than its masks have bits");
+  return run_attention(a, tree_mask, mask_words, plan, stream, "aspire_tree_attention");
 }
 
 int aspire_append_kv(const AspireAppendArgs* a, void* stream) {
@@ -425,14 +465,14 @@ int aspire_append_kv(const AspireAppendArgs* a, void* stream) {
                 static_cast<cudaStream_t>(stream), "aspire_append_kv_kernel launch", p);
 }
 
-int aspire_qkv_prologue(const AspirePrologueArgs* a, void* stream) {
+static int run_prologue(const AspirePrologueArgs* a, const int32_t* positions, void* stream) {
   clear_error();
   if (!a) return set_error(ASPIRE_ERR_INVALID, "aspire_qkv_prologue: null argument");
   if (a->head_dim != kHeadDim || a->page_size != kPageSize)
     return set_error(ASPIRE_ERR_INVALID, "aspire_qkv_prologue: head_dim must be 128 and page_size 16");
   if (a->num_tokens <= 0 || a->num_rows < 0) return ASPIRE_OK;
   if (!a->q || !a->k || !a->v || !a->q_out || !a->kv_cache || !a->append_indptr || !a->page_indptr ||
-      !a->last_page_len || (a->num_rows > 0 && !a->rope_offsets))
+      !a->last_page_len || (a->num_rows > 0 && !a->rope_offsets && !positions))
     return set_error(ASPIRE_ERR_INVALID, "aspire_qkv_prologue: null pointer");
   if (!a->page_indices && (!a->mode_flags || !a->draft_table || !a->block_table))
     return set_error(ASPIRE_ERR_INVALID, "aspire_qkv_prologue: page_indices or the three page tables are required");
@@ -483,6 +523,7 @@ int aspire_qkv_prologue(const AspirePrologueArgs* a, void* stream) {
   p.k_norm_w = static_cast<const __nv_bfloat16*>(a->k_norm_weight);
   p.eps = a->norm_eps;
   p.rope_offsets = a->rope_offsets;
+  p.positions = positions;
   // The constants FlashInfer derives on the host: reciprocals in fp32, the
   // Llama-3.1 smoothing line from double-precision pi.
   p.rcp_theta = 1.0f / a->rope_theta;
@@ -501,6 +542,14 @@ int aspire_qkv_prologue(const AspirePrologueArgs* a, void* stream) {
   const unsigned ny = static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>((units_per_row + 31) / 32, 1), 64));
   return launch(aspire_qkv_prologue_kernel, dim3(static_cast<unsigned>(a->num_rows + 1), ny), dim3(256), 0,
                 static_cast<cudaStream_t>(stream), "aspire_qkv_prologue_kernel launch", p);
+}
+
+int aspire_qkv_prologue(const AspirePrologueArgs* a, void* stream) { return run_prologue(a, nullptr, stream); }
+
+int aspire_qkv_prologue_at(const AspirePrologueArgs* a, const int32_t* positions, void* stream) {
+  clear_error();
+  if (!positions) return set_error(ASPIRE_ERR_INVALID, "aspire_qkv_prologue_at: null positions");
+  return run_prologue(a, positions, stream);
 }
 
 int aspire_build_unified_indices(const AspireIndicesArgs* a, void* stream) {

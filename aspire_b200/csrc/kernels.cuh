@@ -56,6 +56,7 @@ struct PrologueParams {
   const __nv_bfloat16* k_norm_w;
   float eps;
   const int32_t* rope_offsets;  // position of each row's first new token
+  const int32_t* positions;     // each token's own position, or NULL
   float rcp_theta, rcp_scale, smooth_a, smooth_b;
   int32_t num_qo_heads;
 };
@@ -165,6 +166,9 @@ __global__ void aspire_attn_gather_kernel(AttnParams p);
 __global__ void aspire_attn_tc_kernel(AttnParams p, const __grid_constant__ CUtensorMap tmap,
                                       const __grid_constant__ CUtensorMap qmap,
                                       const __grid_constant__ CUtensorMap qmap_pf);
+__global__ void aspire_attn_tree_kernel(AttnParams p, const __grid_constant__ CUtensorMap tmap,
+                                        const __grid_constant__ CUtensorMap qmap,
+                                        const __grid_constant__ CUtensorMap qmap_pf);
 constexpr int kMergeThreads = 128;
 constexpr int kMergeCtasPerSm = 4;
 __global__ void aspire_attn_merge_kernel(AttnParams p);

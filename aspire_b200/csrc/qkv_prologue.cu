@@ -13,7 +13,7 @@
 // permutation sends element i of the first half to 2i and element 64+i to
 // 2i+1.  RoPE rotates the pair (2p, 2p+1) by pos * freq_p with
 // freq_p = theta^(-2p/128) (scaled, with the Llama-3.1 smoothing when set),
-// pos = offsets[b] + (t - append_indptr[b]), using the fast powf / sincosf
+// pos = offsets[b] + (t - append_indptr[b]) or the token's own, using the fast powf / sincosf
 // intrinsics as FlashInfer's kernel does.  Tokens after the last row (bucket
 // padding) get the norm and permutation but no rotation and no append, as in
 // the reference, where the norm runs over the whole tensor and the RoPE and
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(256) aspire_qkv_prologue_kernel(PrologueParams
     page_begin = ap.page_indptr[b];
     page_count = ap.page_indptr[b + 1] - page_begin;
     seq_len = page_count > 0 ? (page_count - 1) * kPageSize + ap.last_page_len[b] : 0;
-    rope_base = p.rope_offsets[b];
+    if (!p.positions) rope_base = p.rope_offsets[b];
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hq = p.num_qo_heads, hkv = ap.num_kv_heads;
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(256) aspire_qkv_prologue_kernel(PrologueParams
     const int s = static_cast<int>(e - int64_t(i) * slots);
     const int64_t t = int64_t(start) + i;
     if (t >= ap.num_tokens) break;
-    const int64_t rope_pos = int64_t(rope_base) + i;
+    const int64_t rope_pos = p.positions ? int64_t(p.positions[t]) : int64_t(rope_base) + i;
     if (s < hq) {
       float v[4];
       transform_row(p, p.q + t * p.q_stride_n + int64_t(s) * p.q_stride_h, p.q_norm_w, !tail, rope_pos, lane, v);

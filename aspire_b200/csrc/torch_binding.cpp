@@ -1,5 +1,6 @@
-// The feed-forward operators' Python calls: argument checks, outputs and the
-// call of the C ABI (include/aspire_b200.h) on torch's current stream.
+// The feed-forward and tree-step operators' Python calls: argument checks,
+// outputs and the call of the C ABI (include/aspire_b200.h) on torch's current
+// stream.
 //
 // A decode step's calls are a few microseconds on the device, less than the
 // same checks take attribute by attribute in Python, so they are made here on
@@ -10,12 +11,14 @@
 // file launches nothing.
 #include <Python.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <initializer_list>
 #include <stdexcept>
 #include <string>
 #include <type_traits>
 #include <utility>
+#include <vector>
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
@@ -39,6 +42,11 @@ struct {
   decltype(&aspire_moe_dispatch) moe_dispatch;
   decltype(&aspire_moe_combine) moe_combine;
   decltype(&aspire_moe_combine_grad) moe_combine_grad;
+  decltype(&aspire_step_tables) step_tables;
+  decltype(&aspire_logits_workspace) logits_workspace;
+  decltype(&aspire_adjust_logits) adjust_logits;
+  decltype(&aspire_tree_accept) tree_accept;
+  decltype(&aspire_tree_attention) tree_attention;
 } abi = {};
 
 // A refused argument; becomes ValueError.
@@ -77,7 +85,7 @@ const Tensor& tensor(PyObject* o) {
   if (!THPVariable_Check(o)) throw Invalid("a tensor is required");
   const Tensor& t = THPVariable_Unpack(o);
   // A tangent would be dropped, not carried through.
-  require(!t._fw_grad(0).defined(), "the feed-forward operators have no forward-mode derivative");
+  require(!t._fw_grad(0).defined(), "the feed-forward and tree-step operators have no forward-mode derivative");
   return t;
 }
 // NULL for None.
@@ -440,6 +448,287 @@ std::pair<Tensor, Tensor> combine_grad(const Tensor& grad_in, const Tensor& rows
   return {d_rows, d_weights};
 }
 
+// ----------------------------------------------------------------- tree step
+// A contiguous int32 vector of `n` entries (any number for n < 0) on `like`'s device.
+int32_t* ints(const Tensor* t, int64_t n, const Tensor& like, const char* name) {
+  if (!t) return nullptr;
+  if (t->scalar_type() != at::kInt || t->dim() != 1 || !t->is_contiguous() || t->device() != like.device() ||
+      (n >= 0 && t->size(0) != n))
+    throw Invalid(std::string(name) + " must be a contiguous int32 vector of the right length on the operands' device");
+  return static_cast<int32_t*>(t->data_ptr());
+}
+
+// A 2-D int32 tensor with contiguous rows.
+int32_t* int_rows(const Tensor& t, int64_t rows, const Tensor& like, const char* name) {
+  if (t.scalar_type() != at::kInt || t.dim() != 2 || t.size(0) != rows || t.device() != like.device() ||
+      (t.size(1) > 1 && rows > 0 && t.stride(1) != 1) || t.size(1) > INT32_MAX)
+    throw Invalid(std::string(name) + " must be a 2-D int32 tensor with contiguous rows on the operands' device");
+  return static_cast<int32_t*>(t.data_ptr());
+}
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// Whether the memory of two tensors, first to last element, has a byte in common.
+bool in_common(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto span = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    return std::make_pair(at, at + uintptr_t((last + 1) * t.element_size()));
+  };
+  const auto x = span(a), y = span(b);
+  return x.first < y.second && y.first < x.second;
+}
+
+struct Tables {
+  Tensor qo_indptr, kv_indptr, kv_len, last_page_len, positions, slots, tree_mask;
+};
+
+Tables step_tables(const Tensor& lengths, const Tensor* new_tokens, const Tensor& table, const Tensor& held,
+                   const Tensor& free_pages, const Tensor& free_count, int64_t tokens, const Tensor* parents,
+                   int64_t max_nodes, int64_t page_size, const Tensor* status) {
+  require(lengths.is_cuda() && lengths.dim() == 1, "lengths must be a 1-D CUDA tensor");
+  const int64_t rows = lengths.size(0);
+  require(rows <= INT32_MAX && tokens >= 0 && tokens <= INT32_MAX, "sizes past 32 bits");
+  require(page_size >= 1 && page_size <= INT32_MAX, "page_size must be positive");
+  require(!parents || (max_nodes >= 1 && max_nodes <= INT32_MAX - 31), "parents need max_nodes, the nodes of the largest tree");
+  AspireStepTablesArgs a = {};
+  a.lengths = ints(&lengths, rows, lengths, "lengths");
+  a.new_tokens = ints(new_tokens, rows, lengths, "new_tokens");
+  a.rows = int32_t(rows);
+  a.page_size = int32_t(page_size);
+  a.block_table = int_rows(table, rows, lengths, "block_table");
+  a.block_table_stride = row_stride(table);
+  a.block_table_cols = int32_t(table.size(1));
+  require(rows <= 1 || table.stride(0) >= table.size(1), "block_table's rows must not overlap");
+  a.held = ints(&held, rows, lengths, "held");
+  a.free_pages = ints(&free_pages, -1, lengths, "free_pages");
+  a.free_capacity = free_pages.size(0);
+  require(a.free_capacity <= INT32_MAX, "sizes past 32 bits");
+  a.free_count = ints(&free_count, 1, lengths, "free_count");
+  a.parents = ints(parents, tokens, lengths, "parents");
+  const Tensor* written[] = {&table, &held, &free_pages, &free_count};
+  const Tensor* read[] = {&lengths, new_tokens, parents};
+  for (int i = 0; i < 4; ++i) {
+    for (int j = i + 1; j < 4; ++j)
+      require(!in_common(*written[i], *written[j]), "block_table, held, free_pages and free_count must not overlap");
+    for (const Tensor* r : read)
+      require(!r || !in_common(*written[i], *r), "what the call changes must not overlap what it reads");
+  }
+  for (const Tensor* w : written) w->unsafeGetTensorImpl()->bump_version();
+  const auto i32 = lengths.options();
+  Tables t;
+  t.qo_indptr = at::empty({rows + 1}, i32);
+  t.kv_indptr = at::empty({rows + 1}, i32);
+  t.kv_len = at::empty({rows}, i32);
+  t.last_page_len = at::empty({rows}, i32);
+  // (Without rows no kernel writes the tokens' tables.)
+  const auto make = [&](at::IntArrayRef size, const auto& options, int64_t fill) {
+    return rows ? at::empty(size, options) : at::full(size, fill, options);
+  };
+  t.positions = make({tokens}, i32, 0);
+  t.slots = make({tokens}, i32.dtype(at::kLong), -1);
+  a.qo_indptr = static_cast<int32_t*>(t.qo_indptr.data_ptr());
+  a.kv_indptr = static_cast<int32_t*>(t.kv_indptr.data_ptr());
+  a.kv_len = static_cast<int32_t*>(t.kv_len.data_ptr());
+  a.last_page_len = static_cast<int32_t*>(t.last_page_len.data_ptr());
+  a.positions = static_cast<int32_t*>(t.positions.data_ptr());
+  a.slots = static_cast<int64_t*>(t.slots.data_ptr());
+  a.tokens = tokens;
+  if (parents) {
+    a.tree_mask_words = int32_t((max_nodes + 31) / 32);
+    t.tree_mask = make({tokens, a.tree_mask_words}, i32, 0);
+    a.tree_mask = static_cast<int32_t*>(t.tree_mask.data_ptr());
+    if (!a.parents) a.parents = a.qo_indptr;  // (no tokens, no address: nothing is read through it)
+  }
+  a.status = status_word(status, lengths);
+  on_device(lengths, [&](void* stream) { check(abi.step_tables(&a, stream), "aspire_step_tables"); });
+  return t;
+}
+
+const float* row_terms(const Tensor* t, int64_t rows, const Tensor& like, const char* name) {
+  if (!t) return nullptr;
+  if (t->scalar_type() != at::kFloat || t->dim() != 1 || t->size(0) != rows || !t->is_contiguous() ||
+      t->device() != like.device())
+    throw Invalid(std::string(name) + " must be contiguous float32 [rows] on the logits' device");
+  return static_cast<const float*>(t->data_ptr());
+}
+
+struct LogitsCall {
+  const Tensor &logits;
+  const Tensor *history, *history_len, *prompt_len, *indptr, *tokens, *tree_mask, *repetition, *frequency, *presence,
+      *bias_indptr, *bias_ids, *bias_values, *allowed, *out;
+  bool want_out, want_ids;
+  const Tensor* status;
+};
+
+std::pair<Tensor, Tensor> adjust_logits(const LogitsCall& c) {
+  const Tensor& x = c.logits;
+  require(x.dim() == 2 && type_of(x) >= 0 && x.is_cuda(),
+          "logits must be a [tokens, vocab] CUDA tensor of float32, bfloat16 or float16");
+  for (const Tensor* t : {&x, c.repetition, c.frequency, c.presence, c.bias_values})
+    require(!t || !at::GradMode::is_enabled() || !t->requires_grad(),
+            "adjusted logits have no gradient: detach the operands or call under torch.no_grad()");
+  const int64_t tokens = x.size(0), vocab = x.size(1);
+  require(vocab >= 1 && vocab <= INT32_MAX && tokens <= INT32_MAX, "tokens or vocab out of range");
+  require(tokens == 0 || vocab == 1 || x.stride(1) == 1, "logits need contiguous rows");
+  const int64_t rows = c.indptr ? c.indptr->numel() - 1 : tokens;
+  require(!c.indptr || rows >= 0, "indptr must be [rows + 1]");
+  require(rows <= 65534, "at most 65534 rows are supported");
+  AspireLogitsArgs a = {};
+  a.logits = x.data_ptr();
+  a.logits_stride = tokens > 1 ? x.stride(0) : vocab;
+  require(a.logits_stride >= vocab, "logits' rows must not overlap");
+  a.type = type_of(x);
+  a.tokens = tokens;
+  a.vocab = int32_t(vocab);
+  a.rows = int32_t(rows);
+  a.indptr = ints(c.indptr, rows + 1, x, "indptr");
+  require(!c.history == !c.history_len, "history and history_len go together");
+  require(!c.prompt_len || c.history, "prompt_len needs a history");
+  if (c.history) {
+    a.history = int_rows(*c.history, rows, x, "history");
+    a.history_stride = row_stride(*c.history);
+    a.history_cols = int32_t(c.history->size(1));
+    a.history_len = ints(c.history_len, rows, x, "history_len");
+    a.prompt_len = ints(c.prompt_len, rows, x, "prompt_len");
+    if (a.history_cols == 0) a.history = nullptr;
+  }
+  a.step_tokens = ints(c.tokens, tokens, x, "tokens");
+  if (c.tree_mask) {
+    require(c.tokens, "tree_mask needs tokens");
+    a.tree_mask = int_rows(*c.tree_mask, tokens, x, "tree_mask");
+    require(c.tree_mask->is_contiguous() && c.tree_mask->size(1) >= 1, "tree_mask must be contiguous [tokens, words]");
+    a.tree_mask_words = int32_t(c.tree_mask->size(1));
+  }
+  a.repetition = row_terms(c.repetition, rows, x, "repetition");
+  a.frequency = row_terms(c.frequency, rows, x, "frequency");
+  a.presence = row_terms(c.presence, rows, x, "presence");
+  require(!c.bias_indptr == !c.bias_ids && !c.bias_ids == !c.bias_values, "bias must be (indptr, ids, values)");
+  if (c.bias_indptr && c.bias_ids->numel() > 0) {
+    a.bias_indptr = ints(c.bias_indptr, rows + 1, x, "bias indptr");
+    a.bias_ids = ints(c.bias_ids, -1, x, "bias ids");
+    a.bias_values = row_terms(c.bias_values, c.bias_ids->numel(), x, "bias values");
+    a.bias_entries = c.bias_ids->numel();
+    require(a.bias_entries < INT32_MAX, "sizes past 32 bits");
+  }
+  if (c.allowed) {
+    a.allowed = int_rows(*c.allowed, tokens, x, "allowed");
+    a.allowed_stride = row_stride(*c.allowed);
+    require(c.allowed->size(1) >= (vocab + 31) / 32, "allowed must be [tokens, vocab / 32 rounded up]");
+  }
+  Tensor out, ids, workspace;
+  if (c.want_out) {
+    if (c.out) {
+      out = *c.out;
+      require(out.scalar_type() == x.scalar_type() && out.sizes() == x.sizes() && out.device() == x.device() &&
+                  (tokens == 0 || vocab == 1 || out.stride(1) == 1),
+              "out must be [tokens, vocab] of the logits' type with contiguous rows on their device");
+      a.out_stride = tokens > 1 ? out.stride(0) : vocab;
+      require(a.out_stride >= vocab, "out's rows must not overlap");
+      require(!(at::GradMode::is_enabled() && out.requires_grad()),
+              "out requires a gradient: give another, or use torch.no_grad()");
+      const Block o = block_of(out, a.out_stride), l = block_of(x, a.logits_stride);
+      require((o.at == l.at && (o.pitch == l.pitch || o.rows <= 1)) || !share(o, l),
+              "out may be the logits themselves, but must not overlap them otherwise");
+      for (const Tensor* t : {c.history, c.history_len, c.prompt_len, c.indptr, c.tokens, c.tree_mask, c.repetition,
+                              c.frequency, c.presence, c.bias_indptr, c.bias_ids, c.bias_values, c.allowed})
+        require(!t || !in_common(out, *t), "out must not overlap what the call reads");
+      out.unsafeGetTensorImpl()->bump_version();
+    } else {
+      out = at::empty({tokens, vocab}, x.options().requires_grad(false));
+      a.out_stride = vocab;
+    }
+    a.out = out.data_ptr();
+  }
+  a.status = status_word(c.status, x);
+  on_device(x, [&](void* stream) {
+    if (c.want_ids) {
+      const auto i32 = x.options().dtype(at::kInt).requires_grad(false);
+      ids = at::empty({tokens}, i32);
+      if (tokens > 0) {
+        a.workspace_bytes = abi.logits_workspace(tokens, a.rows, a.vocab, a.bias_indptr != nullptr);
+        workspace = at::empty({int64_t(a.workspace_bytes / 4)}, i32);
+        a.workspace = workspace.data_ptr();
+        a.ids = static_cast<int32_t*>(ids.data_ptr());
+      }
+    }
+    if (tokens > 0) check(abi.adjust_logits(&a, stream), "aspire_adjust_logits");
+  });
+  return {out, ids};
+}
+
+struct Walked {
+  Tensor count, path, tokens, lengths;
+};
+
+Walked tree_accept(const Tensor& tokens, const Tensor& parents, const Tensor& targets, const Tensor& indptr,
+                   const Tensor& lengths, int64_t max_path, const std::vector<const Tensor*>& caches,
+                   const Tensor* table, const Tensor* status) {
+  require(tokens.is_cuda() && tokens.dim() == 1, "tokens must be a 1-D CUDA tensor");
+  require(max_path >= 1 && max_path <= ASPIRE_MAX_PATH, "max_path must be between 1 and 64");
+  const int64_t total = tokens.size(0), rows = lengths.numel();
+  require(total <= INT32_MAX && rows <= INT32_MAX, "sizes past 32 bits");
+  AspireTreeAcceptArgs a = {};
+  a.tokens = ints(&tokens, total, tokens, "tokens");
+  a.parents = ints(&parents, total, tokens, "parents");
+  a.targets = ints(&targets, total, tokens, "targets");
+  a.lengths = ints(&lengths, rows, tokens, "lengths");
+  a.indptr = ints(&indptr, rows + 1, tokens, "indptr");
+  a.total = total;
+  a.rows = int32_t(rows);
+  a.max_path = int32_t(max_path);
+  std::vector<void*> at;
+  if (!caches.empty()) {
+    require(table, "caches need a block table");
+    a.block_table = int_rows(*table, rows, tokens, "block_table");
+    a.block_table_stride = row_stride(*table);
+    a.block_table_cols = int32_t(table->size(1));
+    const Tensor& first = *caches[0];
+    require(first.dim() == 5 && first.size(1) == 2, "a cache must be [pages, 2, page_size, heads, head_dim]");
+    for (const Tensor* c : caches)
+      require(c->sizes() == first.sizes() && c->scalar_type() == first.scalar_type() && c->is_contiguous() &&
+                  c->device() == tokens.device() && !(at::GradMode::is_enabled() && c->requires_grad()),
+              "caches must be contiguous tensors of one shape and type on the tokens' device, without gradients");
+    for (size_t i = 0; i < caches.size(); ++i)
+      for (size_t j = i + 1; j < caches.size(); ++j)
+        require(!in_common(*caches[i], *caches[j]), "a cache is given twice, or two of them overlap");
+    a.pages = first.size(0);
+    a.token_bytes = first.size(3) * first.size(4) * first.element_size();
+    require(first.size(2) >= 1 && first.size(2) <= INT32_MAX, "bad page size");
+    a.page_size = int32_t(first.size(2));
+    require(a.token_bytes >= 16 && a.token_bytes % 16 == 0, "a token's keys must be a positive multiple of 16 bytes");
+    for (const Tensor* c : caches) {
+      for (const Tensor* t : {&tokens, &parents, &targets, &indptr, &lengths, table})
+        require(!in_common(*c, *t), "a cache overlaps what the call reads");
+      at.push_back(c->data_ptr());
+      c->unsafeGetTensorImpl()->bump_version();
+    }
+  }
+  const auto i32 = tokens.options();
+  Walked w;
+  w.count = at::empty({rows}, i32);
+  w.path = at::empty({rows, max_path}, i32);
+  w.tokens = at::empty({rows, max_path}, i32);
+  w.lengths = at::empty({rows}, i32);
+  a.count = static_cast<int32_t*>(w.count.data_ptr());
+  a.path = static_cast<int32_t*>(w.path.data_ptr());
+  a.out_tokens = static_cast<int32_t*>(w.tokens.data_ptr());
+  a.new_lengths = static_cast<int32_t*>(w.lengths.data_ptr());
+  a.status = status_word(status, tokens);
+  if (rows == 0) return w;
+  on_device(tokens, [&](void* stream) {
+    size_t done = 0;
+    do {  // (more layers than a call takes: the walk is the same each time)
+      a.num_caches = int32_t(std::min(at.size() - done, size_t(ASPIRE_MAX_CACHES)));
+      a.caches = at.data() + done;
+      check(abi.tree_accept(&a, stream), "aspire_tree_accept");
+      done += size_t(a.num_caches);
+    } while (done < at.size());
+  });
+  return w;
+}
+
 // -------------------------------------------------------------------- Python
 PyObject* wrap(const Tensor& t) {
   if (!t.defined()) Py_RETURN_NONE;
@@ -566,9 +855,42 @@ PyObject* py_combine_grad(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// (lengths, new_tokens, block_table, held, free_pages, free_count, tokens, parents, max_nodes, page_size, status)
+PyObject* py_step_tables(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 11, [&] {
+    const Tables t = step_tables(tensor(v[0]), optional(v[1]), tensor(v[2]), tensor(v[3]), tensor(v[4]), tensor(v[5]),
+                                 integer(v[6]), optional(v[7]), integer(v[8]), integer(v[9]), optional(v[10]));
+    return wrap_all(t.qo_indptr, t.kv_indptr, t.kv_len, t.last_page_len, t.positions, t.slots, t.tree_mask);
+  });
+}
+// (logits, history, history_len, prompt_len, indptr, tokens, tree_mask, repetition, frequency, presence, bias indptr,
+// ids, values, allowed, out, want_out, want_ids, status) -> out, ids
+PyObject* py_adjust_logits(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 18, [&] {
+    const LogitsCall c = {tensor(v[0]),    optional(v[1]),  optional(v[2]),  optional(v[3]),  optional(v[4]),
+                          optional(v[5]),  optional(v[6]),  optional(v[7]),  optional(v[8]),  optional(v[9]),
+                          optional(v[10]), optional(v[11]), optional(v[12]), optional(v[13]), optional(v[14]),
+                          v[15] == Py_True, v[16] == Py_True, optional(v[17])};
+    const auto r = adjust_logits(c);
+    return wrap_all(r.first, r.second);
+  });
+}
+// (tokens, parents, targets, indptr, lengths, max_path, caches, block_table, status) -> count, path, tokens, lengths
+PyObject* py_tree_accept(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject* {
+    require(PyList_Check(v[6]) || PyTuple_Check(v[6]), "caches must be a list or tuple of tensors");
+    std::vector<const Tensor*> caches;
+    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(v[6]); ++i)
+      caches.push_back(&tensor(PySequence_Fast_GET_ITEM(v[6], i)));
+    const Walked w = tree_accept(tensor(v[0]), tensor(v[1]), tensor(v[2]), tensor(v[3]), tensor(v[4]), integer(v[5]),
+                                 caches, optional(v[7]), optional(v[8]));
+    return wrap_all(w.count, w.path, w.tokens, w.lengths);
+  });
+}
+
 // (addresses of the entry points, in the order of `abi`)
 PyObject* py_bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
-  return guarded(n, 8, [&]() -> PyObject* {
+  return guarded(n, 13, [&]() -> PyObject* {
     const auto at = [&](int i, auto& fn) {
       fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(PyLong_AsVoidPtr(v[i]));
       if (!fn) throw Invalid("an address is required");
@@ -581,6 +903,11 @@ PyObject* py_bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
     at(5, abi.moe_dispatch);
     at(6, abi.moe_combine);
     at(7, abi.moe_combine_grad);
+    at(8, abi.step_tables);
+    at(9, abi.logits_workspace);
+    at(10, abi.adjust_logits);
+    at(11, abi.tree_accept);
+    at(12, abi.tree_attention);
     Py_RETURN_NONE;
   });
 }
@@ -597,6 +924,9 @@ PyMethodDef kMethods[] = {
     ASPIRE_METHOD("dispatch_grad", py_dispatch_grad),
     ASPIRE_METHOD("combine", py_combine),
     ASPIRE_METHOD("combine_grad", py_combine_grad),
+    ASPIRE_METHOD("step_tables", py_step_tables),
+    ASPIRE_METHOD("adjust_logits", py_adjust_logits),
+    ASPIRE_METHOD("tree_accept", py_tree_accept),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

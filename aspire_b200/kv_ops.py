@@ -9,12 +9,14 @@ so ``torch.compile(fullgraph=True)`` can trace it.
 
 The module also holds the step's other cache and slot bookkeeping:
 ``build_unified_indices``, ``draft_page_spill``, ``qkv_prologue`` (norm +
-RoPE + append) and ``clear_dump_slots`` (dump-state reset of cleared slots).
+RoPE + append), ``clear_dump_slots`` (dump-state reset of cleared slots) and
+``build_step_tables`` (block tables and slot maps from the rows' lengths).
 """
 
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -220,7 +222,7 @@ def qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_append_in
                  norm_eps: float = 1e-6, rope_theta: float = 1e4, rope_scale: float = 1.0,
                  llama31: tuple[float, float, float] | None = None, q_out: torch.Tensor | None = None,
                  page_tables: tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None = None,
-                 status: torch.Tensor | None = None) -> torch.Tensor:
+                 status: torch.Tensor | None = None, positions: torch.Tensor | None = None) -> torch.Tensor:
     """One launch for a layer's attention prologue (C ABI ``aspire_qkv_prologue``):
     ``q_norm`` / ``k_norm`` with the HF-to-interleaved permutation
     (aspire/models/sparse_draft_transformer.py:150-158) when the norm weights
@@ -230,7 +232,10 @@ def qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_append_in
     aspire/models/mixed_transformer.py:159-197) at positions
     ``rope_offsets[b] + (t - kv_append_indptr[b])``, and the paged append of
     the rotated k and of v (``mylib::update_kv_padded``).  Returns the rotated
-    q (``q_out``, which may be ``q`` itself for the reference's in-place form)."""
+    q (``q_out``, which may be ``q`` itself for the reference's in-place form).
+    ``positions`` (int32 [tokens], C ABI ``aspire_qkv_prologue_at``) gives each
+    token its own position, as the nodes of a tree have; ``rope_offsets`` may
+    then be None."""
     total = q.shape[0]
     if q_out is None:
         q_out = torch.empty_like(q)
@@ -248,7 +253,8 @@ def qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_append_in
     for w in (q_norm_weight, k_norm_weight):
         if w is not None and (w.dtype != torch.bfloat16 or w.numel() != q.shape[2] or not w.is_contiguous()):
             raise ValueError("norm weights must be contiguous bfloat16 [head_dim] tensors")
-    ints = [("kv_append_indptr", kv_append_indptr), ("rope_offsets", rope_offsets),
+    ints = [("kv_append_indptr", kv_append_indptr),
+            ("rope_offsets", rope_offsets) if positions is None else ("positions", positions),
             ("kv_page_indptr", kv_page_indptr), ("kv_last_page_len", kv_last_page_len)]
     if kv_page_indices is not None:
         ints.append(("kv_page_indices", kv_page_indices))
@@ -260,7 +266,10 @@ def qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_append_in
     num_rows = kv_last_page_len.shape[0]
     if kv_append_indptr.shape[0] < num_rows + 1 or kv_page_indptr.shape[0] < num_rows + 1:
         raise ValueError("kv_append_indptr / kv_page_indptr need len(kv_last_page_len) + 1 entries")
-    if rope_offsets.shape[0] < num_rows:
+    if positions is not None:
+        if positions.device != q.device or positions.numel() < total:
+            raise ValueError("positions needs one entry per token on q's device")
+    elif rope_offsets.shape[0] < num_rows:
         raise ValueError("rope_offsets needs one entry per row")
     a = _capi.AspirePrologueArgs()
     a.q, a.q_stride_n, a.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1)
@@ -272,7 +281,7 @@ def qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_append_in
     a.q_norm_weight = q_norm_weight.data_ptr() if q_norm_weight is not None else None
     a.k_norm_weight = k_norm_weight.data_ptr() if k_norm_weight is not None else None
     a.norm_eps = float(norm_eps)
-    a.rope_offsets = rope_offsets.data_ptr()
+    a.rope_offsets = rope_offsets.data_ptr() if positions is None else None
     a.rope_theta, a.rope_scale = float(rope_theta), float(rope_scale)
     if llama31 is not None:
         a.low_freq_factor, a.high_freq_factor, a.old_context_len = (float(x) for x in llama31)
@@ -293,9 +302,66 @@ def qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_append_in
         a.block_table_stride = page_tables[2].stride(0)
     a.status = status.data_ptr() if status is not None else None
     stream = torch.cuda.current_stream(q.device).cuda_stream
+    if positions is not None:
+        rc = _capi.load_library().aspire_qkv_prologue_at(ctypes.byref(a), ctypes.c_void_p(positions.data_ptr()),
+                                                         ctypes.c_void_p(stream))
+        _capi.check(rc, "aspire_qkv_prologue_at")
+        return q_out
     rc = _capi.load_library().aspire_qkv_prologue(ctypes.byref(a), ctypes.c_void_p(stream))
     _capi.check(rc, "aspire_qkv_prologue")
     return q_out
+
+
+class StepTables(NamedTuple):
+    """What a step's kernels need of its rows and tokens.
+
+    ``qo_indptr`` int32 ``[rows + 1]``: the rows' tokens; ``kv_indptr`` int32
+    ``[rows + 1]``: their pages, prefix sums both; ``kv_len`` and
+    ``last_page_len`` int32 ``[rows]``; ``positions`` int32 ``[tokens]``;
+    ``slots`` int64 ``[tokens]``: a token's place in the cache, ``page *
+    page_size + offset``, -1 for none; ``tree_mask`` int32 ``[tokens, words]``
+    with parents, else None: bit j % 32 of word j / 32 for each node j of the
+    row that is the token or an ancestor of it."""
+
+    qo_indptr: torch.Tensor
+    kv_indptr: torch.Tensor
+    kv_len: torch.Tensor
+    last_page_len: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    tree_mask: torch.Tensor | None
+
+
+def build_step_tables(lengths: torch.Tensor, new_tokens: torch.Tensor | None, block_table: torch.Tensor,
+                      held: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor, *, tokens: int,
+                      parents: torch.Tensor | None = None, max_nodes: int | None = None, page_size: int = 16,
+                      status: torch.Tensor | None = None) -> StepTables:
+    """Block tables and slot maps of a step from the rows' lengths, on the GPU
+    (C ABI ``aspire_step_tables``): no readback, so the call can be captured in
+    a CUDA graph before ``plan_device``.
+
+    ``lengths`` int32 ``[rows]`` are the committed tokens, ``new_tokens`` (or
+    None) this step's.  Row b ends up with ``ceil((lengths[b] + new_tokens[b])
+    / page_size)`` pages: in place, ``held`` int32 ``[rows]`` counts the pages
+    in the first columns of ``block_table`` int32 ``[rows, columns]``, and
+    ``free_pages`` int32 ``[capacity]`` is a stack with ``free_count`` int32
+    ``[1]`` pages.  Pages that a row no longer needs go back first, their
+    entries become -1; a call with None for the new tokens trims the rows to
+    their committed lengths.  Rows are served in order: where the stack runs
+    out, the row and later ones that miss pages get ``kv_len`` 0 and slots -1,
+    and ``status`` gets ``ASPIRE_STATUS_NO_PAGES``; so do, with
+    ``ASPIRE_STATUS_BAD_ROW``, rows that outgrow the table.
+
+    ``tokens`` is the length of the step's token buffers (padding behind the
+    last row's tokens gets position 0, slot -1 and an empty mask).
+    ``parents`` int32 ``[tokens]`` makes every row a tree: its node 0 is the
+    root, a node's parent is an earlier node of the row (-1: none), its
+    position is the length plus its depth; ``max_nodes`` bounds a row's nodes
+    (a larger tree is not served)."""
+    if parents is not None and max_nodes is None:
+        raise ValueError("parents need max_nodes, the nodes of the largest tree")
+    return StepTables(*_capi.ops().step_tables(lengths, new_tokens, block_table, held, free_pages, free_count, tokens,
+                                               parents, max_nodes or 0, page_size, status))
 
 
 def clear_dump_slots(attention_weights_buffer: torch.Tensor, slot_ids: torch.Tensor, num_heads: int,

@@ -15,7 +15,10 @@
  *   4. planning: on the host, or on the device inside a CUDA graph;
  *   5. the feed-forward block around it: products with 4-bit weights (one
  *      matrix, or one per expert) and the tokens' way to their experts and
- *      back, with its gradients.
+ *      back, with its gradients;
+ *   6. a step of tree speculation: block tables and slot maps from lengths,
+ *      the attention's tree masks, penalties and masks on logits, the accepted
+ *      path with the move of its keys and values.
  *
  * Every entry point takes plain pointers, sizes and a CUDA stream handle
  * (passed as void*); no framework types cross this boundary.  Every entry
@@ -65,6 +68,7 @@ extern "C" {
 #define ASPIRE_STATUS_BAD_ROW 4u   /* attention row past q_rows, or selection
                                       row/argument out of range               */
 #define ASPIRE_STATUS_TIMEOUT 8u   /* a bounded device wait expired; the CTA stopped */
+#define ASPIRE_STATUS_NO_PAGES 16u /* aspire_step_tables: no free pages left for a row */
 
 /* Logit-dump variants (AspireAttnArgs.dump_kind, AspireSelectArgs.dump_kind),
  * the dump kinds of aspire/backends/jit_kernels.py:180-193: */
@@ -220,6 +224,18 @@ typedef struct AspireAttnArgs {
  * Capturable in a CUDA graph; allocates nothing.
  */
 ASPIRE_API int aspire_mixed_attention(const AspireAttnArgs* args, const AspirePlanInfo* plan, void* stream);
+
+/*
+ * The same with a tree mask, int32 [q_rows, mask_words]: the keys of a row's
+ * q_len queries are its last q_len keys, as for the causal mask; every query
+ * sees all keys before those, and of those key j iff bit j % 32 of word j / 32
+ * of the query's mask is set (a key past the last word is hidden).  A query
+ * that sees no key gets zeros and an LSE of -inf.  Keys and values that are
+ * hidden from some query must be finite.  Needs a plan made with causal 0 by
+ * the default routing, and no dump.  No counterpart in the reference.
+ */
+ASPIRE_API int aspire_tree_attention(const AspireAttnArgs* args, const int32_t* tree_mask, int32_t mask_words,
+                                     const AspirePlanInfo* plan, void* stream);
 
 /*
  * Sizes of the two device arrays that aspire_mixed_attention_noalloc uses
@@ -440,6 +456,13 @@ typedef struct AspirePrologueArgs {
  * reference: it replaces three of its ops.
  */
 ASPIRE_API int aspire_qkv_prologue(const AspirePrologueArgs* args, void* stream);
+
+/*
+ * The same with each token's own position, int32 [num_tokens], instead of
+ * rope_offsets (which is not read): the nodes of a tree lie one after another
+ * in the cache, at positions by their depth.
+ */
+ASPIRE_API int aspire_qkv_prologue_at(const AspirePrologueArgs* args, const int32_t* positions, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Mixed page list (device).                                                */
@@ -703,6 +726,141 @@ ASPIRE_API int aspire_set_wait_limit_ns(uint64_t ns);
 
 /* Names of the kernels the library launches, one per line (diagnostics). */
 ASPIRE_API const char* aspire_kernel_names(void);
+
+/* ------------------------------------------------------------------------ */
+/* A step of tree speculation (device).  No counterparts in the reference,   */
+/* which verifies one chain of drafts per row.                               */
+/* ------------------------------------------------------------------------ */
+
+typedef struct AspireStepTablesArgs {
+  const int32_t* lengths;    /* int32 [rows] committed tokens                     */
+  const int32_t* new_tokens; /* int32 [rows] tokens of this step; NULL: none      */
+  int32_t rows;
+  int32_t page_size;
+  int32_t* block_table;      /* int32 [rows, block_table_stride], in place        */
+  int64_t block_table_stride;
+  int32_t block_table_cols;
+  int32_t* held;             /* int32 [rows] pages a row holds, in place          */
+  int32_t* free_pages;       /* int32 [free_capacity] stack, in place             */
+  int32_t* free_count;       /* int32 [1] pages on the stack, in place            */
+  int64_t free_capacity;
+  const int32_t* parents;    /* int32 [tokens]: a node's parent within its row, -1
+                                without one; NULL: each row's tokens are a chain  */
+  int32_t tree_mask_words;   /* words of a token's mask (with parents)            */
+  int64_t tokens;            /* rows of the step's token buffers; 0: no tokens     */
+  int32_t* qo_indptr;        /* int32 [rows + 1] out                              */
+  int32_t* kv_indptr;        /* int32 [rows + 1] out: pages                       */
+  int32_t* kv_len;           /* int32 [rows] out                                  */
+  int32_t* last_page_len;    /* int32 [rows] out                                  */
+  int32_t* positions;        /* int32 [tokens] out                                */
+  int64_t* slots;            /* int64 [tokens] out: page * page_size + offset, -1 */
+  int32_t* tree_mask;        /* int32 [tokens, tree_mask_words] out (with parents) */
+  uint32_t* status;          /* optional device status word                       */
+} AspireStepTablesArgs;
+
+/*
+ * Block tables and slot maps of a step from the rows' lengths.  Row b needs
+ * ceil((lengths[b] + new_tokens[b]) / page_size) pages: those it holds beyond
+ * that go back on the stack of free pages (their table entries become -1),
+ * those it misses come from the top of the stack, for all rows in row order.
+ * Rows are served in order until the stack cannot give a row its pages
+ * (ASPIRE_STATUS_NO_PAGES); that row and later ones that miss pages, rows that
+ * outgrow their table and trees of more nodes than mask bits
+ * (ASPIRE_STATUS_BAD_ROW) keep what they hold and get kv_len 0 and slots -1.
+ * A token's position is its row's length plus its depth; its place in the
+ * cache is the length plus its index.  Tokens behind the last row's get
+ * position 0, slot -1 and an empty mask.  A parent that is not an earlier
+ * node counts as none (ASPIRE_STATUS_BAD_ROW).
+ */
+ASPIRE_API int aspire_step_tables(const AspireStepTablesArgs* args, void* stream);
+
+typedef struct AspireLogitsArgs {
+  const void* logits;        /* [tokens, vocab] of `type`, contiguous rows        */
+  int64_t logits_stride;
+  int32_t type;              /* ASPIRE_T_F32, ASPIRE_T_BF16 or ASPIRE_T_F16       */
+  int64_t tokens;
+  int32_t vocab;
+  int32_t rows;
+  const int32_t* indptr;     /* int32 [rows + 1]: row b's tokens; NULL: token b   */
+  const int32_t* history;    /* int32 [rows, history_stride] token ids, or NULL   */
+  int64_t history_stride;
+  int32_t history_cols;
+  const int32_t* history_len;/* int32 [rows] (with history)                       */
+  const int32_t* prompt_len; /* int32 [rows]: the history's first tokens that only
+                                the repetition penalty counts; NULL: none         */
+  const int32_t* step_tokens;/* int32 [tokens]: the step's own tokens, or NULL    */
+  const int32_t* tree_mask;  /* int32 [tokens, tree_mask_words]: which of its row's
+                                tokens precede a token (itself included); NULL:
+                                those before it and itself                        */
+  int32_t tree_mask_words;
+  const float* repetition;   /* fp32 [rows] each, or NULL                         */
+  const float* frequency;
+  const float* presence;
+  const int32_t* bias_indptr;/* int32 [rows + 1], or NULL                         */
+  const int32_t* bias_ids;   /* int32 [bias_entries]                              */
+  const float* bias_values;  /* fp32 [bias_entries]                               */
+  int64_t bias_entries;
+  const int32_t* allowed;    /* int32 [tokens, allowed_stride]: bit v % 32 of word
+                                v / 32 says that v may follow; NULL: all may      */
+  int64_t allowed_stride;
+  void* out;                 /* [tokens, vocab] of `type`, may be logits; NULL    */
+  int64_t out_stride;
+  int32_t* ids;              /* int32 [tokens] best tokens, or NULL               */
+  void* workspace;           /* with ids: aspire_logits_workspace bytes           */
+  size_t workspace_bytes;
+  uint32_t* status;          /* optional device status word                       */
+} AspireLogitsArgs;
+
+/* Bytes of workspace that a call with these sizes needs for its best tokens. */
+ASPIRE_API size_t aspire_logits_workspace(int64_t tokens, int32_t rows, int32_t vocab, int32_t with_bias);
+
+/*
+ * Penalties for repeated tokens, biases and grammar masks on logits (out), and
+ * the best token of the result (ids), in fp32.  Of token v with c occurrences
+ * in the row's history behind its prompt and on the token's path:
+ *   x = x > 0 ? x / repetition : x * repetition   (v anywhere in history or path)
+ *   x = x - frequency * c - presence * (c > 0);  x = x + bias;  -inf if not allowed
+ * A token that a row's biases list twice takes the later one.  Ids outside
+ * [0, vocab) are ignored.  The best token is the largest value, the lowest id
+ * on ties; NaN and -inf are never chosen (-1 if nothing else is left).  Tokens
+ * of no row keep their logits and get -1.
+ */
+ASPIRE_API int aspire_adjust_logits(const AspireLogitsArgs* args, void* stream);
+
+#define ASPIRE_MAX_CACHES 128
+#define ASPIRE_MAX_PATH 64
+typedef struct AspireTreeAcceptArgs {
+  const int32_t* tokens;     /* int32 [total] the nodes' tokens                   */
+  const int32_t* parents;    /* int32 [total] a node's parent within its row      */
+  const int32_t* targets;    /* int32 [total] the target's choice after each node */
+  const int32_t* indptr;     /* int32 [rows + 1]                                  */
+  const int32_t* lengths;    /* int32 [rows] committed tokens before the step     */
+  int64_t total;
+  int32_t rows;
+  int32_t max_path;          /* 1 .. ASPIRE_MAX_PATH                              */
+  int32_t* count;            /* int32 [rows] out: nodes walked                    */
+  int32_t* path;             /* int32 [rows, max_path] out, -1 behind the path    */
+  int32_t* out_tokens;       /* int32 [rows, max_path] out, -1 behind the path    */
+  int32_t* new_lengths;      /* int32 [rows] out, apart from lengths              */
+  void* const* caches;       /* host array of num_caches device pointers: one
+                                layer's [pages, 2, page_size, token_bytes] each    */
+  int32_t num_caches;        /* 0 .. ASPIRE_MAX_CACHES                            */
+  int64_t pages;
+  int32_t page_size;
+  int64_t token_bytes;       /* K (or V) bytes of a token, a multiple of 16       */
+  const int32_t* block_table;/* int32 [rows, block_table_stride]                  */
+  int64_t block_table_stride;
+  int32_t block_table_cols;
+  uint32_t* status;          /* optional device status word                       */
+} AspireTreeAcceptArgs;
+
+/*
+ * Walks each row's tree from node 0 along the target's choices (the first
+ * child whose token is targets[node]) and moves the walked nodes' keys and
+ * values from places lengths[b] + node to lengths[b] + 0, 1, 2, ... in every
+ * cache.  A place whose page is missing is not moved (ASPIRE_STATUS_BAD_PAGE).
+ */
+ASPIRE_API int aspire_tree_accept(const AspireTreeAcceptArgs* args, void* stream);
 
 #ifdef __cplusplus
 }

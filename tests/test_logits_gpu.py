@@ -1,0 +1,207 @@
+"""Penalties, biases and grammar masks on logits against the definition: in 64
+bits with the bound of the fp32 roundings, and the best token against the same
+formula in fp32, step by step."""
+
+import math
+import random
+
+import pytest
+import torch
+
+from aspire_b200.logits import adjust_logits, pick_tokens
+import tree_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def _pack(allowed):
+    t, v = allowed.shape
+    words = (v + 31) // 32
+    bits = torch.zeros(t, words * 32, dtype=torch.int64)
+    bits[:, :v] = allowed.long()
+    w = (bits.view(t, words, 32) << torch.arange(32)).sum(2)
+    return torch.where(w >= 2 ** 31, w - 2 ** 32, w).to(torch.int32)
+
+
+class Case:
+    def __init__(self, seed, sizes, vocab, dtype, hist=50, bias=0, allowed=False, tree=True, path=True, prompt=True,
+                 terms=("repetition", "frequency", "presence"), pad=0, row_pad=0, dense=False):
+        rng = random.Random(seed)
+        g = torch.Generator().manual_seed(seed)
+        rows, total = len(sizes), sum(sizes)
+        t = total + pad
+        self.base = (torch.randn(t, vocab + row_pad, generator=g) * 3).to(dtype)
+        self.logits = self.base[:, :vocab]
+        span = max(2, vocab // 4) if not dense else 5
+        ident = lambda: rng.choice([rng.randrange(min(span, vocab)), rng.randrange(vocab), vocab - 1, 0])  # noqa: E731
+        self.history = [[ident() for _ in range(rng.choice([0, 1, hist, rng.randint(0, hist)]))] for _ in range(rows)]
+        self.prompts = [rng.choice([0, len(h) // 2, len(h)]) if prompt else 0 for h in self.history]
+        self.row_of = [b for b, n in enumerate(sizes) for _ in range(n)] + [-1] * pad
+        self.tokens = [ident() for _ in range(t)]
+        paths = [p for n in sizes for p in (ref.ancestors(ref.random_parents(rng, n)) if n else [])]
+        if not tree:
+            paths = [list(range(i + 1)) for n in sizes for i in range(n)]
+        words = (max(sizes + [1]) + 31) // 32
+        self.mask = ref.mask_words(paths, words) + [[-1] * words] * pad
+        at = ref.indptr(sizes)
+        self.paths = [[self.tokens[at[b] + j] for j in p] if path else [] for b, p in zip(self.row_of, paths)] + [[]] * pad
+        f32 = lambda: torch.rand(rows, generator=g) + 0.5  # noqa: E731
+        self.terms = {k: f32() if k in terms else None for k in ("repetition", "frequency", "presence")}
+        self.bias = None
+        if bias:
+            lists = [[(ident(), rng.uniform(-9, 9)) for _ in range(rng.choice([0, bias]))] for _ in range(rows)]
+            self.bias_lists = lists
+            self.bias = [dict(p) for p in lists]  # (of a token listed twice the later value)
+        self.allowed = (torch.rand(t, vocab, generator=g) < 0.5) if allowed else None
+        if allowed and total > 1:
+            self.allowed[1] = False  # nothing may follow
+        self.sizes, self.tree, self.path, self.prompt = sizes, tree, path, prompt
+
+    def args(self, dev):
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+        cols = max([len(h) for h in self.history] + [0]) + 2
+        # What lies behind a history's end must not count.
+        hist = [h + [0] * (cols - len(h)) for h in self.history]
+        kw = dict(history=i32(hist), history_len=i32([len(h) for h in self.history]), indptr=i32(ref.indptr(self.sizes)))
+        if self.prompt:
+            kw["prompt_len"] = i32(self.prompts)
+        if self.path:
+            kw["tokens"] = i32(self.tokens)
+            if self.tree:
+                kw["tree_mask"] = i32(self.mask)
+        kw.update({k: v.to(dev) for k, v in self.terms.items() if v is not None})
+        if self.bias is not None:
+            flat = [p for r in self.bias_lists for p in r]
+            kw["bias"] = (i32(ref.indptr([len(r) for r in self.bias_lists])), i32([a for a, _ in flat]),
+                          torch.tensor([w for _, w in flat], dtype=torch.float32, device=dev))
+        if self.allowed is not None:
+            kw["allowed"] = _pack(self.allowed).to(dev)
+        return kw
+
+    def check(self, dev):
+        x32, x64, bound = ref.adjust(self.logits, self.row_of, self.history, self.prompts, self.paths, *(
+            self.terms[k] for k in ("repetition", "frequency", "presence")), self.bias, self.allowed)
+        base = self.base.to(dev)
+        logits = base[:, :self.logits.shape[1]]
+        kw = self.args(dev)
+        got = adjust_logits(logits, **kw)
+        ids = pick_tokens(logits, **kw)
+        assert torch.equal(base.cpu(), self.base), "the logits were changed"
+        # The fp32 steps and their one rounding, and the definition with its bound.
+        assert torch.equal(got.cpu(), x32.to(self.logits.dtype))
+        d = (got.double().cpu() - x64).abs()
+        fin = torch.isfinite(x64)
+        assert bool((d[fin] <= bound[fin]).all())
+        assert bool((got.double().cpu()[~fin] == x64[~fin]).all())
+        assert ids.cpu().tolist() == ref.pick(x32, self.row_of)
+        # In place, the columns behind the vocabulary untouched.
+        assert adjust_logits(logits, out=logits, **kw) is logits
+        assert torch.equal(logits, got)
+        assert torch.equal(base[:, self.logits.shape[1]:].cpu(), self.base[:, self.logits.shape[1]:])
+
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes,vocab", [([1], 1), ([1], 31), ([3, 0, 2], 1000), ([1, 1, 1], 32001), ([40, 7], 517),
+                                         ([2, 5], 60000)])
+def test_everything_at_once(cuda_device, sizes, vocab, dtype):
+    Case(vocab, sizes, vocab, dtype, bias=9, allowed=True, pad=2).check(cuda_device)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("row_pad", [1, 3, 8])
+def test_rows_at_any_alignment(cuda_device, dtype, row_pad):
+    Case(row_pad, [2, 3], 4099, dtype, bias=5, allowed=True, row_pad=row_pad).check(cuda_device)
+
+
+@pytest.mark.parametrize("terms", [(), ("repetition",), ("frequency",), ("presence",)])
+def test_terms_alone(cuda_device, terms):
+    Case(len(terms), [4, 1, 9], 777, torch.bfloat16, terms=terms).check(cuda_device)
+
+
+@pytest.mark.parametrize("kw", [dict(tree=False), dict(path=False), dict(prompt=False), dict(hist=0),
+                                dict(hist=5000, dense=True), dict(bias=300, dense=True), dict(hist=3000, bias=40)])
+def test_what_counts(cuda_device, kw):
+    Case(3, [5, 2, 0, 33], 2500, torch.float32, **kw).check(cuda_device)
+
+
+def test_one_row_a_token_without_indptr(cuda_device):
+    c = Case(5, [1] * 6, 3001, torch.bfloat16)
+    kw = c.args(cuda_device)
+    x = c.logits.to(cuda_device)
+    want = pick_tokens(x, **kw)
+    kw.pop("indptr")
+    assert torch.equal(pick_tokens(x, **kw), want)
+
+
+def test_nothing_but_logits(cuda_device):
+    x = torch.randn(3, 5000, device=cuda_device).to(torch.bfloat16)
+    assert torch.equal(adjust_logits(x), x)
+    assert torch.equal(pick_tokens(x).long(), torch.tensor(ref.pick(x.float().cpu(), [0] * 3), device=cuda_device))
+
+
+def test_ties_nan_and_infinities(cuda_device):
+    x = torch.zeros(6, 70000, device=cuda_device)
+    x[0, [5, 6, 69999]] = 3.0
+    x[1, 1000] = math.nan
+    x[1, 60000] = 2.0
+    x[2] = -math.inf
+    x[3] = math.nan
+    x[4, 40000] = math.inf
+    x[4, 50000] = math.inf
+    x[5] = -math.inf
+    x[5, 69999] = -1e38
+    want = [5, 60000, -1, -1, 40000, 69999]
+    for dtype in (torch.float32, torch.bfloat16):
+        assert pick_tokens(x.to(dtype)).tolist() == want
+    # NaN and infinities in places that are not allowed are -inf.
+    allowed = torch.zeros(6, 70000, dtype=torch.bool)
+    allowed[:, 7:90] = True
+    words = _pack(allowed).to(cuda_device)
+    assert pick_tokens(x, allowed=words).tolist() == [7, 7, -1, -1, 7, -1]
+    y = adjust_logits(x, allowed=words)
+    assert bool((y.cpu()[~allowed] == -math.inf).all())
+
+
+def test_ids_outside_the_vocabulary_do_not_count(cuda_device):
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)  # noqa: E731
+    x = torch.randn(1, 300, device=cuda_device)
+    y = adjust_logits(x, history=i32([[-1, 300, 2 ** 31 - 1, -2 ** 31]]), history_len=i32([4]), tokens=i32([400]),
+                      frequency=torch.ones(1, device=cuda_device),
+                      bias=(i32([0, 2]), i32([-3, 300]), torch.ones(2, device=cuda_device)))
+    assert torch.equal(x, y)
+
+
+def test_lengths_and_prefix_sums_out_of_range(cuda_device):
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)  # noqa: E731
+    x = torch.zeros(2, 300, device=cuda_device)
+    one = torch.ones(2, device=cuda_device)
+    status = i32([0])
+    y = adjust_logits(x, history=i32([[4, 5], [6, 7]]), history_len=i32([99, -3]), frequency=one)
+    assert y[0, [4, 5]].tolist() == [-1.0, -1.0] and bool((y[1] == 0).all())
+    adjust_logits(x, indptr=i32([0, 5, 2]), frequency=one, status=status)
+    assert int(status) == 4
+    status.zero_()
+    adjust_logits(x, bias=(i32([0, 9, 9]), i32([1, 2]), one), status=status)
+    assert int(status) == 4
+
+
+def test_replayed_with_other_histories(cuda_device):
+    c = Case(8, [3, 4], 9001, torch.bfloat16, bias=7, allowed=True)
+    kw = c.args(cuda_device)
+    x = c.logits.to(cuda_device)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        pick_tokens(x, **kw)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ids, out = pick_tokens(x, **kw), adjust_logits(x, **kw)
+    for n in (1, 0, 30):
+        kw["history_len"].fill_(n)
+        kw["history"].random_(0, 9001)
+        g.replay()
+        assert torch.equal(ids, pick_tokens(x, **kw)) and torch.equal(out, adjust_logits(x, **kw))

@@ -1,0 +1,275 @@
+"""Attention of trees of drafted tokens over the paged cache (``run`` with a
+tree mask) against the definition in 64 bits, with the bound of the kernels'
+roundings."""
+
+import math
+import random
+
+import pytest
+import torch
+
+from aspire_b200.attention import HolisticAttentionWrapper, first_last_dump_jit_args
+import tree_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+class Case:
+    """Rows of (keys before the nodes, nodes); masks by `kind`: trees, random
+    bits, nothing, everything."""
+
+    def __init__(self, dev, rows, heads, kv_heads, kind="tree", seed=0, extra_words=0, pad=0, scale=1.0, pages_pad=3):
+        rng = random.Random(seed)
+        g = torch.Generator().manual_seed(seed)
+        nodes = [n for _, n in rows]
+        self.ends = [a + n for a, n in rows]
+        self.starts = ref.indptr(nodes)
+        total = self.starts[-1] + pad
+        per = [-(-e // 16) for e in self.ends]
+        order = list(range(sum(per) + pages_pad))
+        rng.shuffle(order)
+        at = ref.indptr(per)
+        self.kv_indptr = at
+        self.pages = [order[at[b]:at[b + 1]] for b in range(len(rows))]
+        self.cache = torch.randn(len(order), 2, 16, kv_heads, 128, generator=g).to(torch.bfloat16)
+        # Places behind a row's end hold what an earlier owner of the page left.
+        for b, e in enumerate(self.ends):
+            if e % 16:
+                self.cache[self.pages[b][-1], :, e % 16:] = math.nan
+        self.q = (torch.randn(total, heads, 128, generator=g) * scale).to(torch.bfloat16)
+        words = (max(nodes + [1]) + 31) // 32 + extra_words
+        self.seen, mask = [], []
+        for n in nodes:
+            s = torch.zeros(n, n, dtype=torch.bool)
+            if kind == "tree" and n:
+                for i, path in enumerate(ref.ancestors(ref.random_parents(rng, n))):
+                    s[i, path] = True
+            elif kind == "random":
+                s = torch.rand(n, n, generator=g) < 0.4
+            elif kind == "all":
+                s[:] = True
+            elif kind == "chain":
+                s = torch.ones(n, n).tril().bool()
+            self.seen.append(s)
+            mask += ref.mask_words([r.nonzero()[:, 0].tolist() for r in s], words)
+        mask += [[-1] * words] * pad
+        self.mask = torch.tensor(mask, dtype=torch.int32, device=dev).view(total, words)
+        self.dev, self.heads, self.kv_heads, self.rows = dev, heads, kv_heads, rows
+
+    def plan(self, device_plan=False, tables=False, wrapper=None):
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+        w = wrapper or HolisticAttentionWrapper(torch.empty(1, device=self.dev))
+        flat = i32([p for r in self.pages for p in r] or [0]).to(self.dev)
+        if tables:
+            cols = max(len(r) for r in self.pages)
+            t = i32([r + [10 ** 6] * (cols - len(r)) for r in self.pages]).to(self.dev)
+            w.set_page_tables(torch.ones(len(self.rows), dtype=torch.int32, device=self.dev), t, t)
+            flat = None
+        shape = (self.heads, self.kv_heads, 128, 16)
+        if device_plan:
+            last = i32([(e - 1) % 16 + 1 if e else 0 for e in self.ends]).to(self.dev)
+            w.plan_device(i32(self.starts).to(self.dev), i32(self.kv_indptr).to(self.dev), last, *shape,
+                          paged_kv_indices=flat, causal=False)
+        else:
+            w.plan_host(i32(self.starts), i32(self.kv_indptr), i32(self.ends), flat, *shape, causal=False)
+        return w
+
+    def check(self, out, lse, rows=None):
+        exp, else_, bound, lbound = ref.tree_attention(self.q, self.cache.nan_to_num(0), self.pages, self.starts,
+                                                       self.ends, self.seen)
+        n = self.starts[-1]
+        d = (out.double().cpu() - exp).abs()[:n]
+        bad = ~(d <= bound[:n])
+        assert not bool(bad.any()), f"{int(bad.sum())} of {bad.numel()} out, worst {(d / bound[:n].clamp(min=1e-300)).max():.3g}"
+        none = else_[:n] == -math.inf
+        got = lse.double().cpu()[:n]
+        assert torch.equal(got == -math.inf, none)
+        assert bool((out.cpu()[:n][none] == 0).all())
+        assert bool(((got - else_[:n]).abs()[~none] <= lbound[:n][~none]).all())
+
+    def run(self, **kw):
+        w = self.plan(**kw)
+        out, lse = w.run(self.q.to(self.dev), self.cache.to(self.dev), tree_mask=self.mask, return_lse=True)
+        assert w.device_status() == 0
+        return out, lse
+
+
+ROWS = {
+    "one": [(0, 1)],
+    "short": [(130, 5)],
+    "no_prefix": [(0, 7), (0, 33), (0, 1)],
+    "tile_edges": [(128 - 3, 6), (128, 9), (127, 2), (64 - 5, 12), (256 - 16, 16), (1, 127)],
+    "idle_rows": [(40, 0), (300, 11), (0, 0), (17, 3)],
+    "ragged": [(700, 13), (33, 31), (1000, 20), (5, 8), (511, 1)],
+    "split": [(3001, 9)],
+    "wide": [(900, 64), (100, 33), (1, 100), (63, 65)],
+    "more_than_an_item": [(200, 140)],
+}
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 1), (8, 8), (10, 2)])
+@pytest.mark.parametrize("rows", list(ROWS))
+def test_trees(cuda_device, rows, heads, kv_heads):
+    c = Case(cuda_device, ROWS[rows], heads, kv_heads, seed=len(rows) * 7 + heads)
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(16, 2), (48, 1), (17, 1), (3, 1)])
+def test_group_sizes(cuda_device, heads, kv_heads):
+    c = Case(cuda_device, [(250, 5), (120, 17), (0, 2), (64, 40)], heads, kv_heads, seed=heads)
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("kind", ["random", "none", "all", "chain"])
+@pytest.mark.parametrize("rows", ["no_prefix", "tile_edges", "wide"])
+def test_any_mask(cuda_device, rows, kind):
+    """Masks need not be trees; rows that see nothing give zeros."""
+    c = Case(cuda_device, ROWS[rows], 4, 1, kind=kind, seed=3, extra_words=1)
+    c.check(*c.run())
+
+
+def test_large_logits(cuda_device):
+    """The running maximum moves and rescales inside the nodes' own tiles too."""
+    c = Case(cuda_device, [(900, 14), (90, 70)], 4, 1, seed=4, scale=8.0)
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("rows", ["ragged", "wide", "split", "idle_rows"])
+def test_page_tables_and_device_plans(cuda_device, rows):
+    c = Case(cuda_device, ROWS[rows], 8, 2, seed=5)
+    first = c.run()
+    c.check(*first)
+    for kw in (dict(tables=True), dict(device_plan=True), dict(device_plan=True, tables=True)):
+        out, lse = c.run(**kw)
+        c.check(out, lse)
+
+
+def test_a_chain_is_the_causal_attention(cuda_device):
+    c = Case(cuda_device, [(1200, 9), (60, 3), (400, 40)], 8, 2, kind="chain", seed=6)
+    out, lse = c.run()
+    w = HolisticAttentionWrapper(torch.empty(1, device=cuda_device))
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    w.plan_host(i32(c.starts), i32(c.kv_indptr), i32(c.ends),
+                i32([p for r in c.pages for p in r]).to(cuda_device), 8, 2, 128, 16, causal=True)
+    c.check(*w.run(c.q.to(cuda_device), c.cache.to(cuda_device), return_lse=True))
+    c.check(out, lse)
+
+
+def test_strides_and_rows_behind_the_last(cuda_device):
+    c = Case(cuda_device, [(140, 6), (31, 50)], 4, 2, seed=7, pad=5)
+    w = c.plan()
+    wide = torch.zeros(c.q.shape[0], 8, 256, dtype=torch.bfloat16, device=cuda_device)
+    wide[:, 1::2, 64:192] = c.q.to(cuda_device)
+    back = torch.full((c.q.shape[0], 4, 264), 7.0, dtype=torch.bfloat16, device=cuda_device)
+    lse = torch.full((c.q.shape[0], 4), 7.0, device=cuda_device)
+    out = w.run(wide[:, 1::2, 64:192], c.cache.to(cuda_device), tree_mask=c.mask, out=back[:, :, 8:136], lse=lse)
+    c.check(out, lse)
+    n = c.starts[-1]
+    assert bool((back[n:] == 7).all()) and bool((lse[n:] == 7).all())
+    assert bool((back[:n, :, :8] == 7).all()) and bool((back[:n, :, 136:] == 7).all())
+
+
+def test_with_the_append_inside(cuda_device):
+    c = Case(cuda_device, [(140, 6), (31, 5), (0, 3)], 8, 2, seed=8)
+    n = c.starts[-1]
+    k = torch.randn(n, 2, 128).to(torch.bfloat16)
+    v = torch.randn(n, 2, 128).to(torch.bfloat16)
+    cache = c.cache.to(cuda_device)
+    w = c.plan()
+    out, lse = w.run(c.q.to(cuda_device), cache, tree_mask=c.mask, return_lse=True,
+                     append=(k.to(cuda_device), v.to(cuda_device)))
+    for b, (a, m) in enumerate(c.rows):
+        for i in range(m):
+            page = c.pages[b][(a + i) // 16]
+            c.cache[page, 0, (a + i) % 16] = k[c.starts[b] + i]
+            c.cache[page, 1, (a + i) % 16] = v[c.starts[b] + i]
+    c.check(out, lse)
+    assert torch.equal(cache.cpu().nan_to_num(9), c.cache.nan_to_num(9))
+
+
+def test_nodes_past_the_mask_are_hidden_under_device_plans(cuda_device):
+    c = Case(cuda_device, [(50, 40), (20, 70)], 4, 1, kind="all", seed=9)
+    c.mask = c.mask[:, :1].contiguous()
+    for s in c.seen:
+        s[:, 32:] = False
+    c.check(*c.run(device_plan=True))
+
+
+def test_bad_pages_are_reported(cuda_device):
+    c = Case(cuda_device, [(50, 6)], 4, 1, seed=10)
+    c.pages[0][1] = 10 ** 6
+    w = c.plan()
+    w.run(c.q.to(cuda_device), c.cache.to(cuda_device), tree_mask=c.mask)
+    assert w.device_status() == 1
+
+
+def test_replayed_with_other_masks_and_lengths(cuda_device):
+    cases = [Case(cuda_device, rows, 8, 2, seed=s, extra_words=e) for s, (rows, e) in enumerate(
+        [([(700, 12), (90, 3), (10, 40)], 0), ([(300, 30), (11, 20), (0, 5)], 1), ([(3, 1), (1500, 33), (0, 21)], 0)])]
+    dev = cuda_device
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    starts, kvp, last = (torch.zeros(k, dtype=torch.int32, device=dev) for k in (4, 4, 3))
+    flat = torch.zeros(400, dtype=torch.int32, device=dev)
+    q = torch.zeros(55, 8, 128, dtype=torch.bfloat16, device=dev)
+    cache = torch.zeros(200, 2, 16, 2, 128, dtype=torch.bfloat16, device=dev)
+    mask = torch.zeros(55, 2, dtype=torch.int32, device=dev)
+    w = HolisticAttentionWrapper(torch.empty(1, device=dev))
+
+    def load(c):
+        n = c.starts[-1]
+        starts.copy_(i32(c.starts))
+        kvp.copy_(i32(c.kv_indptr))
+        last.copy_(i32([(e - 1) % 16 + 1 for e in c.ends]))
+        ids = i32([p for r in c.pages for p in r])
+        flat[:ids.numel()].copy_(ids)
+        q[:n].copy_(c.q)
+        cache[:c.cache.shape[0]].copy_(c.cache)
+        mask[:n].copy_(c.mask)
+
+    def step():
+        w.plan_device(starts, kvp, last, 8, 2, 128, 16, paged_kv_indices=flat, causal=False)
+        return w.run(q, cache, tree_mask=mask, return_lse=True)
+
+    load(cases[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out, lse = step()
+    torch.cuda.synchronize()
+    cases[0].check(out, lse)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = step()
+    for c in cases[1:] + cases[:1]:
+        load(c)
+        g.replay()
+        c.check(out, lse)
+    assert w.device_status() == 0
+
+
+def test_results_repeat_bit_by_bit(cuda_device):
+    c = Case(cuda_device, [(2600, 12), (900, 50)], 8, 2, seed=12)
+    out, lse = c.run()
+    for _ in range(3):
+        o, l = c.run()
+        assert torch.equal(o, out) and torch.equal(l, lse)
+
+
+def test_refusals(cuda_device):
+    c = Case(cuda_device, [(50, 40)], 4, 1, seed=13)
+    q, kv = c.q.to(cuda_device), c.cache.to(cuda_device)
+    w = c.plan()
+    for mask in (c.mask.long(), c.mask[:, 0], c.mask[:-1], c.mask.cpu(), c.mask.repeat(1, 2)[:, ::2], c.mask[:, :0]):
+        with pytest.raises(ValueError):
+            w.run(q, kv, tree_mask=mask)
+    with pytest.raises(ValueError, match="more queries"):
+        w.run(q, kv, tree_mask=c.mask[:, :1].contiguous())
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    w.plan_host(i32(c.starts), i32(c.kv_indptr), i32(c.ends), i32(c.pages[0]).to(cuda_device), 4, 1, 128, 16, causal=True)
+    with pytest.raises(ValueError, match="causal"):
+        w.run(q, kv, tree_mask=c.mask)
+    d = HolisticAttentionWrapper(torch.empty(1, device=cuda_device), jit_args=first_last_dump_jit_args())
+    c.plan(wrapper=d)
+    dump = torch.empty(4 * 2 * 96, dtype=torch.float16, device=cuda_device)
+    with pytest.raises(ValueError, match="dump"):
+        d.run(q, kv, dump, 4, 96, tree_mask=c.mask)
