@@ -486,7 +486,7 @@ _SIGNATURES = {
          ctypes.c_void_p],
     ),
     "aspire_step_tables": (ctypes.c_int, [ctypes.POINTER(AspireStepTablesArgs), ctypes.c_void_p]),
-    "aspire_logits_workspace": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]),
+    "aspire_logits_workspace": (ctypes.c_size_t, [ctypes.POINTER(AspireLogitsArgs)]),
     "aspire_adjust_logits": (ctypes.c_int, [ctypes.POINTER(AspireLogitsArgs), ctypes.c_void_p]),
     "aspire_tree_accept": (ctypes.c_int, [ctypes.POINTER(AspireTreeAcceptArgs), ctypes.c_void_p]),
     "aspire_draft_page_spill": (ctypes.c_int, [ctypes.POINTER(AspireSpillArgs), ctypes.c_void_p]),

@@ -190,8 +190,8 @@ const char* aspire_kernel_names(void) {
          "aspire_draft_spill_kernel\naspire_clear_dump_kernel\n"
          "aspire_w4_small_kernel\naspire_w4_tc_kernel\naspire_moe_route_kernel\naspire_moe_sort_kernel\naspire_moe_route_grad_kernel\n"
          "aspire_moe_dispatch_kernel\naspire_moe_combine_kernel\naspire_moe_combine_grad_kernel\n"
-         "aspire_attn_tree_kernel\naspire_step_tables_kernel\naspire_step_tokens_kernel\naspire_logits_kernel\n"
-         "aspire_pick_kernel\naspire_tree_accept_kernel\n";
+         "aspire_attn_tree_kernel\naspire_step_tables_kernel\naspire_step_tokens_kernel\naspire_logits_mark_kernel\n"
+         "aspire_logits_kernel\naspire_logits_pick_kernel\naspire_tree_accept_kernel\n";
 }
 
 int aspire_plan_host_only(const int32_t* qo_indptr, const int32_t* kv_indptr,

@@ -29,27 +29,7 @@ int invalid(const char* who, const char* what) {
   return set_error(ASPIRE_ERR_INVALID, std::string(who) + ": " + what);
 }
 
-SmemOptIn g_logits_smem[3];  // by ASPIRE_T_*
-
-// Vocabulary entries of a CTA and how many CTAs share a row.
-struct Slicing {
-  int32_t slice, slices;
-};
-
-// Shared memory of a slice: a bit and a count an entry, with biases an entry's number too.
-size_t slice_bytes(int64_t slice, bool bias) { return size_t((slice + 31) / 32 * 4 + slice * (bias ? 8 : 4)); }
-
-constexpr int64_t kSliceStep = 256;
-constexpr int64_t kMostSlice = 25600;  // 103 KB: two CTAs fit an SM
-
-Slicing slicing(int32_t rows, int32_t vocab, bool bias, int sms) {
-  const int64_t most = bias ? kMostSlice / 2 : kMostSlice;
-  const int64_t least = (int64_t(vocab) + most - 1) / most;
-  int64_t n = std::max<int64_t>(least, (2 * int64_t(sms) + rows - 1) / std::max(rows, 1));
-  n = std::min<int64_t>(n, (int64_t(vocab) + kSliceStep - 1) / kSliceStep);
-  const int64_t slice = ((int64_t(vocab) + n - 1) / n + kSliceStep - 1) / kSliceStep * kSliceStep;
-  return {int32_t(slice), int32_t((int64_t(vocab) + slice - 1) / slice)};
-}
+SmemOptIn g_mark_smem[2], g_logits_smem[3][2];
 
 int step_tables(const AspireStepTablesArgs* a, void* stream) {
   const char* who = "aspire_step_tables";
@@ -99,8 +79,58 @@ int step_tables(const AspireStepTablesArgs* a, void* stream) {
                 st, "aspire_step_tokens_kernel launch", p);
 }
 
-size_t logits_workspace(int64_t tokens, int32_t rows, int32_t vocab, bool bias, int sms) {
-  return size_t(tokens) * size_t(slicing(rows, vocab, bias, sms).slices) * 8;
+// Whether anything touches single entries of the logits.
+bool has_marks(const AspireLogitsArgs* a) {
+  const bool penalties = a->repetition || a->frequency || a->presence;
+  return a->rows > 0 && (a->bias_indptr || (penalties && (a->history || a->step_tokens)));
+}
+
+int32_t blocks_of(int32_t vocab) { return int32_t((int64_t(vocab) + kLogitsBlock - 1) / kLogitsBlock); }
+
+// Entries of the marking CTAs' lists.
+size_t list_entries(const AspireLogitsArgs* a, int ranks) {
+  return size_t(ranks) * (size_t(a->rows) * size_t(a->history ? a->history_cols : 0) + size_t(a->tokens) +
+                          size_t(a->bias_indptr ? a->bias_entries : 0));
+}
+
+// The workspace's parts, from `base` on; returns their bytes.
+size_t lay_out(const AspireLogitsArgs* a, char* base, int sms, LogitsParams* p) {
+  // As many marking CTAs a row as the counts need, more for few rows.
+  const int cols = a->history ? a->history_cols : 0;
+  const int most = cols > kMarkNarrow ? kMarkMaxWide : kMarkMaxBlocks;
+  const int all = blocks_of(a->vocab), need = (all + most - 1) / most;
+  const int ranks = std::max(need, std::min({8, all, sms / std::max(a->rows, 1)}));
+  p->mark_blocks = (all + ranks - 1) / ranks;
+  p->mark_ranks = (all + p->mark_blocks - 1) / p->mark_blocks;
+  size_t at = 0;
+  const auto part = [&](size_t bytes) {
+    char* here = base + at;
+    at += (bytes + 15) / 16 * 16;
+    return here;
+  };
+  if (a->ids) {
+    p->keys = reinterpret_cast<unsigned long long*>(part(size_t(a->tokens) * 8));
+    p->arrived = reinterpret_cast<uint32_t*>(part(size_t(a->tokens) * 4));
+  }
+  if (has_marks(a)) {
+    const size_t blocks = size_t(a->rows) * size_t(all);
+    const size_t entries = list_entries(a, p->mark_ranks);
+    p->table = reinterpret_cast<int2*>(part(blocks * (kLogitsBlock / kLogitsUnit) * 8));
+    p->touched = reinterpret_cast<uint32_t*>(part(blocks * kLogitsBlock / 8));
+    p->list = reinterpret_cast<int2*>(part(entries * 8));
+    if (a->bias_indptr) p->list_bias = reinterpret_cast<uint2*>(part(entries * 8));
+  }
+  return at;
+}
+
+int launch_marks(const LogitsParams& p, cudaStream_t st) {
+  const bool wide = p.history_cols > kMarkNarrow;
+  const size_t smem = p.list ? mark_smem_bytes(p.mark_blocks, wide) : 0;
+  const LogitsKernel mark = mark_kernel(wide);
+  int rc = ensure_smem(reinterpret_cast<const void*>(mark), smem, g_mark_smem[wide]);
+  if (rc) return rc;
+  return launch(mark, dim3(unsigned(p.mark_ranks), unsigned(std::max(p.rows, 1))), dim3(kMarkThreads), smem, st,
+                "aspire_logits_mark_kernel launch", p);
 }
 
 int adjust_logits(const AspireLogitsArgs* a, void* stream) {
@@ -109,7 +139,8 @@ int adjust_logits(const AspireLogitsArgs* a, void* stream) {
   if (a->type < ASPIRE_T_F32 || a->type > ASPIRE_T_F16) return invalid(who, "type must be ASPIRE_T_F32, _BF16 or _F16");
   if (a->tokens < 0 || a->tokens > INT32_MAX || a->rows < 0 || a->rows > 65534 || a->vocab < 1)
     return invalid(who, "tokens, rows (at most 65534) or vocab out of range");
-  if (!a->out && !a->ids) return invalid(who, "neither out nor ids is given");
+  if (!a->out == !a->ids) return invalid(who, "give either out or ids");
+  if (a->vocab > 1 << 30) return invalid(who, "vocab must be at most 2^30");
   if (a->tokens == 0) return ASPIRE_OK;
   if (!a->logits) return invalid(who, "null logits");
   if (a->logits_stride < a->vocab || (a->out && a->out_stride < a->vocab))
@@ -125,10 +156,12 @@ int adjust_logits(const AspireLogitsArgs* a, void* stream) {
   int sms = 0;
   int rc = current_sm_count(&sms);
   if (rc) return rc;
-  const Slicing cut = slicing(a->rows, a->vocab, a->bias_indptr != nullptr, sms);
-  if (a->ids && (!a->workspace || a->workspace_bytes < size_t(a->tokens) * size_t(cut.slices) * 8))
-    return set_error(ASPIRE_ERR_CAPACITY, std::string(who) + ": workspace too small");
-  LogitsParams p;
+  LogitsParams p = {};
+  const size_t wanted = lay_out(a, static_cast<char*>(a->workspace), sms, &p);
+  if (p.list && list_entries(a, p.mark_ranks) > size_t(INT32_MAX))
+    return invalid(who, "histories, tokens and biases past 2^31 entries together");
+  if (wanted > 0 && (!a->workspace || a->workspace_bytes < wanted || (reinterpret_cast<uintptr_t>(a->workspace) & 15)))
+    return set_error(ASPIRE_ERR_CAPACITY, std::string(who) + ": workspace missing, too small or not 16-byte aligned");
   p.logits = a->logits;
   p.logits_stride = a->logits_stride;
   p.out = a->out;
@@ -139,7 +172,7 @@ int adjust_logits(const AspireLogitsArgs* a, void* stream) {
   p.indptr = a->indptr;
   p.history = a->history;
   p.history_stride = a->history_stride;
-  p.history_cols = a->history_cols;
+  p.history_cols = a->history ? a->history_cols : 0;
   p.history_len = a->history_len;
   p.prompt_len = a->prompt_len;
   p.step_tokens = a->step_tokens;
@@ -154,27 +187,22 @@ int adjust_logits(const AspireLogitsArgs* a, void* stream) {
   p.bias_entries = a->bias_entries;
   p.allowed = a->allowed;
   p.allowed_stride = a->allowed_stride;
-  p.slice = cut.slice;
-  p.slices = cut.slices;
-  p.best_value = a->ids ? static_cast<float*>(a->workspace) : nullptr;
-  p.best_id = a->ids ? static_cast<int32_t*>(a->workspace) + a->tokens * cut.slices : nullptr;
   p.ids = a->ids;
   p.status = a->status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool tail = a->indptr && a->out && a->out != a->logits;
-  if (a->rows > 0 || tail) {
-    const LogitsKernel kernel = logits_kernel(a->type);
-    const size_t smem = slice_bytes(p.slice, p.bias_indptr != nullptr);
-    rc = ensure_smem(reinterpret_cast<const void*>(kernel), smem, g_logits_smem[a->type]);
-    if (rc) return rc;
-    rc = launch(kernel, dim3(unsigned(p.slices), unsigned(p.rows + (tail ? 1 : 0))), dim3(kLogitsThreads), smem, st,
-                "aspire_logits_kernel launch", p);
+  if (p.list || p.keys) {
+    rc = launch_marks(p, st);
     if (rc) return rc;
   }
-  if (!a->ids) return ASPIRE_OK;
-  const int64_t per = kPickThreads / 32;
-  return launch(aspire_pick_kernel, dim3(unsigned((a->tokens + per - 1) / per)), dim3(kPickThreads), 0, st,
-                "aspire_pick_kernel launch", p);
+  // As many CTAs a token as are resident at once.
+  const int slice = logits_slice(a->type);
+  const int64_t slices = (int64_t(a->vocab) + slice - 1) / slice;
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(slices, int64_t(kLogitsCtas) * sms / a->tokens));
+  const LogitsKernel kernel = logits_kernel(a->type, a->ids != nullptr);
+  rc = ensure_smem(reinterpret_cast<const void*>(kernel), logits_smem_bytes(), g_logits_smem[a->type][a->ids ? 1 : 0]);
+  if (rc) return rc;
+  return launch(kernel, dim3(unsigned(a->tokens), unsigned(parts)), dim3(kLogitsThreads), logits_smem_bytes(), st,
+                "aspire_logits_kernel launch", p);
 }
 
 int tree_accept(const AspireTreeAcceptArgs* a, void* stream) {
@@ -232,10 +260,12 @@ int aspire_step_tables(const AspireStepTablesArgs* args, void* stream) {
   return aspire::guarded([&] { return aspire::step_tables(args, stream); });
 }
 
-size_t aspire_logits_workspace(int64_t tokens, int32_t rows, int32_t vocab, int32_t with_bias) {
+size_t aspire_logits_workspace(const AspireLogitsArgs* args) {
+  if (!args || args->tokens <= 0 || args->rows < 0 || args->vocab < 1 || args->history_cols < 0 || args->bias_entries < 0)
+    return 0;
+  aspire::LogitsParams p = {};
   int sms = 0;
-  if (tokens <= 0 || rows < 0 || vocab < 1 || aspire::current_sm_count(&sms)) return 0;
-  return aspire::logits_workspace(tokens, rows, vocab, with_bias != 0, sms);
+  return aspire::current_sm_count(&sms) ? 0 : aspire::lay_out(args, nullptr, sms, &p);
 }
 
 int aspire_adjust_logits(const AspireLogitsArgs* args, void* stream) {

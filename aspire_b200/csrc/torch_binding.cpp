@@ -643,17 +643,18 @@ std::pair<Tensor, Tensor> adjust_logits(const LogitsCall& c) {
   }
   a.status = status_word(c.status, x);
   on_device(x, [&](void* stream) {
+    const auto i32 = x.options().dtype(at::kInt).requires_grad(false);
     if (c.want_ids) {
-      const auto i32 = x.options().dtype(at::kInt).requires_grad(false);
       ids = at::empty({tokens}, i32);
-      if (tokens > 0) {
-        a.workspace_bytes = abi.logits_workspace(tokens, a.rows, a.vocab, a.bias_indptr != nullptr);
-        workspace = at::empty({int64_t(a.workspace_bytes / 4)}, i32);
-        a.workspace = workspace.data_ptr();
-        a.ids = static_cast<int32_t*>(ids.data_ptr());
-      }
+      a.ids = static_cast<int32_t*>(ids.data_ptr());
     }
-    if (tokens > 0) check(abi.adjust_logits(&a, stream), "aspire_adjust_logits");
+    if (tokens == 0) return;
+    a.workspace_bytes = abi.logits_workspace(&a);
+    if (a.workspace_bytes) {
+      workspace = at::empty({int64_t(a.workspace_bytes / 4)}, i32);
+      a.workspace = workspace.data_ptr();
+    }
+    check(abi.adjust_logits(&a, stream), "aspire_adjust_logits");
   });
   return {out, ids};
 }

@@ -39,7 +39,7 @@ __global__ void aspire_step_tokens_kernel(StepTablesParams p);
 struct LogitsParams {
   const void* logits;
   int64_t logits_stride;      // elements between tokens
-  void* out;                  // NULL: pick only
+  void* out;
   int64_t out_stride;
   int64_t tokens;
   int32_t vocab;
@@ -62,18 +62,32 @@ struct LogitsParams {
   int64_t bias_entries;
   const int32_t* allowed;     // [tokens, allowed_stride] words or NULL
   int64_t allowed_stride;
-  int32_t slice;              // vocabulary entries of a CTA
-  int32_t slices;
-  float* best_value;          // [tokens, slices], NULL: no pick
-  int32_t* best_id;
-  int32_t* ids;               // [tokens]
+  int32_t* ids;               // [tokens]: the best tokens, or NULL: adjusted logits to out
+  // Workspace.  The marking CTAs' lists lie one after another (list_base).
+  unsigned long long* keys;   // [tokens], with ids
+  uint32_t* arrived;          // [tokens], with ids: slices done
+  int2* list;                 // touched ids with their counts and flags; NULL: nothing touches the logits
+  uint2* list_bias;           // with biases, of ids that have one: 1 + the entry's number, the bias
+  int2* table;                // [rows, blocks * kLogitsBlock / kLogitsUnit]: a unit's part of the list
+  uint32_t* touched;          // [rows, blocks, kLogitsBlock / 32] bitmap
+  int32_t mark_ranks;         // CTAs that mark a row
+  int32_t mark_blocks;        // blocks of each
   uint32_t* status;
 };
-constexpr int kLogitsThreads = 256;
+constexpr int kLogitsBlock = 4096;  // vocabulary entries, the steps of a marking CTA's share
+constexpr int kLogitsUnit = 512;    // vocabulary entries that share an entry of the table
+constexpr int kMarkThreads = 1024;
+constexpr int kMarkMaxBlocks = 21;  // of a CTA with 16-bit counts: 216 KB of counts and bits
+constexpr int kMarkMaxWide = 12;    // with 32-bit ones: 219 KB
+constexpr int kMarkNarrow = 65535;  // history up to which 16 bits count
 using LogitsKernel = void (*)(LogitsParams);
-LogitsKernel logits_kernel(int type);  // aspire_logits_kernel of an ASPIRE_T_*
-__global__ void aspire_pick_kernel(LogitsParams p);
-constexpr int kPickThreads = 128;
+LogitsKernel mark_kernel(bool wide);  // aspire_logits_mark_kernel
+size_t mark_smem_bytes(int blocks, bool wide);
+constexpr int kLogitsThreads = 256;
+constexpr int kLogitsCtas = 3;  // of an SM
+LogitsKernel logits_kernel(int type, bool pick);  // aspire_logits_kernel of an ASPIRE_T_*
+int logits_slice(int type);                       // vocabulary entries of one of its CTAs at a time
+size_t logits_smem_bytes();
 
 constexpr int kAcceptCaches = 128;
 struct AcceptParams {

@@ -803,19 +803,20 @@ typedef struct AspireLogitsArgs {
   const int32_t* allowed;    /* int32 [tokens, allowed_stride]: bit v % 32 of word
                                 v / 32 says that v may follow; NULL: all may      */
   int64_t allowed_stride;
-  void* out;                 /* [tokens, vocab] of `type`, may be logits; NULL    */
+  void* out;                 /* [tokens, vocab] of `type`, may be logits, or ...  */
   int64_t out_stride;
-  int32_t* ids;              /* int32 [tokens] best tokens, or NULL               */
-  void* workspace;           /* with ids: aspire_logits_workspace bytes           */
+  int32_t* ids;              /* ... int32 [tokens] best tokens (logits stay)      */
+  void* workspace;           /* aspire_logits_workspace bytes, 16-byte aligned    */
   size_t workspace_bytes;
   uint32_t* status;          /* optional device status word                       */
 } AspireLogitsArgs;
 
-/* Bytes of workspace that a call with these sizes needs for its best tokens. */
-ASPIRE_API size_t aspire_logits_workspace(int64_t tokens, int32_t rows, int32_t vocab, int32_t with_bias);
+/* Bytes of workspace that a call with these arguments needs (its pointers are
+ * compared with NULL, nothing is read through them). */
+ASPIRE_API size_t aspire_logits_workspace(const AspireLogitsArgs* args);
 
 /*
- * Penalties for repeated tokens, biases and grammar masks on logits (out), and
+ * Penalties for repeated tokens, biases and grammar masks on logits (out), or
  * the best token of the result (ids), in fp32.  Of token v with c occurrences
  * in the row's history behind its prompt and on the token's path:
  *   x = x > 0 ? x / repetition : x * repetition   (v anywhere in history or path)
@@ -823,7 +824,7 @@ ASPIRE_API size_t aspire_logits_workspace(int64_t tokens, int32_t rows, int32_t 
  * A token that a row's biases list twice takes the later one.  Ids outside
  * [0, vocab) are ignored.  The best token is the largest value, the lowest id
  * on ties; NaN and -inf are never chosen (-1 if nothing else is left).  Tokens
- * of no row keep their logits and get -1.
+ * of no row keep their logits and get -1. 
  */
 ASPIRE_API int aspire_adjust_logits(const AspireLogitsArgs* args, void* stream);
 

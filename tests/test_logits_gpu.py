@@ -205,3 +205,38 @@ def test_replayed_with_other_histories(cuda_device):
         kw["history"].random_(0, 9001)
         g.replay()
         assert torch.equal(ids, pick_tokens(x, **kw)) and torch.equal(out, adjust_logits(x, **kw))
+
+
+def test_histories_past_16_bits(cuda_device):
+    """70000 tokens, some of them more than 65535 times."""
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)  # noqa: E731
+    n = 70000
+    history = torch.full((2, n), 7, dtype=torch.int32, device=cuda_device)
+    history[0, 66000:] = 2999
+    history[1, :100] = 5
+    x = torch.zeros(2, 3000, device=cuda_device)
+    y = adjust_logits(x, history=history, history_len=i32([n, n]), prompt_len=i32([10, 50]),
+                      frequency=torch.ones(2, device=cuda_device))
+    want = torch.zeros(2, 3000)
+    want[0, 7], want[0, 2999], want[1, 5], want[1, 7] = -65990, -4000, -50, -69900
+    assert torch.equal(y.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 140001), (torch.bfloat16, 270000)])
+def test_many_tokens_of_large_vocabularies(cuda_device, dtype, vocab):
+    """More chunks a warp than it looks up at once, against the same rows in small calls."""
+    g = torch.Generator(device=cuda_device).manual_seed(1)
+    rows = 460
+    x = (torch.randn(rows, vocab, generator=g, device=cuda_device) * 3).to(dtype)
+    history = (torch.rand(rows, 3000, generator=g, device=cuda_device).pow(2) * vocab).int()
+    length = torch.full((rows,), 3000, dtype=torch.int32, device=cuda_device)
+    terms = {k: torch.rand(rows, generator=g, device=cuda_device) + 0.5 for k in ("repetition", "frequency", "presence")}
+    whole, ids = (f(x, history=history, history_len=length, **terms) for f in (adjust_logits, pick_tokens))
+    for a in range(0, rows, 46):
+        part = slice(a, a + 46)
+        kw = dict(history=history[part], history_len=length[part], **{k: v[part] for k, v in terms.items()})
+        assert torch.equal(adjust_logits(x[part], **kw), whole[part])
+        assert torch.equal(pick_tokens(x[part], **kw), ids[part])
+    # (Of equal values the lowest id: the rounded logits cannot tell which the larger one was.)
+    top = whole.float().max(1).values
+    assert bool((whole.float().gather(1, ids.long()[:, None])[:, 0] == top).all())

@@ -67,7 +67,8 @@ def test_adjust_logits_abi(built_library):
         return ctypes.byref(a)
 
     for kw, text in [(dict(type=3), "type"), (dict(type=-1), "type"), (dict(vocab=0), "vocab"), (dict(rows=65535), "rows"),
-                     (dict(tokens=-1), "range"), (dict(out=None), "neither"), (dict(logits=None), "null"),
+                     (dict(tokens=-1), "range"), (dict(out=None), "either"), (dict(ids=P), "either"),
+                     (dict(vocab=2 ** 30 + 1, logits_stride=2 ** 31, out_stride=2 ** 31), "2^30"), (dict(logits=None), "null"),
                      (dict(logits_stride=99), "apart"), (dict(out_stride=99), "apart"), (dict(rows=1), "indptr"),
                      (dict(history=P), "history_len"), (dict(tree_mask=P), "step_tokens"),
                      (dict(tree_mask=P, step_tokens=P), "words"), (dict(bias_indptr=P, bias_entries=3), "bias"),
