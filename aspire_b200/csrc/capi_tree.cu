@@ -36,7 +36,7 @@ int step_tables(const AspireStepTablesArgs* a, void* stream) {
   if (!a) return invalid(who, "null argument");
   if (a->rows < 0 || a->tokens < 0 || a->tokens > INT32_MAX) return invalid(who, "rows or tokens out of range");
   if (a->page_size < 1) return invalid(who, "page_size must be > 0");
-  if (a->free_capacity < 0 || a->free_capacity > INT32_MAX || a->block_table_cols < 0)
+  if (a->free_capacity < 0 || a->free_capacity > INT32_MAX || a->block_table_cols < 0 || a->block_table_cols >= 1 << 22)
     return invalid(who, "free_capacity or block_table_cols out of range");
   if (!a->qo_indptr || !a->kv_indptr || !a->free_count || (a->free_capacity > 0 && !a->free_pages))
     return invalid(who, "null pointer");
@@ -71,12 +71,12 @@ int step_tables(const AspireStepTablesArgs* a, void* stream) {
   p.tree_mask = a->tree_mask;
   p.status = a->status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  int rc = launch(aspire_step_tables_kernel, dim3(1), dim3(kTablesThreads), 0, st, "aspire_step_tables_kernel launch",
-                  p);
-  if (rc || a->tokens == 0 || a->rows == 0) return rc;
-  const int64_t blocks = (a->tokens + kStepTokensThreads - 1) / kStepTokensThreads;
-  return launch(aspire_step_tokens_kernel, dim3(unsigned(std::min<int64_t>(blocks, 4096))), dim3(kStepTokensThreads), 0,
-                st, "aspire_step_tokens_kernel launch", p);
+  const bool few = a->tokens > 0 && a->tokens <= kFewTokens && a->rows <= kTablesThreads && a->rows > 0;
+  int rc = launch(step_tables_kernel(few), dim3(1), dim3(kTablesThreads), 0, st, "aspire_step_tables_kernel launch", p);
+  if (rc || few || a->tokens == 0 || a->rows == 0) return rc;
+  const int64_t per = int64_t(kStepTokensThreads) * 4;
+  return launch(aspire_step_tokens_kernel, dim3(unsigned(std::min<int64_t>((a->tokens + per - 1) / per, 4096))),
+                dim3(kStepTokensThreads), 0, st, "aspire_step_tokens_kernel launch", p);
 }
 
 // Whether anything touches single entries of the logits.
@@ -247,8 +247,12 @@ int tree_accept(const AspireTreeAcceptArgs* a, void* stream) {
   p.token_bytes = a->token_bytes;
   p.num_caches = a->num_caches;
   p.status = a->status;
-  return launch(aspire_tree_accept_kernel, dim3(unsigned(a->rows), unsigned(std::max(a->num_caches, 1))),
-                dim3(kAcceptThreads), 0, static_cast<cudaStream_t>(stream), "aspire_tree_accept_kernel launch", p);
+  // About four CTAs an SM: fewer walk a row's tree more seldom, more have more reads under way.
+  int sms = 0;
+  const int rc = current_sm_count(&sms);
+  if (rc) return rc;
+  const int shares = std::max(1, std::min(a->num_caches, (4 * sms + a->rows - 1) / a->rows));
+  return launch(aspire_tree_accept_kernel, dim3(unsigned(a->rows), unsigned(shares)), dim3(kAcceptThreads), 0, static_cast<cudaStream_t>(stream), "aspire_tree_accept_kernel launch", p);
 }
 
 }  // namespace

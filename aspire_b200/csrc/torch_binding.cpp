@@ -467,16 +467,18 @@ int32_t* int_rows(const Tensor& t, int64_t rows, const Tensor& like, const char*
 }
 int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
-// Whether the memory of two tensors, first to last element, has a byte in common.
+// A tensor's memory, first to last element.
+std::pair<uintptr_t, uintptr_t> span_of(const Tensor& t) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
+  if (t.numel() == 0) return {at, at};
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  return {at, at + uintptr_t((last + 1) * t.element_size())};
+}
+
+// Whether two tensors' memory has a byte in common.
 bool in_common(const Tensor& a, const Tensor& b) {
-  if (a.numel() == 0 || b.numel() == 0) return false;
-  const auto span = [](const Tensor& t) {
-    int64_t last = 0;
-    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-    const uintptr_t at = reinterpret_cast<uintptr_t>(t.data_ptr());
-    return std::make_pair(at, at + uintptr_t((last + 1) * t.element_size()));
-  };
-  const auto x = span(a), y = span(b);
+  const auto x = span_of(a), y = span_of(b);
   return x.first < y.second && y.first < x.second;
 }
 
@@ -687,24 +689,34 @@ Walked tree_accept(const Tensor& tokens, const Tensor& parents, const Tensor& ta
     a.block_table_cols = int32_t(table->size(1));
     const Tensor& first = *caches[0];
     require(first.dim() == 5 && first.size(1) == 2, "a cache must be [pages, 2, page_size, heads, head_dim]");
-    for (const Tensor* c : caches)
+    const bool grads = at::GradMode::is_enabled();
+    const size_t bytes = first.nbytes();
+    std::vector<uintptr_t> starts;
+    at.reserve(caches.size());
+    starts.reserve(caches.size());
+    for (const Tensor* c : caches) {
       require(c->sizes() == first.sizes() && c->scalar_type() == first.scalar_type() && c->is_contiguous() &&
-                  c->device() == tokens.device() && !(at::GradMode::is_enabled() && c->requires_grad()),
+                  c->device() == tokens.device() && !(grads && c->requires_grad()),
               "caches must be contiguous tensors of one shape and type on the tokens' device, without gradients");
-    for (size_t i = 0; i < caches.size(); ++i)
-      for (size_t j = i + 1; j < caches.size(); ++j)
-        require(!in_common(*caches[i], *caches[j]), "a cache is given twice, or two of them overlap");
+      at.push_back(c->data_ptr());
+      starts.push_back(reinterpret_cast<uintptr_t>(at.back()));
+    }
+    std::sort(starts.begin(), starts.end());
+    for (size_t i = 1; i < starts.size(); ++i)
+      require(bytes == 0 || starts[i] - starts[i - 1] >= bytes, "a cache is given twice, or two of them overlap");
+    for (const Tensor* t : {&tokens, &parents, &targets, &indptr, &lengths, table}) {
+      const auto s = span_of(*t);
+      const auto next = std::upper_bound(starts.begin(), starts.end(), s.first);
+      require(s.first == s.second || bytes == 0 ||
+                  ((next == starts.end() || s.second <= *next) && (next == starts.begin() || *(next - 1) + bytes <= s.first)),
+              "a cache overlaps what the call reads");
+    }
     a.pages = first.size(0);
     a.token_bytes = first.size(3) * first.size(4) * first.element_size();
     require(first.size(2) >= 1 && first.size(2) <= INT32_MAX, "bad page size");
     a.page_size = int32_t(first.size(2));
     require(a.token_bytes >= 16 && a.token_bytes % 16 == 0, "a token's keys must be a positive multiple of 16 bytes");
-    for (const Tensor* c : caches) {
-      for (const Tensor* t : {&tokens, &parents, &targets, &indptr, &lengths, table})
-        require(!in_common(*c, *t), "a cache overlaps what the call reads");
-      at.push_back(c->data_ptr());
-      c->unsafeGetTensorImpl()->bump_version();
-    }
+    for (const Tensor* c : caches) c->unsafeGetTensorImpl()->bump_version();
   }
   const auto i32 = tokens.options();
   Walked w;

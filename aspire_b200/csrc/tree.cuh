@@ -32,7 +32,9 @@ struct StepTablesParams {
   uint32_t* status;
 };
 constexpr int kTablesThreads = 1024;
-__global__ void aspire_step_tables_kernel(StepTablesParams p);
+constexpr int kFewTokens = 4096;  // that the tables' kernel does itself, if their rows are one tile
+using TablesKernel = void (*)(StepTablesParams);
+TablesKernel step_tables_kernel(bool few);  // aspire_step_tables_kernel
 constexpr int kStepTokensThreads = 256;
 __global__ void aspire_step_tokens_kernel(StepTablesParams p);
 

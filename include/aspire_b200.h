@@ -739,7 +739,7 @@ typedef struct AspireStepTablesArgs {
   int32_t page_size;
   int32_t* block_table;      /* int32 [rows, block_table_stride], in place        */
   int64_t block_table_stride;
-  int32_t block_table_cols;
+  int32_t block_table_cols;  /* less than 2^22                                    */
   int32_t* held;             /* int32 [rows] pages a row holds, in place          */
   int32_t* free_pages;       /* int32 [free_capacity] stack, in place             */
   int32_t* free_count;       /* int32 [1] pages on the stack, in place            */

@@ -47,7 +47,7 @@ def test_step_tables_abi(built_library):
         return ctypes.byref(a)
 
     for kw, text in [(dict(rows=-1), "range"), (dict(tokens=-1), "range"), (dict(page_size=0), "page_size"),
-                     (dict(free_capacity=-1), "range"), (dict(block_table_cols=-1), "range"), (dict(lengths=None), "null"),
+                     (dict(free_capacity=-1), "range"), (dict(block_table_cols=-1), "range"), (dict(block_table_cols=2 ** 22), "range"), (dict(lengths=None), "null"),
                      (dict(block_table=None), "null"), (dict(held=None), "null"), (dict(free_count=None), "null"),
                      (dict(free_pages=None), "null"), (dict(kv_len=None), "null"), (dict(positions=None), "positions"),
                      (dict(slots=None), "slots"), (dict(parents=P), "mask"), (dict(tree_mask_words=1), "parents"),
