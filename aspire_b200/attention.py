@@ -131,6 +131,9 @@ class HolisticAttentionWrapper:
         self._has_jit = jit_args is not None
 
         self._plan_info: Optional[_capi.AspirePlanInfo] = None
+        self._plan_host_arrays: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None
+        self._plan_trees = False
+        self._tree_args: Optional[_capi.AspireAttnArgs] = None
         self._kv_indices: Optional[torch.Tensor] = None
         self._page_tables: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None
         self._page_size = 0
@@ -152,6 +155,7 @@ class HolisticAttentionWrapper:
         plan's ``paged_kv_indices`` may then be None.  The tensors must stay
         allocated (CUDA graphs capture their addresses).  ``None`` turns the
         tables off."""
+        self._tree_args = None
         if mode_flags is None:
             self._page_tables = None
             return
@@ -207,8 +211,11 @@ class HolisticAttentionWrapper:
         head_dim_vo: Optional[int] = None,
         causal: bool = False,
         sm_scale: Optional[float] = None,
+        trees: bool = False,
     ) -> None:
-        """Plans from host arrays with no device readback or synchronisation."""
+        """Plans from host arrays with no device readback or synchronisation.
+        ``trees`` (not causal) plans for ``run`` with a ``tree_mask``, and for
+        nothing else: other tiles of the rows and lengths of the chunks."""
         if head_dim_vo is not None and head_dim_vo != head_dim_qk:
             raise ValueError("head_dim_vo must equal head_dim_qk")
         if paged_kv_indices is None and self._page_tables is None:
@@ -219,7 +226,20 @@ class HolisticAttentionWrapper:
         batch = int(kvl.shape[0])
         if qo.shape[0] < batch + 1 or kvp.shape[0] < batch + 1:
             raise ValueError("qo_indptr / kv_indptr need batch_size + 1 entries")
+        if trees and causal:
+            raise ValueError("a plan for trees is not causal")
+        self._plan_arrays(qo, kvp, kvl, (int(num_qo_heads), int(num_kv_heads), int(head_dim_qk), int(page_size)),
+                          _capi.PLAN_TREE if trees else 1 if causal else 0)
+        self._kv_indices = paged_kv_indices
+        self._page_size = int(page_size)
+        self._sm_scale = sm_scale
+        self._causal = bool(causal)
+        self._num_qo_heads = int(num_qo_heads)
+        self._num_kv_heads = int(num_kv_heads)
 
+    def _plan_arrays(self, qo: torch.Tensor, kvp: torch.Tensor, kvl: torch.Tensor, shape: Tuple[int, int, int, int],
+                     mode: int) -> None:
+        batch = int(kvl.shape[0])
         slot = self._pinned_slot
         event = self._pinned_ring_events[slot]
         if event is not None:
@@ -228,8 +248,7 @@ class HolisticAttentionWrapper:
         info = _capi.AspirePlanInfo()
         stream = torch.cuda.current_stream(self._device).cuda_stream
         rc = self._lib.aspire_plan(
-            _ptr_i32(qo), _ptr_i32(kvp), _ptr_i32(kvl), batch, int(num_qo_heads), int(num_kv_heads),
-            int(head_dim_qk), int(page_size), 1 if causal else 0, self._num_sms,
+            _ptr_i32(qo), _ptr_i32(kvp), _ptr_i32(kvl), batch, *shape, mode, self._num_sms,
             ctypes.c_void_p(buf.data_ptr()), buf.numel(),
             ctypes.c_void_p(self._int_workspace.data_ptr()), self._int_workspace.numel(),
             self._float_workspace.numel(), ctypes.c_void_p(stream), ctypes.byref(info),
@@ -245,12 +264,10 @@ class HolisticAttentionWrapper:
         self._plan_q_total = int(qo[batch])
         self._plan_max_kv_len = int(kvl.max()) if batch else 0
         self._plan_rows = batch
-        self._kv_indices = paged_kv_indices
-        self._page_size = int(page_size)
-        self._sm_scale = sm_scale
-        self._causal = bool(causal)
-        self._num_qo_heads = int(num_qo_heads)
-        self._num_kv_heads = int(num_kv_heads)
+        # (What a plan that is not causal is made from, should its rows turn out to be trees.)
+        self._plan_host_arrays = (qo, kvp, kvl) if mode == 0 else None
+        self._plan_trees = mode == _capi.PLAN_TREE
+        self._tree_args = None
 
     def plan_device(
         self,
@@ -265,6 +282,7 @@ class HolisticAttentionWrapper:
         causal: bool = False,
         sm_scale: Optional[float] = None,
         batch_size: Optional[int] = None,
+        trees: bool = False,
     ) -> None:
         """Plans on the device from device arrays (C ABI ``aspire_plan_device``):
         no readback and no synchronisation, so the call can be captured in a
@@ -274,7 +292,9 @@ class HolisticAttentionWrapper:
         Row b attends ``max(pages_b - 1, 0) * page_size + last_page_len[b]``
         tokens.  Problems found on the device (a malformed row, a plan beyond
         the workspaces) are reported in ``device_status()`` and the program
-        then writes nothing."""
+        then writes nothing.  ``trees`` as for ``plan_host``."""
+        if trees and causal:
+            raise ValueError("a plan for trees is not causal")
         batch = int(paged_kv_last_page_len.shape[0] if batch_size is None else batch_size)
         for name, t in (("qo_indptr", qo_indptr), ("paged_kv_indptr", paged_kv_indptr),
                         ("paged_kv_last_page_len", paged_kv_last_page_len)):
@@ -289,12 +309,15 @@ class HolisticAttentionWrapper:
         stream = torch.cuda.current_stream(self._device).cuda_stream
         rc = self._lib.aspire_plan_device(
             _dev_i32(qo_indptr), _dev_i32(paged_kv_indptr), _dev_i32(paged_kv_last_page_len), batch, int(num_qo_heads), int(num_kv_heads),
-            int(head_dim_qk), int(page_size), 1 if causal else 0, self._num_sms,
+            int(head_dim_qk), int(page_size), _capi.PLAN_TREE if trees else 1 if causal else 0, self._num_sms,
             ctypes.c_void_p(self._int_workspace.data_ptr()), self._int_workspace.numel(),
             self._float_workspace.numel(), ctypes.c_void_p(stream), ctypes.byref(info),
         )
         _capi.check(rc, "aspire_plan_device")
         self._plan_info = info
+        self._plan_host_arrays = None
+        self._plan_trees = bool(trees)
+        self._tree_args = None
         self._plan_q_total = 0      # checked on the device: rows past q are skipped
         self._plan_max_kv_len = 0   # checked on the device: dump writes past kv_stride are skipped
         self._plan_rows = batch
@@ -334,9 +357,24 @@ class HolisticAttentionWrapper:
         of those, key j iff bit j % 32 of word j / 32 of its mask is set, as
         ``build_step_tables`` makes it.  A query that sees no key gets zeros
         and an LSE of -inf.  Keys and values that some query does not see must
-        be finite.  The plan must be made with ``causal=False``; no dump."""
+        be finite.  The plan must not be causal; no dump.  A plan made on the
+        host without ``trees=True`` is made again for trees by the first such
+        call outside a graph's capture."""
         if self._plan_info is None:
             raise RuntimeError("run() before plan()/plan_host()")
+        if tree_mask is not None:
+            if self._causal:
+                raise ValueError("tree_mask needs a plan made with causal=False")
+            if self._has_jit and self._dump_kind != "noop":
+                raise ValueError("a dump variant takes no tree_mask")
+            if self._plan_host_arrays is not None and not torch.cuda.is_current_stream_capturing():
+                heads = (self._num_qo_heads, self._num_kv_heads)
+                self._plan_arrays(*self._plan_host_arrays, (*heads, 128, self._page_size), _capi.PLAN_TREE)
+            if append is None:
+                return self._run_trees(q, _unpack_paged_kv_cache(paged_kv_cache, self._kv_layout), tree_mask, out,
+                                       lse, return_lse)
+        elif self._plan_trees:
+            raise ValueError("the plan was made for trees: give a tree_mask")
         kv = _unpack_paged_kv_cache(paged_kv_cache, self._kv_layout)
         if q.dtype != torch.bfloat16 or kv.dtype != torch.bfloat16:
             raise ValueError("q and paged_kv_cache must be bfloat16")
@@ -393,10 +431,6 @@ class HolisticAttentionWrapper:
             if tree_mask.dtype != torch.int32 or tree_mask.dim() != 2 or not tree_mask.is_contiguous() or \
                     tree_mask.device != q.device or tree_mask.shape[0] < q.shape[0] or tree_mask.shape[1] < 1:
                 raise ValueError("tree_mask must be a contiguous int32 [tokens, words] tensor on q's device")
-            if self._causal:
-                raise ValueError("tree_mask needs a plan made with causal=False")
-            if dump is not None:
-                raise ValueError("a dump variant takes no tree_mask")
         sm_scale = self._sm_scale if self._sm_scale is not None else 1.0 / math.sqrt(q.shape[2])
         a = _capi.AspireAttnArgs()
         a.q = q.data_ptr()
@@ -459,6 +493,33 @@ class HolisticAttentionWrapper:
         if return_lse:
             return out, lse
         return out
+
+    def _run_trees(self, q, kv, tree_mask, out, lse, return_lse):
+        """``run`` with a tree mask, its checks and its call compiled."""
+        a = self._tree_args
+        if a is None:
+            a = _capi.AspireAttnArgs()
+            if self._kv_indices is not None and self._page_tables is None:
+                a.kv_indices = self._kv_indices.data_ptr()
+            else:
+                if self._page_tables is None:
+                    raise RuntimeError("no page list: plan with paged_kv_indices or call set_page_tables()")
+                mode_flags, draft_table, block_table = self._page_tables
+                a.mode_flags = mode_flags.data_ptr()
+                a.draft_table, a.draft_stride = draft_table.data_ptr(), draft_table.stride(0)
+                a.block_table, a.block_table_stride = block_table.data_ptr(), block_table.stride(0)
+            a.sm_scale = float(self._sm_scale) if self._sm_scale is not None else 1.0 / math.sqrt(128)
+            a.num_qo_heads, a.num_kv_heads = self._num_qo_heads, self._num_kv_heads
+            a.page_size = self._page_size
+            a.int_ws, a.int_ws_bytes = self._int_workspace.data_ptr(), self._int_workspace.numel()
+            a.float_ws, a.float_ws_bytes = self._float_workspace.data_ptr(), self._float_workspace.numel()
+            self._tree_args = a
+            self._tree_addresses = ctypes.addressof(a), ctypes.addressof(self._plan_info)
+        if q.device != self._device:
+            raise ValueError("q must be on the wrapper's device")
+        out, lse = _capi.ops().tree_attention(q, kv, tree_mask, out, lse, bool(return_lse), *self._tree_addresses,
+                                              self._plan_q_total)
+        return (out, lse) if return_lse else out
 
     # ------------------------------------------------------------- diagnostics
     def device_status(self) -> int:

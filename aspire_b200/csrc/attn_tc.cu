@@ -68,21 +68,27 @@ constexpr int kPvWarp = 11;           // decode phase: the P.V issuer
 constexpr int kSeqReaders = 11;       // V producer, the two MMA warps and the 8 softmax warps
 constexpr int kKStages = 2;
 constexpr int kVStages = 3;
-constexpr int kNMax = kTcQTile;
 constexpr uint32_t kTmemCols = pf::kTmemCols;  // the decode phase uses [0, 256)
-constexpr uint32_t kQHalfBytes = kNMax * 128;
-constexpr uint32_t kPBufBytes = (kNMax / 8) * kTile * 16;
 constexpr float kLazyLog2 = 8.0f;                  // max growth tolerated before a rescale
 
 __host__ __device__ constexpr uint32_t col_s(int b) { return uint32_t(b) * 64u; }
 constexpr uint32_t kColO = 128;
 
+// kNMax: columns of an item's products at most.  The tree kernel has 64, so
+// that a tree's 16 nodes of a group of 4 are one pass over the keys; its
+// finished rows leave through the P buffers, which its larger buffers leave no
+// other room for (kStageInP).
+template <int kColumns>
 struct TcShared {
+  static constexpr int kNMax = kColumns;
+  static constexpr bool kStageInP = kColumns > kTcQTile;
+  static constexpr uint32_t kQHalfBytes = kNMax * 128;
+  static constexpr uint32_t kPBufBytes = (kNMax / 8) * kTile * 16;
   uint8_t k[kKStages][kSlotBytes];
   uint8_t v[kVStages][kSlotBytes];
   uint8_t q[2][kQHalfBytes];
   uint8_t p[2][kPBufBytes];
-  uint8_t out_stage[kNMax * kHeadDim * 4];  // finished rows (fp32 partial or bf16) on their way out
+  uint8_t out_stage[kStageInP ? 16 : kNMax * kHeadDim * 4];  // finished rows (fp32 partial or bf16) on their way out
   float red[2][4][kNMax];
   float red_l[4][kNMax];
   float alpha[2][kNMax];
@@ -101,10 +107,17 @@ struct TcShared {
   uint32_t tmem_base;
   int abort_flag;
 };
-static_assert(sizeof(TcShared) + 1024 <= 227 * 1024, "tcgen05 kernel shared memory too large");
-// The prefill phase's buffers overlay the decode phase's data buffers only.
-static_assert(sizeof(pf::Buffers) <= offsetof(TcShared, red), "prefill buffers overlap decode state");
-static_assert(kNMax % 16 == 0 && kNMax <= 64, "N tile must be a multiple of 16 and fit a 64-column buffer");
+template <class Sh>
+constexpr bool shared_fits() {
+  static_assert(sizeof(Sh) + 1024 <= 227 * 1024, "tcgen05 kernel shared memory too large");
+  // The prefill phase's buffers overlay the decode phase's data buffers only.
+  static_assert(sizeof(pf::Buffers) <= offsetof(Sh, red), "prefill buffers overlap decode state");
+  static_assert(Sh::kNMax % 16 == 0 && Sh::kNMax <= 64, "N tile must be a multiple of 16 and fit a 64-column buffer");
+  return true;
+}
+using DecodeShared = TcShared<kTcQTile>;
+using TreeShared = TcShared<kTreeQTile>;
+static_assert(shared_fits<DecodeShared>() && shared_fits<TreeShared>(), "");
 
 // Columns N of an item's products: its packed rows rounded up to 16, or the
 // wider width its plan gives it (WorkItem::cols: the planners give the long
@@ -114,21 +127,24 @@ static_assert(kNMax % 16 == 0 && kNMax <= 64, "N tile must be a multiple of 16 a
 // rows' own width and kNMax is ignored, so every role derives the same N.
 // Launches with the dump keep the exact widths (their dump path is longer
 // per column).
+template <class Sh>
 __device__ __forceinline__ int item_columns(const WorkItem& it, bool use_cols) {
   const int exact = (it.pq_end - it.pq_begin + 15) / 16 * 16;
-  return use_cols && it.cols > exact && it.cols <= kNMax && it.cols % 16 == 0 ? it.cols : exact;
+  return use_cols && it.cols > exact && it.cols <= Sh::kNMax && it.cols % 16 == 0 ? it.cols : exact;
 }
 
 // Barrier of one softmax warpgroup's 128 threads on an mbarrier (bounded, so that a warp
 // that stopped on a timeout cannot leave the others blocked).  The result is the
 // lane's own; group_sync_warp's is the warp's.
-__device__ __forceinline__ bool group_sync(TcShared& sm, uint64_t& grp, uint32_t& uses, uint32_t* status) {
+template <class Sh>
+__device__ __forceinline__ bool group_sync(Sh& sm, uint64_t& grp, uint32_t& uses, uint32_t* status) {
   ptx::mbar_arrive(ptx::smem_addr(&grp));
   const uint32_t parity = uses & 1;
   ++uses;
   return wait_bar(sm, grp, parity, status);
 }
-__device__ __forceinline__ bool group_sync_warp(TcShared& sm, uint64_t& grp, uint32_t& uses, uint32_t* status) {
+template <class Sh>
+__device__ __forceinline__ bool group_sync_warp(Sh& sm, uint64_t& grp, uint32_t& uses, uint32_t* status) {
   return __all_sync(0xffffffffu, group_sync(sm, grp, uses, status)) != 0;
 }
 
@@ -145,7 +161,8 @@ __device__ __forceinline__ bool group_sync_warp(TcShared& sm, uint64_t& grp, uin
 // the CTA's shared memory), so each loop adds offsets to a base descriptor.
 
 // QK^T of every tile, and the query-tile loads (warp 1).
-__device__ void run_qk(const AttnParams& p, const CUtensorMap* qmap, TcShared& sm, int lane, uint32_t& k,
+template <class Sh>
+__device__ void run_qk(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, int lane, uint32_t& k,
                        bool use_cols) {
   const uint32_t tmem = sm.tmem_base;
   uint32_t g = 0, items_done = 0;
@@ -155,7 +172,7 @@ __device__ void run_qk(const AttnParams& p, const CUtensorMap* qmap, TcShared& s
   const uint64_t qdesc0 = ptx::smem_desc(q0, 16, 1024, ptx::kLayoutSw128);
   bool q_pending = false;  // a query-tile load is in flight
 
-  int ii = next_item_with_tiles(p, sm, k, lane, kNMax);
+  int ii = next_item_with_tiles(p, sm, k, lane, Sh::kNMax);
   if (ii == -2) ok = false;
   if (ii >= 0) {
     if (lane == 0) issue_q(p, qmap, sm, ii, p.q_box_tokens);
@@ -164,7 +181,7 @@ __device__ void run_qk(const AttnParams& p, const CUtensorMap* qmap, TcShared& s
   while (ii >= 0 && ok) {
     const WorkItem it = load_item(p.plan, ii);
     const int nt = n_tiles_of(it);
-    const uint32_t N = uint32_t(item_columns(it, use_cols));
+    const uint32_t N = uint32_t(item_columns<Sh>(it, use_cols));
     const uint32_t idesc_qk = ptx::idesc_bf16(128, N, false, false);
     if (!wait_bar_warp(sm, sm.q_full, items_done & 1, p.status)) {
       ok = false;
@@ -181,7 +198,7 @@ __device__ void run_qk(const AttnParams& p, const CUtensorMap* qmap, TcShared& s
 #pragma unroll
         for (int kk = 0; kk < 128 / 16; ++kk) {
           const uint32_t koff = uint32_t(kk / 4) * kHalfBytes + uint32_t(kk % 4) * 32;
-          const uint32_t qoff = uint32_t(kk / 4) * kQHalfBytes + uint32_t(kk % 4) * 32;
+          const uint32_t qoff = uint32_t(kk / 4) * Sh::kQHalfBytes + uint32_t(kk % 4) * 32;
           ptx::mma_bf16(tmem + col_s(sb), kdesc0 + (koff >> 4), qdesc0 + (qoff >> 4), idesc_qk, kk > 0 ? 1u : 0u);
         }
         ptx::mma_commit(ptx::smem_addr(&sm.s_full[sb]));
@@ -192,7 +209,7 @@ __device__ void run_qk(const AttnParams& p, const CUtensorMap* qmap, TcShared& s
     }
     if (!ok) break;
     // The next item's query tile loads while this item's last PV and epilogue run.
-    const int nxt = next_item_with_tiles(p, sm, k, lane, kNMax);
+    const int nxt = next_item_with_tiles(p, sm, k, lane, Sh::kNMax);
     if (nxt == -2) {
       ok = false;
       break;
@@ -218,18 +235,19 @@ __device__ void run_qk(const AttnParams& p, const CUtensorMap* qmap, TcShared& s
 }
 
 // P.V of every tile into the O accumulator (warp 11).
-__device__ void run_pv(const AttnParams& p, TcShared& sm, int lane, uint32_t& k, bool use_cols) {
+template <class Sh>
+__device__ void run_pv(const AttnParams& p, Sh& sm, int lane, uint32_t& k, bool use_cols) {
   const uint32_t tmem = sm.tmem_base;
   uint32_t g = 0, items_done = 0;
   bool ok = true;
   const uint32_t v0 = ptx::smem_addr(sm.v[0]);
   const uint32_t p0 = ptx::smem_addr(sm.p[0]);
-  int ii = next_item_with_tiles(p, sm, k, lane, kNMax);
+  int ii = next_item_with_tiles(p, sm, k, lane, Sh::kNMax);
   if (ii == -2) ok = false;
   while (ii >= 0 && ok) {
     const WorkItem it = load_item(p.plan, ii);
     const int nt = n_tiles_of(it);
-    const uint32_t N = uint32_t(item_columns(it, use_cols));
+    const uint32_t N = uint32_t(item_columns<Sh>(it, use_cols));
     const uint32_t idesc_pv = ptx::idesc_bf16(128, N, true, true);
     for (int t = 0; t < nt && ok; ++t, ++g) {
       const uint32_t vs = g % kVStages, pb = g % 2;
@@ -244,7 +262,7 @@ __device__ void run_pv(const AttnParams& p, TcShared& sm, int lane, uint32_t& k,
       ptx::tc_fence_after();
       if (lane == 0 && ready) {
         const uint64_t vdesc0 = ptx::smem_desc(v0 + vs * kSlotBytes, kHalfBytes, 1024, ptx::kLayoutSw128);
-        const uint64_t pdesc0 = ptx::smem_desc(p0 + pb * kPBufBytes, 128, kTile * 16, ptx::kLayoutNone);
+        const uint64_t pdesc0 = ptx::smem_desc(p0 + pb * Sh::kPBufBytes, 128, kTile * 16, ptx::kLayoutNone);
 #pragma unroll
         for (int kk = 0; kk < kTile / 16; ++kk)
           ptx::mma_bf16(tmem + kColO, vdesc0 + uint64_t(kk * 2048 >> 4), pdesc0 + uint64_t(kk * 256 >> 4), idesc_pv,
@@ -256,7 +274,7 @@ __device__ void run_pv(const AttnParams& p, TcShared& sm, int lane, uint32_t& k,
     }
     if (!ok) break;
     ++items_done;
-    ii = next_item_with_tiles(p, sm, k, lane, kNMax);
+    ii = next_item_with_tiles(p, sm, k, lane, Sh::kNMax);
     if (ii == -2) ok = false;
   }
   if (lane == 0) ptx::mma_commit(ptx::smem_addr(&sm.done_pv));
@@ -320,11 +338,13 @@ __device__ __forceinline__ float reduce_scatter8(float* v, int lane) {
   return v[0];
 }
 
-// Per-warp reduction of NH (8, 16 or 24) columns over the 32 lanes, written to
-// out[0..NH).  Destroys v.
+// Per-warp reduction of NH (8, 16, 24 or 32) columns over the 32 lanes, written
+// to out[0..NH).  Destroys v.
 template <int NH, bool kMax>
 __device__ __forceinline__ void warp_columns(float* v, float* out, int lane) {
-  if constexpr (NH == 8) {
+  if constexpr (NH == 32) {
+    out[lane] = reduce_scatter32<kMax>(v, lane);
+  } else if constexpr (NH == 8) {
     const float r8 = reduce_scatter8<kMax>(v, lane);
     if (lane < 8) out[lane] = r8;
   } else {
@@ -337,10 +357,11 @@ __device__ __forceinline__ void warp_columns(float* v, float* out, int lane) {
   }
 }
 
-// NH consecutive TMEM columns of this warp's lanes (NH = 8, 16 or 24).
+// NH consecutive TMEM columns of this warp's lanes (NH = 8, 16, 24 or 32).
 template <int NH>
 __device__ __forceinline__ void tmem_load_cols(uint32_t taddr, float* v) {
-  if constexpr (NH >= 16) ptx::tmem_ld16(taddr, v);
+  if constexpr (NH == 32) ptx::tmem_ld32(taddr, v);
+  if constexpr (NH == 16 || NH == 24) ptx::tmem_ld16(taddr, v);
   if constexpr (NH == 8) ptx::tmem_ld8(taddr, v);
   if constexpr (NH == 24) ptx::tmem_ld8(taddr + 16, v + 16);
 }
@@ -396,8 +417,8 @@ __device__ __forceinline__ uint32_t tree_columns(const AttnParams& p, const Work
   return seen;
 }
 
-template <int NH, bool kDump, bool kTree>
-__device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& it, bool causal, int r,
+template <int NH, bool kDump, bool kTree, class Sh>
+__device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bool causal, int r,
                              int ctid, int wg, int wq, int lane, uint32_t& g, uint32_t& grp_uses) {
   constexpr int N = 2 * NH;
   const int c0 = wg * NH;
@@ -519,6 +540,8 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
     // (The next tile's flag was read two tiles ago, before this thread passed the
     // last barrier: it is free to be cleared.)
     const int next_flag = flag == 2 ? 0 : flag + 1;
+    // The previous item's rows have left the P buffers before this item's P is written.
+    if (Sh::kStageInP && t == 0 && ctid == 0) ptx::bulk_wait_read();
     if (exceed) flags[flag][wq] = 1;
     if (lane == 0) flags[next_flag][wq] = 0;
     failed |= !group_sync(sm, grp, grp_uses, p.status);
@@ -569,6 +592,7 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
         if constexpr (NH >= 16) ptx::tmem_st16(tmem_lane + kColO + c0, ov);
         if constexpr (NH == 8) ptx::tmem_st8(tmem_lane + kColO + c0, ov);
         if constexpr (NH == 24) ptx::tmem_st8(tmem_lane + kColO + c0 + 16, ov + 16);
+        if constexpr (NH == 32) ptx::tmem_st16(tmem_lane + kColO + c0 + 16, ov + 16);
         ptx::tmem_wait_st();
         ptx::tc_fence_before();
       }
@@ -630,30 +654,36 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
   }
   // The previous item's bulk stores (issued by this group's thread 0) have
   // read the group's staging rows before anyone rewrites them.
-  if (ctid == 0) ptx::bulk_wait_read();
+  if (!Sh::kStageInP && ctid == 0) ptx::bulk_wait_read();
   if (!group_sync_warp(sm, grp, grp_uses, p.status)) return false;
 
   // Normalised rows are staged in shared memory and leave by bulk stores, so
   // the threads move on to the next item at once.
   const int d = r;  // this thread's output dim
-  uint8_t* stage = sm.out_stage;
+  // Row c0 + j of the item, of row_bytes: in the output stage or, by halves of
+  // the group's rows, in its parts of the two P buffers.
+  const auto staged = [&](int j, int row_bytes) -> uint8_t* {
+    if constexpr (Sh::kStageInP)
+      return sm.p[j / (NH / 2)] + (c0 / 8) * (kTile * 16) + (j % (NH / 2)) * row_bytes;
+    else
+      return sm.out_stage + (c0 + j) * row_bytes;
+  };
   const bool final_rows = it.n_chunks <= 1;
   const int row_end = min(c0 + NH, nrows);  // this group's rows are [c0, row_end)
   if (final_rows) {
-    __nv_bfloat16* st = reinterpret_cast<__nv_bfloat16*>(stage);
 #pragma unroll
     for (int j = 0; j < NH; ++j)
-      if (c0 + j < nrows) st[(c0 + j) * kHeadDim + d] = __float2bfloat16_rn(o_fin[j] * sm.inv_l[c0 + j]);
+      if (c0 + j < nrows)
+        reinterpret_cast<__nv_bfloat16*>(staged(j, kHeadDim * 2))[d] = __float2bfloat16_rn(o_fin[j] * sm.inv_l[c0 + j]);
     if (ctid < NH && c0 + ctid < nrows && p.lse) {
       int q_idx, head;
       packed_row(p, it, it.pq_begin + c0 + ctid, q_idx, head);
       if (int64_t(it.q_start) + q_idx < p.q_rows) p.lse[(int64_t(it.q_start) + q_idx) * p.num_qo_heads + head] = my_lse;
     }
   } else {
-    float* st = reinterpret_cast<float*>(stage);
 #pragma unroll
     for (int j = 0; j < NH; ++j)
-      if (c0 + j < nrows) st[(c0 + j) * kHeadDim + d] = o_fin[j] * sm.inv_l[c0 + j];
+      if (c0 + j < nrows) reinterpret_cast<float*>(staged(j, kHeadDim * 4))[d] = o_fin[j] * sm.inv_l[c0 + j];
     if (ctid < NH && c0 + ctid < nrows)
       partial_lse_ptr(p)[int64_t(it.partial_base) + int64_t(it.chunk) * nrows + c0 + ctid] = my_lse;
   }
@@ -661,7 +691,6 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
   if (!group_sync_warp(sm, grp, grp_uses, p.status)) return false;
   if (ctid == 0 && c0 < row_end) {
     if (final_rows) {
-      const uint32_t src = ptx::smem_addr(stage);
       for (int j = c0; j < row_end; ++j) {
         int q_idx, head;
         packed_row(p, it, it.pq_begin + j, q_idx, head);
@@ -670,20 +699,24 @@ __device__ bool consume_item(const AttnParams& p, TcShared& sm, const WorkItem& 
           continue;
         }
         __nv_bfloat16* dst = p.out + (int64_t(it.q_start) + q_idx) * p.o_stride_n + int64_t(head) * p.o_stride_h;
-        ptx::bulk_store(dst, src + uint32_t(j) * kHeadDim * 2, kHeadDim * 2);
+        ptx::bulk_store(dst, ptx::smem_addr(staged(j - c0, kHeadDim * 2)), kHeadDim * 2);
       }
     } else {
-      const uint32_t src = ptx::smem_addr(stage) + uint32_t(c0) * kHeadDim * 4;
       const int64_t base = int64_t(it.partial_base) + int64_t(it.chunk) * nrows + c0;
-      ptx::bulk_store(p.partial_o + base * kHeadDim, src, uint32_t(row_end - c0) * kHeadDim * 4);
+      const int rows = row_end - c0, part = Sh::kStageInP ? min(rows, NH / 2) : rows;  // rows in one piece
+      ptx::bulk_store(p.partial_o + base * kHeadDim, ptx::smem_addr(staged(0, kHeadDim * 4)),
+                      uint32_t(part) * kHeadDim * 4);
+      if (part < rows)
+        ptx::bulk_store(p.partial_o + (base + part) * kHeadDim, ptx::smem_addr(staged(part, kHeadDim * 4)),
+                        uint32_t(rows - part) * kHeadDim * 4);
     }
     ptx::bulk_commit();
   }
   return true;
 }
 
-template <bool kTree>
-__device__ void consume_items(const AttnParams& p, TcShared& sm, bool causal, int warp, int lane, uint32_t& k,
+template <bool kTree, class Sh>
+__device__ void consume_items(const AttnParams& p, Sh& sm, bool causal, int warp, int lane, uint32_t& k,
                               bool use_cols) {
   const int wq = warp & 3;
   const int wg = (warp - kFirstSoftmaxWarp) / 4;  // softmax warpgroup 0 or 1
@@ -696,7 +729,7 @@ __device__ void consume_items(const AttnParams& p, TcShared& sm, bool causal, in
     if (ii < 0) return;
     const WorkItem it = load_item(p.plan, ii);
     const int nrows = it.pq_end - it.pq_begin;
-    if (!item_valid(p, it, kNMax)) {
+    if (!item_valid(p, it, Sh::kNMax)) {
       if (ctid == 0 && wg == 0) record_status(p.status, ASPIRE_STATUS_BAD_PLAN);
       continue;
     }
@@ -705,7 +738,7 @@ __device__ void consume_items(const AttnParams& p, TcShared& sm, bool causal, in
       for (int j = wg; j < nrows; j += 2) store_final(p, it, it.pq_begin + j, r, 0.f, -INFINITY);
       continue;
     }
-    const int N = item_columns(it, use_cols);
+    const int N = item_columns<Sh>(it, use_cols);
     // Items whose columns include dumped rows (query 0 or the last query, as
     // the dump kind and the row's flag have it) take the instantiation that
     // carries the dump path.
@@ -728,15 +761,17 @@ __device__ void consume_items(const AttnParams& p, TcShared& sm, bool causal, in
         ok = consume_item<8, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
       else if (N == 32)
         ok = consume_item<16, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
-      else
+      else if (Sh::kNMax == 48 || N == 48)
         ok = consume_item<24, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+      else if constexpr (Sh::kNMax > 48)
+        ok = consume_item<32, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
     }
     if (!ok) return;
   }
 }
 
-template <bool kTree>
-__device__ void run_consumer(const AttnParams& p, TcShared& sm, bool causal, int warp, int lane, uint32_t& k,
+template <bool kTree, class Sh>
+__device__ void run_consumer(const AttnParams& p, Sh& sm, bool causal, int warp, int lane, uint32_t& k,
                              bool use_cols) {
   consume_items<kTree>(p, sm, causal, warp, lane, k, use_cols);
   // The bulk stores of each group's last item (issued by its thread 0) finish
@@ -750,7 +785,8 @@ __device__ __forceinline__ void attn_tc(const AttnParams& p, const CUtensorMap& 
   pdl_launch_dependents();
   extern __shared__ __align__(1024) uint8_t tc_smem_raw[];
   const uint32_t raw = ptx::smem_addr(tc_smem_raw);
-  TcShared& sm = *reinterpret_cast<TcShared*>(tc_smem_raw + ((1024 - (raw & 1023)) & 1023));
+  using Sh = TcShared<kTree ? kTreeQTile : kTcQTile>;
+  Sh& sm = *reinterpret_cast<Sh*>(tc_smem_raw + ((1024 - (raw & 1023)) & 1023));
   pf::Buffers& pbuf = *reinterpret_cast<pf::Buffers*>(&sm);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -823,11 +859,11 @@ __device__ __forceinline__ void attn_tc(const AttnParams& p, const CUtensorMap& 
   // Phase 1: the decode list.
   if (n_tc > 0) {
     if (warp == 0) {
-      run_producer<kKStages>(p, &tmap, sm, sm.k, sm.k_full, sm.k_empty, 0, true, tc_first, n_tc, kHdrTcClaim, kNMax,
-                             lane, k);
+      run_producer<kKStages>(p, &tmap, sm, sm.k, sm.k_full, sm.k_empty, 0, true, tc_first, n_tc, kHdrTcClaim,
+                             Sh::kNMax, lane, k);
     } else if (warp == kVProducerWarp) {
       run_producer<kVStages>(p, &tmap, sm, sm.v, sm.v_full, sm.v_empty, 1, false, tc_first, n_tc, kHdrTcClaim,
-                             kNMax, lane, k);
+                             Sh::kNMax, lane, k);
     } else if (warp == 1) {
       run_qk(p, &qmap, sm, lane, k, use_cols);
     } else if (warp == kPvWarp) {
@@ -883,7 +919,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   attn_tc<true>(p, tmap, qmap, qmap_pf);
 }
 
-size_t tc_smem_bytes() { return sizeof(TcShared) + 1024; }
+size_t tc_smem_bytes(bool tree) { return (tree ? sizeof(TreeShared) : sizeof(DecodeShared)) + 1024; }
 
 int tc_threads() { return kTcThreads; }
 

@@ -236,13 +236,13 @@ int aspire_plan_device(const int32_t* qo_indptr, const int32_t* kv_indptr, const
   p.batch = batch_size;
   p.group = group;
   p.num_kv_heads = num_kv_heads;
-  p.causal = causal;
+  p.causal = causal == kPlanTree ? kPlanTree : causal ? kPlanCausal : kPlanAll;
   p.num_sms = num_ctas;
   p.plan = reinterpret_cast<int32_t*>(static_cast<char*>(dev_int_ws) + kStatusBytes);
   p.plan_words = int64_t((dev_int_ws_bytes - kStatusBytes) / 4);
   p.float_ws_bytes = int64_t(float_ws_bytes);
   p.status = static_cast<uint32_t*>(dev_int_ws);
-  int rc = launch(aspire_plan_device_kernel, dim3(1), dim3(kDevPlanThreads), 0, static_cast<cudaStream_t>(stream),
+  int rc = launch(plan_device_kernel(p.causal == kPlanTree), dim3(1), dim3(kDevPlanThreads), 0, static_cast<cudaStream_t>(stream),
                   "aspire_plan_device_kernel launch", p);
   if (rc) return rc;
   std::memset(info, 0, sizeof(*info));
@@ -257,7 +257,7 @@ int aspire_plan_device(const int32_t* qo_indptr, const int32_t* kv_indptr, const
   info->float_bytes = int64_t(float_ws_bytes);
   info->num_qo_heads = num_qo_heads;
   info->num_kv_heads = num_kv_heads;
-  info->causal = causal ? 1 : 0;
+  info->causal = p.causal;
   info->batch_size = batch_size;
   info->max_q_len = -1;
   info->tc_enabled = 1;
@@ -346,7 +346,7 @@ int run_attention(const AspireAttnArgs* a, const int32_t* tree_mask, int32_t mas
   p.num_qo_heads = a->num_qo_heads;
   p.num_kv_heads = a->num_kv_heads;
   p.group = group;
-  p.q_box_tokens = static_cast<int32_t>(std::min<int64_t>(kTcQTile / group, a->q_rows));
+  p.q_box_tokens = static_cast<int32_t>(std::min<int64_t>((tree_mask ? kTreeQTile : kTcQTile) / group, a->q_rows));
   p.pf_box_tokens = static_cast<int32_t>(std::min<int64_t>(kPfQTile / group, a->q_rows));
   p.q_rows = a->q_rows;
   p.plan = reinterpret_cast<const int32_t*>(static_cast<const char*>(a->int_ws) + kStatusBytes);
@@ -370,7 +370,7 @@ int run_attention(const AspireAttnArgs* a, const int32_t* tree_mask, int32_t mas
     if (rc) return rc;
   }
   if (run_tc) {
-    const size_t smem = tc_smem_bytes();
+    const size_t smem = tc_smem_bytes(tree_mask != nullptr);
     const auto kernel = tree_mask ? &aspire_attn_tree_kernel : &aspire_attn_tc_kernel;
     rc = ensure_smem(reinterpret_cast<const void*>(kernel), smem, tree_mask ? g_tree_smem : g_tc_smem);
     if (rc) return rc;
@@ -400,6 +400,8 @@ extern "C" {
 
 int aspire_mixed_attention(const AspireAttnArgs* a, const AspirePlanInfo* plan, void* stream) {
   clear_error();
+  if (plan && plan->causal == kPlanTree)
+    return set_error(ASPIRE_ERR_INVALID, "aspire_mixed_attention: a plan for trees needs aspire_tree_attention");
   return run_attention(a, nullptr, 0, plan, stream, "aspire_mixed_attention");
 }
 
@@ -408,7 +410,8 @@ int aspire_tree_attention(const AspireAttnArgs* a, const int32_t* tree_mask, int
   clear_error();
   if (!a || !plan || !tree_mask) return set_error(ASPIRE_ERR_INVALID, "aspire_tree_attention: null argument");
   if (mask_words <= 0) return set_error(ASPIRE_ERR_INVALID, "aspire_tree_attention: mask_words must be > 0");
-  if (plan->causal) return set_error(ASPIRE_ERR_INVALID, "aspire_tree_attention: the plan must be made with causal 0");
+  if (plan->causal == kPlanCausal)
+    return set_error(ASPIRE_ERR_INVALID, "aspire_tree_attention: the plan must not be causal");
   if (a->dump) return set_error(ASPIRE_ERR_INVALID, "aspire_tree_attention: no dump under a tree mask");
   if (a->num_kv_heads <= 0 || !plan->tc_enabled || a->num_qo_heads / a->num_kv_heads > kTcQTile || !all_rows_tc())
     return set_error(ASPIRE_ERR_INVALID,

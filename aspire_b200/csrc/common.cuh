@@ -201,6 +201,8 @@ __host__ __device__ inline bool pad_long_items(int64_t n_decode_items, int64_t n
 constexpr int kGatherQTile = 4;
 // Packed query rows handled by one tcgen05 item (N of the MMA after padding).
 constexpr int kTcQTile = 48;
+// The same under a tree mask: 16 nodes of a group of 4 in one pass over the keys.
+constexpr int kTreeQTile = 64;
 // Prefill items: two halves of up to kPfQTile packed query rows (the M of
 // the MMA), whole query positions per half, sharing every K/V tile.  Rows
 // with at least kPfMinRows packed query rows (long queries: prefill chunks)
@@ -210,5 +212,56 @@ constexpr int kPfMinRows = 128;
 constexpr int kPfMaxRows = 2 * kPfQTile;
 __host__ __device__ constexpr int pf_half_rows(int group) { return (kPfQTile / group) * group; }
 __host__ __device__ constexpr int pf_item_rows(int group) { return 2 * pf_half_rows(group); }
+
+// What a plan is made for (the planners' `causal` argument): a plan for trees
+// is not causal and runs under a tree mask only.  Its decode items have up to
+// kTreeQTile packed rows and every longer row is a prefill item, one pass over
+// the keys either way (8 rows of 16k keys, 16 nodes of a group of 4: 123 us
+// against 168 with tiles of 48 rows; 24 nodes: 185 as a prefill item, 165 in
+// two decode passes; 31 nodes: 189 against 253 in three).
+enum PlanMode : int { kPlanAll = 0, kPlanCausal = 1, kPlanTree = 2 };
+__host__ __device__ constexpr int decode_tile_rows(int mode) { return mode == kPlanTree ? kTreeQTile : kTcQTile; }
+__host__ __device__ constexpr int prefill_min_rows(int mode) { return mode == kPlanTree ? kTreeQTile + 1 : kPfMinRows; }
+
+// Chunk length of plans for trees: of kTreePlans candidates (about one, two or
+// three items per CTA; the longest group whole, in two or in three pieces) the
+// one whose estimated makespan is the shortest.  In tenths of a 128-token tile
+// of a decode item of up to 32 columns (1.75 us): wider tiles count more
+// (tree_tile10), an item's boundary kItemCost10, a split group's rows what
+// their partials' way out and back costs, the merge kMergeCost10.  The
+// makespan is the larger of the even share of all items and the rounds of
+// full-length ones.  Measured over fixed lengths of 256 to 131200 (16 rows of
+// 2k-8k with 8-16 nodes: best 81 us, the rule's 84; 8 rows of 4k-16k with
+// 32-64: 136, 136; one row of 32k with 8: 41, 41; 2 rows of 131k: 132, 140).
+constexpr int kTreePlans = 6;
+__host__ __device__ inline int64_t tree_chunk(int64_t total_tokens, int64_t max_span, int64_t num_sms, int k) {
+  const int64_t n = k < 3 ? num_sms * (k + 1) : k - 2;
+  int64_t chunk = ((k < 3 ? total_tokens : max_span) + n - 1) / n;
+  chunk = chunk < 256 ? 256 : chunk;
+  return (chunk + 127) / 128 * 128;
+}
+__host__ __device__ inline int64_t tree_tile10(int kind, int rows, int group) {
+  if (kind == 2) return rows > pf_half_rows(group) ? 16 : 13;
+  return rows > 48 ? 12 : rows > 32 ? 11 : 10;
+}
+// A group's part of the estimate for chunk length `chunk`.
+struct TreeCost {
+  int64_t work10, full, full10, split;  // all items, full-length ones, the longest of those, whether any group splits
+};
+__host__ __device__ inline void add_tree_cost(TreeCost& c, int64_t span, int64_t chunk, int64_t tile10, int64_t rows) {
+  const int64_t n = span > 0 ? (span + chunk - 1) / chunk : 1;
+  const int64_t item = kItemCost10 + (n > 1 ? rows * 10 / 64 : 0);  // (1 KB a row out and back, 64 KB a tile)
+  c.work10 += (span + 127) / 128 * tile10 + n * item;
+  const int64_t longest = span < chunk ? span : chunk;
+  const int64_t item10 = (longest + 127) / 128 * tile10 + item;
+  if (2 * longest > chunk) c.full += n > 1 ? span / chunk : 1;
+  if (item10 > c.full10) c.full10 = item10;
+  if (n > 1) c.split = 1;
+}
+__host__ __device__ inline int64_t tree_makespan(const TreeCost& c, int64_t num_sms) {
+  const int64_t even = (c.work10 + num_sms - 1) / num_sms, rounds = (c.full + num_sms - 1) / num_sms * c.full10;
+  const int64_t most = even > rounds ? even : rounds;
+  return (most > c.full10 ? most : c.full10) + (c.split ? kMergeCost10 : 0);
+}
 
 }  // namespace aspire

@@ -73,7 +73,8 @@ struct DevPlanParams {
   uint32_t* status;
 };
 constexpr int kDevPlanThreads = 1024;
-__global__ void aspire_plan_device_kernel(DevPlanParams p);
+using DevPlanKernel = void (*)(DevPlanParams);
+DevPlanKernel plan_device_kernel(bool trees);  // aspire_plan_device_kernel
 
 struct SelectParams {
   const void* dump;  // fp16 or fp32 (dump_f32) [rows, num_heads, dump_slots, kv_stride]
@@ -176,7 +177,7 @@ __global__ void aspire_append_kv_kernel(AppendParams p);
 __global__ void aspire_select_pages_kernel(SelectParams p);
 
 size_t gather_smem_bytes();
-size_t tc_smem_bytes();
+size_t tc_smem_bytes(bool tree);
 int tc_threads();
 bool tc_kernel_available();
 size_t select_smem_bytes(int pages_per_slot, int sort_cap);

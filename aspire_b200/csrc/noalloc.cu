@@ -84,6 +84,8 @@ extern "C" int aspire_mixed_attention_noalloc(const AspireAttnArgs* args, const 
                      "aspire_plan_host_only (an aspire_plan_device plan has no host copy to upload)");
   // Every argument is checked before the shared arrays are touched, so a
   // rejected call leaves the previous call's plan and status in place.
+  if (plan->causal == kPlanTree)
+    return set_error(ASPIRE_ERR_INVALID, "aspire_mixed_attention_noalloc: a plan for trees needs aspire_tree_attention");
   int rc = check_attention_args(args, plan, "aspire_mixed_attention_noalloc");
   if (rc) return rc;
   if (plan->int_bytes <= 0 || size_t(plan->int_bytes) + kStatusBytes > kNoAllocIntBytes)

@@ -65,7 +65,7 @@ struct RowShape {
 // logits).
 __device__ __forceinline__ int32_t tile_span(const DevPlanParams& p, const RowShape& s, int32_t pq_begin,
                                              int32_t pq_end) {
-  if (!p.causal || pq_begin < p.group) return s.kl;
+  if (p.causal != kPlanCausal || pq_begin < p.group) return s.kl;
   const int64_t q_last = (pq_end - 1) / p.group;
   const int64_t lim = int64_t(s.kl) - s.ql + q_last + 1;
   return int32_t(max(int64_t(0), min(int64_t(s.kl), lim)));
@@ -85,8 +85,8 @@ __device__ __forceinline__ RowShape row_shape(const DevPlanParams& p, int b) {
   r.ql = r.valid ? ql : 0;
   r.kl = r.valid ? kl : 0;
   r.nq = r.ql * p.group;
-  r.kind = r.nq >= kPfMinRows ? 2 : 1;
-  r.tile = r.kind == 2 ? pf_item_rows(p.group) : (kTcQTile / p.group) * p.group;
+  r.kind = r.nq >= prefill_min_rows(p.causal) ? 2 : 1;
+  r.tile = r.kind == 2 ? pf_item_rows(p.group) : (decode_tile_rows(p.causal) / p.group) * p.group;
   r.ntq = (r.nq + r.tile - 1) / r.tile;
   return r;
 }
@@ -98,11 +98,12 @@ __device__ __forceinline__ int cost_bucket(int64_t tokens) {
 
 }  // namespace
 
+template <bool kTrees>
 __global__ void __launch_bounds__(kDevPlanThreads) aspire_plan_device_kernel(DevPlanParams p) {
   pdl_begin();
   __shared__ int64_t warp_sums[32];
   __shared__ int32_t bucket[2][kCostBuckets];  // per kernel list: decode (1), prefill (2)
-  __shared__ int bad, max_span, min_span, long_cols;
+  __shared__ int bad, max_span, min_span, long_cols, longest10;
   const int tid = threadIdx.x, nthreads = blockDim.x;
   if (tid == 0) {
     bad = 0;
@@ -136,7 +137,40 @@ __global__ void __launch_bounds__(kDevPlanThreads) aspire_plan_device_kernel(Dev
   block_exclusive_scan(tokens, warp_sums, &total_tokens);  // (its barriers publish max_span)
   const bool similar = 2 * int64_t(min_span) >= max_span;
   int64_t chunk = chunk_for(total_tokens, p.num_sms, similar ? kItemsPerCtaUniform : kItemsPerCtaMixed);
-  if (!similar) {
+  if constexpr (kTrees) {
+    TreeCost cost[kTreePlans] = {};
+    for (int b = r0; b < r1; ++b) {
+      const RowShape s = row_shape(p, b);
+      if (s.ql <= 0) continue;
+      for (int qt = 0; qt < s.ntq; ++qt) {
+        const int32_t rows = min(s.nq, (qt + 1) * s.tile) - qt * s.tile;
+        for (int k = 0; k < kTreePlans; ++k) {
+          TreeCost one = {};
+          add_tree_cost(one, s.kl, tree_chunk(total_tokens, max_span, p.num_sms, k), tree_tile10(s.kind, rows, p.group), rows);
+          cost[k].work10 += p.num_kv_heads * one.work10;
+          cost[k].full += p.num_kv_heads * one.full;
+          cost[k].full10 = max(cost[k].full10, one.full10);
+          cost[k].split |= one.split;
+        }
+      }
+    }
+    int64_t best = INT64_MAX;
+    for (int k = 0; k < kTreePlans; ++k) {
+      TreeCost all;
+      block_exclusive_scan(cost[k].work10, warp_sums, &all.work10);
+      block_exclusive_scan(cost[k].full, warp_sums, &all.full);
+      if (tid == 0) longest10 = 0;
+      __syncthreads();
+      atomicMax(&longest10, int(min(cost[k].full10, int64_t(INT_MAX))));
+      all.split = __syncthreads_or(int(cost[k].split));
+      all.full10 = longest10;
+      __syncthreads();
+      if (tree_makespan(all, p.num_sms) < best) {
+        best = tree_makespan(all, p.num_sms);
+        chunk = tree_chunk(total_tokens, max_span, p.num_sms, k);
+      }
+    }
+  } else if (!similar) {
     // Long groups cut into one piece per SM when that packs the grid (long_group_chunk).
     int64_t my_long = 0, my_short = 0;
     for (int b = r0; b < r1; ++b) {
@@ -156,7 +190,7 @@ __global__ void __launch_bounds__(kDevPlanThreads) aspire_plan_device_kernel(Dev
     const int64_t c = long_group_chunk(n_long, max_span, short_work10, p.num_sms);
     if (c > 0) chunk = c;
   }
-  {
+  if constexpr (!kTrees) {
     // Whole groups when they balance about as well (whole_groups_cheaper),
     // else 256-token chunks for small split plans (small_plan_chunk).
     int64_t my_groups = 0, my_chunk_items = 0;
@@ -302,7 +336,7 @@ __global__ void __launch_bounds__(kDevPlanThreads) aspire_plan_device_kernel(Dev
     w[kHdrNumItems] = int32_t(tot_items);
     w[kHdrNumGatherCtas] = gather_ctas;
     w[kHdrNumTcCtas] = p.num_sms * kTcCtasPerSm;
-    w[kHdrCausal] = p.causal ? 1 : 0;
+    w[kHdrCausal] = p.causal == kPlanCausal ? 1 : 0;
     w[kHdrOffGatherIndptr] = int32_t(off_gather);
     w[kHdrTcFirst] = 0;
     w[kHdrOffItems] = int32_t(off_items);
@@ -319,6 +353,10 @@ __global__ void __launch_bounds__(kDevPlanThreads) aspire_plan_device_kernel(Dev
     w[kHdrChunkTokens] = int32_t(chunk);
     w[kHdrMagic] = kPlanMagic;
   }
+}
+
+DevPlanKernel plan_device_kernel(bool trees) {
+  return trees ? &aspire_plan_device_kernel<true> : &aspire_plan_device_kernel<false>;
 }
 
 }  // namespace aspire

@@ -108,6 +108,9 @@ int plan_impl(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t*
     return set_error(ASPIRE_ERR_INVALID,
                      "aspire_plan: num_qo_heads must be a positive multiple of num_kv_heads");
   if (num_sms <= 0) return set_error(ASPIRE_ERR_INVALID, "aspire_plan: num_sms must be > 0");
+  if (causal != kPlanTree) causal = causal ? kPlanCausal : kPlanAll;
+  if (causal == kPlanTree && (!tc_enabled || num_qo_heads / num_kv_heads > kTcQTile))
+    return set_error(ASPIRE_ERR_INVALID, "aspire_plan: trees need tcgen05 and at most 48 query heads per KV head");
   const int gather_ctas = num_sms * kGatherCtasPerSm;
   const int tc_ctas = num_sms * kTcCtasPerSm;
   const int group = num_qo_heads / num_kv_heads;
@@ -140,16 +143,18 @@ int plan_impl(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t*
     // so that one TMA box loads it.
     const bool wide = tc_enabled && group <= kTcQTile &&
                       (nq > kGatherQTile || nq >= tc_min_rows || kl >= tc_min_kv);
+    if (causal == kPlanTree && !wide)
+      return set_error(ASPIRE_ERR_INVALID, "aspire_plan: trees need the default routing");
     // Long queries (prefill chunks) go to the prefill phase: items of two
     // 128-row halves (whole query positions each) that share every K/V tile.
-    const bool prefill = wide && nq >= kPfMinRows;
-    const int tile = prefill ? pf_item_rows(group) : wide ? (kTcQTile / group) * group : kGatherQTile;
+    const bool prefill = wide && nq >= prefill_min_rows(causal);
+    const int tile = prefill ? pf_item_rows(group) : wide ? (decode_tile_rows(causal) / group) * group : kGatherQTile;
     const int kind = prefill ? 2 : (wide ? 1 : 0);
     for (int h = 0; h < num_kv_heads; ++h) {
       for (int p0 = 0; p0 < nq; p0 += tile) {
         const int32_t p1 = std::min(nq, p0 + tile);
         GroupDesc g{b, h, q0, ql, kv_indptr[b], kl, p0, p1, kind,
-                    visible_span(kl, ql, p0, p1, group, causal != 0)};
+                    visible_span(kl, ql, p0, p1, group, causal == kPlanCausal)};
         groups.push_back(g);
         total_tokens += std::max<int32_t>(g.span, 1);
       }
@@ -166,7 +171,19 @@ int plan_impl(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t*
   }
   const bool similar = 2 * int64_t(min_span) >= max_span;
   int64_t chunk = chunk_for(total_tokens, num_sms, similar ? kItemsPerCtaUniform : kItemsPerCtaMixed);
-  if (!similar) {
+  if (causal == kPlanTree) {
+    int64_t best = INT64_MAX;
+    for (int k = 0; k < kTreePlans; ++k) {
+      const int64_t length = tree_chunk(total_tokens, max_span, num_sms, k);
+      TreeCost cost{};
+      for (const GroupDesc& g : groups)
+        add_tree_cost(cost, g.span, length, tree_tile10(g.kind, g.pq_end - g.pq_begin, group), g.pq_end - g.pq_begin);
+      if (tree_makespan(cost, num_sms) < best) {
+        best = tree_makespan(cost, num_sms);
+        chunk = length;
+      }
+    }
+  } else if (!similar) {
     int64_t n_long = 0, short_work10 = 0;
     for (const GroupDesc& g : groups) {
       if (long_group(g.span, max_span))
@@ -177,7 +194,7 @@ int plan_impl(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t*
     const int64_t c = long_group_chunk(n_long, max_span, short_work10, num_sms);
     if (c > 0) chunk = c;
   }
-  {
+  if (causal != kPlanTree) {
     int64_t n_chunk_items = 0;
     for (const GroupDesc& g : groups) n_chunk_items += g.span > 0 ? (g.span + chunk - 1) / chunk : 1;
     if (whole_groups_cheaper(int64_t(groups.size()), max_span, total_tokens, chunk, n_chunk_items, num_sms))
@@ -285,7 +302,7 @@ int plan_impl(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t*
   w[kHdrNumItems] = num_items;
   w[kHdrNumGatherCtas] = gather_ctas;
   w[kHdrNumTcCtas] = tc_ctas;
-  w[kHdrCausal] = causal ? 1 : 0;
+  w[kHdrCausal] = causal == kPlanCausal ? 1 : 0;
   w[kHdrOffGatherIndptr] = static_cast<int32_t>(off_gather);
   w[kHdrTcFirst] = n_gather;
   w[kHdrTcClaim] = 0;
@@ -322,7 +339,7 @@ int plan_impl(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t*
   info->float_bytes = float_bytes;
   info->num_qo_heads = num_qo_heads;
   info->num_kv_heads = num_kv_heads;
-  info->causal = causal ? 1 : 0;
+  info->causal = causal;
   info->batch_size = batch_size;
   info->max_q_len = max_q_len;
   info->tc_enabled = tc_enabled ? 1 : 0;

@@ -482,6 +482,30 @@ bool in_common(const Tensor& a, const Tensor& b) {
   return x.first < y.second && y.first < x.second;
 }
 
+// Tensors of one type in one allocation, each 16-byte aligned: a step has many
+// small tables, and an allocation is most of what a small tensor costs.
+class Pieces {
+ public:
+  Pieces(std::initializer_list<int64_t> counts, const at::TensorOptions& options, int64_t size) : step_(16 / size) {
+    int64_t total = 0;
+    for (const int64_t c : counts) total += (c + step_ - 1) / step_ * step_;
+    all_ = at::empty({total}, options);
+  }
+  // The next piece, of these sizes.
+  Tensor take(at::IntArrayRef sizes) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all_.storage()), all_.key_set(), all_.dtype());
+    c10::TensorImpl* impl = t.unsafeGetTensorImpl();
+    impl->set_storage_offset(at_);
+    impl->set_sizes_contiguous(sizes);
+    at_ += (t.numel() + step_ - 1) / step_ * step_;
+    return t;
+  }
+
+ private:
+  Tensor all_;
+  int64_t step_, at_ = 0;
+};
+
 struct Tables {
   Tensor qo_indptr, kv_indptr, kv_len, last_page_len, positions, slots, tree_mask;
 };
@@ -520,16 +544,14 @@ Tables step_tables(const Tensor& lengths, const Tensor* new_tokens, const Tensor
   for (const Tensor* w : written) w->unsafeGetTensorImpl()->bump_version();
   const auto i32 = lengths.options();
   Tables t;
-  t.qo_indptr = at::empty({rows + 1}, i32);
-  t.kv_indptr = at::empty({rows + 1}, i32);
-  t.kv_len = at::empty({rows}, i32);
-  t.last_page_len = at::empty({rows}, i32);
-  // (Without rows no kernel writes the tokens' tables.)
-  const auto make = [&](at::IntArrayRef size, const auto& options, int64_t fill) {
-    return rows ? at::empty(size, options) : at::full(size, fill, options);
-  };
-  t.positions = make({tokens}, i32, 0);
-  t.slots = make({tokens}, i32.dtype(at::kLong), -1);
+  const int64_t words = parents ? (max_nodes + 31) / 32 : 0;
+  Pieces pieces({rows + 1, rows + 1, rows, rows, tokens, tokens * words}, i32, 4);
+  t.qo_indptr = pieces.take({rows + 1});
+  t.kv_indptr = pieces.take({rows + 1});
+  t.kv_len = pieces.take({rows});
+  t.last_page_len = pieces.take({rows});
+  t.positions = pieces.take({tokens});
+  t.slots = at::empty({tokens}, i32.dtype(at::kLong));
   a.qo_indptr = static_cast<int32_t*>(t.qo_indptr.data_ptr());
   a.kv_indptr = static_cast<int32_t*>(t.kv_indptr.data_ptr());
   a.kv_len = static_cast<int32_t*>(t.kv_len.data_ptr());
@@ -538,10 +560,15 @@ Tables step_tables(const Tensor& lengths, const Tensor* new_tokens, const Tensor
   a.slots = static_cast<int64_t*>(t.slots.data_ptr());
   a.tokens = tokens;
   if (parents) {
-    a.tree_mask_words = int32_t((max_nodes + 31) / 32);
-    t.tree_mask = make({tokens, a.tree_mask_words}, i32, 0);
+    a.tree_mask_words = int32_t(words);
+    t.tree_mask = pieces.take({tokens, words});
     a.tree_mask = static_cast<int32_t*>(t.tree_mask.data_ptr());
     if (!a.parents) a.parents = a.qo_indptr;  // (no tokens, no address: nothing is read through it)
+  }
+  if (rows == 0) {  // (no kernel writes the tokens' tables)
+    t.positions.zero_();
+    t.slots.fill_(-1);
+    if (parents) t.tree_mask.zero_();
   }
   a.status = status_word(status, lengths);
   on_device(lengths, [&](void* stream) { check(abi.step_tables(&a, stream), "aspire_step_tables"); });
@@ -720,10 +747,11 @@ Walked tree_accept(const Tensor& tokens, const Tensor& parents, const Tensor& ta
   }
   const auto i32 = tokens.options();
   Walked w;
-  w.count = at::empty({rows}, i32);
-  w.path = at::empty({rows, max_path}, i32);
-  w.tokens = at::empty({rows, max_path}, i32);
-  w.lengths = at::empty({rows}, i32);
+  Pieces pieces({rows, rows * max_path, rows * max_path, rows}, i32, 4);
+  w.count = pieces.take({rows});
+  w.path = pieces.take({rows, max_path});
+  w.tokens = pieces.take({rows, max_path});
+  w.lengths = pieces.take({rows});
   a.count = static_cast<int32_t*>(w.count.data_ptr());
   a.path = static_cast<int32_t*>(w.path.data_ptr());
   a.out_tokens = static_cast<int32_t*>(w.tokens.data_ptr());
@@ -740,6 +768,62 @@ Walked tree_accept(const Tensor& tokens, const Tensor& parents, const Tensor& ta
     } while (done < at.size());
   });
   return w;
+}
+
+// `fixed` holds what a plan's calls share (heads, pages, workspaces, scale); q_total the query rows it addresses.
+std::pair<Tensor, Tensor> tree_attention(const Tensor& q, const Tensor& cache, const Tensor& mask,
+                                         const Tensor* out_given, const Tensor* lse_given, bool want_lse,
+                                         const AspireAttnArgs& fixed, const AspirePlanInfo& plan, int64_t q_total) {
+  require(q.scalar_type() == at::kBFloat16 && cache.scalar_type() == at::kBFloat16, "q and paged_kv_cache must be bfloat16");
+  require(cache.dim() == 5 && cache.size(1) == 2 && cache.is_contiguous() && cache.device() == q.device(),
+          "paged_kv_cache must be a contiguous [pages, 2, page_size, num_kv_heads, head_dim] tensor on q's device");
+  require(q.is_cuda() && q.dim() == 3 && q.size(1) == fixed.num_qo_heads && q.size(2) == cache.size(4),
+          "q's shape does not match the plan");
+  require(q.stride(2) == 1, "q head_dim must be contiguous");
+  require(cache.size(2) == fixed.page_size && cache.size(3) == fixed.num_kv_heads,
+          "paged_kv_cache geometry does not match the plan");
+  require(q.size(0) >= q_total, "q has fewer rows than the plan addresses");
+  require(!at::GradMode::is_enabled() || !(q.requires_grad() || cache.requires_grad()),
+          "the attention has no gradient: detach the operands or call under torch.no_grad()");
+  require(mask.scalar_type() == at::kInt && mask.dim() == 2 && mask.is_contiguous() && mask.device() == q.device() &&
+              mask.size(0) >= q.size(0) && mask.size(1) >= 1 && mask.size(1) <= INT32_MAX,
+          "tree_mask must be a contiguous int32 [tokens, words] tensor on q's device");
+  Tensor out, lse;
+  if (out_given) {
+    out = *out_given;
+    require(out.scalar_type() == q.scalar_type() && out.sizes() == q.sizes() && out.stride(2) == 1 &&
+                out.device() == q.device(),
+            "out must match q's shape and type with a contiguous head_dim on its device");
+    out.unsafeGetTensorImpl()->bump_version();
+  } else {
+    out = at::empty(q.sizes(), q.options().requires_grad(false));
+  }
+  if (lse_given) {
+    lse = *lse_given;
+    require(lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.dim() == 2 && lse.size(0) == q.size(0) &&
+                lse.size(1) == q.size(1) && lse.device() == q.device(),
+            "lse must be a contiguous fp32 [tokens, num_qo_heads] tensor");
+    lse.unsafeGetTensorImpl()->bump_version();
+  } else if (want_lse) {
+    lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat).requires_grad(false));
+  }
+  AspireAttnArgs a = fixed;
+  a.q = q.data_ptr();
+  a.q_stride_n = q.stride(0);
+  a.q_stride_h = q.stride(1);
+  a.q_rows = q.size(0);
+  a.head_dim = int32_t(q.size(2));
+  a.kv_cache = cache.data_ptr();
+  a.num_pages_total = cache.size(0);
+  a.out = out.data_ptr();
+  a.o_stride_n = out.stride(0);
+  a.o_stride_h = out.stride(1);
+  a.lse = lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr;
+  on_device(q, [&](void* stream) {
+    check(abi.tree_attention(&a, static_cast<const int32_t*>(mask.data_ptr()), int32_t(mask.size(1)), &plan, stream),
+          "aspire_tree_attention");
+  });
+  return {out, lse};
 }
 
 // -------------------------------------------------------------------- Python
@@ -901,6 +985,19 @@ PyObject* py_tree_accept(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// (q, cache, mask, out, lse, want_lse, address of the plan's AspireAttnArgs, of its AspirePlanInfo, q_total) -> out, lse
+PyObject* py_tree_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject* {
+    const void* fixed = PyLong_AsVoidPtr(v[6]);
+    const void* plan = PyLong_AsVoidPtr(v[7]);
+    if (!fixed || !plan) throw Invalid("an address is required");
+    const auto r = tree_attention(tensor(v[0]), tensor(v[1]), tensor(v[2]), optional(v[3]), optional(v[4]),
+                                  v[5] == Py_True, *static_cast<const AspireAttnArgs*>(fixed),
+                                  *static_cast<const AspirePlanInfo*>(plan), integer(v[8]));
+    return wrap_all(r.first, r.second);
+  });
+}
+
 // (addresses of the entry points, in the order of `abi`)
 PyObject* py_bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
   return guarded(n, 13, [&]() -> PyObject* {
@@ -940,6 +1037,7 @@ PyMethodDef kMethods[] = {
     ASPIRE_METHOD("step_tables", py_step_tables),
     ASPIRE_METHOD("adjust_logits", py_adjust_logits),
     ASPIRE_METHOD("tree_accept", py_tree_accept),
+    ASPIRE_METHOD("tree_attention", py_tree_attention),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

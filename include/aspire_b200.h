@@ -62,6 +62,8 @@ extern "C" {
 #define ASPIRE_ERR_CAPACITY (-3) /* a workspace or plan buffer is too small      */
 #define ASPIRE_ERR_DEVICE (-4)   /* a kernel reported bad input via the status word */
 
+#define ASPIRE_PLAN_TREE 2 /* `causal` of a plan for aspire_tree_attention        */
+
 /* Device status word bits (written by kernels instead of faulting). */
 #define ASPIRE_STATUS_BAD_PAGE 1u  /* a page id >= num_pages_total was skipped */
 #define ASPIRE_STATUS_BAD_PLAN 2u  /* a work item was inconsistent and skipped */
@@ -131,6 +133,8 @@ typedef struct AspirePlanInfo {
  * cudaMemcpyAsync; the caller must not reuse host_buf until that copy has
  * completed (the wrapper fences a small ring of pinned buffers with events).
  * num_ctas <= 0 selects one CTA per SM of the current device.
+ * causal: 0, 1, or ASPIRE_PLAN_TREE for a plan of aspire_tree_attention (not
+ * causal, its own tiling of the rows; no other call takes it).
  */
 ASPIRE_API int aspire_plan(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_len,
                 int32_t batch_size, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
@@ -231,8 +235,10 @@ ASPIRE_API int aspire_mixed_attention(const AspireAttnArgs* args, const AspirePl
  * sees all keys before those, and of those key j iff bit j % 32 of word j / 32
  * of the query's mask is set (a key past the last word is hidden).  A query
  * that sees no key gets zeros and an LSE of -inf.  Keys and values that are
- * hidden from some query must be finite.  Needs a plan made with causal 0 by
- * the default routing, and no dump.  No counterpart in the reference.
+ * hidden from some query must be finite.  Needs a plan made with causal
+ * ASPIRE_PLAN_TREE (or 0, which is slower for rows of more than 48 packed
+ * queries) by the default routing, and no dump.  No counterpart in the
+ * reference.
  */
 ASPIRE_API int aspire_tree_attention(const AspireAttnArgs* args, const int32_t* tree_mask, int32_t mask_words,
                                      const AspirePlanInfo* plan, void* stream);

@@ -56,7 +56,7 @@ class Case:
         self.mask = torch.tensor(mask, dtype=torch.int32, device=dev).view(total, words)
         self.dev, self.heads, self.kv_heads, self.rows = dev, heads, kv_heads, rows
 
-    def plan(self, device_plan=False, tables=False, wrapper=None):
+    def plan(self, device_plan=False, tables=False, wrapper=None, trees=False):
         i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
         w = wrapper or HolisticAttentionWrapper(torch.empty(1, device=self.dev))
         flat = i32([p for r in self.pages for p in r] or [0]).to(self.dev)
@@ -69,9 +69,9 @@ class Case:
         if device_plan:
             last = i32([(e - 1) % 16 + 1 if e else 0 for e in self.ends]).to(self.dev)
             w.plan_device(i32(self.starts).to(self.dev), i32(self.kv_indptr).to(self.dev), last, *shape,
-                          paged_kv_indices=flat, causal=False)
+                          paged_kv_indices=flat, causal=False, trees=trees)
         else:
-            w.plan_host(i32(self.starts), i32(self.kv_indptr), i32(self.ends), flat, *shape, causal=False)
+            w.plan_host(i32(self.starts), i32(self.kv_indptr), i32(self.ends), flat, *shape, causal=False, trees=trees)
         return w
 
     def check(self, out, lse, rows=None):
@@ -139,9 +139,53 @@ def test_page_tables_and_device_plans(cuda_device, rows):
     c = Case(cuda_device, ROWS[rows], 8, 2, seed=5)
     first = c.run()
     c.check(*first)
-    for kw in (dict(tables=True), dict(device_plan=True), dict(device_plan=True, tables=True)):
+    for kw in (dict(tables=True), dict(device_plan=True), dict(device_plan=True, tables=True), dict(trees=True),
+               dict(device_plan=True, trees=True)):
         out, lse = c.run(**kw)
         c.check(out, lse)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 1), (16, 2), (10, 2)])
+@pytest.mark.parametrize("rows", ["ragged", "wide", "split", "tile_edges"])
+def test_device_plans_for_trees_hold_the_host_plans_items(cuda_device, rows, heads, kv_heads):
+    c = Case(cuda_device, ROWS[rows], heads, kv_heads, seed=14)
+    lists = []
+    for device_plan in (False, True):
+        w = c.plan(device_plan=device_plan, trees=True)
+        torch.cuda.synchronize()
+        words = w._int_workspace[256:].view(torch.int32).cpu()
+        n, at = int(words[1]), int(words[5])
+        items = words[at:at + 16 * n].view(n, 16)
+        # (Where a group's partial rows lie and which descriptor it has is the planner's own.)
+        lists.append((n, int(words[4]), int(words[15]), int(words[17]),
+                      sorted(tuple(r[:12].tolist()) + (int(r[13]) >= 0, int(r[14]), int(r[15])) for r in items)))
+    assert lists[0] == lists[1]
+
+
+def test_a_plain_plan_is_made_again_for_trees_outside_captures(cuda_device):
+    c = Case(cuda_device, [(300, 16), (40, 25)], 4, 1, seed=15)
+    q, kv = c.q.to(cuda_device), c.cache.to(cuda_device)
+    w = c.plan()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        out, lse = w.run(q, kv, tree_mask=c.mask, return_lse=True)
+    assert w.plan_info.causal == 0
+    g.replay()
+    c.check(out, lse)
+    c.check(*w.run(q, kv, tree_mask=c.mask, return_lse=True))
+    assert w.plan_info.causal == 2
+    g.replay()
+    c.check(out, lse)
+    with pytest.raises(ValueError, match="tree_mask"):
+        w.run(q, kv)
+    with pytest.raises(ValueError, match="causal"):
+        w.plan_host(torch.tensor(c.starts), torch.tensor(c.kv_indptr), torch.tensor(c.ends), w._kv_indices, 4, 1, 128, 16,
+                    causal=True, trees=True)
+    c.plan(wrapper=w)
+    assert w.run(q, kv).shape == q.shape
 
 
 def test_a_chain_is_the_causal_attention(cuda_device):
@@ -227,7 +271,7 @@ def test_replayed_with_other_masks_and_lengths(cuda_device):
         mask[:n].copy_(c.mask)
 
     def step():
-        w.plan_device(starts, kvp, last, 8, 2, 128, 16, paged_kv_indices=flat, causal=False)
+        w.plan_device(starts, kvp, last, 8, 2, 128, 16, paged_kv_indices=flat, trees=True)
         return w.run(q, cache, tree_mask=mask, return_lse=True)
 
     load(cases[0])

@@ -129,6 +129,42 @@ def test_tree_attention_abi(built_library):
     _refused(lib, call(plan=dict(tc_enabled=1, causal=1)), "causal")
 
 
+@pytest.mark.parametrize("group", [1, 3, 4, 8, 17, 48])
+@pytest.mark.parametrize("rows", [[(100, 5)], [(5000, 12), (0, 3), (77, 0), (900, 40)], [(40000, 16)] * 3,
+                                  [(3000, 100), (128, 64), (64, 1)] * 4])
+def test_plans_for_trees_cover_every_key_once(built_library, rows, group):
+    import numpy as np
+
+    i32 = lambda a: np.ascontiguousarray(a, dtype=np.int32)  # noqa: E731
+    ptr = lambda a: a.ctypes.data_as(_capi.c_int32_p)  # noqa: E731
+    qo = i32(np.cumsum([0] + [n for _, n in rows]))
+    kvl = i32([a + n for a, n in rows])
+    kvp = i32(np.cumsum([0] + [-(-k // 16) for k in kvl]))
+    buf = np.zeros(1 << 23, dtype=np.uint8)
+    info = _capi.AspirePlanInfo()
+    rc = built_library.aspire_plan_host_only(ptr(qo), ptr(kvp), ptr(kvl), len(kvl), 2 * group, 2, 128, 16,
+                                             _capi.PLAN_TREE, 148, buf.ctypes.data_as(ctypes.c_void_p), buf.nbytes,
+                                             1 << 31, ctypes.byref(info))
+    assert rc == 0 and info.causal == _capi.PLAN_TREE
+    w = buf.view(np.int32)
+    assert w[10] == 0  # not causal
+    items = w[w[5]:w[5] + 16 * info.num_items].reshape(-1, 16)
+    seen = {}
+    for row, head, _, q_len, _, kv_len, t0, t1, p0, p1, chunk, chunks, base, merge, kind, cols in items.tolist():
+        assert kind == (2 if q_len * group > 64 else 1)
+        assert 0 < p1 - p0 <= (256 if kind == 2 else 64) and p0 % group == 0
+        assert t0 % 128 == 0 and cols <= 64 and (merge >= 0) == (chunks > 1)
+        seen.setdefault((row, head, p0, p1), []).append((t0, t1))
+    for b, (a, n) in enumerate(rows):
+        for h in range(2):
+            tiles = sorted(k for k in seen if k[:2] == (b, h))
+            assert [t[2] for t in tiles] + [n * group] == [0] + [t[3] for t in tiles] or n == 0
+            for t in tiles:
+                ranges = sorted(seen[t])
+                assert ranges[0][0] == 0 and ranges[-1][1] == a + n
+                assert all(x[1] == y[0] for x, y in zip(ranges, ranges[1:]))
+
+
 def test_prologue_at_abi(built_library):
     lib = built_library
     a = _capi.AspirePrologueArgs()
