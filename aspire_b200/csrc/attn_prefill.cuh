@@ -121,7 +121,7 @@ __device__ __forceinline__ void issue_q(const AttnParams& p, const CUtensorMap* 
 // The MMA warp of half h.  Both warps walk every item and tile in the same
 // order (the K/V ring and the query buffer are shared); warp 0 also loads
 // the query rows and clears the V tiles' tail rows.
-template <class Sh>
+template <bool kTree, class Sh>
 __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Buffers& buf, int h, int lane,
                         uint32_t& k) {
   Barriers& b = sm.pf;
@@ -140,7 +140,8 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
 
   // QK_h of sub-tile j of the item (its K tile in stage ks).  The warp goes on or
   // stops as one, by all lanes' `ready`.
-  auto issue_qk = [&](int j, int ks, bool ready) -> bool {
+  const uint64_t qdesc_h = qdesc0;
+  auto issue_qk = [&](int j, int ks, bool ready, uint64_t qdesc0) -> bool {
     if (lane == 0 && ready) {
       const uint64_t kdesc0 = ptx::smem_desc(k0 + uint32_t(ks) * kSlotBytes + uint32_t(j & 1) * (kSub * 128), 16,
                                              1024, ptx::kLayoutSw128);
@@ -176,6 +177,103 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
     q_pending = true;
     __syncwarp();
   }
+  // The next item's query rows load while this item's last PVs and epilogue run.
+  // False (and ok cleared) on a timeout.
+  auto next_queries = [&]() -> bool {
+    const int nxt = next_item_with_tiles(p, sm, k, lane, kPfMaxRows);
+    if (nxt == -2) return ok = false;
+    if (nxt >= 0 && leader) {
+      if (!wait_bar_warp(sm, b.q_empty, items_done & 1, p.status)) return ok = false;
+      if (lane == 0) issue_q(p, qmap, buf, b, nxt);
+      q_pending = true;
+      __syncwarp();
+    }
+    ++items_done;
+    ii = nxt;
+    return true;
+  };
+  // An item whose tiles alternate between the halves (kSplitTiles): half h
+  // computes tiles h, h + 2, ... with the rows in the first query buffer.  Of
+  // the other half's tiles it releases K when its own tile before it begins
+  // (so that the ring can load on) and V when that tile is done, each after it
+  // has landed: an arrival never runs ahead of its phase.
+  auto split_item = [&](const WorkItem& it, int nt) -> bool {
+    const uint64_t qdesc_s = ptx::smem_desc(ptx::smem_addr(buf.q[0][0]), 16, 1024, ptx::kLayoutSw128);
+    auto give_k = [&](int t) -> bool {
+      if (t >= nt) return true;
+      const uint32_t gt = g + uint32_t(t);
+      if (!wait_bar_warp(sm, b.k_full[gt % kKStages], (gt / kKStages) & 1, p.status)) return false;
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&b.k_empty[gt % kKStages]));
+      __syncwarp();
+      return true;
+    };
+    auto give_v = [&](int t) -> bool {
+      if (t >= nt) return true;
+      const uint32_t gt = g + uint32_t(t);
+      if (!wait_bar_warp(sm, b.v_full[gt % kVStages], (gt / kVStages) & 1, p.status)) return false;
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&b.v_empty[gt % kVStages]));
+      __syncwarp();
+      return true;
+    };
+    const int own = (nt - h + 1) / 2;  // tiles of this half
+    if (h == 1 && !give_k(0)) return false;
+    if (own > 0) {
+      const uint32_t gt = g + uint32_t(h);
+      if (!wait_bar_warp(sm, b.k_full[gt % kKStages], (gt / kKStages) & 1, p.status)) return false;
+      for (int j = 0; j < 2; ++j) {
+        const bool ready = nth == 0 || wait_bar(sm, b.pv_done[h][j], (nth - 1) & 1, p.status);
+        ptx::tc_fence_after();
+        if (!issue_qk(j, gt % kKStages, ready, qdesc_s)) return false;
+      }
+      release_k(gt % kKStages, own == 1, true);
+    } else {
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_addr(&b.q_empty));
+      __syncwarp();
+    }
+    if (h == 1 && !give_v(0)) return false;
+    for (int i = 0; i < own; ++i) {
+      const int t = h + 2 * i;
+      const uint32_t gt = g + uint32_t(t), th = nth + uint32_t(i);
+      const int vs = gt % kVStages;
+      if (!give_k(t + 1)) return false;
+      bool ready = wait_bar(sm, b.v_full[vs], (gt / kVStages) & 1, p.status);
+      if (ready) clear_v_tail(buf.v[vs], it.tok_end - (it.tok_begin + t * kTile), lane);
+      // (Every lane's part of the tail is cleared before lane 0 goes on.)
+      if (!__all_sync(0xffffffffu, ready)) return false;
+      for (int bj = 0; bj < 2; ++bj) {
+        // The item's first PV overwrites O_h: the previous item's epilogue has read it.
+        ready = i > 0 || bj > 0 || nit == 0 || wait_bar(sm, b.o_free[h], (nit - 1) & 1, p.status);
+        ready = ready && wait_bar(sm, b.p_full[h][bj], th & 1, p.status);
+        ptx::tc_fence_after();
+        if (lane == 0 && ready) {
+          const uint64_t vdesc0 = ptx::smem_desc(v0 + uint32_t(vs) * kSlotBytes + uint32_t(bj) * (kSub / 16) * 2048,
+                                                 kHalfBytes, 1024, ptx::kLayoutSw128);
+#pragma unroll
+          for (int kk = 0; kk < kSub / 16; ++kk)
+            ptx::mma_bf16_ts(tmem + col_o(h), tmem + col_s(h, bj) + uint32_t(kk) * 8,
+                             vdesc0 + uint64_t(kk * 2048 >> 4), idesc_pv, (i > 0 || bj > 0 || kk > 0) ? 1u : 0u);
+          ptx::mma_commit(ptx::smem_addr(&b.pv_done[h][bj]));
+        }
+        if (!__all_sync(0xffffffffu, ready)) return false;
+        if (i + 1 < own) {
+          // The half's next tile reuses S buffer bj once this PV has read P from it.
+          const uint32_t gt2 = gt + 2;
+          ready = bj == 1 || wait_bar(sm, b.k_full[gt2 % kKStages], (gt2 / kKStages) & 1, p.status);
+          ready = ready && wait_bar(sm, b.pv_done[h][bj], th & 1, p.status);
+          ptx::tc_fence_after();
+          if (!issue_qk(bj, gt2 % kKStages, ready, qdesc_s)) return false;
+          if (bj == 1) release_k(gt2 % kKStages, i + 1 == own - 1, true);
+        }
+      }
+      if (lane == 0) ptx::mma_commit(ptx::smem_addr(&b.v_empty[vs]));
+      __syncwarp();
+      if (!give_v(t + 1)) return false;
+    }
+    g += uint32_t(nt);
+    nth += uint32_t(own);
+    if (own > 0) ++nit;
+    return true;
+  };
   while (ii >= 0 && ok) {
     const WorkItem it = load_item(p.plan, ii);
     const int nt = n_tiles_of(it);
@@ -188,6 +286,16 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
       break;
     }
     q_pending = false;
+    if constexpr (kTree) {
+      if (it.cols == kSplitTiles) {
+        if (!split_item(it, nt)) {
+          ok = false;
+          break;
+        }
+        if (!next_queries()) break;
+        continue;
+      }
+    }
     // Scores of the first tile's two sub-tiles, once each S buffer is free
     // (the previous item's last PV on it has completed).
     if (!wait_bar_warp(sm, b.k_full[g % kKStages], (g / kKStages) & 1, p.status)) {
@@ -198,7 +306,7 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
       for (int j = 0; j < 2 && ok; ++j) {
         const bool ready = nth == 0 || wait_bar(sm, b.pv_done[h][j], (nth - 1) & 1, p.status);
         ptx::tc_fence_after();
-        ok = issue_qk(j, g % kKStages, ready);
+        ok = issue_qk(j, g % kKStages, ready, qdesc_h);
       }
       if (!ok) break;
     }
@@ -245,7 +353,7 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
             if (bj == 0) ready = wait_bar(sm, b.k_full[gt2 % kKStages], (gt2 / kKStages) & 1, p.status);
             ready = ready && wait_bar(sm, b.pv_done[h][bj], th & 1, p.status);
             ptx::tc_fence_after();
-            ok = issue_qk(j + 2, gt2 % kKStages, ready);
+            ok = issue_qk(j + 2, gt2 % kKStages, ready, qdesc_h);
             if (!ok) break;
             if (bj == 1) release_k(gt2 % kKStages, t + 1 == nt - 1, true);
           }
@@ -275,23 +383,7 @@ __device__ void run_mma(const AttnParams& p, const CUtensorMap* qmap, Sh& sm, Bu
       nth += uint32_t(nt);
       ++nit;
     }
-    // The next item's query rows load while this item's last PVs and epilogue run.
-    const int nxt = next_item_with_tiles(p, sm, k, lane, kPfMaxRows);
-    if (nxt == -2) {
-      ok = false;
-      break;
-    }
-    if (nxt >= 0 && leader) {
-      if (!wait_bar_warp(sm, b.q_empty, items_done & 1, p.status)) {
-        ok = false;
-        break;
-      }
-      if (lane == 0) issue_q(p, qmap, buf, b, nxt);
-      q_pending = true;
-      __syncwarp();
-    }
-    ++items_done;
-    ii = nxt;
+    if (!next_queries()) break;
   }
   // A query load still in flight lands before the CTA reuses its memory.
   if (q_pending) drain_bar(b.q_full, items_done & 1);
@@ -360,8 +452,9 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
   Barriers& b = sm.pf;
   const int group = p.group;
   const int nrows = it.pq_end - it.pq_begin;
-  const int nj = 2 * n_tiles_of(it);
-  const int j_row = h * pf_half_rows(group) + r;  // row within the item
+  const bool split = kTree && it.cols == kSplitTiles;  // both halves hold the same rows, every other tile each
+  const int nj = 2 * (split ? (n_tiles_of(it) - h + 1) / 2 : n_tiles_of(it));
+  const int j_row = (split ? 0 : h * pf_half_rows(group)) + r;  // row within the item
   const bool valid = r < pf_half_rows(group) && j_row < nrows;
   const int pq = it.pq_begin + j_row;
   const int q_idx = pq / group;
@@ -395,7 +488,7 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
     const uint32_t th = gt + uint32_t(j >> 1);
     failed |= !wait_bar(sm, b.s_full[h][bj], th & 1, p.status);
     ptx::tc_fence_after();
-    const int sub0 = it.tok_begin + j * kSub;
+    const int sub0 = it.tok_begin + (split ? (2 * (j >> 1) + h) * kTile + (j & 1) * kSub : j * kSub);
     const uint32_t s_addr = tmem_lane + col_s(h, bj);
     float s[kSub];
     ptx::tmem_ld32(s_addr, s);
@@ -476,7 +569,7 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
   const float lse = l > 0.f ? m_ref + lg2(l) : -INFINITY;
   const int64_t tok = int64_t(it.q_start) + q_idx;
   const bool final_rows = it.n_chunks <= 1;
-  const int64_t prow = int64_t(it.partial_base) + int64_t(it.chunk) * nrows + j_row;
+  const int64_t prow = int64_t(it.partial_base) + int64_t(it.chunk + (split ? h : 0)) * nrows + j_row;
   bool store = valid;
   if (store && final_rows && tok >= p.q_rows) {
     record_status(p.status, ASPIRE_STATUS_BAD_ROW);
@@ -538,7 +631,16 @@ __device__ void consume_items(const AttnParams& p, Sh& sm, bool causal, int h, i
       for (int jr = h; jr < nrows; jr += 2) store_final(p, it, it.pq_begin + jr, r, 0.f, -INFINITY);
       continue;
     }
-    if (h >= halves_of(p, it)) continue;
+    if (kTree && it.cols == kSplitTiles) {
+      if (h == 1 && n_tiles_of(it) == 1) {  // no tile of its own: a partial of no weight
+        const int64_t base = int64_t(it.partial_base) + int64_t(it.chunk + 1) * nrows;
+        for (int jr = 0; jr < nrows; ++jr) p.partial_o[(base + jr) * kHeadDim + r] = 0.f;
+        if (r < nrows) partial_lse_ptr(p)[base + r] = -INFINITY;
+        continue;
+      }
+    } else if (h >= halves_of(p, it)) {
+      continue;
+    }
     if (!consume_item<kTree>(p, sm, it, causal, h, r, tmem_lane, gt)) return;
   }
 }

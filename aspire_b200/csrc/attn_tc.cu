@@ -889,7 +889,7 @@ __device__ __forceinline__ void attn_tc(const AttnParams& p, const CUtensorMap& 
                                    kHdrPfClaim, kPfMaxRows, lane, k);
       } else if (warp == 1 || warp == kPvWarp) {
         // One MMA-issuing warp per item half.
-        pf::run_mma(p, &qmap_pf, sm, pbuf, warp == 1 ? 0 : 1, lane, k);
+        pf::run_mma<kTree>(p, &qmap_pf, sm, pbuf, warp == 1 ? 0 : 1, lane, k);
       } else {
         pf::consume_items<kTree>(p, sm, causal, (warp - kFirstSoftmaxWarp) / 4, warp & 3, lane, k);
       }

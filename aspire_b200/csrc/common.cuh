@@ -223,6 +223,20 @@ enum PlanMode : int { kPlanAll = 0, kPlanCausal = 1, kPlanTree = 2 };
 __host__ __device__ constexpr int decode_tile_rows(int mode) { return mode == kPlanTree ? kTreeQTile : kTcQTile; }
 __host__ __device__ constexpr int prefill_min_rows(int mode) { return mode == kPlanTree ? kTreeQTile + 1 : kPfMinRows; }
 
+// A prefill item of one half of a plan for trees whose key tiles alternate
+// between the two halves' warps (WorkItem::cols, unused by other prefill
+// items): both hold the same rows, half h's partials are chunk `chunk` + h of
+// the item's group.  One half alone is bound by its softmax (2.4 us a tile).
+// Taken where the group is split anyway, in long pieces: 8 rows of 16k keys and
+// 32 nodes of a group of 4, pieces of 7168: 187 -> 158 us; 32 rows of 4k whole:
+// 163 -> 172; 4 rows of 2k, pieces of 512: 32 -> 38.
+constexpr int32_t kSplitTiles = 1;
+constexpr int64_t kSplitMinTokens = 2048;
+__host__ __device__ inline int32_t item_parts(int mode, int kind, int32_t rows, int group, int64_t n_chunks,
+                                              int64_t chunk) {
+  return mode == kPlanTree && kind == 2 && rows <= pf_half_rows(group) && n_chunks > 1 && chunk >= kSplitMinTokens ? 2 : 1;
+}
+
 // Chunk length of plans for trees: of kTreePlans candidates (about one, two or
 // three items per CTA; the longest group whole, in two or in three pieces) the
 // one whose estimated makespan is the shortest.  In tenths of a 128-token tile

@@ -225,10 +225,11 @@ __global__ void __launch_bounds__(kDevPlanThreads) aspire_plan_device_kernel(Dev
       const int32_t span = tile_span(p, s, qt * s.tile, pq1);
       const int32_t nch = span_chunks(span, chunk);
       const int32_t heads = p.num_kv_heads;
+      const int32_t parts = kTrees ? item_parts(kPlanTree, s.kind, rows, p.group, nch, chunk) : 1;
       n_items += int64_t(heads) * nch;
       if (nch > 1) {
         n_merge += heads;
-        n_prow += int64_t(heads) * rows * nch;
+        n_prow += int64_t(heads) * rows * nch * parts;
         n_units += int64_t(heads) * rows;
         atomicAdd(&hist[cost_bucket(chunk)], heads * (nch - 1));
       }
@@ -291,18 +292,19 @@ __global__ void __launch_bounds__(kDevPlanThreads) aspire_plan_device_kernel(Dev
         const int32_t pq0 = qt * s.tile, pq1 = min(s.nq, pq0 + s.tile), rows = pq1 - pq0;
         const int32_t span = tile_span(p, s, pq0, pq1);
         const int32_t nch = span_chunks(span, chunk);
+        const int32_t parts = kTrees ? item_parts(kPlanTree, s.kind, rows, p.group, nch, chunk) : 1;
         int32_t merge_id = -1, pbase = 0;
         if (nch > 1) {
           merge_id = int32_t(off_merge++);
           pbase = int32_t(off_prow);
-          off_prow += int64_t(nch) * rows;
+          off_prow += int64_t(nch) * parts * rows;
           MergeDesc md{};
           md.q_start = p.qo_indptr[b];
           md.pq_begin = pq0;
           md.nrows = rows;
           md.kv_head = h;
           md.partial_base = pbase;
-          md.n_chunks = nch;
+          md.n_chunks = nch * parts;
           merges[merge_id] = md;
           for (int j = 0; j < rows; ++j) units[off_unit++] = (merge_id << 8) | j;
         }
@@ -318,12 +320,12 @@ __global__ void __launch_bounds__(kDevPlanThreads) aspire_plan_device_kernel(Dev
           it.tok_end = int32_t(min(int64_t(c + 1) * chunk, int64_t(span)));
           it.pq_begin = pq0;
           it.pq_end = pq1;
-          it.chunk = c;
-          it.n_chunks = nch;
+          it.chunk = c * parts;
+          it.n_chunks = nch * parts;
           it.partial_base = pbase;
           it.merge_id = merge_id;
           it.kind = s.kind;
-          it.cols = s.kind == 1 && long_group(span, max_span) ? pad_cols : 0;
+          it.cols = parts == 2 ? kSplitTiles : s.kind == 1 && long_group(span, max_span) ? pad_cols : 0;
           const int slot = atomicAdd(&slots[cost_bucket(it.tok_end - it.tok_begin)], 1);
           items[slot] = it;
         }

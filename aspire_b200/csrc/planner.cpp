@@ -224,20 +224,22 @@ int plan_impl(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t*
     const int32_t n_chunks =
         g.span > 0 ? static_cast<int32_t>((g.span + chunk - 1) / chunk) : 1;
     const int32_t rows = g.pq_end - g.pq_begin;
+    // Items whose tiles alternate between the halves leave two partials each.
+    const int32_t parts = item_parts(causal, g.kind, rows, group, n_chunks, chunk);
     int32_t merge_id = -1, partial_base = 0;
     if (n_chunks > 1) {
       merge_id = num_merge++;
-      if (partial_rows + int64_t(n_chunks) * rows > INT32_MAX)
+      if (partial_rows + int64_t(n_chunks) * parts * rows > INT32_MAX)
         return set_error(ASPIRE_ERR_CAPACITY, "aspire_plan: too many partial rows");
       partial_base = static_cast<int32_t>(partial_rows);
-      partial_rows += int64_t(n_chunks) * rows;
+      partial_rows += int64_t(n_chunks) * parts * rows;
       MergeDesc md{};
       md.q_start = g.q_start;
       md.pq_begin = g.pq_begin;
       md.nrows = rows;
       md.kv_head = g.kv_head;
       md.partial_base = partial_base;
-      md.n_chunks = n_chunks;
+      md.n_chunks = n_chunks * parts;
       merges.push_back(md);
       for (int32_t j = 0; j < rows; ++j) merge_units.push_back((merge_id << 8) | j);
     }
@@ -253,12 +255,12 @@ int plan_impl(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t*
       it.tok_end = static_cast<int32_t>(std::min<int64_t>(int64_t(c + 1) * chunk, g.span));
       it.pq_begin = g.pq_begin;
       it.pq_end = g.pq_end;
-      it.chunk = c;
-      it.n_chunks = n_chunks;
+      it.chunk = c * parts;
+      it.n_chunks = n_chunks * parts;
       it.partial_base = partial_base;
       it.merge_id = merge_id;
       it.kind = g.kind;
-      it.cols = g.kind == 1 && long_group(g.span, max_span) ? pad_cols : 0;
+      it.cols = parts == 2 ? kSplitTiles : g.kind == 1 && long_group(g.span, max_span) ? pad_cols : 0;
       (g.kind == 2 ? pf_items : g.kind == 1 ? tc_items : gather_items).push_back(it);
     }
   }

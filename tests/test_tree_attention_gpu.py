@@ -162,6 +162,25 @@ def test_device_plans_for_trees_hold_the_host_plans_items(cuda_device, rows, hea
     assert lists[0] == lists[1]
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(4, 1), (8, 2), (16, 4)])
+@pytest.mark.parametrize("rows,sms", [([(4200, 17), (1432, 30), (50, 32)], 3), ([(9000, 17), (3060, 30), (50, 32)], 4),
+                                      ([(5000, 33), (6001, 21), (8, 40)], 3)])
+@pytest.mark.parametrize("kind", ["tree", "random"])
+def test_items_whose_tiles_alternate_between_the_halves(cuda_device, rows, sms, heads, kv_heads, kind):
+    """Long pieces of rows of one half; a group's last item may have one tile,
+    so that the other half has none."""
+    c = Case(cuda_device, rows, heads, kv_heads, kind=kind, seed=16)
+    wrappers = [HolisticAttentionWrapper(torch.empty(1, device=cuda_device), num_sms=sms * kv_heads) for _ in range(2)]
+    for w, device_plan in zip(wrappers, (False, True)):
+        c.plan(wrapper=w, trees=True, device_plan=device_plan)
+        torch.cuda.synchronize()
+        words = w._int_workspace[256:].view(torch.int32).cpu()
+        items = words[int(words[5]):int(words[5]) + 16 * int(words[1])].view(-1, 16)
+        assert int(((items[:, 14] == 2) & (items[:, 15] == 1)).sum()) >= 2 * kv_heads
+        c.check(*w.run(c.q.to(cuda_device), c.cache.to(cuda_device), tree_mask=c.mask, return_lse=True))
+        assert w.device_status() == 0
+
+
 def test_a_plain_plan_is_made_again_for_trees_outside_captures(cuda_device):
     c = Case(cuda_device, [(300, 16), (40, 25)], 4, 1, seed=15)
     q, kv = c.q.to(cuda_device), c.cache.to(cuda_device)
