@@ -230,6 +230,9 @@ class HolisticAttentionWrapper:
             raise ValueError("a plan for trees is not causal")
         self._plan_arrays(qo, kvp, kvl, (int(num_qo_heads), int(num_kv_heads), int(head_dim_qk), int(page_size)),
                           _capi.PLAN_TREE if trees else 1 if causal else 0)
+        # What a plan that is not causal is made from, should its rows turn out to be trees (the caller may
+        # write the next step into its arrays before that).
+        self._plan_host_arrays = None if causal or trees else (qo[:batch + 1].clone(), kvp[:batch + 1].clone(), kvl.clone())
         self._kv_indices = paged_kv_indices
         self._page_size = int(page_size)
         self._sm_scale = sm_scale
@@ -264,10 +267,16 @@ class HolisticAttentionWrapper:
         self._plan_q_total = int(qo[batch])
         self._plan_max_kv_len = int(kvl.max()) if batch else 0
         self._plan_rows = batch
-        # (What a plan that is not causal is made from, should its rows turn out to be trees.)
-        self._plan_host_arrays = (qo, kvp, kvl) if mode == 0 else None
         self._plan_trees = mode == _capi.PLAN_TREE
         self._tree_args = None
+
+    def _plan_again(self, mode: int) -> bool:
+        """Makes a plain host plan that is not causal again for trees, or back;
+        False where there is none or a graph is being captured."""
+        if self._plan_host_arrays is None or torch.cuda.is_current_stream_capturing():
+            return False
+        self._plan_arrays(*self._plan_host_arrays, (self._num_qo_heads, self._num_kv_heads, 128, self._page_size), mode)
+        return True
 
     def plan_device(
         self,
@@ -359,7 +368,7 @@ class HolisticAttentionWrapper:
         and an LSE of -inf.  Keys and values that some query does not see must
         be finite.  The plan must not be causal; no dump.  A plan made on the
         host without ``trees=True`` is made again for trees by the first such
-        call outside a graph's capture."""
+        call outside a graph's capture, and back by one without a mask."""
         if self._plan_info is None:
             raise RuntimeError("run() before plan()/plan_host()")
         if tree_mask is not None:
@@ -367,13 +376,12 @@ class HolisticAttentionWrapper:
                 raise ValueError("tree_mask needs a plan made with causal=False")
             if self._has_jit and self._dump_kind != "noop":
                 raise ValueError("a dump variant takes no tree_mask")
-            if self._plan_host_arrays is not None and not torch.cuda.is_current_stream_capturing():
-                heads = (self._num_qo_heads, self._num_kv_heads)
-                self._plan_arrays(*self._plan_host_arrays, (*heads, 128, self._page_size), _capi.PLAN_TREE)
+            if not self._plan_trees:
+                self._plan_again(_capi.PLAN_TREE)
             if append is None:
                 return self._run_trees(q, _unpack_paged_kv_cache(paged_kv_cache, self._kv_layout), tree_mask, out,
                                        lse, return_lse)
-        elif self._plan_trees:
+        elif self._plan_trees and not self._plan_again(0):
             raise ValueError("the plan was made for trees: give a tree_mask")
         kv = _unpack_paged_kv_cache(paged_kv_cache, self._kv_layout)
         if q.dtype != torch.bfloat16 or kv.dtype != torch.bfloat16:

@@ -124,6 +124,14 @@ __device__ __forceinline__ float* partial_lse_ptr(const AttnParams& p) {
   return p.partial_o + off;
 }
 
+// Whether a kernel can run the plan that the workspace holds by now (a replayed
+// one may find another than it was captured with): under a tree mask any that
+// is not causal, otherwise any that is not for trees.
+__device__ __forceinline__ bool plan_runs(const int32_t* plan, bool tree_mask) {
+  const int32_t magic = plan[kHdrMagic];
+  return tree_mask ? magic == kTreePlanMagic || (magic == kPlanMagic && plan[kHdrCausal] == 0) : magic == kPlanMagic;
+}
+
 __device__ __forceinline__ void record_status(uint32_t* status, uint32_t bits) {
   if (status) atomicOr(status, bits);
 }

@@ -22,7 +22,7 @@ namespace aspire {
 __global__ void __launch_bounds__(kMergeThreads) aspire_attn_merge_kernel(AttnParams p) {
   pdl_begin();
   const int32_t* plan = p.plan;
-  if (plan[kHdrMagic] != kPlanMagic) return;
+  if (!plan_runs(plan, p.tree_mask != nullptr)) return;
   // The tcgen05 kernel of this call has finished: rearm its item counters for
   // the next launch of the same plan (graph replays upload no new plan).
   if (blockIdx.x == 0 && threadIdx.x == 0) {

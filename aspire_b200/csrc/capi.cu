@@ -307,7 +307,7 @@ int run_attention(const AspireAttnArgs* a, const int32_t* tree_mask, int32_t mas
     return set_error(ASPIRE_ERR_CAPACITY, w + ": int workspace smaller than plan");
   if (size_t(plan->float_bytes) > a->float_ws_bytes)
     return set_error(ASPIRE_ERR_CAPACITY, w + ": float workspace smaller than plan");
-  if (plan->num_merge > 0 && !a->float_ws)
+  if (plan->num_merge > 0 && plan->float_bytes > 0 && !a->float_ws)
     return set_error(ASPIRE_ERR_INVALID, w + ": split-KV needs a float workspace");
   const int group = a->num_qo_heads / a->num_kv_heads;
   // The tcgen05 kernel takes rows only when a whole query position fits its tile.

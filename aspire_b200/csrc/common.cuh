@@ -41,7 +41,8 @@ enum PlanHeader : int {
   kHdrChunkTokens = 17,      // the plan's common split-KV chunk length (tokens)
   kHdrWords = 32,
 };
-constexpr int32_t kPlanMagic = 0x41535042;  // "ASPB"
+constexpr int32_t kPlanMagic = 0x41535042;      // "ASPB"
+constexpr int32_t kTreePlanMagic = 0x41535054;  // "ASPT": a plan for trees
 
 // One unit of work: a KV chunk of one (request row, KV head, packed-query tile).
 struct WorkItem {
@@ -244,7 +245,8 @@ __host__ __device__ inline int32_t item_parts(int mode, int kind, int32_t rows, 
 // (tree_tile10), an item's boundary kItemCost10, a split group's rows what
 // their partials' way out and back costs, the merge kMergeCost10.  The
 // makespan is the larger of the even share of all items and the rounds of
-// full-length ones.  Measured over fixed lengths of 256 to 131200 (16 rows of
+// full-length ones.  Candidates whose partials the float workspace has no room
+// for are passed over; the whole groups have none.  Measured over fixed lengths of 256 to 131200 (16 rows of
 // 2k-8k with 8-16 nodes: best 81 us, the rule's 84; 8 rows of 4k-16k with
 // 32-64: 136, 136; one row of 32k with 8: 41, 41; 2 rows of 131k: 132, 140).
 constexpr int kTreePlans = 6;
@@ -260,9 +262,11 @@ __host__ __device__ inline int64_t tree_tile10(int kind, int rows, int group) {
 }
 // A group's part of the estimate for chunk length `chunk`.
 struct TreeCost {
-  int64_t work10, full, full10, split;  // all items, full-length ones, the longest of those, whether any group splits
+  int64_t work10, full, full10;  // all items, full-length ones, the longest of those
+  int64_t partials;              // rows of the split groups' partials (0: none splits)
 };
-__host__ __device__ inline void add_tree_cost(TreeCost& c, int64_t span, int64_t chunk, int64_t tile10, int64_t rows) {
+__host__ __device__ inline void add_tree_cost(TreeCost& c, int64_t span, int64_t chunk, int kind, int rows, int group) {
+  const int64_t tile10 = tree_tile10(kind, rows, group);
   const int64_t n = span > 0 ? (span + chunk - 1) / chunk : 1;
   const int64_t item = kItemCost10 + (n > 1 ? rows * 10 / 64 : 0);  // (1 KB a row out and back, 64 KB a tile)
   c.work10 += (span + 127) / 128 * tile10 + n * item;
@@ -270,12 +274,15 @@ __host__ __device__ inline void add_tree_cost(TreeCost& c, int64_t span, int64_t
   const int64_t item10 = (longest + 127) / 128 * tile10 + item;
   if (2 * longest > chunk) c.full += n > 1 ? span / chunk : 1;
   if (item10 > c.full10) c.full10 = item10;
-  if (n > 1) c.split = 1;
+  if (n > 1) c.partials += n * item_parts(kPlanTree, kind, rows, group, n, chunk) * rows;
+}
+__host__ __device__ inline bool tree_fits(const TreeCost& c, int64_t float_ws_bytes) {
+  return c.partials <= INT32_MAX && c.partials * (kHeadDim + 1) * 4 <= float_ws_bytes;
 }
 __host__ __device__ inline int64_t tree_makespan(const TreeCost& c, int64_t num_sms) {
   const int64_t even = (c.work10 + num_sms - 1) / num_sms, rounds = (c.full + num_sms - 1) / num_sms * c.full10;
   const int64_t most = even > rounds ? even : rounds;
-  return (most > c.full10 ? most : c.full10) + (c.split ? kMergeCost10 : 0);
+  return (most > c.full10 ? most : c.full10) + (c.partials > 0 ? kMergeCost10 : 0);
 }
 
 }  // namespace aspire

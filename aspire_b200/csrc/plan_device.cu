@@ -146,11 +146,11 @@ __global__ void __launch_bounds__(kDevPlanThreads) aspire_plan_device_kernel(Dev
         const int32_t rows = min(s.nq, (qt + 1) * s.tile) - qt * s.tile;
         for (int k = 0; k < kTreePlans; ++k) {
           TreeCost one = {};
-          add_tree_cost(one, s.kl, tree_chunk(total_tokens, max_span, p.num_sms, k), tree_tile10(s.kind, rows, p.group), rows);
+          add_tree_cost(one, s.kl, tree_chunk(total_tokens, max_span, p.num_sms, k), s.kind, rows, p.group);
           cost[k].work10 += p.num_kv_heads * one.work10;
           cost[k].full += p.num_kv_heads * one.full;
           cost[k].full10 = max(cost[k].full10, one.full10);
-          cost[k].split |= one.split;
+          cost[k].partials += p.num_kv_heads * one.partials;
         }
       }
     }
@@ -162,10 +162,10 @@ __global__ void __launch_bounds__(kDevPlanThreads) aspire_plan_device_kernel(Dev
       if (tid == 0) longest10 = 0;
       __syncthreads();
       atomicMax(&longest10, int(min(cost[k].full10, int64_t(INT_MAX))));
-      all.split = __syncthreads_or(int(cost[k].split));
+      block_exclusive_scan(cost[k].partials, warp_sums, &all.partials);
       all.full10 = longest10;
       __syncthreads();
-      if (tree_makespan(all, p.num_sms) < best) {
+      if (tree_fits(all, p.float_ws_bytes) && tree_makespan(all, p.num_sms) < best) {
         best = tree_makespan(all, p.num_sms);
         chunk = tree_chunk(total_tokens, max_span, p.num_sms, k);
       }
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kDevPlanThreads) aspire_plan_device_kernel(Dev
     w[kHdrPfFirst] = int32_t(n_decode);
     w[kHdrPfClaim] = 0;
     w[kHdrChunkTokens] = int32_t(chunk);
-    w[kHdrMagic] = kPlanMagic;
+    w[kHdrMagic] = kTrees ? kTreePlanMagic : kPlanMagic;
   }
 }
 

@@ -177,8 +177,8 @@ int plan_impl(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t*
       const int64_t length = tree_chunk(total_tokens, max_span, num_sms, k);
       TreeCost cost{};
       for (const GroupDesc& g : groups)
-        add_tree_cost(cost, g.span, length, tree_tile10(g.kind, g.pq_end - g.pq_begin, group), g.pq_end - g.pq_begin);
-      if (tree_makespan(cost, num_sms) < best) {
+        add_tree_cost(cost, g.span, length, g.kind, g.pq_end - g.pq_begin, group);
+      if (tree_fits(cost, int64_t(float_ws_bytes)) && tree_makespan(cost, num_sms) < best) {
         best = tree_makespan(cost, num_sms);
         chunk = length;
       }
@@ -300,7 +300,7 @@ int plan_impl(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t*
 
   int32_t* w = static_cast<int32_t*>(host_buf);
   std::memset(w, 0, kHdrWords * 4);
-  w[kHdrMagic] = kPlanMagic;
+  w[kHdrMagic] = causal == kPlanTree ? kTreePlanMagic : kPlanMagic;
   w[kHdrNumItems] = num_items;
   w[kHdrNumGatherCtas] = gather_ctas;
   w[kHdrNumTcCtas] = tc_ctas;

@@ -17,10 +17,13 @@
 // kv_len 0 and slots of -1, and the status word says so.
 //
 // aspire_step_tables_kernel: one CTA, 1024 rows at a time; scans in registers,
-// then a warp per row for its pages.  Pages are pushed for all rows before any is popped, with a CTA
-// barrier between.  It does the tokens too where they are few; many are left
-// to aspire_step_tokens_kernel on the whole grid.  Both are bound by latency
-// up to some ten thousand tokens, by the bytes written beyond.
+// then the rows' pages, a warp for four rows at a time (256 rows of 16 to 64
+// pages: 31 us both ways against 36 with one row at a time).  Pages are pushed
+// for all rows before any is popped, with a CTA barrier between.  It does the
+// tokens too where they are few, one a thread (64 rows of 16 nodes, both ways:
+// 20.6 us; four a thread, 22.7), and many are left to aspire_step_tokens_kernel
+// on the whole grid.  Both are bound by latency up to some ten thousand tokens,
+// by the bytes written beyond.
 #include "tree.cuh"
 
 namespace aspire {
@@ -113,10 +116,11 @@ __device__ __forceinline__ int32_t ancestors(const StepTablesParams& p, const in
 }
 
 // Tokens [t0, t0 + kPer) of the step: positions, slots, masks.  `indptr` are
-// the rows' prefix sums, `parents` the step's, wherever they lie.
-constexpr int kPer = 4;
+// the rows' prefix sums, `lens` and `limits` their lengths and keys, `parents`
+// the step's, wherever they lie.
+template <int kPer>
 __device__ __forceinline__ void tokens_of(const StepTablesParams& p, int64_t t0, const int32_t* indptr,
-                                          const int32_t* parents, bool wide) {
+                                          const int32_t* lens, const int32_t* limits, const int32_t* parents, bool wide) {
   const int32_t total = indptr[p.rows];
   int32_t position[kPer];
   int64_t slot[kPer];
@@ -137,8 +141,8 @@ __device__ __forceinline__ void tokens_of(const StepTablesParams& p, int64_t t0,
       b = row_of(indptr, p.rows, int32_t(t));
       start = indptr[b];
       end = indptr[b + 1];
-      len = max(p.lengths[b], 0);
-      limit = __ldcg(p.kv_len + b);
+      len = max(lens[b], 0);
+      limit = limits[b];
       col = -1;
     }
     const int32_t i = int32_t(t) - start;
@@ -154,11 +158,13 @@ __device__ __forceinline__ void tokens_of(const StepTablesParams& p, int64_t t0,
       if (page >= 0) slot[k] = int64_t(page) * size + (place - c * size);
     }
   }
-  if (wide && t0 + kPer <= p.tokens) {
-    *reinterpret_cast<int4*>(p.positions + t0) = make_int4(position[0], position[1], position[2], position[3]);
-    *reinterpret_cast<longlong2*>(p.slots + t0) = make_longlong2(slot[0], slot[1]);
-    *reinterpret_cast<longlong2*>(p.slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
-    return;
+  if constexpr (kPer == 4) {
+    if (wide && t0 + kPer <= p.tokens) {
+      *reinterpret_cast<int4*>(p.positions + t0) = make_int4(position[0], position[1], position[2], position[3]);
+      *reinterpret_cast<longlong2*>(p.slots + t0) = make_longlong2(slot[0], slot[1]);
+      *reinterpret_cast<longlong2*>(p.slots + t0 + 2) = make_longlong2(slot[2], slot[3]);
+      return;
+    }
   }
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
@@ -175,6 +181,44 @@ __device__ __forceinline__ bool wide_tables(const StepTablesParams& p) {
 
 }  // namespace
 
+namespace {
+
+// Pages of a tile's rows, `many` of each, a warp for kRows rows at a time with
+// their loads under way together: f(row, i) is the value of a row's page i,
+// g(row, i, value) stores it.
+template <int kRows, typename F, typename G>
+__device__ __forceinline__ void each_page(const int32_t* many, int rows, F&& f, G&& g) {
+  constexpr int kWarps = kTablesThreads / 32, kPages = kRows > 1 ? 2 : 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int r0 = warp; r0 < rows; r0 += kRows * kWarps) {
+    int more = 0;
+    int32_t v[kRows][kPages];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const int r = r0 + k * kWarps, n = r < rows ? many[r] : 0;
+      more |= n > 32 * kPages;
+#pragma unroll
+      for (int u = 0; u < kPages; ++u)
+        if (lane + 32 * u < n) v[k][u] = f(r, lane + 32 * u);
+    }
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const int r = r0 + k * kWarps, n = r < rows ? many[r] : 0;
+#pragma unroll
+      for (int u = 0; u < kPages; ++u)
+        if (lane + 32 * u < n) g(r, lane + 32 * u, v[k][u]);
+    }
+    if (!more) continue;
+    for (int k = 0; k < kRows && r0 + k * kWarps < rows; ++k) {
+      const int r = r0 + k * kWarps, n = many[r];
+#pragma unroll 4
+      for (int i = lane + 32 * kPages; i < n; i += 32) g(r, i, f(r, i));
+    }
+  }
+}
+
+}  // namespace
+
 // kFew: the tokens are done here, one a thread and round.
 template <bool kFew>
 __global__ void __launch_bounds__(kTablesThreads) aspire_step_tables_kernel(StepTablesParams p) {
@@ -185,9 +229,11 @@ __global__ void __launch_bounds__(kTablesThreads) aspire_step_tables_kernel(Step
   __shared__ int32_t many[kTablesThreads];   // and how many
   __shared__ int32_t taken_s;                // pages of the served rows
   __shared__ int32_t indptr_s[kFew ? kTablesThreads + 1 : 1];
+  __shared__ int32_t len_s[kFew ? kTablesThreads : 1], limit_s[kFew ? kTablesThreads : 1];
   __shared__ int32_t parents_s[kFew ? kFewTokens : 1];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t capacity = p.free_capacity;
+  constexpr int kRows = kFew ? 1 : 4;
+  const int tid = threadIdx.x;
+  const int64_t capacity = min(p.free_capacity, int64_t(INT32_MAX));  // (the count has 32 bits)
   uint32_t bad = 0;
   int32_t parent[kFew ? kFewTokens / kTablesThreads : 1];
   if constexpr (kFew) {  // on their way while the rows are done
@@ -216,22 +262,22 @@ __global__ void __launch_bounds__(kTablesThreads) aspire_step_tables_kernel(Step
     }
     uint64_t total;
     const uint64_t before = scan_exclusive(pair(n, need), sums[0], &total);
-    at[tid] = int32_t(given + int64_t(before & 0xffffffffu));
+    at[tid] = int32_t(min(given + int64_t(before & 0xffffffffu), int64_t(INT32_MAX)));
     many[tid] = n;
     need_before = int64_t(before >> 32);
     __syncthreads();
     const int rows = int(min(int64_t(kTablesThreads), p.rows - r0));
-    for (int r = warp; (total & 0xffffffffu) && r < rows; r += kTablesThreads / 32) {
-      int32_t* row = p.table + (r0 + r) * p.table_stride + first[r];
-      for (int i = lane; i < many[r]; i += 32) {
-        const int64_t place = count + at[r] + i;
-        if (place < capacity)
-          p.free_pages[place] = row[i];
-        else
-          bad |= ASPIRE_STATUS_BAD_ROW;  // more pages given back than the pool has
-        row[i] = -1;
-      }
-    }
+    if (total & 0xffffffffu)
+      each_page<kRows>(
+          many, rows, [&](int r, int i) { return p.table[(r0 + r) * p.table_stride + first[r] + i]; },
+          [&](int r, int i, int32_t page) {
+            const int64_t place = count + at[r] + i;
+            if (place < capacity)
+              p.free_pages[place] = page;
+            else
+              bad |= ASPIRE_STATUS_BAD_ROW;  // more pages given back than the pool has
+            p.table[(r0 + r) * p.table_stride + first[r] + i] = -1;
+          });
     given += int64_t(total & 0xffffffffu);
     missing += int64_t(total >> 32);
     if (!one_tile) __syncthreads();
@@ -277,7 +323,11 @@ __global__ void __launch_bounds__(kTablesThreads) aspire_step_tables_kernel(Step
       const int32_t end = served ? r.len + r.fresh : 0;
       const int32_t start = int32_t(min(qo, int64_t(INT32_MAX)));  // (past the step's buffers in any case)
       p.qo_indptr[b] = start;
-      if (kFew) indptr_s[tid] = start;
+      if (kFew) {
+        indptr_s[tid] = start;
+        len_s[tid] = r.len;
+        limit_s[tid] = end;
+      }
       p.kv_indptr[b] = int32_t(min(kv, int64_t(INT32_MAX)));
       p.kv_len[b] = end;
       p.last_page_len[b] = end > 0 ? (end - 1) % p.page_size + 1 : 0;
@@ -288,11 +338,11 @@ __global__ void __launch_bounds__(kTablesThreads) aspire_step_tables_kernel(Step
     many[tid] = served ? n : 0;
     __syncthreads();
     const int rows = int(min(int64_t(kTablesThreads), p.rows - r0));
-    for (int w = warp; missing > 0 && w < rows; w += kTablesThreads / 32) {
-      int32_t* row = p.table + (r0 + w) * p.table_stride + first[w];
-      const int32_t* src = p.free_pages + (avail - taken_s) + at[w];
-      for (int i = lane; i < many[w]; i += 32) row[i] = src[i];
-    }
+    const int32_t* src = p.free_pages + (avail - taken_s);
+    if (missing > 0)
+      each_page<kRows>(
+          many, rows, [&](int r, int i) { return src[at[r] + i]; },
+          [&](int r, int i, int32_t page) { p.table[(r0 + r) * p.table_stride + first[r] + i] = page; });
     new_at += int64_t(new_total);
     page_at += int64_t(page_total);
     if (!one_tile) __syncthreads();
@@ -310,9 +360,8 @@ __global__ void __launch_bounds__(kTablesThreads) aspire_step_tables_kernel(Step
     for (int k = 0; k < kFewTokens / kTablesThreads; ++k)
       if (p.parents && tid + k * kTablesThreads < p.tokens) parents_s[tid + k * kTablesThreads] = parent[k];
     __syncthreads();  // (the tables' new pages are written)
-    const bool wide = wide_tables(p);
-    for (int64_t t = int64_t(tid) * kPer; t < p.tokens; t += kTablesThreads * kPer)
-      tokens_of(p, t, indptr_s, p.parents ? parents_s : nullptr, wide);
+    for (int64_t t = tid; t < p.tokens; t += kTablesThreads)
+      tokens_of<1>(p, t, indptr_s, len_s, limit_s, p.parents ? parents_s : nullptr, false);
   }
 }
 
@@ -328,10 +377,11 @@ __global__ void __launch_bounds__(kStepTokensThreads) aspire_step_tokens_kernel(
     indptr = indptr_s;
   }
   __syncthreads();
+  constexpr int kPer = 4;
   const bool wide = wide_tables(p);
   const int64_t step = int64_t(gridDim.x) * kStepTokensThreads * kPer;
   for (int64_t t = (int64_t(blockIdx.x) * kStepTokensThreads + threadIdx.x) * kPer; t < p.tokens; t += step)
-    tokens_of(p, t, indptr, p.parents, wide);
+    tokens_of<kPer>(p, t, indptr, p.lengths, p.kv_len, p.parents, wide);
 }
 
 }  // namespace aspire

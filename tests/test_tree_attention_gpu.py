@@ -198,13 +198,70 @@ def test_a_plain_plan_is_made_again_for_trees_outside_captures(cuda_device):
     assert w.plan_info.causal == 2
     g.replay()
     c.check(out, lse)
+    plain = w.run(q, kv)  # and back
+    assert w.plan_info.causal == 0 and torch.equal(plain.nan_to_num(9), c.plan().run(q, kv).nan_to_num(9))
+    g.replay()
+    c.check(out, lse)
+    c.check(*w.run(q, kv, tree_mask=c.mask, return_lse=True))
+    t = c.plan(trees=True)
     with pytest.raises(ValueError, match="tree_mask"):
-        w.run(q, kv)
+        t.run(q, kv)
     with pytest.raises(ValueError, match="causal"):
         w.plan_host(torch.tensor(c.starts), torch.tensor(c.kv_indptr), torch.tensor(c.ends), w._kv_indices, 4, 1, 128, 16,
                     causal=True, trees=True)
     c.plan(wrapper=w)
     assert w.run(q, kv).shape == q.shape
+
+
+def test_the_callers_arrays_may_change_before_the_first_run(cuda_device):
+    c = Case(cuda_device, [(300, 16), (40, 25)], 4, 1, seed=17)
+    w = HolisticAttentionWrapper(torch.empty(1, device=cuda_device))
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    arrays = i32(c.starts), i32(c.kv_indptr), i32(c.ends)
+    w.plan_host(*arrays, i32([p for r in c.pages for p in r]).to(cuda_device), 4, 1, 128, 16)
+    for a in arrays:
+        a.fill_(1)
+    c.check(*w.run(c.q.to(cuda_device), c.cache.to(cuda_device), tree_mask=c.mask, return_lse=True))
+
+
+def test_a_replay_that_finds_another_kind_of_plan_writes_nothing(cuda_device):
+    c = Case(cuda_device, [(300, 16), (40, 25)], 4, 1, seed=18)
+    q, kv = c.q.to(cuda_device), c.cache.to(cuda_device).nan_to_num(0)
+    w = c.plan()
+    w.run(q, kv)
+    torch.cuda.synchronize()
+    outs, graphs = [], []
+    for mask in (None, c.mask):
+        g = torch.cuda.CUDAGraph()
+        out = torch.full_like(q, 7)
+        with torch.cuda.graph(g):
+            w.run(q, kv, out=out, tree_mask=mask)
+        graphs.append(g), outs.append(out)
+    w.run(q, kv, tree_mask=c.mask)  # now for trees
+    graphs[0].replay()
+    assert w.device_status() == 2 and bool((outs[0] == 7).all())  # BAD_PLAN
+    w.clear_device_status()
+    graphs[1].replay()
+    assert w.device_status() == 0 and torch.equal(outs[1], w.run(q, kv, tree_mask=c.mask))
+    outs[1].fill_(7)
+    shape = w._kv_indices, 4, 1, 128, 16
+    w.plan_host(torch.tensor(c.starts), torch.tensor(c.kv_indptr), torch.tensor(c.ends), *shape, causal=True)
+    graphs[1].replay()
+    assert w.device_status() == 2 and bool((outs[1] == 7).all())
+    w.clear_device_status()
+    graphs[0].replay()
+    assert w.device_status() == 0 and torch.equal(outs[0], w.run(q, kv))
+
+
+@pytest.mark.parametrize("device_plan", [False, True])
+def test_little_float_workspace(cuda_device, device_plan):
+    """Plans for trees split no further than the workspace has room for."""
+    c = Case(cuda_device, [(3000, 9), (700, 33)], 8, 2, seed=19)
+    for room in (0, 64 << 10, 600 << 10):
+        w = HolisticAttentionWrapper(torch.empty(1, device=cuda_device), float_workspace_bytes=room)
+        c.plan(wrapper=w, device_plan=device_plan, trees=True)
+        c.check(*w.run(c.q.to(cuda_device), c.cache.to(cuda_device), tree_mask=c.mask, return_lse=True))
+        assert w.device_status() == 0
 
 
 def test_a_chain_is_the_causal_attention(cuda_device):

@@ -165,6 +165,24 @@ def test_plans_for_trees_cover_every_key_once(built_library, rows, group):
                 assert all(x[1] == y[0] for x, y in zip(ranges, ranges[1:]))
 
 
+@pytest.mark.parametrize("room", [0, 100_000, 1_000_000, 1 << 31])
+@pytest.mark.parametrize("rows", [[(5000, 12), (900, 40)], [(130000, 4)], [(600, 80)] * 48])
+def test_plans_for_trees_fit_the_float_workspace(built_library, rows, room):
+    import numpy as np
+
+    i32 = lambda a: np.ascontiguousarray(a, dtype=np.int32)  # noqa: E731
+    ptr = lambda a: a.ctypes.data_as(_capi.c_int32_p)  # noqa: E731
+    qo = i32(np.cumsum([0] + [n for _, n in rows]))
+    kvl = i32([a + n for a, n in rows])
+    kvp = i32(np.cumsum([0] + [-(-k // 16) for k in kvl]))
+    buf = np.zeros(1 << 23, dtype=np.uint8)
+    info = _capi.AspirePlanInfo()
+    rc = built_library.aspire_plan_host_only(ptr(qo), ptr(kvp), ptr(kvl), len(kvl), 64, 8, 128, 16, _capi.PLAN_TREE,
+                                             148, buf.ctypes.data_as(ctypes.c_void_p), buf.nbytes, room,
+                                             ctypes.byref(info))
+    assert rc == 0 and info.float_bytes <= room
+
+
 def test_prologue_at_abi(built_library):
     lib = built_library
     a = _capi.AspirePrologueArgs()
