@@ -547,8 +547,10 @@ __global__ void __launch_bounds__(kLogitsThreads, kLogitsCtas) aspire_logits_ker
           int path = 0;
           if (__any_sync(0xffffffffu, (flags & kInStep) != 0))
             path = on_path(p, r.span, t, (flags & kInStep) != 0, now[k].x, lane);
-          if (i0 + 32 * k + lane < end) {
-            T* x = stage + (now[k].x - w.chunk * W::kChunk);
+          // (Rows that overlap share their lists' memory: an entry may be another row's.)
+          const int32_t e = now[k].x - w.chunk * W::kChunk;
+          if (i0 + 32 * k + lane < end && uint32_t(e) < uint32_t(a.n)) {
+            T* x = stage + e;
             *x = from_float<T>(r.adjusted(to_float(*x), flags, path, own[k]));
           }
         }
@@ -716,8 +718,9 @@ __global__ void __launch_bounds__(kLogitsThreads, kLogitsCtas) aspire_logits_pic
           const int i = i0 + 32 * k + lane;
           if (i0 + 32 * k >= end) break;
           const int32_t v = entry[k].x;
-          const float x = i < end ? to_float(stage[v - v0]) : -INFINITY;
-          const bool live = i < end && (raises || x >= bar) && (!allowed || ((allowed[v >> 5] >> (v & 31)) & 1));
+          const bool here = i < end && uint32_t(v - v0) < uint32_t(a.n);  // (rows that overlap share their lists' memory)
+          const float x = here ? to_float(stage[v - v0]) : -INFINITY;
+          const bool live = here && (raises || x >= bar) && (!allowed || ((allowed[v >> 5] >> (v & 31)) & 1));
           const uint32_t flags = live ? uint32_t(entry[k].y) : 0u;
           if (!__any_sync(0xffffffffu, live)) continue;
           int path = 0;

@@ -807,6 +807,11 @@ std::pair<Tensor, Tensor> tree_attention(const Tensor& q, const Tensor& cache, c
   } else if (want_lse) {
     lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat).requires_grad(false));
   }
+  if (out_given)
+    require(!in_common(out, cache) && !in_common(out, mask), "out must not overlap the cache or the mask");
+  if (lse_given)
+    require(!in_common(lse, cache) && !in_common(lse, mask) && !in_common(lse, q) && !in_common(lse, out),
+            "lse must not overlap the other operands");
   AspireAttnArgs a = fixed;
   a.q = q.data_ptr();
   a.q_stride_n = q.stride(0);

@@ -3,7 +3,7 @@
 A step of tree speculation::
 
     t = build_step_tables(lengths, new_tokens, *pool, tokens=T, parents=parents, max_nodes=N)
-    wrapper.plan_device(t.qo_indptr, t.kv_indptr, t.last_page_len, ..., causal=False)
+    wrapper.plan_device(t.qo_indptr, t.kv_indptr, t.last_page_len, ..., trees=True)
     # per layer: qkv_prologue(..., positions=t.positions), then
     wrapper.run(q, cache, tree_mask=t.tree_mask)
     targets = pick_tokens(logits, indptr=t.qo_indptr, tokens=tokens, tree_mask=t.tree_mask, ...)

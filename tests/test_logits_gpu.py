@@ -188,6 +188,23 @@ def test_lengths_and_prefix_sums_out_of_range(cuda_device):
     assert int(status) == 4
 
 
+@pytest.mark.parametrize("vocab", [1000, 40003])
+def test_rows_that_overlap(cuda_device, vocab):
+    """Prefix sums that go back: rows whose lists share memory stay within their logits, and the status says so."""
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)  # noqa: E731
+    x = torch.randn(40, vocab, generator=torch.Generator().manual_seed(1)).to(cuda_device)
+    tokens = i32([(7919 * i) % vocab for i in range(40)])
+    status = i32([0])
+    kw = dict(indptr=i32([0, 30, 2, 40, 1, 40]), tokens=tokens, frequency=torch.ones(5, device=cuda_device), status=status)
+    for _ in range(3):
+        out = adjust_logits(x, **kw)
+        ids = pick_tokens(x, **kw)
+        assert int(status) == 4
+        changed = (out != x).nonzero()
+        assert set(changed[:, 1].tolist()) <= set(tokens.tolist())
+        assert bool(((ids >= -1) & (ids < vocab)).all())
+
+
 def test_replayed_with_other_histories(cuda_device):
     c = Case(8, [3, 4], 9001, torch.bfloat16, bias=7, allowed=True)
     kw = c.args(cuda_device)

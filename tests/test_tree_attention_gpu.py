@@ -393,3 +393,17 @@ def test_refusals(cuda_device):
     dump = torch.empty(4 * 2 * 96, dtype=torch.float16, device=cuda_device)
     with pytest.raises(ValueError, match="dump"):
         d.run(q, kv, dump, 4, 96, tree_mask=c.mask)
+
+
+def test_outputs_that_overlap_are_refused(cuda_device):
+    c = Case(cuda_device, [(30, 4)], 4, 1, seed=20)
+    w, q, kv = c.plan(trees=True), c.q.to(cuda_device), c.cache.to(cuda_device)
+    lse = torch.empty(4, 4, device=cuda_device)
+    for kw in (dict(out=kv.view(-1)[:q.numel()].view(q.shape)), dict(lse=q.view(-1).view(torch.float32)[:16].view(4, 4)),
+               dict(out=lse.new_empty(1024).view(torch.bfloat16).view(q.shape), lse=None)):
+        if kw.get("lse", lse) is None:
+            kw["lse"] = kw["out"].view(-1).view(torch.float32)[:16].view(4, 4)
+        with pytest.raises(ValueError, match="overlap"):
+            w.run(q, kv, tree_mask=c.mask, **kw)
+    out = w.run(q, kv, tree_mask=c.mask)
+    assert torch.equal(w.run(q, kv, tree_mask=c.mask, out=q), out)  # in place of the queries
