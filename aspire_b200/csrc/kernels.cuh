@@ -172,6 +172,7 @@ __global__ void aspire_attn_tree_kernel(AttnParams p, const __grid_constant__ CU
                                         const __grid_constant__ CUtensorMap qmap_pf);
 constexpr int kMergeThreads = 128;
 constexpr int kMergeCtasPerSm = 4;
+constexpr int kMergeManyUnits = 2;  // rows per warp past which a warp takes four rows together
 __global__ void aspire_attn_merge_kernel(AttnParams p);
 __global__ void aspire_append_kv_kernel(AppendParams p);
 __global__ void aspire_select_pages_kernel(SelectParams p);
