@@ -238,51 +238,89 @@ __host__ __device__ inline int32_t item_parts(int mode, int kind, int32_t rows, 
   return mode == kPlanTree && kind == 2 && rows <= pf_half_rows(group) && n_chunks > 1 && chunk >= kSplitMinTokens ? 2 : 1;
 }
 
-// Chunk length of plans for trees: of kTreePlans candidates (about one, two or
-// three items per CTA; the longest group whole, in two or in three pieces) the
-// one whose estimated makespan is the shortest.  In tenths of a 128-token tile
-// of a decode item of up to 32 columns (1.75 us): wider tiles count more
-// (tree_tile10), an item's boundary kItemCost10, a split group's rows what
-// their partials' way out and back costs, the merge kMergeCost10.  The
-// makespan is the larger of the even share of all items and the rounds of
-// full-length ones.  Candidates whose partials the float workspace has no room
-// for are passed over; the whole groups have none.  Measured over fixed lengths of 256 to 131200 (16 rows of
-// 2k-8k with 8-16 nodes: best 81 us, the rule's 84; 8 rows of 4k-16k with
-// 32-64: 136, 136; one row of 32k with 8: 41, 41; 2 rows of 131k: 132, 140).
-constexpr int kTreePlans = 6;
+// Chunk length of plans for trees: of kTreePlans candidates the one whose
+// estimated makespan is the shortest, the longest of equals.  They are the even
+// share of one, two or three items per CTA, the same somewhat longer (so that
+// the groups' last pieces find room beside the full ones: 2 rows of 131k and
+// 57k keys, 10240 tokens 143 us, 10368 to 11904 132), and the longest group
+// whole, in two or in three pieces.  The estimate counts in twentieths of the
+// 1.4 us that a 128-token tile takes from memory when all SMs read
+// (kTreeEven20).  An SM by itself takes a decode tile in less and a prefill
+// tile in more (tree_tile20: 1.2 us; 2.1 for one half, bound by its softmax,
+// 2.4 for two, 1.55 where the halves alternate).  An item's boundary costs 4 us,
+// a split group's row what its partial's way out and back does, the merge 3 us.
+// The makespan is the largest of the memory's share, the longest item, and for
+// each of the upper eight lengths in sixteenths of a piece what the CTAs get that
+// take most items as long.  Candidates whose partials the float workspace has
+// no room for are passed over; the whole groups have none.  Best over fixed
+// lengths of 256 to 131200, and this rule: 16 rows of 2k-8k with 8-16 nodes 80
+// and 85 us; 8 rows of 4k-16k with 32-64 nodes 127, 132; 2 rows of 131k and 57k
+// 131, 135.  8 rows of 16k with 16 nodes: 104 (128 items; 192 items, 123).
+constexpr int kTreePlans = 11;
+constexpr int kTreeBins = 8;  // lengths in (8 + i, 9 + i] sixteenths of a piece
+constexpr int32_t kTreeEven20 = 20, kTreeItem20 = 58, kTreeMerge20 = 40;
 __host__ __device__ inline int64_t tree_chunk(int64_t total_tokens, int64_t max_span, int64_t num_sms, int k) {
-  const int64_t n = k < 3 ? num_sms * (k + 1) : k - 2;
-  int64_t chunk = ((k < 3 ? total_tokens : max_span) + n - 1) / n;
-  chunk = chunk < 256 ? 256 : chunk;
-  return (chunk + 127) / 128 * 128;
+  const int64_t whole = ((max_span > 256 ? max_span : 256) + 127) / 128 * 128;
+  int64_t chunk;
+  if (k < 8) {  // items per CTA, sixteenths longer
+    const int items = k < 4 ? 1 : k < 6 ? 2 : 3, longer = k < 4 ? (k < 3 ? k : 4) : (k & 1) * 2;
+    const int64_t shares = num_sms * items * 16;
+    chunk = (total_tokens * (16 + longer) + shares - 1) / shares;
+  } else {
+    chunk = (max_span + k - 8) / (k - 7);
+  }
+  chunk = ((chunk > 256 ? chunk : 256) + 127) / 128 * 128;
+  return chunk < whole ? chunk : whole;
 }
-__host__ __device__ inline int64_t tree_tile10(int kind, int rows, int group) {
-  if (kind == 2) return rows > pf_half_rows(group) ? 16 : 13;
-  return rows > 48 ? 12 : rows > 32 ? 11 : 10;
+__host__ __device__ inline int32_t tree_tile20(int kind, int rows, int group, int parts) {
+  if (kind != 2) return 17;
+  return parts > 1 ? 22 : rows > pf_half_rows(group) ? 34 : 30;
 }
-// A group's part of the estimate for chunk length `chunk`.
-struct TreeCost {
-  int64_t work10, full, full10;  // all items, full-length ones, the longest of those
-  int64_t partials;              // rows of the split groups' partials (0: none splits)
+// A group's part of the estimate for chunk length `chunk`: its work, the cost
+// of its longest piece, its full pieces, the bin of its last one (-1: none), its
+// partials' rows.
+struct TreeGroup {
+  int64_t work20, partials;
+  int32_t item20, full, last_bin;
 };
-__host__ __device__ inline void add_tree_cost(TreeCost& c, int64_t span, int64_t chunk, int kind, int rows, int group) {
-  const int64_t tile10 = tree_tile10(kind, rows, group);
-  const int64_t n = span > 0 ? (span + chunk - 1) / chunk : 1;
-  const int64_t item = kItemCost10 + (n > 1 ? rows * 10 / 64 : 0);  // (1 KB a row out and back, 64 KB a tile)
-  c.work10 += (span + 127) / 128 * tile10 + n * item;
-  const int64_t longest = span < chunk ? span : chunk;
-  const int64_t item10 = (longest + 127) / 128 * tile10 + item;
-  if (2 * longest > chunk) c.full += n > 1 ? span / chunk : 1;
-  if (item10 > c.full10) c.full10 = item10;
-  if (n > 1) c.partials += n * item_parts(kPlanTree, kind, rows, group, n, chunk) * rows;
+__host__ __device__ inline TreeGroup tree_group(uint32_t span, uint32_t chunk, int kind, int rows, int group) {
+  TreeGroup g;
+  const uint32_t tiles = (span + 127) / 128, piece = chunk / 128;
+  const uint32_t n = tiles > 0 ? (tiles + piece - 1) / piece : 1;
+  const int parts = item_parts(kPlanTree, kind, rows, group, n, chunk);
+  const int32_t tile20 = tree_tile20(kind, rows, group, parts);
+  const int32_t item = kTreeItem20 + (n > 1 ? rows * 20 / 64 : 0);  // (1 KB a row out and back, 64 KB a tile)
+  g.work20 = int64_t(tiles) * (tile20 > kTreeEven20 ? tile20 : kTreeEven20) + int64_t(n) * item;
+  g.item20 = int32_t(tiles < piece ? tiles : piece) * tile20 + item;
+  g.full = int32_t(tiles / piece);
+  const uint32_t last = tiles - uint32_t(g.full) * piece, sixteenths = (16 * last + piece - 1) / piece;
+  g.last_bin = sixteenths > 8 ? int32_t(sixteenths) - 9 : -1;
+  g.partials = n > 1 ? int64_t(n) * parts * rows : 0;
+  return g;
 }
+// Their sums.
+struct TreeCost {
+  unsigned long long work20, partials;  // all items; rows of the split groups' partials (0: none splits)
+  int32_t item20;                       // the longest item
+  uint32_t bins[kTreeBins];             // items by length, the full ones in the last
+};
 __host__ __device__ inline bool tree_fits(const TreeCost& c, int64_t float_ws_bytes) {
-  return c.partials <= INT32_MAX && c.partials * (kHeadDim + 1) * 4 <= float_ws_bytes;
+  return c.partials <= INT32_MAX && int64_t(c.partials) * (kHeadDim + 1) * 4 <= float_ws_bytes;
+}
+__host__ __device__ inline bool tree_better(int64_t makespan, int64_t chunk, int64_t best, int64_t best_chunk) {
+  return makespan < best || (makespan == best && best != INT64_MAX && chunk > best_chunk);
 }
 __host__ __device__ inline int64_t tree_makespan(const TreeCost& c, int64_t num_sms) {
-  const int64_t even = (c.work10 + num_sms - 1) / num_sms, rounds = (c.full + num_sms - 1) / num_sms * c.full10;
-  const int64_t most = even > rounds ? even : rounds;
-  return (most > c.full10 ? most : c.full10) + (c.partials > 0 ? kMergeCost10 : 0);
+  int64_t most = (int64_t(c.work20) + num_sms - 1) / num_sms;
+  if (c.item20 > most) most = c.item20;
+  int64_t items = 0;
+  for (int i = kTreeBins - 1; i >= 0; --i) {
+    items += c.bins[i];
+    const int64_t rounds = (items + num_sms - 1) / num_sms;
+    const int64_t length20 = i == kTreeBins - 1 ? c.item20 : int64_t(c.item20) * (17 + 2 * i) / 32;
+    if (rounds * length20 > most) most = rounds * length20;
+  }
+  return most + (c.partials > 0 ? kTreeMerge20 : 0);
 }
 
 }  // namespace aspire

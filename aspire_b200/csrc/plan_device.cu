@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kDevPlanThreads) aspire_plan_device_kernel(Dev
   pdl_begin();
   __shared__ int64_t warp_sums[32];
   __shared__ int32_t bucket[2][kCostBuckets];  // per kernel list: decode (1), prefill (2)
-  __shared__ int bad, max_span, min_span, long_cols, longest10;
+  __shared__ int bad, max_span, min_span, long_cols;
   const int tid = threadIdx.x, nthreads = blockDim.x;
   if (tid == 0) {
     bad = 0;
@@ -138,38 +138,38 @@ __global__ void __launch_bounds__(kDevPlanThreads) aspire_plan_device_kernel(Dev
   const bool similar = 2 * int64_t(min_span) >= max_span;
   int64_t chunk = chunk_for(total_tokens, p.num_sms, similar ? kItemsPerCtaUniform : kItemsPerCtaMixed);
   if constexpr (kTrees) {
-    TreeCost cost[kTreePlans] = {};
-    for (int b = r0; b < r1; ++b) {
+    // A thread for a row and a candidate at a time.
+    __shared__ TreeCost cost[kTreePlans];
+    for (int i = tid; i < int(sizeof(cost) / 4); i += nthreads) reinterpret_cast<uint32_t*>(cost)[i] = 0;
+    __syncthreads();
+    for (int64_t i = tid; i < int64_t(p.batch) * kTreePlans; i += nthreads) {
+      const int b = int(i / kTreePlans), k = int(i % kTreePlans);
       const RowShape s = row_shape(p, b);
       if (s.ql <= 0) continue;
+      const uint32_t length = uint32_t(tree_chunk(total_tokens, max_span, p.num_sms, k));
+      TreeCost& c = cost[k];
       for (int qt = 0; qt < s.ntq; ++qt) {
         const int32_t rows = min(s.nq, (qt + 1) * s.tile) - qt * s.tile;
-        for (int k = 0; k < kTreePlans; ++k) {
-          TreeCost one = {};
-          add_tree_cost(one, s.kl, tree_chunk(total_tokens, max_span, p.num_sms, k), s.kind, rows, p.group);
-          cost[k].work10 += p.num_kv_heads * one.work10;
-          cost[k].full += p.num_kv_heads * one.full;
-          cost[k].full10 = max(cost[k].full10, one.full10);
-          cost[k].partials += p.num_kv_heads * one.partials;
-        }
+        const TreeGroup t = tree_group(uint32_t(s.kl), length, s.kind, rows, p.group);
+        atomicAdd(&c.work20, (unsigned long long)(p.num_kv_heads * t.work20));
+        if (t.partials > 0) atomicAdd(&c.partials, (unsigned long long)(p.num_kv_heads * t.partials));
+        atomicMax(&c.item20, t.item20);
+        if (t.full > 0) atomicAdd(&c.bins[kTreeBins - 1], uint32_t(p.num_kv_heads * t.full));
+        if (t.last_bin >= 0) atomicAdd(&c.bins[t.last_bin], uint32_t(p.num_kv_heads));
       }
     }
+    __syncthreads();
+    __shared__ int64_t makespan[kTreePlans];
+    if (tid < kTreePlans)
+      makespan[tid] = tree_fits(cost[tid], p.float_ws_bytes) ? tree_makespan(cost[tid], p.num_sms) : INT64_MAX;
+    __syncthreads();
     int64_t best = INT64_MAX;
-    for (int k = 0; k < kTreePlans; ++k) {
-      TreeCost all;
-      block_exclusive_scan(cost[k].work10, warp_sums, &all.work10);
-      block_exclusive_scan(cost[k].full, warp_sums, &all.full);
-      if (tid == 0) longest10 = 0;
-      __syncthreads();
-      atomicMax(&longest10, int(min(cost[k].full10, int64_t(INT_MAX))));
-      block_exclusive_scan(cost[k].partials, warp_sums, &all.partials);
-      all.full10 = longest10;
-      __syncthreads();
-      if (tree_fits(all, p.float_ws_bytes) && tree_makespan(all, p.num_sms) < best) {
-        best = tree_makespan(all, p.num_sms);
-        chunk = tree_chunk(total_tokens, max_span, p.num_sms, k);
+    for (int k = 0; k < kTreePlans; ++k)
+      if (const int64_t length = tree_chunk(total_tokens, max_span, p.num_sms, k);
+          tree_better(makespan[k], length, best, chunk)) {
+        best = makespan[k];
+        chunk = length;
       }
-    }
   } else if (!similar) {
     // Long groups cut into one piece per SM when that packs the grid (long_group_chunk).
     int64_t my_long = 0, my_short = 0;

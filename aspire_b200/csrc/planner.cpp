@@ -176,9 +176,15 @@ int plan_impl(const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t*
     for (int k = 0; k < kTreePlans; ++k) {
       const int64_t length = tree_chunk(total_tokens, max_span, num_sms, k);
       TreeCost cost{};
-      for (const GroupDesc& g : groups)
-        add_tree_cost(cost, g.span, length, g.kind, g.pq_end - g.pq_begin, group);
-      if (tree_fits(cost, int64_t(float_ws_bytes)) && tree_makespan(cost, num_sms) < best) {
+      for (const GroupDesc& g : groups) {
+        const TreeGroup t = tree_group(uint32_t(g.span), uint32_t(length), g.kind, g.pq_end - g.pq_begin, group);
+        cost.work20 += t.work20;
+        cost.partials += t.partials;
+        cost.item20 = std::max(cost.item20, t.item20);
+        cost.bins[kTreeBins - 1] += t.full;
+        if (t.last_bin >= 0) ++cost.bins[t.last_bin];
+      }
+      if (tree_fits(cost, int64_t(float_ws_bytes)) && tree_better(tree_makespan(cost, num_sms), length, best, chunk)) {
         best = tree_makespan(cost, num_sms);
         chunk = length;
       }
