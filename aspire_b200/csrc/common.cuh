@@ -217,9 +217,10 @@ __host__ __device__ constexpr int pf_item_rows(int group) { return 2 * pf_half_r
 // What a plan is made for (the planners' `causal` argument): a plan for trees
 // is not causal and runs under a tree mask only.  Its decode items have up to
 // kTreeQTile packed rows and every longer row is a prefill item, one pass over
-// the keys either way (8 rows of 16k keys, 16 nodes of a group of 4: 123 us
-// against 168 with tiles of 48 rows; 24 nodes: 185 as a prefill item, 165 in
-// two decode passes; 31 nodes: 189 against 253 in three).
+// the keys either way (8 rows of 16k keys in pieces of 7168, 16 nodes of a group
+// of 4: 123 us against 168 with tiles of 48 rows; 24 nodes: 150 as a prefill
+// item whose tiles alternate, 165 in two decode passes; 31 nodes: 155 against
+// 253 in three).
 enum PlanMode : int { kPlanAll = 0, kPlanCausal = 1, kPlanTree = 2 };
 __host__ __device__ constexpr int decode_tile_rows(int mode) { return mode == kPlanTree ? kTreeQTile : kTcQTile; }
 __host__ __device__ constexpr int prefill_min_rows(int mode) { return mode == kPlanTree ? kTreeQTile + 1 : kPfMinRows; }
@@ -228,11 +229,12 @@ __host__ __device__ constexpr int prefill_min_rows(int mode) { return mode == kP
 // between the two halves' warps (WorkItem::cols, unused by other prefill
 // items): both hold the same rows, half h's partials are chunk `chunk` + h of
 // the item's group.  One half alone is bound by its softmax (2.4 us a tile).
-// Taken where the group is split anyway, in long pieces: 8 rows of 16k keys and
-// 32 nodes of a group of 4, pieces of 7168: 187 -> 158 us; 32 rows of 4k whole:
-// 163 -> 172; 4 rows of 2k, pieces of 512: 32 -> 38.
+// Taken where the group is split anyway, in long pieces.  24 nodes of a group
+// of 4: 8 rows of 16k keys, pieces of 7168, 185 -> 150 us; 32 rows of 4k, 3584,
+// 178 -> 154; 3 rows of 9k, 1536, 54 -> 51; 8 rows of 2k, 1024, 47 -> 49; one
+// row of 8k, 512, 29 -> 35.
 constexpr int32_t kSplitTiles = 1;
-constexpr int64_t kSplitMinTokens = 2048;
+constexpr int64_t kSplitMinTokens = 1536;
 __host__ __device__ inline int32_t item_parts(int mode, int kind, int32_t rows, int group, int64_t n_chunks,
                                               int64_t chunk) {
   return mode == kPlanTree && kind == 2 && rows <= pf_half_rows(group) && n_chunks > 1 && chunk >= kSplitMinTokens ? 2 : 1;
