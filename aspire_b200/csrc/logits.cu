@@ -103,8 +103,8 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {
 // 16 bits where the history allows (kWide: 32): two CTAs then hold 152000
 // entries, and 64 rows are one wave.  Bound by the latency of its few steps
 // and by its instructions, so what it reads is requested before anything
-// waits.  64 rows with histories of up to 16384 over 151936 entries: 15 us;
-// one row with 900: 4 us.
+// waits.  64 rows with histories of up to 16384 over 151936 entries: 19.6 us
+// with cold caches; one row with 900 over eight CTAs: 8.7.
 template <bool kWide>
 __global__ void __launch_bounds__(kMarkThreads, 1) aspire_logits_mark_kernel(LogitsParams p) {
   // (The next kernel reads the logits before it waits for this one, so it may
@@ -484,7 +484,9 @@ struct Listed {
 
 // The adjusted logits of token blockIdx.x.  The warps work on their own: no
 // barrier, three chunks of each on their way while it adjusts the listed
-// entries of one where they lie, in shared memory.
+// entries of one where they lie, in shared memory.  64 rows of 151936 fp32
+// logits with some 4 to 16 thousand entries listed each: 23.6 us for 78 MB; both
+// kernels in a graph 37.
 template <typename T>
 __global__ void __launch_bounds__(kLogitsThreads, kLogitsCtas) aspire_logits_kernel(LogitsParams p) {
   using W = Walk<T>;
