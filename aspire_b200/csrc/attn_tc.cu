@@ -671,19 +671,33 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
   const bool final_rows = it.n_chunks <= 1;
   const int row_end = min(c0 + NH, nrows);  // this group's rows are [c0, row_end)
   if (final_rows) {
+    if constexpr (Sh::kStageInP) {
 #pragma unroll
-    for (int j = 0; j < NH; ++j)
-      if (c0 + j < nrows)
-        reinterpret_cast<__nv_bfloat16*>(staged(j, kHeadDim * 2))[d] = __float2bfloat16_rn(o_fin[j] * sm.inv_l[c0 + j]);
+      for (int j = 0; j < NH; ++j)
+        if (c0 + j < nrows)
+          reinterpret_cast<__nv_bfloat16*>(staged(j, kHeadDim * 2))[d] = __float2bfloat16_rn(o_fin[j] * sm.inv_l[c0 + j]);
+    } else {
+      __nv_bfloat16* st = reinterpret_cast<__nv_bfloat16*>(sm.out_stage);
+#pragma unroll
+      for (int j = 0; j < NH; ++j)
+        if (c0 + j < nrows) st[(c0 + j) * kHeadDim + d] = __float2bfloat16_rn(o_fin[j] * sm.inv_l[c0 + j]);
+    }
     if (ctid < NH && c0 + ctid < nrows && p.lse) {
       int q_idx, head;
       packed_row(p, it, it.pq_begin + c0 + ctid, q_idx, head);
       if (int64_t(it.q_start) + q_idx < p.q_rows) p.lse[(int64_t(it.q_start) + q_idx) * p.num_qo_heads + head] = my_lse;
     }
   } else {
+    if constexpr (Sh::kStageInP) {
 #pragma unroll
-    for (int j = 0; j < NH; ++j)
-      if (c0 + j < nrows) reinterpret_cast<float*>(staged(j, kHeadDim * 4))[d] = o_fin[j] * sm.inv_l[c0 + j];
+      for (int j = 0; j < NH; ++j)
+        if (c0 + j < nrows) reinterpret_cast<float*>(staged(j, kHeadDim * 4))[d] = o_fin[j] * sm.inv_l[c0 + j];
+    } else {
+      float* st = reinterpret_cast<float*>(sm.out_stage);
+#pragma unroll
+      for (int j = 0; j < NH; ++j)
+        if (c0 + j < nrows) st[(c0 + j) * kHeadDim + d] = o_fin[j] * sm.inv_l[c0 + j];
+    }
     if (ctid < NH && c0 + ctid < nrows)
       partial_lse_ptr(p)[int64_t(it.partial_base) + int64_t(it.chunk) * nrows + c0 + ctid] = my_lse;
   }
@@ -699,16 +713,23 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
           continue;
         }
         __nv_bfloat16* dst = p.out + (int64_t(it.q_start) + q_idx) * p.o_stride_n + int64_t(head) * p.o_stride_h;
-        ptx::bulk_store(dst, ptx::smem_addr(staged(j - c0, kHeadDim * 2)), kHeadDim * 2);
+        const uint32_t src = Sh::kStageInP ? ptx::smem_addr(staged(j - c0, kHeadDim * 2))
+                                           : ptx::smem_addr(sm.out_stage) + uint32_t(j) * kHeadDim * 2;
+        ptx::bulk_store(dst, src, kHeadDim * 2);
       }
     } else {
       const int64_t base = int64_t(it.partial_base) + int64_t(it.chunk) * nrows + c0;
-      const int rows = row_end - c0, part = Sh::kStageInP ? min(rows, NH / 2) : rows;  // rows in one piece
-      ptx::bulk_store(p.partial_o + base * kHeadDim, ptx::smem_addr(staged(0, kHeadDim * 4)),
-                      uint32_t(part) * kHeadDim * 4);
-      if (part < rows)
-        ptx::bulk_store(p.partial_o + (base + part) * kHeadDim, ptx::smem_addr(staged(part, kHeadDim * 4)),
-                        uint32_t(rows - part) * kHeadDim * 4);
+      if constexpr (Sh::kStageInP) {
+        const int rows = row_end - c0, part = min(rows, NH / 2);  // rows in one piece
+        ptx::bulk_store(p.partial_o + base * kHeadDim, ptx::smem_addr(staged(0, kHeadDim * 4)),
+                        uint32_t(part) * kHeadDim * 4);
+        if (part < rows)
+          ptx::bulk_store(p.partial_o + (base + part) * kHeadDim, ptx::smem_addr(staged(part, kHeadDim * 4)),
+                          uint32_t(rows - part) * kHeadDim * 4);
+      } else {
+        ptx::bulk_store(p.partial_o + base * kHeadDim, ptx::smem_addr(sm.out_stage) + uint32_t(c0) * kHeadDim * 4,
+                        uint32_t(row_end - c0) * kHeadDim * 4);
+      }
     }
     ptx::bulk_commit();
   }
