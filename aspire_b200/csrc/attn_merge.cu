@@ -107,7 +107,11 @@ __device__ __forceinline__ void merge_rows(const AttnParams& p, const MergeDesc*
 __global__ void __launch_bounds__(kMergeThreads) aspire_attn_merge_kernel(AttnParams p) {
   pdl_begin();
   const int32_t* plan = p.plan;
-  if (!plan_runs(plan, p.tree_mask != nullptr)) return;
+  if (!plan_runs(plan, p.tree_mask != nullptr)) {
+    // (Reported here: a status written by the attention kernel costs its prefill phase 3 %.)
+    if (plan[kHdrMagic] != 0 && blockIdx.x == 0 && threadIdx.x == 0) record_status(p.status, ASPIRE_STATUS_BAD_PLAN);
+    return;
+  }
   // The tcgen05 kernel of this call has finished: rearm its item counters for
   // the next launch of the same plan (graph replays upload no new plan).
   if (blockIdx.x == 0 && threadIdx.x == 0) {

@@ -866,9 +866,7 @@ __device__ __forceinline__ void attn_tc(const AttnParams& p, const CUtensorMap& 
   // The plan and every input are outputs of earlier kernels (or copies).
   pdl_wait();
   const int32_t* plan = p.plan;
-  const bool runs = plan_runs(plan, kTree);
-  if (!runs && plan[kHdrMagic] != 0 && blockIdx.x == 0 && threadIdx.x == 0) record_status(p.status, ASPIRE_STATUS_BAD_PLAN);
-  const bool live = runs && int(blockIdx.x) < plan[kHdrNumTcCtas];
+  const bool live = plan_runs(plan, kTree) && int(blockIdx.x) < plan[kHdrNumTcCtas];
   const int tc_first = live ? plan[kHdrTcFirst] : 0;
   const int pf_first = live ? plan[kHdrPfFirst] : 0;
   const int n_tc = live ? pf_first - tc_first : 0;
