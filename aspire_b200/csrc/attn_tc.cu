@@ -100,6 +100,7 @@ struct TcShared {
   uint64_t v_full[kVStages], v_empty[kVStages];
   uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2];
   uint64_t o_free, q_full, q_empty, done, done_pv, grp[2];
+  uint64_t stage_free;  // (kStageInP) both groups' rows of an item have left the P buffers, where the next is of another width
   pf::Barriers pf;  // prefill phase
   uint64_t seq_full[kSeqDepth], seq_empty[kSeqDepth];
   int seq[kSeqDepth];
@@ -419,7 +420,8 @@ __device__ __forceinline__ uint32_t tree_columns(const AttnParams& p, const Work
 
 template <int NH, bool kDump, bool kTree, class Sh>
 __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bool causal, int r,
-                             int ctid, int wg, int wq, int lane, uint32_t& g, uint32_t& grp_uses) {
+                             int ctid, int wg, int wq, int lane, uint32_t& g, uint32_t& grp_uses, int& staged_cols,
+                             uint32_t& width_changes) {
   constexpr int N = 2 * NH;
   const int c0 = wg * NH;
   const int nrows = it.pq_end - it.pq_begin;
@@ -468,6 +470,11 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
   // next vote, so that no lane leaves alone; a vote after every wait would cost
   // the tile loop 4 %.  After a failure no output counts (ASPIRE_STATUS_TIMEOUT).
   bool failed = false;
+  // kStageInP: the previous item's rows lie in the group's part of the P buffers,
+  // which its width gives it.  An item of another width writes its P over the
+  // other group's rows too, which that group may still be storing.
+  const bool other_width = Sh::kStageInP && staged_cols != 0 && staged_cols != N;
+  staged_cols = N;
   int flag = 0;  // the first tile sets its flags whatever they hold
 
   for (int t = 0; t < nt; ++t) {
@@ -541,7 +548,10 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
     // last barrier: it is free to be cleared.)
     const int next_flag = flag == 2 ? 0 : flag + 1;
     // The previous item's rows have left the P buffers before this item's P is written.
-    if (Sh::kStageInP && t == 0 && ctid == 0) ptx::bulk_wait_read();
+    if (Sh::kStageInP && t == 0 && ctid == 0) {
+      ptx::bulk_wait_read();
+      if (other_width) ptx::mbar_arrive(ptx::smem_addr(&sm.stage_free));
+    }
     if (exceed) flags[flag][wq] = 1;
     if (lane == 0) flags[next_flag][wq] = 0;
     failed |= !group_sync(sm, grp, grp_uses, p.status);
@@ -611,6 +621,10 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
     }
     // P^T as bf16, MN-major without swizzle: 8 queries x 16 B per token, token-major.
     failed |= !wait_bar(sm, sm.p_empty[b], ph ^ 1, p.status);
+    if (Sh::kStageInP && t == 0 && other_width) {
+      failed |= !wait_bar(sm, sm.stage_free, width_changes & 1, p.status);
+      ++width_changes;
+    }
     uint8_t* pbuf = sm.p[b] + (c0 / 8) * (kTile * 16);
 #pragma unroll
     for (int c = 0; c < NH / 8; ++c) {
@@ -743,7 +757,8 @@ __device__ void consume_items(const AttnParams& p, Sh& sm, bool causal, int warp
   const int wg = (warp - kFirstSoftmaxWarp) / 4;  // softmax warpgroup 0 or 1
   const int r = wq * 32 + lane;                    // TMEM lane = S-tile token = O-tile dim
   const int ctid = (warp - kFirstSoftmaxWarp - 4 * wg) * 32 + lane;  // 0..127 within the group
-  uint32_t g = 0, grp_uses = 0;
+  uint32_t g = 0, grp_uses = 0, width_changes = 0;
+  int staged_cols = 0;  // width of the previous item
   for (;;) {
     if (__any_sync(0xffffffffu, aborted(sm))) return;
     const int ii = seq_read(sm, k, lane, p.status);
@@ -771,21 +786,28 @@ __device__ void consume_items(const AttnParams& p, Sh& sm, bool causal, int warp
       if constexpr (kTree) {
         ok = false;
       } else if (N == 16) {
-        ok = consume_item<8, true, false>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+        ok = consume_item<8, true, false>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses, staged_cols,
+                                          width_changes);
       } else if (N == 32) {
-        ok = consume_item<16, true, false>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+        ok = consume_item<16, true, false>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses, staged_cols,
+                                           width_changes);
       } else {
-        ok = consume_item<24, true, false>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+        ok = consume_item<24, true, false>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses, staged_cols,
+                                           width_changes);
       }
     } else {
       if (N == 16)
-        ok = consume_item<8, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+        ok = consume_item<8, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses, staged_cols,
+                                           width_changes);
       else if (N == 32)
-        ok = consume_item<16, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+        ok = consume_item<16, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses, staged_cols,
+                                            width_changes);
       else if (Sh::kNMax == 48 || N == 48)
-        ok = consume_item<24, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+        ok = consume_item<24, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses, staged_cols,
+                                            width_changes);
       else if constexpr (Sh::kNMax > 48)
-        ok = consume_item<32, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses);
+        ok = consume_item<32, false, kTree>(p, sm, it, causal, r, ctid, wg, wq, lane, g, grp_uses, staged_cols,
+                                            width_changes);
     }
     if (!ok) return;
   }
@@ -836,6 +858,7 @@ __device__ __forceinline__ void attn_tc(const AttnParams& p, const CUtensorMap& 
     ptx::mbar_init(ptx::smem_addr(&sm.done_pv), 1);
     ptx::mbar_init(ptx::smem_addr(&sm.grp[0]), 128);
     ptx::mbar_init(ptx::smem_addr(&sm.grp[1]), 128);
+    ptx::mbar_init(ptx::smem_addr(&sm.stage_free), 2);
     pf::init_barriers(sm.pf);
     for (int s = 0; s < kSeqDepth; ++s) {
       ptx::mbar_init(ptx::smem_addr(&sm.seq_full[s]), 1);

@@ -181,6 +181,38 @@ def test_items_whose_tiles_alternate_between_the_halves(cuda_device, rows, sms, 
         assert w.device_status() == 0
 
 
+def _short_rows_of_four_widths():
+    rng = random.Random(21)
+    return [(rng.randint(0, 500), rng.choice([4, 8, 12, 16])) for _ in range(48)]
+
+
+def _long_rows_of_four_widths():
+    rng = random.Random(403)
+    return [(rng.randint(900, 9000), rng.choice([4, 8, 12, 16])) for _ in range(rng.randint(2, 30))]
+
+
+@pytest.mark.parametrize("rows,sms", [(_short_rows_of_four_widths(), 1), (_short_rows_of_four_widths(), 2),
+                                      (_long_rows_of_four_widths(), 11)])
+def test_consecutive_items_of_other_widths(cuda_device, rows, sms):
+    """A CTA's items have 16, 32, 48 and 64 columns in turn, whole and split ones."""
+    c = Case(cuda_device, rows, 8, 2, seed=21)
+    w = HolisticAttentionWrapper(torch.empty(1, device=cuda_device), num_sms=sms)
+    c.plan(wrapper=w, trees=True)
+    torch.cuda.synchronize()
+    words = w._int_workspace[256:].view(torch.int32).cpu()
+    items = words[int(words[5]):int(words[5]) + 16 * int(words[1])].view(-1, 16)
+    columns = torch.maximum((items[:, 9] - items[:, 8] + 15) // 16 * 16, items[:, 15])
+    assert columns.unique().tolist() == [16, 32, 48, 64] and items.shape[0] > 2 * sms
+    assert bool((items[:, 11] > 1).any()) == (sms == 11)
+    q, kv = c.q.to(cuda_device), c.cache.to(cuda_device)
+    out, lse = w.run(q, kv, tree_mask=c.mask, return_lse=True)
+    c.check(out, lse)
+    for _ in range(20):
+        o, l = w.run(q, kv, tree_mask=c.mask, return_lse=True)
+        assert torch.equal(o, out) and torch.equal(l, lse)
+    assert w.device_status() == 0
+
+
 def test_a_plain_plan_is_made_again_for_trees_outside_captures(cuda_device):
     c = Case(cuda_device, [(300, 16), (40, 25)], 4, 1, seed=15)
     q, kv = c.q.to(cuda_device), c.cache.to(cuda_device)
