@@ -424,6 +424,10 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
                              uint32_t& width_changes) {
   constexpr int N = 2 * NH;
   const int c0 = wg * NH;
+  // The group's places in the shared statistics start at s0, whatever the item's
+  // width: a group may begin the next item, of another width, while the other
+  // group still ends this one.
+  const int s0 = wg * (Sh::kNMax / 2);
   const int nrows = it.pq_end - it.pq_begin;
   const int nt = n_tiles_of(it);
   const uint32_t tmem_lane = sm.tmem_base + (uint32_t(wq * 32) << 16);
@@ -538,7 +542,7 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
     mask_s(sv);
 
     // Lazy running max: does any logit of the tile exceed its column's reference by > 2^8?
-    const float* mr = sm.mref[cur] + c0;
+    const float* mr = sm.mref[cur] + s0;
     bool exceed = (t == 0);
     if (t > 0) {
 #pragma unroll
@@ -563,11 +567,11 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
       // TMEM afterwards).  Thread j < NH then updates column c0 + j's reference
       // (mref[cur ^ 1]) and its rescale factor alpha; the per-column work is
       // spread over threads so that this once-per-item path stays short.
-      warp_columns<NH, true>(sv, sm.red[t & 1][wq] + c0, lane);
+      warp_columns<NH, true>(sv, sm.red[t & 1][wq] + s0, lane);
       if (ctid == 0) grew[t & 1] = 0;
       if (!group_sync_warp(sm, grp, grp_uses, p.status)) return false;
       if (ctid < NH) {
-        const int c = c0 + ctid;
+        const int c = s0 + ctid;
         const float mo = t > 0 ? sm.mref[cur][c] : -INFINITY;
         const float tmax = fmaxf(fmaxf(sm.red[t & 1][0][c], sm.red[t & 1][1][c]),
                                  fmaxf(sm.red[t & 1][2][c], sm.red[t & 1][3][c]));
@@ -584,7 +588,7 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
       if (!group_sync_warp(sm, grp, grp_uses, p.status)) return false;
       cur ^= 1;
       if (t > 0 && grew[t & 1]) {
-        const float* alpha_s = sm.alpha[t & 1] + c0;
+        const float* alpha_s = sm.alpha[t & 1] + s0;
 #pragma unroll
         for (int j = 0; j < NH; ++j) l[j] *= alpha_s[j];
         // Rescale this group's O columns once the previous tile's PV has
@@ -611,7 +615,7 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
       ptx::mbar_arrive(ptx::smem_addr(&sm.s_empty[b]));
     }
     {
-      const float* m = sm.mref[cur] + c0;
+      const float* m = sm.mref[cur] + s0;
 #pragma unroll
       for (int j = 0; j < NH; ++j) {
         const float pv = (m[j] == -INFINITY) ? 0.f : ex2(fmaf(sv[j], scale, -m[j]));
@@ -657,11 +661,11 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
 
   // Column sums of l across the group's 128 threads; thread j < NH then turns
   // column c0 + j into its reciprocal and LSE once.
-  warp_columns<NH, false>(l, sm.red_l[wq] + c0, lane);
+  warp_columns<NH, false>(l, sm.red_l[wq] + s0, lane);
   if (!group_sync_warp(sm, grp, grp_uses, p.status)) return false;
   float my_lse = -INFINITY;  // LSE of column c0 + ctid
   if (ctid < NH) {
-    const int c = c0 + ctid;
+    const int c = s0 + ctid;
     const float L = sm.red_l[0][c] + sm.red_l[1][c] + sm.red_l[2][c] + sm.red_l[3][c];
     sm.inv_l[c] = L > 0.f ? 1.f / L : 0.f;
     my_lse = L > 0.f ? sm.mref[cur][c] + lg2(L) : -INFINITY;
@@ -689,12 +693,12 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
 #pragma unroll
       for (int j = 0; j < NH; ++j)
         if (c0 + j < nrows)
-          reinterpret_cast<__nv_bfloat16*>(staged(j, kHeadDim * 2))[d] = __float2bfloat16_rn(o_fin[j] * sm.inv_l[c0 + j]);
+          reinterpret_cast<__nv_bfloat16*>(staged(j, kHeadDim * 2))[d] = __float2bfloat16_rn(o_fin[j] * sm.inv_l[s0 + j]);
     } else {
       __nv_bfloat16* st = reinterpret_cast<__nv_bfloat16*>(sm.out_stage);
 #pragma unroll
       for (int j = 0; j < NH; ++j)
-        if (c0 + j < nrows) st[(c0 + j) * kHeadDim + d] = __float2bfloat16_rn(o_fin[j] * sm.inv_l[c0 + j]);
+        if (c0 + j < nrows) st[(c0 + j) * kHeadDim + d] = __float2bfloat16_rn(o_fin[j] * sm.inv_l[s0 + j]);
     }
     if (ctid < NH && c0 + ctid < nrows && p.lse) {
       int q_idx, head;
@@ -705,12 +709,12 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
     if constexpr (Sh::kStageInP) {
 #pragma unroll
       for (int j = 0; j < NH; ++j)
-        if (c0 + j < nrows) reinterpret_cast<float*>(staged(j, kHeadDim * 4))[d] = o_fin[j] * sm.inv_l[c0 + j];
+        if (c0 + j < nrows) reinterpret_cast<float*>(staged(j, kHeadDim * 4))[d] = o_fin[j] * sm.inv_l[s0 + j];
     } else {
       float* st = reinterpret_cast<float*>(sm.out_stage);
 #pragma unroll
       for (int j = 0; j < NH; ++j)
-        if (c0 + j < nrows) st[(c0 + j) * kHeadDim + d] = o_fin[j] * sm.inv_l[c0 + j];
+        if (c0 + j < nrows) st[(c0 + j) * kHeadDim + d] = o_fin[j] * sm.inv_l[s0 + j];
     }
     if (ctid < NH && c0 + ctid < nrows)
       partial_lse_ptr(p)[int64_t(it.partial_base) + int64_t(it.chunk) * nrows + c0 + ctid] = my_lse;

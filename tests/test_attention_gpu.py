@@ -167,6 +167,26 @@ def test_edge_rows(cuda_device):
     assert torch.isinf(lse[r0:r1]).all()
 
 
+@pytest.mark.parametrize("sms", [1])
+def test_consecutive_items_of_other_widths(cuda_device, sms):
+    """A CTA's items have 16, 32 and 48 columns in turn; the results repeat."""
+    rng = np.random.default_rng(33)
+    q_lens = rng.choice([1, 4, 6, 8, 10, 12], 40).tolist() + [9, 5, 2]
+    lay = _custom_layout(q_lens, rng.integers(12, 500, 40).tolist() + [6000, 5000, 4000], hq=8, hkv=2, seed=33)
+    if not any(k in os.environ for k in ROUTING_VARS):  # the plan's shape under the default routing
+        rows, cols = _tc_item_columns(lay, sms)
+        assert np.unique(np.maximum((rows + 15) // 16 * 16, cols)).tolist() == [16, 32, 48]
+        assert (len(rows) > 2 * lay.batch) == (sms > 1), "some rows are split with 5 CTAs, none with one"
+    q, kv = make_inputs(lay, cuda_device, seed=33)
+    w = HolisticAttentionWrapper(torch.empty(1, device=cuda_device), num_sms=sms)
+    out, lse, _, _ = run_attention(lay, q, kv, wrapper=w)
+    ref_out, ref_lse, _ = oracle_attention(lay, q, kv)
+    assert_attention_close(out, lse, ref_out, ref_lse)
+    for _ in range(10):
+        o, l, _, _ = run_attention(lay, q, kv, wrapper=w)
+        assert torch.equal(o, out) and torch.equal(l, lse)
+
+
 @pytest.mark.parametrize("hq,hkv", [(32, 8), (16, 8), (40, 8)])
 def test_prefill_rows(cuda_device, hq, hkv):
     """Long-query causal rows (prefill chunks, with and without a cached
