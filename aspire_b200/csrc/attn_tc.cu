@@ -678,13 +678,15 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
   // Normalised rows are staged in shared memory and leave by bulk stores, so
   // the threads move on to the next item at once.
   const int d = r;  // this thread's output dim
-  // Row c0 + j of the item, of row_bytes: in the output stage or, by halves of
-  // the group's rows, in its parts of the two P buffers.
+  // Row c0 + j of the item, of row_bytes: in the group's half of the output stage
+  // (the same half for all widths and row sizes, so that the other group's rows
+  // are never written over) or, by halves of the group's rows, in its parts of
+  // the two P buffers.
   const auto staged = [&](int j, int row_bytes) -> uint8_t* {
     if constexpr (Sh::kStageInP)
       return sm.p[j / (NH / 2)] + (c0 / 8) * (kTile * 16) + (j % (NH / 2)) * row_bytes;
     else
-      return sm.out_stage + (c0 + j) * row_bytes;
+      return sm.out_stage + s0 * (kHeadDim * 4) + j * row_bytes;
   };
   const bool final_rows = it.n_chunks <= 1;
   const int row_end = min(c0 + NH, nrows);  // this group's rows are [c0, row_end)
@@ -695,10 +697,10 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
         if (c0 + j < nrows)
           reinterpret_cast<__nv_bfloat16*>(staged(j, kHeadDim * 2))[d] = __float2bfloat16_rn(o_fin[j] * sm.inv_l[s0 + j]);
     } else {
-      __nv_bfloat16* st = reinterpret_cast<__nv_bfloat16*>(sm.out_stage);
+      __nv_bfloat16* st = reinterpret_cast<__nv_bfloat16*>(staged(0, kHeadDim * 2));
 #pragma unroll
       for (int j = 0; j < NH; ++j)
-        if (c0 + j < nrows) st[(c0 + j) * kHeadDim + d] = __float2bfloat16_rn(o_fin[j] * sm.inv_l[s0 + j]);
+        if (c0 + j < nrows) st[j * kHeadDim + d] = __float2bfloat16_rn(o_fin[j] * sm.inv_l[s0 + j]);
     }
     if (ctid < NH && c0 + ctid < nrows && p.lse) {
       int q_idx, head;
@@ -711,10 +713,10 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
       for (int j = 0; j < NH; ++j)
         if (c0 + j < nrows) reinterpret_cast<float*>(staged(j, kHeadDim * 4))[d] = o_fin[j] * sm.inv_l[s0 + j];
     } else {
-      float* st = reinterpret_cast<float*>(sm.out_stage);
+      float* st = reinterpret_cast<float*>(staged(0, kHeadDim * 4));
 #pragma unroll
       for (int j = 0; j < NH; ++j)
-        if (c0 + j < nrows) st[(c0 + j) * kHeadDim + d] = o_fin[j] * sm.inv_l[s0 + j];
+        if (c0 + j < nrows) st[j * kHeadDim + d] = o_fin[j] * sm.inv_l[s0 + j];
     }
     if (ctid < NH && c0 + ctid < nrows)
       partial_lse_ptr(p)[int64_t(it.partial_base) + int64_t(it.chunk) * nrows + c0 + ctid] = my_lse;
@@ -731,9 +733,7 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
           continue;
         }
         __nv_bfloat16* dst = p.out + (int64_t(it.q_start) + q_idx) * p.o_stride_n + int64_t(head) * p.o_stride_h;
-        const uint32_t src = Sh::kStageInP ? ptx::smem_addr(staged(j - c0, kHeadDim * 2))
-                                           : ptx::smem_addr(sm.out_stage) + uint32_t(j) * kHeadDim * 2;
-        ptx::bulk_store(dst, src, kHeadDim * 2);
+        ptx::bulk_store(dst, ptx::smem_addr(staged(j - c0, kHeadDim * 2)), kHeadDim * 2);
       }
     } else {
       const int64_t base = int64_t(it.partial_base) + int64_t(it.chunk) * nrows + c0;
@@ -745,7 +745,7 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
           ptx::bulk_store(p.partial_o + (base + part) * kHeadDim, ptx::smem_addr(staged(part, kHeadDim * 4)),
                           uint32_t(rows - part) * kHeadDim * 4);
       } else {
-        ptx::bulk_store(p.partial_o + base * kHeadDim, ptx::smem_addr(sm.out_stage) + uint32_t(c0) * kHeadDim * 4,
+        ptx::bulk_store(p.partial_o + base * kHeadDim, ptx::smem_addr(staged(0, kHeadDim * 4)),
                         uint32_t(row_end - c0) * kHeadDim * 4);
       }
     }

@@ -167,9 +167,10 @@ def test_edge_rows(cuda_device):
     assert torch.isinf(lse[r0:r1]).all()
 
 
-@pytest.mark.parametrize("sms", [1])
+@pytest.mark.parametrize("sms", [1, 5])
 def test_consecutive_items_of_other_widths(cuda_device, sms):
-    """A CTA's items have 16, 32 and 48 columns in turn; the results repeat."""
+    """A CTA's items have 16, 32 and 48 columns in turn, with 5 CTAs whole rows
+    (bf16 outputs) and split ones (fp32 partials); the results repeat."""
     rng = np.random.default_rng(33)
     q_lens = rng.choice([1, 4, 6, 8, 10, 12], 40).tolist() + [9, 5, 2]
     lay = _custom_layout(q_lens, rng.integers(12, 500, 40).tolist() + [6000, 5000, 4000], hq=8, hkv=2, seed=33)
