@@ -448,6 +448,7 @@ class AspireTreeAcceptArgs(ctypes.Structure):
         ("block_table_stride", ctypes.c_int64),
         ("block_table_cols", ctypes.c_int32),
         ("status", ctypes.c_void_p),
+        ("kv_len", ctypes.c_void_p),
     ]
 
 

@@ -247,6 +247,7 @@ int tree_accept(const AspireTreeAcceptArgs* a, void* stream) {
   p.token_bytes = a->token_bytes;
   p.num_caches = a->num_caches;
   p.status = a->status;
+  p.kv_len = a->kv_len;
   // About four CTAs an SM: fewer walk a row's tree more seldom, more have more reads under way.
   int sms = 0;
   const int rc = current_sm_count(&sms);

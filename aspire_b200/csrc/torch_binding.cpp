@@ -694,7 +694,7 @@ struct Walked {
 
 Walked tree_accept(const Tensor& tokens, const Tensor& parents, const Tensor& targets, const Tensor& indptr,
                    const Tensor& lengths, int64_t max_path, const std::vector<const Tensor*>& caches,
-                   const Tensor* table, const Tensor* status) {
+                   const Tensor* table, const Tensor* status, const Tensor* kv_len) {
   require(tokens.is_cuda() && tokens.dim() == 1, "tokens must be a 1-D CUDA tensor");
   require(max_path >= 1 && max_path <= ASPIRE_MAX_PATH, "max_path must be between 1 and 64");
   const int64_t total = tokens.size(0), rows = lengths.numel();
@@ -705,6 +705,7 @@ Walked tree_accept(const Tensor& tokens, const Tensor& parents, const Tensor& ta
   a.targets = ints(&targets, total, tokens, "targets");
   a.lengths = ints(&lengths, rows, tokens, "lengths");
   a.indptr = ints(&indptr, rows + 1, tokens, "indptr");
+  a.kv_len = ints(kv_len, rows, tokens, "kv_len");
   a.total = total;
   a.rows = int32_t(rows);
   a.max_path = int32_t(max_path);
@@ -731,7 +732,8 @@ Walked tree_accept(const Tensor& tokens, const Tensor& parents, const Tensor& ta
     std::sort(starts.begin(), starts.end());
     for (size_t i = 1; i < starts.size(); ++i)
       require(bytes == 0 || starts[i] - starts[i - 1] >= bytes, "a cache is given twice, or two of them overlap");
-    for (const Tensor* t : {&tokens, &parents, &targets, &indptr, &lengths, table}) {
+    for (const Tensor* t : {&tokens, &parents, &targets, &indptr, &lengths, table, kv_len}) {
+      if (!t) continue;
       const auto s = span_of(*t);
       const auto next = std::upper_bound(starts.begin(), starts.end(), s.first);
       require(s.first == s.second || bytes == 0 ||
@@ -977,15 +979,16 @@ PyObject* py_adjust_logits(PyObject*, PyObject* const* v, Py_ssize_t n) {
     return wrap_all(r.first, r.second);
   });
 }
-// (tokens, parents, targets, indptr, lengths, max_path, caches, block_table, status) -> count, path, tokens, lengths
+// (tokens, parents, targets, indptr, lengths, max_path, caches, block_table, status, kv_len) -> count, path, tokens,
+// lengths
 PyObject* py_tree_accept(PyObject*, PyObject* const* v, Py_ssize_t n) {
-  return guarded(n, 9, [&]() -> PyObject* {
+  return guarded(n, 10, [&]() -> PyObject* {
     require(PyList_Check(v[6]) || PyTuple_Check(v[6]), "caches must be a list or tuple of tensors");
     std::vector<const Tensor*> caches;
     for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(v[6]); ++i)
       caches.push_back(&tensor(PySequence_Fast_GET_ITEM(v[6], i)));
     const Walked w = tree_accept(tensor(v[0]), tensor(v[1]), tensor(v[2]), tensor(v[3]), tensor(v[4]), integer(v[5]),
-                                 caches, optional(v[7]), optional(v[8]));
+                                 caches, optional(v[7]), optional(v[8]), optional(v[9]));
     return wrap_all(w.count, w.path, w.tokens, w.lengths);
   });
 }

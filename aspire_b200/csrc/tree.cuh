@@ -113,6 +113,7 @@ struct AcceptParams {
   int64_t token_bytes;     // bytes of one token's K (or V) of all heads, a multiple of 16
   int32_t num_caches;
   uint32_t* status;
+  const int32_t* kv_len;   // [rows] or NULL
   char* caches[kAcceptCaches];
 };
 constexpr int kAcceptThreads = 256;

@@ -8,6 +8,10 @@
 //   then the target's next token), length + count committed tokens;
 //   cache place length + node_d  ->  length + d  (K and V, all heads).
 //
+// Given the step's key counts (kv_len), the walk keeps to nodes whose keys the
+// cache holds: those at places below kv_len, none of a row that got no pages,
+// up to the first whose place has no page.
+//
 // A CTA serves one row and some of the layers.  Its tree is read to shared
 // memory at once and walked there by the first warp; every CTA of the row walks
 // alike, which costs less than a second launch.  Then each thread moves the
@@ -77,7 +81,8 @@ __global__ void __launch_bounds__(kAcceptThreads) aspire_tree_accept_kernel(cons
     bad = ASPIRE_STATUS_BAD_ROW;
     hi = lo = 0;
   }
-  const int n = int(hi - lo);
+  int n = int(hi - lo);
+  if (p.kv_len) n = int(min(int64_t(n), max(int64_t(p.kv_len[b]) - length, int64_t(0))));
   const bool held = n <= kTree;
   if (held)
     for (int i = tid; i < n; i += kAcceptThreads) {
@@ -91,19 +96,21 @@ __global__ void __launch_bounds__(kAcceptThreads) aspire_tree_accept_kernel(cons
     const int count = walk(held ? tokens : p.tokens + lo, held ? parents : p.parents + lo, want, n, p.max_path, lane, path);
     __syncwarp();
     // The moves: nodes that lie behind their places, all of a path's from the first such on.
-    int first = count;
+    int first = count, kept = count;
     for (int d = lane; d < count; d += 32) {
       if (path[d] != d) first = min(first, d);
-      if (p.num_caches > 0 && path[d] != d) {
+      if (p.num_caches > 0 && (path[d] != d || p.kv_len)) {
         from[d] = place_offset(p, b, length + path[d], bad);
         to[d] = place_offset(p, b, length + d, bad);
         if (from[d] < 0) to[d] = -1;
+        if (p.kv_len && to[d] < 0) kept = min(kept, d);
       }
     }
     first = __reduce_min_sync(0xffffffffu, first);
+    kept = __reduce_min_sync(0xffffffffu, kept);
     if (lane == 0) {
-      walked = count;
-      moves = first;
+      walked = kept;
+      moves = min(first, kept);
     }
   }
   __syncthreads();

@@ -859,6 +859,9 @@ typedef struct AspireTreeAcceptArgs {
   int64_t block_table_stride;
   int32_t block_table_cols;
   uint32_t* status;          /* optional device status word                       */
+  const int32_t* kv_len;     /* int32 [rows]: the step's keys of each row, as
+                                aspire_step_tables gives them; NULL: all nodes
+                                are taken to be in the cache                      */
 } AspireTreeAcceptArgs;
 
 /*
@@ -866,6 +869,9 @@ typedef struct AspireTreeAcceptArgs {
  * child whose token is targets[node]) and moves the walked nodes' keys and
  * values from places lengths[b] + node to lengths[b] + 0, 1, 2, ... in every
  * cache.  A place whose page is missing is not moved (ASPIRE_STATUS_BAD_PAGE).
+ * With kv_len only nodes whose keys are in the cache are walked: those at places
+ * below kv_len[b] (0 where aspire_step_tables found no pages, so that such a row
+ * commits nothing) and, given caches, none from the first without a page on.
  */
 ASPIRE_API int aspire_tree_accept(const AspireTreeAcceptArgs* args, void* stream);
 

@@ -105,6 +105,32 @@ def test_places_without_a_page_are_not_moved(cuda_device):
     assert int(status) == 5
 
 
+def test_only_nodes_with_keys_in_the_cache_are_walked(cuda_device):
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)  # noqa: E731
+    status = i32([0])
+    cache = torch.randn(6, 2, 16, 1, 128, device=cuda_device).to(torch.bfloat16)
+    before = cache.clone()
+    # Rows 0 and 1: no page at their second node's place (no page of the cache; behind the table).  Row 2 got no
+    # pages, row 3 has all that it needs, row 4 is row 3 with a key less.
+    args = (i32([1, 2, 3] * 5), i32([-1, 0, 0] * 5), i32([3, 7, 8] * 5), i32([0, 3, 6, 9, 12, 15]),
+            i32([14, 31, 6, 2, 2]), 4)
+    table = i32([[0, 9], [1, 2], [3, 3], [4, -1], [5, -1]])
+    a = accept_tree(*args, caches=[cache], block_table=table, kv_len=i32([17, 34, 0, 5, 4]), status=status)
+    assert a.count.tolist() == [1, 1, 0, 2, 1]
+    assert a.path.tolist() == [[0, -1, -1, -1]] * 2 + [[-1] * 4, [0, 2, -1, -1], [0, -1, -1, -1]]
+    assert a.tokens.tolist() == [[3, -1, -1, -1]] * 2 + [[-1] * 4, [3, 8, -1, -1], [3, -1, -1, -1]]
+    assert a.lengths.tolist() == [15, 32, 6, 4, 3]
+    before[4, :, 3] = before[4, :, 4]
+    assert torch.equal(cache, before)
+    assert int(status) == 1
+    # The walk alone knows no pages.
+    a = accept_tree(*args, kv_len=i32([17, 34, 0, 5, -3]))
+    assert a.count.tolist() == [2, 2, 0, 2, 0]
+    for bad in (i32([1] * 4), i32([1] * 5).long(), i32([1] * 5).cpu()):
+        with pytest.raises(ValueError, match="kv_len"):
+            accept_tree(*args, kv_len=bad)
+
+
 def test_captured_and_replayed(cuda_device):
     i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)  # noqa: E731
     tokens, parents, targets = i32([1, 2, 3, 4]), i32([-1, 0, 0, 2]), i32([3, 0, 4, 0])

@@ -156,3 +156,87 @@ def test_steps(cuda_device, prompts, seed, captured):
             for place, out in by_place.items():
                 t = start[b] + place
                 assert bool(((out.double().cpu() - exp[t]).abs() <= bound[t]).all()), (l, b, place)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_step_in_which_the_pages_run_out(cuda_device, captured):
+    """The last row's pages are not there at first: it commits nothing, keeps
+    its length and its pages, and is served once another row has left."""
+    dev, prompts, nodes = cuda_device, [20, 30, 13], len(TREE)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    rng = random.Random(9)
+    m = Model(dev, 3, 9)
+    committed = [[rng.randrange(VOCAB) for _ in range(n)] for n in prompts]
+    m.chain(i32([v for c in committed for v in c]), i32(prompts), i32([0] * 3))  # 2, 2 and 1 pages
+    m.count.fill_(2)  # 3, 3 and 2 pages are needed for the trees
+    trees = [[rng.randrange(VOCAB)] + [i % VOCAB for i in range(1, nodes)] for _ in prompts]
+    tokens, parents = i32([v for t in trees for v in t]), i32(TREE * 3)
+    lengths, new, status = i32(prompts), i32([nodes] * 3), i32([0])
+    frequency, history = torch.zeros(3, device=dev), i32([c + [0] * (16 * COLS - len(c)) for c in committed])
+
+    def step():
+        t = build_step_tables(lengths, new, *m.pool, tokens=3 * nodes, parents=parents, max_nodes=nodes, status=status)
+        m.wrapper.plan_device(t.qo_indptr, t.kv_indptr, t.last_page_len, HEADS, KV, 128, 16, trees=True)
+        outs = []
+        for l in range(LAYERS):
+            q = m.keys(l, tokens, t, positions=t.positions)
+            outs.append(m.wrapper.run(q, m.caches[l], tree_mask=t.tree_mask))
+        logits = (torch.cat([o.flatten(1) for o in outs], 1).double() @ m.out).float()
+        targets = pick_tokens(logits, history=history, history_len=lengths, indptr=t.qo_indptr, tokens=tokens,
+                              tree_mask=t.tree_mask, frequency=frequency, status=status)
+        a = accept_tree(tokens, parents, targets, t.qo_indptr, lengths, MOST, caches=m.caches, block_table=m.table,
+                        kv_len=t.kv_len, status=status)
+        build_step_tables(a.lengths, None, *m.pool, tokens=0, status=status)
+        return t, targets, a
+
+    graph = None
+    if captured:
+        new.zero_()
+        step()
+        new.fill_(nodes)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            t, targets, a = step()
+
+    def check(served, bits):
+        nonlocal t, targets, a
+        if captured:
+            graph.replay()
+        else:
+            t, targets, a = step()
+        assert int(status) == bits and m.wrapper.device_status() == 0
+        starts, want = t.qo_indptr.tolist(), targets.tolist()
+        for b in range(3):
+            tree = trees[b][:starts[b + 1] - starts[b]]
+            path = ref.walk(tree, TREE[:len(tree)], want[starts[b]:starts[b + 1]], MOST) if b in served else []
+            assert a.path[b].tolist() == path + [-1] * (MOST - len(path))
+            assert a.lengths[b] == len(committed[b]) + len(path)
+            committed[b] += [tree[j] for j in path]
+        assert m.held.tolist() == [-(-len(c) // 16) for c in committed]
+
+    if not captured:
+        t = targets = a = None
+    first = m.caches[0][m.table[2, 0].long()].clone()
+    check({0, 1}, 16)
+    assert len(committed[2]) == 13 and torch.equal(m.caches[0][m.table[2, 0].long()], first)
+    # Row 0 leaves.
+    status.zero_()
+    committed[0] = []
+    lengths.copy_(i32([0] + [len(c) for c in committed[1:]]))
+    new.copy_(i32([0, 1, nodes]))
+    trees = [trees[0], [rng.randrange(VOCAB)], trees[2]]
+    tokens.copy_(i32(trees[1] + trees[2] + [0] * (2 * nodes - 1)))
+    parents.copy_(i32([-1] + TREE + [-1] * (2 * nodes - 1)))
+    history.copy_(i32([c + [0] * (16 * COLS - len(c)) for c in committed]))
+    check({0, 1, 2}, 0)
+    assert len(committed[2]) > 13
+
+    # The same keys and values as the tokens' own chain, bit for bit.
+    c = Model(dev, 3, 9)
+    c.chain(i32([v for r in committed for v in r]), i32([len(r) for r in committed]), i32([0] * 3))
+    for l in range(LAYERS):
+        for b, r in enumerate(committed):
+            ours, chain = ((x.caches[l][x.table[b, :-(-len(r) // 16)].long()].transpose(1, 2).flatten(0, 1)[:len(r)])
+                           for x in (m, c))
+            assert torch.equal(ours, chain)
