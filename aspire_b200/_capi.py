@@ -29,6 +29,7 @@ STATUS_BAD_PLAN = 2
 STATUS_BAD_ROW = 4
 STATUS_TIMEOUT = 8
 STATUS_NO_PAGES = 16
+STATUS_NO_TOKEN = 32
 PLAN_TREE = 2
 MAX_CACHES = 128
 MAX_PATH = 64

@@ -3,7 +3,8 @@
 //
 //   node_0 = 0;  node_{d+1} = the first child of node_d whose token is
 //   targets[node_d], the target's choice after node_d; the walk ends where no
-//   child has it, or at max_path nodes;
+//   child has it, at max_path nodes, or before a node without a choice
+//   (targets[node] < 0): what is committed are tokens, and -1 is none;
 //   count = nodes walked, tokens_d = targets[node_d] (the accepted drafts,
 //   then the target's next token), length + count committed tokens;
 //   cache place length + node_d  ->  length + d  (K and V, all heads).
@@ -39,17 +40,21 @@ __device__ __forceinline__ int64_t place_offset(const AcceptParams& p, int b, in
   return (int64_t(page) * 2 * p.page_size + pos % p.page_size) * p.token_bytes;
 }
 
-// The walk, by one warp; `path` gets the nodes.
+// The walk, by one warp; `path` gets the nodes.  `dead` is set where it ends before a node without a choice.
 __device__ __forceinline__ int walk(const int32_t* tokens, const int32_t* parents, const int32_t* targets, int n,
-                                    int max_path, int lane, int32_t* path) {
+                                    int max_path, int lane, int32_t* path, bool& dead) {
   int count = 0, node = 0;
   bool more = n > 0;
   while (more) {
+    const int32_t want = targets[node];
+    if (want < 0) {
+      dead = true;
+      break;
+    }
     if (lane == 0) path[count] = node;
     ++count;
     more = false;
     if (count == max_path) break;
-    const int32_t want = targets[node];
     for (int c0 = node + 1; c0 < n; c0 += 32) {  // children come after their parent
       const int c = c0 + lane;
       const uint32_t found = __ballot_sync(0xffffffffu, c < n && parents[c] == node && tokens[c] == want);
@@ -93,7 +98,10 @@ __global__ void __launch_bounds__(kAcceptThreads) aspire_tree_accept_kernel(cons
   __syncthreads();
   const int32_t* want = held ? targets : p.targets + lo;
   if (tid < 32) {
-    const int count = walk(held ? tokens : p.tokens + lo, held ? parents : p.parents + lo, want, n, p.max_path, lane, path);
+    bool dead = false;
+    const int count =
+        walk(held ? tokens : p.tokens + lo, held ? parents : p.parents + lo, want, n, p.max_path, lane, path, dead);
+    if (dead) bad |= ASPIRE_STATUS_NO_TOKEN;
     __syncwarp();
     // The moves: nodes that lie behind their places, all of a path's from the first such on.
     int first = count, kept = count;

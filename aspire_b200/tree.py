@@ -26,7 +26,8 @@ from . import _capi
 
 class Accepted(NamedTuple):
     """``count`` int32 ``[rows]``: nodes on the accepted path, the root
-    included (0 for a row without nodes, or without keys in the cache); ``path`` int32 ``[rows, max_path]``:
+    included (0 for a row without nodes, without keys in the cache, or without
+    a choice after its root); ``path`` int32 ``[rows, max_path]``:
     those nodes; ``tokens`` int32 ``[rows, max_path]``: the tokens committed,
     the target's choice after each of them (the accepted drafts, then one
     more); -1 behind the path.  ``lengths`` int32 ``[rows]``: the lengths plus
@@ -58,6 +59,11 @@ def accept_tree(tokens: torch.Tensor, parents: torch.Tensor, targets: torch.Tens
     :func:`aspire_b200.kv_ops.build_step_tables` gives them: a row that got no
     pages has 0 and commits nothing, its length stays, and a later step may
     serve it.  The walk then also ends before a node whose place has no page.
-    Without ``kv_len`` the keys of all nodes are taken to be in the cache."""
+    Without ``kv_len`` the keys of all nodes are taken to be in the cache.
+
+    A negative target is no token (``pick_tokens`` gives -1 where nothing is
+    allowed) and no draft's: the walk ends before its node, which stays the
+    row's last committed token and so the root of its next tree, and
+    ``status`` gets ``ASPIRE_STATUS_NO_TOKEN``."""
     return Accepted(*_capi.ops().tree_accept(tokens, parents, targets, indptr, lengths, max_path, caches, block_table,
                                              status, kv_len))

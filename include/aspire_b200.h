@@ -71,6 +71,7 @@ extern "C" {
                                       row/argument out of range               */
 #define ASPIRE_STATUS_TIMEOUT 8u   /* a bounded device wait expired; the CTA stopped */
 #define ASPIRE_STATUS_NO_PAGES 16u /* aspire_step_tables: no free pages left for a row */
+#define ASPIRE_STATUS_NO_TOKEN 32u /* aspire_tree_accept: a node on a path has no choice */
 
 /* Logit-dump variants (AspireAttnArgs.dump_kind, AspireSelectArgs.dump_kind),
  * the dump kinds of aspire/backends/jit_kernels.py:180-193: */
@@ -839,7 +840,8 @@ ASPIRE_API int aspire_adjust_logits(const AspireLogitsArgs* args, void* stream);
 typedef struct AspireTreeAcceptArgs {
   const int32_t* tokens;     /* int32 [total] the nodes' tokens                   */
   const int32_t* parents;    /* int32 [total] a node's parent within its row      */
-  const int32_t* targets;    /* int32 [total] the target's choice after each node */
+  const int32_t* targets;    /* int32 [total] the target's choice after each node,
+                                negative for none (as aspire_adjust_logits' ids)  */
   const int32_t* indptr;     /* int32 [rows + 1]                                  */
   const int32_t* lengths;    /* int32 [rows] committed tokens before the step     */
   int64_t total;
@@ -872,6 +874,10 @@ typedef struct AspireTreeAcceptArgs {
  * With kv_len only nodes whose keys are in the cache are walked: those at places
  * below kv_len[b] (0 where aspire_step_tables found no pages, so that such a row
  * commits nothing) and, given caches, none from the first without a page on.
+ * The walk ends before a node without a choice (ASPIRE_STATUS_NO_TOKEN): each
+ * node of the path commits the token after it, so such a node stays the row's
+ * last committed token, whose keys are not in the cache; at node 0 the row
+ * commits nothing.
  */
 ASPIRE_API int aspire_tree_accept(const AspireTreeAcceptArgs* args, void* stream);
 

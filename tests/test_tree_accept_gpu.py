@@ -131,6 +131,29 @@ def test_only_nodes_with_keys_in_the_cache_are_walked(cuda_device):
             accept_tree(*args, kv_len=bad)
 
 
+def test_a_node_without_a_choice_is_not_committed(cuda_device):
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)  # noqa: E731
+    # Drafts of -1 are padding: 0 -> 2 -> 3 -> 4 in each row, without a choice after node 0, 2 and 4, and with all.
+    tokens, parents = [1, -1, 5, 6, -1], [-1, 0, 0, 2, 3]
+    targets = [[-1, 0, 6, -7, 9], [5, 0, -1, 9, 9], [5, 0, 6, -(2 ** 31), 9], [5, 0, 6, 9, -1]]
+    cache = torch.randn(4, 2, 16, 1, 128, device=cuda_device).to(torch.bfloat16)
+    want = cache.clone()
+    for b, moved in enumerate([[], [], [2], [2, 3]]):
+        for d, node in enumerate(moved):
+            want[b, :, 3 + d + 1] = cache[b, :, 3 + node]
+    status = i32([0])
+    a = accept_tree(i32(tokens * 4), i32(parents * 4), i32([v for r in targets for v in r]), i32([0, 5, 10, 15, 20]),
+                    i32([3] * 4), 5, caches=[cache], block_table=i32([[0], [1], [2], [3]]), status=status)
+    assert a.path.tolist() == [[-1] * 5, [0] + [-1] * 4, [0, 2, -1, -1, -1], [0, 2, 3, -1, -1]]
+    assert a.tokens.tolist() == [[-1] * 5, [5] + [-1] * 4, [5, 6, -1, -1, -1], [5, 6, 9, -1, -1]]
+    assert a.count.tolist() == [0, 1, 2, 3] and a.lengths.tolist() == [3, 4, 5, 6]
+    assert torch.equal(cache, want)
+    assert int(status) == 32
+    # The path's end comes first.
+    a = accept_tree(i32(tokens), i32(parents), i32(targets[2]), i32([0, 5]), i32([3]), 2, status=status.zero_())
+    assert a.path[0].tolist() == [0, 2] and int(status) == 0
+
+
 def test_captured_and_replayed(cuda_device):
     i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda_device)  # noqa: E731
     tokens, parents, targets = i32([1, 2, 3, 4]), i32([-1, 0, 0, 2]), i32([3, 0, 4, 0])
