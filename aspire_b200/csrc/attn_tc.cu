@@ -398,6 +398,12 @@ __device__ __noinline__ void dump_columns(const AttnParams& p, int lo, int hi, i
 // column's running statistics (reference max, sum, rescale factor) live with
 // its owner, so the two groups never wait for each other; they meet only on
 // the S / P / O barriers shared with the MMA warp.
+// Bits [lo, hi) of a word, 0 <= lo < hi <= 32, without a shift by 32, which the language leaves undefined.
+__host__ __device__ constexpr uint32_t bits_between(int lo, int hi) {
+  return (0xffffffffu >> (32 - hi)) & (0xffffffffu << lo);
+}
+static_assert(bits_between(0, 32) == 0xffffffffu && bits_between(28, 32) == 0xf0000000u && bits_between(0, 1) == 1u, "");
+
 // Which of the columns [c0, c0 + NH) see the item's key `tok` under the tree
 // mask, bit j for column c0 + j: all of them a key before the row's nodes, else
 // the columns of the queries whose mask names the node.
@@ -412,7 +418,7 @@ __device__ __forceinline__ uint32_t tree_columns(const AttnParams& p, const Work
   for (int c = c0; c < end; ++q) {
     const int next = min(end, (q + 1) * p.group - it.pq_begin);
     if ((tree_word(p, int64_t(it.q_start) + q, node >> 5) >> (node & 31)) & 1)
-      seen |= ((1u << (next - c0)) - 1u) & ~((1u << (c - c0)) - 1u);
+      seen |= bits_between(c - c0, next - c0);
     c = next;
   }
   return seen;
