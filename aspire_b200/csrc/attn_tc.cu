@@ -581,7 +581,9 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
         const float mo = t > 0 ? sm.mref[cur][c] : -INFINITY;
         const float tmax = fmaxf(fmaxf(sm.red[t & 1][0][c], sm.red[t & 1][1][c]),
                                  fmaxf(sm.red[t & 1][2][c], sm.red[t & 1][3][c]));
-        const float mn = fmaxf(mo, tmax * scale);
+        // (Tree: columns behind the item's rows hold other rows' queries.  No logit
+        // exceeds a reference of +inf, so those decide nothing, and their P is 0.)
+        const float mn = kTree && c0 + ctid >= nrows ? INFINITY : fmaxf(mo, tmax * scale);
         sm.mref[cur ^ 1][c] = mn;
         sm.alpha[t & 1][c] = (mo == -INFINITY) ? 0.f : (mn == mo ? 1.f : ex2(mo - mn));
         if (mn != mo && mo != -INFINITY) grew[t & 1] = 1;

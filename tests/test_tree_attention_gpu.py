@@ -407,6 +407,23 @@ def test_results_repeat_bit_by_bit(cuda_device):
         assert torch.equal(o, out) and torch.equal(l, lse)
 
 
+@pytest.mark.parametrize("heads,kv_heads,nodes", [(4, 1, 5), (8, 2, 13), (5, 1, 7), (2, 1, 5)])
+def test_neighbours_queries_leave_no_trace(cuda_device, heads, kv_heads, nodes):
+    """The columns behind an item's rows hold the next row's queries, which must
+    not decide when its own references move: small, large or not finite, the
+    row's outputs keep their bits."""
+    c = Case(cuda_device, [(1500, nodes), (700, nodes)], heads, kv_heads, seed=22, scale=4.0)
+    w, kv = c.plan(trees=True), c.cache.to(cuda_device)
+    runs = []
+    for scale in (0.0, 1.0, 30.0, math.inf):
+        q = c.q.to(cuda_device)
+        q[nodes:] *= scale  # (inf and NaN in the last)
+        runs.append(w.run(q, kv, tree_mask=c.mask, return_lse=True))
+    c.check(*runs[1])
+    for out, lse in runs:
+        assert torch.equal(out[:nodes], runs[0][0][:nodes]) and torch.equal(lse[:nodes], runs[0][1][:nodes])
+
+
 def test_refusals(cuda_device):
     c = Case(cuda_device, [(50, 40)], 4, 1, seed=13)
     q, kv = c.q.to(cuda_device), c.cache.to(cuda_device)
