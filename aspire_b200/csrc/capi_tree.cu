@@ -87,10 +87,16 @@ bool has_marks(const AspireLogitsArgs* a) {
 
 int32_t blocks_of(int32_t vocab) { return int32_t((int64_t(vocab) + kLogitsBlock - 1) / kLogitsBlock); }
 
-// Entries of the marking CTAs' lists.
-size_t list_entries(const AspireLogitsArgs* a, int ranks) {
-  return size_t(ranks) * (size_t(a->rows) * size_t(a->history ? a->history_cols : 0) + size_t(a->tokens) +
-                          size_t(a->bias_indptr ? a->bias_entries : 0));
+// Entries of the marking CTAs' lists.  One lists no more than its row's history,
+// tokens and biases, and no more than its own part of the vocabulary: the lists
+// lie as the former or, `list_stride` apart, as the latter, whichever is less.
+size_t list_entries(const AspireLogitsArgs* a, LogitsParams* p) {
+  const size_t ranks = size_t(p->mark_ranks);
+  const size_t given = ranks * (size_t(a->rows) * size_t(a->history ? a->history_cols : 0) + size_t(a->tokens) +
+                                size_t(a->bias_indptr ? a->bias_entries : 0));
+  const size_t share = size_t(p->mark_blocks) * kLogitsBlock, parts = ranks * size_t(a->rows) * share;
+  p->list_stride = parts < given ? int32_t(share) : 0;
+  return std::min(given, parts);
 }
 
 // The workspace's parts, from `base` on; returns their bytes.
@@ -114,7 +120,7 @@ size_t lay_out(const AspireLogitsArgs* a, char* base, int sms, LogitsParams* p) 
   }
   if (has_marks(a)) {
     const size_t blocks = size_t(a->rows) * size_t(all);
-    const size_t entries = list_entries(a, p->mark_ranks);
+    const size_t entries = list_entries(a, p);
     p->table = reinterpret_cast<int2*>(part(blocks * (kLogitsBlock / kLogitsUnit) * 8));
     p->touched = reinterpret_cast<uint32_t*>(part(blocks * kLogitsBlock / 8));
     p->list = reinterpret_cast<int2*>(part(entries * 8));
@@ -158,7 +164,7 @@ int adjust_logits(const AspireLogitsArgs* a, void* stream) {
   if (rc) return rc;
   LogitsParams p = {};
   const size_t wanted = lay_out(a, static_cast<char*>(a->workspace), sms, &p);
-  if (p.list && list_entries(a, p.mark_ranks) > size_t(INT32_MAX))
+  if (p.list && list_entries(a, &p) > size_t(INT32_MAX))
     return invalid(who, "histories, tokens and biases past 2^31 entries together");
   if (wanted > 0 && (!a->workspace || a->workspace_bytes < wanted || (reinterpret_cast<uintptr_t>(a->workspace) & 15)))
     return set_error(ASPIRE_ERR_CAPACITY, std::string(who) + ": workspace missing, too small or not 16-byte aligned");

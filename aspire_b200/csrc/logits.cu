@@ -78,8 +78,10 @@ __device__ __forceinline__ RowSpan row_span(const LogitsParams& p, int b) {
   }
   return s;
 }
-// Where a marking CTA's list starts: each has room for the row's whole history, tokens and biases.
+// Where a marking CTA's list starts: each has room for the row's whole history,
+// tokens and biases, or for its part of the vocabulary.
 __device__ __forceinline__ int64_t list_base(const LogitsParams& p, int b, int rank, int ranks, const RowSpan& s) {
+  if (p.list_stride) return (int64_t(b) * ranks + rank) * p.list_stride;
   return ranks * (int64_t(b) * p.history_cols + s.lo + s.from) +
          rank * (p.history_cols + (s.hi - s.lo) + (s.to - s.from));
 }

@@ -65,7 +65,7 @@ struct LogitsParams {
   const int32_t* allowed;     // [tokens, allowed_stride] words or NULL
   int64_t allowed_stride;
   int32_t* ids;               // [tokens]: the best tokens, or NULL: adjusted logits to out
-  // Workspace.  The marking CTAs' lists lie one after another (list_base).
+  // Workspace.  Where the marking CTAs' lists lie: list_base.
   unsigned long long* keys;   // [tokens], with ids
   uint32_t* arrived;          // [tokens], with ids: slices done
   int2* list;                 // touched ids with their counts and flags; NULL: nothing touches the logits
@@ -74,6 +74,7 @@ struct LogitsParams {
   uint32_t* touched;          // [rows, blocks, kLogitsBlock / 32] bitmap
   int32_t mark_ranks;         // CTAs that mark a row
   int32_t mark_blocks;        // blocks of each
+  int32_t list_stride;        // entries from a marking CTA's list to the next, or 0: as many as its row can touch
   uint32_t* status;
 };
 constexpr int kLogitsBlock = 4096;  // vocabulary entries, the steps of a marking CTA's share

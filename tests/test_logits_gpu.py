@@ -8,6 +8,7 @@ import random
 import pytest
 import torch
 
+from aspire_b200 import _capi
 from aspire_b200.logits import adjust_logits, pick_tokens
 import tree_reference as ref
 
@@ -257,3 +258,39 @@ def test_many_tokens_of_large_vocabularies(cuda_device, dtype, vocab):
     # (Of equal values the lowest id: the rounded logits cannot tell which the larger one was.)
     top = whole.float().max(1).values
     assert bool((whole.float().gather(1, ids.long()[:, None])[:, 0] == top).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes,vocab", [([3, 0, 2], 1000), ([40, 7, 1], 9001), ([2, 5], 60000)])
+def test_long_buffers_of_short_histories(cuda_device, sizes, vocab, dtype):
+    """The marks' lists lie by the vocabulary's parts where those are less than the rows' buffers."""
+    c = Case(vocab + 1, sizes, vocab, dtype, hist=200, bias=30, allowed=True, pad=1)
+    kw, x = c.args(cuda_device), c.logits.to(cuda_device)
+    want = adjust_logits(x, **kw), pick_tokens(x, **kw)
+    for cols in (5000, 70000):
+        longer = torch.randint(0, vocab, (len(sizes), cols), dtype=torch.int32, device=cuda_device)
+        longer[:, :kw["history"].shape[1]] = kw["history"]
+        for b, h in enumerate(c.history):
+            longer[b, :len(h)] = torch.tensor(h, dtype=torch.int32, device=cuda_device)
+        kw["history"] = longer
+        assert torch.equal(adjust_logits(x, **kw), want[0]) and torch.equal(pick_tokens(x, **kw), want[1])
+
+
+def test_lists_are_bounded_by_the_vocabulary(cuda_device):
+    """4096 rows of 2^19 history columns: 2^31 places, of which 4096 rows of 5000 entries can be touched."""
+    rows, cols, vocab = 4096, 2 ** 19, 5000
+    g = torch.Generator(device=cuda_device).manual_seed(2)
+    one = torch.randint(0, vocab, (1, cols), generator=g, device=cuda_device, dtype=torch.int32)
+    length = torch.tensor([0, 1, 17, 1000], device=cuda_device, dtype=torch.int32).repeat(rows // 4)
+    length[0] = cols
+    y = adjust_logits(torch.zeros(rows, vocab, device=cuda_device), history=one.expand(rows, cols), history_len=length,
+                      frequency=torch.ones(rows, device=cuda_device))
+    for b in (0, 1, 2, 3, rows - 2, rows - 1):
+        counts = torch.bincount(one[0, :int(length[b])].long(), minlength=vocab)
+        assert torch.equal(y[b], -counts.float())
+    assert torch.equal(y[4:8].repeat(rows // 4 - 1, 1), y[4:])
+    # The workspace of 64 rows: what 151936 entries a row can fill, not what 131072 columns a marking CTA could.
+    a = _capi.AspireLogitsArgs()
+    a.logits, a.type, a.tokens, a.rows, a.vocab, a.logits_stride, a.out, a.out_stride = 256, 0, 64, 64, 151936, 151936, 256, 151936
+    a.history, a.history_len, a.history_cols, a.history_stride, a.frequency = 256, 256, 131072, 131072, 256
+    assert 64 * 151936 * 8 <= _capi.load_library().aspire_logits_workspace(a) <= 1.1 * 64 * 151936 * 8
