@@ -482,6 +482,39 @@ bool in_common(const Tensor& a, const Tensor& b) {
   return x.first < y.second && y.first < x.second;
 }
 
+// Whether two [tokens, heads, dim] tensors with contiguous dims have a byte in
+// common.  Vectors of one buffer may lie between one another's (the parts of a
+// fused projection): by rows first, vector by vector only where rows cross.
+bool share_vectors(const Tensor& a, const Tensor& b) {
+  if (!in_common(a, b)) return false;
+  const auto rows_of = [](const Tensor& t) {
+    const int64_t size = t.element_size();
+    return Block{reinterpret_cast<uintptr_t>(t.data_ptr()), t.size(0), ((t.size(1) - 1) * t.stride(1) + t.size(2)) * size,
+                 t.stride(0) * size};
+  };
+  if (!share(rows_of(a), rows_of(b))) return false;
+  const auto vectors_of = [](const Tensor& t) {
+    std::vector<uintptr_t> at;
+    at.reserve(size_t(t.size(0) * t.size(1)));
+    for (int64_t n = 0; n < t.size(0); ++n)
+      for (int64_t h = 0; h < t.size(1); ++h)
+        at.push_back(reinterpret_cast<uintptr_t>(t.data_ptr()) + uintptr_t((n * t.stride(0) + h * t.stride(1)) * t.element_size()));
+    std::sort(at.begin(), at.end());
+    return at;
+  };
+  const std::vector<uintptr_t> x = vectors_of(a), y = vectors_of(b);
+  const uintptr_t xb = uintptr_t(a.size(2) * a.element_size()), yb = uintptr_t(b.size(2) * b.element_size());
+  for (size_t i = 0, j = 0; i < x.size() && j < y.size();) {
+    if (x[i] + xb <= y[j])
+      ++i;
+    else if (y[j] + yb <= x[i])
+      ++j;
+    else
+      return true;
+  }
+  return false;
+}
+
 // Tensors of one type in one allocation, each 16-byte aligned: a step has many
 // small tables, and an allocation is most of what a small tensor costs.
 class Pieces {
@@ -796,7 +829,8 @@ std::pair<Tensor, Tensor> tree_attention(const Tensor& q, const Tensor& cache, c
     require(out.scalar_type() == q.scalar_type() && out.sizes() == q.sizes() && out.stride(2) == 1 &&
                 out.device() == q.device(),
             "out must match q's shape and type with a contiguous head_dim on its device");
-    out.unsafeGetTensorImpl()->bump_version();
+    require(!(at::GradMode::is_enabled() && out.requires_grad()),
+            "out requires a gradient: give another, or use torch.no_grad()");
   } else {
     out = at::empty(q.sizes(), q.options().requires_grad(false));
   }
@@ -805,15 +839,23 @@ std::pair<Tensor, Tensor> tree_attention(const Tensor& q, const Tensor& cache, c
     require(lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.dim() == 2 && lse.size(0) == q.size(0) &&
                 lse.size(1) == q.size(1) && lse.device() == q.device(),
             "lse must be a contiguous fp32 [tokens, num_qo_heads] tensor");
-    lse.unsafeGetTensorImpl()->bump_version();
+    require(!(at::GradMode::is_enabled() && lse.requires_grad()),
+            "lse requires a gradient: give another, or use torch.no_grad()");
   } else if (want_lse) {
     lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat).requires_grad(false));
   }
-  if (out_given)
+  if (out_given) {
     require(!in_common(out, cache) && !in_common(out, mask), "out must not overlap the cache or the mask");
+    // (An item reads its queries before it writes their rows, and no other item reads them.)
+    const bool same = out.data_ptr() == q.data_ptr() && (q.size(0) <= 1 || out.stride(0) == q.stride(0)) &&
+                      (q.size(1) <= 1 || out.stride(1) == q.stride(1));
+    require(same || !share_vectors(out, q), "out may be q itself, but must not overlap it otherwise");
+  }
   if (lse_given)
     require(!in_common(lse, cache) && !in_common(lse, mask) && !in_common(lse, q) && !in_common(lse, out),
             "lse must not overlap the other operands");
+  if (out_given) out.unsafeGetTensorImpl()->bump_version();
+  if (lse_given) lse.unsafeGetTensorImpl()->bump_version();
   AspireAttnArgs a = fixed;
   a.q = q.data_ptr();
   a.q_stride_n = q.stride(0);

@@ -407,6 +407,32 @@ def test_results_repeat_bit_by_bit(cuda_device):
         assert torch.equal(o, out) and torch.equal(l, lse)
 
 
+def test_outputs_that_overlap_the_queries(cuda_device):
+    c = Case(cuda_device, [(300, 5), (40, 20)], 4, 2, seed=23)
+    w, kv, n = c.plan(trees=True), c.cache.to(cuda_device), c.starts[-1]
+    buf = torch.zeros(n + 1, 12, 128, dtype=torch.bfloat16, device=cuda_device)
+    flat = torch.zeros(2 * n * 4 * 128, dtype=torch.bfloat16, device=cuda_device)
+    for q, out in [(buf[:-1, :4], buf[1:, :4]), (buf[:-1, :4], buf[:-1, 3:7]), (buf[:-1, :4], buf[:-1, :8:2]),
+                   (buf[:-1, :8:2], buf[:-1, 2:10:2]), (buf[:-1, :4], buf.view(-1)[8:8 + 512 * n].view(n, 4, 128))]:
+        before = buf.clone()
+        with pytest.raises(ValueError, match="q itself"):
+            w.run(q, kv, tree_mask=c.mask, out=out)
+        assert torch.equal(buf, before)
+    # Between one another's rows or heads, or itself.
+    want = w.run(c.q.to(cuda_device), kv, tree_mask=c.mask)
+    for q, out in [(buf[:-1, :4], buf[:-1, 4:8]), (buf[:-1, :8:2], buf[:-1, 1:8:2]), (buf[:-1, 2:10:2], buf[:-1, 2:10:2]),
+                   (flat[:n * 512].view(4, n, 128).transpose(0, 1), flat[n * 512:].view(4, n, 128).transpose(0, 1))]:
+        q.copy_(c.q)
+        version = out._version
+        assert torch.equal(w.run(q, kv, tree_mask=c.mask, out=out), want) and out._version > version
+    for kw in (dict(out=torch.zeros_like(want, requires_grad=True)),
+               dict(lse=torch.zeros(n, 4, device=cuda_device, requires_grad=True))):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            w.run(c.q.to(cuda_device), kv, tree_mask=c.mask, **kw)
+        with torch.no_grad():
+            w.run(c.q.to(cuda_device), kv, tree_mask=c.mask, **kw)
+
+
 @pytest.mark.parametrize("heads,kv_heads,nodes", [(4, 1, 5), (8, 2, 13), (5, 1, 7), (2, 1, 5)])
 def test_neighbours_queries_leave_no_trace(cuda_device, heads, kv_heads, nodes):
     """The columns behind an item's rows hold the next row's queries, which must
