@@ -378,10 +378,9 @@ class HolisticAttentionWrapper:
                 raise ValueError("a dump variant takes no tree_mask")
             if not self._plan_trees:
                 self._plan_again(_capi.PLAN_TREE)
-            if append is None:
-                return self._run_trees(q, _unpack_paged_kv_cache(paged_kv_cache, self._kv_layout), tree_mask, out,
-                                       lse, return_lse)
-        elif self._plan_trees and not self._plan_again(0):
+            return self._run_trees(q, _unpack_paged_kv_cache(paged_kv_cache, self._kv_layout), tree_mask, out, lse,
+                                   return_lse, append)
+        if self._plan_trees and not self._plan_again(0):
             raise ValueError("the plan was made for trees: give a tree_mask")
         kv = _unpack_paged_kv_cache(paged_kv_cache, self._kv_layout)
         if q.dtype != torch.bfloat16 or kv.dtype != torch.bfloat16:
@@ -435,10 +434,6 @@ class HolisticAttentionWrapper:
                                            or dump_flags.numel() < self._plan_rows):
                 raise ValueError("mode_flags must be a contiguous int32 tensor with one entry per row")
 
-        if tree_mask is not None:
-            if tree_mask.dtype != torch.int32 or tree_mask.dim() != 2 or not tree_mask.is_contiguous() or \
-                    tree_mask.device != q.device or tree_mask.shape[0] < q.shape[0] or tree_mask.shape[1] < 1:
-                raise ValueError("tree_mask must be a contiguous int32 [tokens, words] tensor on q's device")
         sm_scale = self._sm_scale if self._sm_scale is not None else 1.0 / math.sqrt(q.shape[2])
         a = _capi.AspireAttnArgs()
         a.q = q.data_ptr()
@@ -489,20 +484,14 @@ class HolisticAttentionWrapper:
         a.float_ws = self._float_workspace.data_ptr()
         a.float_ws_bytes = self._float_workspace.numel()
         stream = torch.cuda.current_stream(q.device).cuda_stream
-        if tree_mask is not None:
-            rc = self._lib.aspire_tree_attention(ctypes.byref(a), ctypes.c_void_p(tree_mask.data_ptr()),
-                                                 tree_mask.shape[1], ctypes.byref(self._plan_info),
-                                                 ctypes.c_void_p(stream))
-            _capi.check(rc, "aspire_tree_attention")
-        else:
-            rc = self._lib.aspire_mixed_attention(ctypes.byref(a), ctypes.byref(self._plan_info),
-                                                  ctypes.c_void_p(stream))
-            _capi.check(rc, "aspire_mixed_attention")
+        rc = self._lib.aspire_mixed_attention(ctypes.byref(a), ctypes.byref(self._plan_info),
+                                              ctypes.c_void_p(stream))
+        _capi.check(rc, "aspire_mixed_attention")
         if return_lse:
             return out, lse
         return out
 
-    def _run_trees(self, q, kv, tree_mask, out, lse, return_lse):
+    def _run_trees(self, q, kv, tree_mask, out, lse, return_lse, append):
         """``run`` with a tree mask, its checks and its call compiled."""
         a = self._tree_args
         if a is None:
@@ -525,8 +514,9 @@ class HolisticAttentionWrapper:
             self._tree_addresses = ctypes.addressof(a), ctypes.addressof(self._plan_info)
         if q.device != self._device:
             raise ValueError("q must be on the wrapper's device")
+        k_new, v_new = append if append is not None else (None, None)
         out, lse = _capi.ops().tree_attention(q, kv, tree_mask, out, lse, bool(return_lse), *self._tree_addresses,
-                                              self._plan_q_total)
+                                              self._plan_q_total, k_new, v_new)
         return (out, lse) if return_lse else out
 
     # ------------------------------------------------------------- diagnostics

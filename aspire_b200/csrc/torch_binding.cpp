@@ -808,7 +808,8 @@ Walked tree_accept(const Tensor& tokens, const Tensor& parents, const Tensor& ta
 // `fixed` holds what a plan's calls share (heads, pages, workspaces, scale); q_total the query rows it addresses.
 std::pair<Tensor, Tensor> tree_attention(const Tensor& q, const Tensor& cache, const Tensor& mask,
                                          const Tensor* out_given, const Tensor* lse_given, bool want_lse,
-                                         const AspireAttnArgs& fixed, const AspirePlanInfo& plan, int64_t q_total) {
+                                         const AspireAttnArgs& fixed, const AspirePlanInfo& plan, int64_t q_total,
+                                         const Tensor* k_new, const Tensor* v_new) {
   require(q.scalar_type() == at::kBFloat16 && cache.scalar_type() == at::kBFloat16, "q and paged_kv_cache must be bfloat16");
   require(cache.dim() == 5 && cache.size(1) == 2 && cache.is_contiguous() && cache.device() == q.device(),
           "paged_kv_cache must be a contiguous [pages, 2, page_size, num_kv_heads, head_dim] tensor on q's device");
@@ -823,6 +824,20 @@ std::pair<Tensor, Tensor> tree_attention(const Tensor& q, const Tensor& cache, c
   require(mask.scalar_type() == at::kInt && mask.dim() == 2 && mask.is_contiguous() && mask.device() == q.device() &&
               mask.size(0) >= q.size(0) && mask.size(1) >= 1 && mask.size(1) <= INT32_MAX,
           "tree_mask must be a contiguous int32 [tokens, words] tensor on q's device");
+  require(!k_new == !v_new, "append needs both the new keys and the new values");
+  for (const Tensor* t : {k_new, v_new}) {
+    if (!t) continue;
+    const std::string name = t == k_new ? "k_new" : "v_new";
+    if (t->scalar_type() != at::kBFloat16 || t->dim() != 3 || t->stride(2) != 1 || t->device() != q.device())
+      throw Invalid(name + " must be a bf16 [tokens, num_kv_heads, 128] tensor on q's device");
+    if (t->size(1) != cache.size(3) || t->size(2) != q.size(2) || t->size(0) < q.size(0))
+      throw Invalid(name + "'s shape does not match the plan");
+    require(!at::GradMode::is_enabled() || !t->requires_grad(),
+            "the attention has no gradient: detach the operands or call under torch.no_grad()");
+    // (The append writes the cache.)
+    require(!in_common(*t, cache) && !in_common(q, cache) && !in_common(mask, cache),
+            "the cache must not overlap what the call reads");
+  }
   Tensor out, lse;
   if (out_given) {
     out = *out_given;
@@ -850,10 +865,15 @@ std::pair<Tensor, Tensor> tree_attention(const Tensor& q, const Tensor& cache, c
     const bool same = out.data_ptr() == q.data_ptr() && (q.size(0) <= 1 || out.stride(0) == q.stride(0)) &&
                       (q.size(1) <= 1 || out.stride(1) == q.stride(1));
     require(same || !share_vectors(out, q), "out may be q itself, but must not overlap it otherwise");
+    for (const Tensor* t : {k_new, v_new})
+      require(!t || !share_vectors(out, *t), "out must not overlap the new keys and values");
   }
-  if (lse_given)
+  if (lse_given) {
     require(!in_common(lse, cache) && !in_common(lse, mask) && !in_common(lse, q) && !in_common(lse, out),
             "lse must not overlap the other operands");
+    for (const Tensor* t : {k_new, v_new}) require(!t || !in_common(lse, *t), "lse must not overlap the other operands");
+  }
+  if (k_new) cache.unsafeGetTensorImpl()->bump_version();
   if (out_given) out.unsafeGetTensorImpl()->bump_version();
   if (lse_given) lse.unsafeGetTensorImpl()->bump_version();
   AspireAttnArgs a = fixed;
@@ -868,6 +888,14 @@ std::pair<Tensor, Tensor> tree_attention(const Tensor& q, const Tensor& cache, c
   a.o_stride_n = out.stride(0);
   a.o_stride_h = out.stride(1);
   a.lse = lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr;
+  if (k_new) {
+    a.k_new = k_new->data_ptr();
+    a.k_new_stride_n = k_new->stride(0);
+    a.k_new_stride_h = k_new->stride(1);
+    a.v_new = v_new->data_ptr();
+    a.v_new_stride_n = v_new->stride(0);
+    a.v_new_stride_h = v_new->stride(1);
+  }
   on_device(q, [&](void* stream) {
     check(abi.tree_attention(&a, static_cast<const int32_t*>(mask.data_ptr()), int32_t(mask.size(1)), &plan, stream),
           "aspire_tree_attention");
@@ -1035,15 +1063,17 @@ PyObject* py_tree_accept(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
-// (q, cache, mask, out, lse, want_lse, address of the plan's AspireAttnArgs, of its AspirePlanInfo, q_total) -> out, lse
+// (q, cache, mask, out, lse, want_lse, address of the plan's AspireAttnArgs, of its AspirePlanInfo, q_total, k_new,
+// v_new) -> out, lse
 PyObject* py_tree_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
-  return guarded(n, 9, [&]() -> PyObject* {
+  return guarded(n, 11, [&]() -> PyObject* {
     const void* fixed = PyLong_AsVoidPtr(v[6]);
     const void* plan = PyLong_AsVoidPtr(v[7]);
     if (!fixed || !plan) throw Invalid("an address is required");
     const auto r = tree_attention(tensor(v[0]), tensor(v[1]), tensor(v[2]), optional(v[3]), optional(v[4]),
                                   v[5] == Py_True, *static_cast<const AspireAttnArgs*>(fixed),
-                                  *static_cast<const AspirePlanInfo*>(plan), integer(v[8]));
+                                  *static_cast<const AspirePlanInfo*>(plan), integer(v[8]), optional(v[9]),
+                                  optional(v[10]));
     return wrap_all(r.first, r.second);
   });
 }

@@ -339,6 +339,28 @@ def test_with_the_append_inside(cuda_device):
     assert torch.equal(cache.cpu().nan_to_num(9), c.cache.nan_to_num(9))
 
 
+def test_the_append_checks_its_operands(cuda_device):
+    c = Case(cuda_device, [(140, 6), (31, 5)], 8, 2, seed=24)
+    w, cache, n = c.plan(trees=True), c.cache.to(cuda_device), c.starts[-1]
+    buf = torch.zeros(n, 12, 128, dtype=torch.bfloat16, device=cuda_device)  # a fused projection's output
+    q, k, v = buf[:, :8], buf[:, 8:10], buf[:, 10:]
+    part = cache[0, 0, :11]
+    before = cache.clone()
+    for kw, text in [(dict(append=(k, v), out=buf[:, 2:10]), "overlap"), (dict(append=(k, v), out=buf[:, 4:]), "overlap"),
+                     (dict(append=(part, v)), "overlap"), (dict(append=(k, part)), "overlap"),
+                     (dict(append=(k, None)), "both"), (dict(append=(k[:-1], v)), "k_new"), (dict(append=(k, v[:, :1])), "v_new"),
+                     (dict(append=(k.float(), v)), "k_new"), (dict(append=(k, v.cpu())), "v_new"),
+                     (dict(append=(k, v.detach().clone().requires_grad_())), "gradient")]:
+        with pytest.raises(ValueError, match=text):
+            w.run(q, cache, tree_mask=c.mask, **kw)
+        assert torch.equal(cache.nan_to_num(9), before.nan_to_num(9))
+    with pytest.raises(ValueError, match="gradient"):
+        w.run(q.detach().clone().requires_grad_(), cache, tree_mask=c.mask, append=(k, v))
+    version = cache._version
+    w.run(q, cache, tree_mask=c.mask, append=(k, v), out=q)
+    assert cache._version > version
+
+
 def test_nodes_past_the_mask_are_hidden_under_device_plans(cuda_device):
     c = Case(cuda_device, [(50, 40), (20, 70)], 4, 1, kind="all", seed=9)
     c.mask = c.mask[:, :1].contiguous()
