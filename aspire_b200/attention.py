@@ -36,6 +36,7 @@ from . import _capi
 FLOAT_WORKSPACE_BYTES = 128 * 1024 * 1024
 INT_WORKSPACE_BYTES = 8 * 1024 * 1024
 PINNED_RING_DEPTH = 4
+TREE_DECODE_ROWS = 64  # packed query rows of a decode item of a plan for trees
 
 _WRAPPER_REGISTRY: dict[int, "HolisticAttentionWrapper"] = {}
 
@@ -368,7 +369,8 @@ class HolisticAttentionWrapper:
         and an LSE of -inf.  Keys and values that some query does not see must
         be finite.  The plan must not be causal; no dump.  A plan made on the
         host without ``trees=True`` is made again for trees by the first such
-        call outside a graph's capture, and back by one without a mask."""
+        call outside a graph's capture, and back by one without a mask, or
+        with an append of rows that a plan for trees has no decode items for."""
         if self._plan_info is None:
             raise RuntimeError("run() before plan()/plan_host()")
         if tree_mask is not None:
@@ -376,8 +378,12 @@ class HolisticAttentionWrapper:
                 raise ValueError("tree_mask needs a plan made with causal=False")
             if self._has_jit and self._dump_kind != "noop":
                 raise ValueError("a dump variant takes no tree_mask")
-            if not self._plan_trees:
-                self._plan_again(_capi.PLAN_TREE)
+            # (The append is made inside decode items, of which a plan for trees has none for rows of more than
+            # 64 packed queries; a plain plan has them up to 127.)
+            packed = self._plan_info.max_q_len * (self._num_qo_heads // self._num_kv_heads)
+            trees = append is None or packed <= TREE_DECODE_ROWS
+            if self._plan_trees != trees:
+                self._plan_again(_capi.PLAN_TREE if trees else 0)
             return self._run_trees(q, _unpack_paged_kv_cache(paged_kv_cache, self._kv_layout), tree_mask, out, lse,
                                    return_lse, append)
         if self._plan_trees and not self._plan_again(0):

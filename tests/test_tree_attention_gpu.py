@@ -339,6 +339,35 @@ def test_with_the_append_inside(cuda_device):
     assert torch.equal(cache.cpu().nan_to_num(9), c.cache.nan_to_num(9))
 
 
+def test_the_append_inside_larger_trees(cuda_device):
+    """Rows of 65 to 127 packed queries are decode items of a plain plan, but not of one for trees."""
+    c = Case(cuda_device, [(140, 20), (31, 5), (700, 31)], 8, 2, seed=25)
+    n, q = c.starts[-1], c.q.to(cuda_device)
+    k, v = (torch.randn(n, 2, 128, generator=torch.Generator().manual_seed(s)).to(torch.bfloat16) for s in (1, 2))
+    cache = c.cache.to(cuda_device)
+    w = c.plan()
+    c.check(*w.run(q, cache, tree_mask=c.mask, return_lse=True))
+    assert w.plan_info.causal == 2 and w.plan_info.num_items_prefill > 0
+    for _ in range(2):
+        out, lse = w.run(q, cache, tree_mask=c.mask, return_lse=True, append=(k.to(cuda_device), v.to(cuda_device)))
+        assert w.plan_info.causal == 0 and w.plan_info.num_items_prefill == 0
+    for b, (a, m) in enumerate(c.rows):
+        for i in range(m):
+            page = c.pages[b][(a + i) // 16]
+            c.cache[page, 0, (a + i) % 16] = k[c.starts[b] + i]
+            c.cache[page, 1, (a + i) % 16] = v[c.starts[b] + i]
+    c.check(out, lse)
+    assert torch.equal(cache.cpu().nan_to_num(9), c.cache.nan_to_num(9))
+    c.check(*w.run(q, cache, tree_mask=c.mask, return_lse=True))
+    assert w.plan_info.causal == 2 and w.device_status() == 0
+    # More than a plain plan's decode items hold: refused, and the plan stays the caller's.
+    c = Case(cuda_device, [(140, 32)], 8, 2, seed=26)
+    w = c.plan()
+    with pytest.raises(ValueError, match="append"):
+        w.run(c.q.to(cuda_device), c.cache.to(cuda_device), tree_mask=c.mask, append=(k[:32].to(cuda_device), v[:32].to(cuda_device)))
+    assert w.plan_info.causal == 0
+
+
 def test_the_append_checks_its_operands(cuda_device):
     c = Case(cuda_device, [(140, 6), (31, 5)], 8, 2, seed=24)
     w, cache, n = c.plan(trees=True), c.cache.to(cuda_device), c.starts[-1]
