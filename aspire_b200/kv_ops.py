@@ -215,6 +215,15 @@ def draft_page_spill(mode_flags: torch.Tensor, dec_lens: torch.Tensor, draft_cac
     _capi.check(rc, "aspire_draft_page_spill")
 
 
+def _in_common(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors' memory, first to last element, has a byte in common."""
+    def span(t):
+        at = t.data_ptr()
+        return at, at + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * (t.numel() > 0)
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_append_indptr: torch.Tensor,
                  rope_offsets: torch.Tensor, kv_cache: torch.Tensor, kv_page_indices: torch.Tensor | None,
                  kv_page_indptr: torch.Tensor, kv_last_page_len: torch.Tensor, page_size: int = 16, *,
@@ -235,7 +244,8 @@ def qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_append_in
     q (``q_out``, which may be ``q`` itself for the reference's in-place form).
     ``positions`` (int32 [tokens], C ABI ``aspire_qkv_prologue_at``) gives each
     token its own position, as the nodes of a tree have; ``rope_offsets`` may
-    then be None."""
+    then be None, and operands that require a gradient are refused where
+    gradients are enabled."""
     total = q.shape[0]
     if q_out is None:
         q_out = torch.empty_like(q)
@@ -269,6 +279,11 @@ def qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_append_in
     if positions is not None:
         if positions.device != q.device or positions.numel() < total:
             raise ValueError("positions needs one entry per token on q's device")
+        if torch.is_grad_enabled() and any(
+                t is not None and t.requires_grad for t in (q, k, v, q_out, kv_cache, q_norm_weight, k_norm_weight)):
+            raise ValueError("the prologue of trees has no gradient: detach the operands or call under torch.no_grad()")
+        if _in_common(positions, q_out) or _in_common(positions, kv_cache):
+            raise ValueError("positions must not overlap q_out or the cache")
     elif rope_offsets.shape[0] < num_rows:
         raise ValueError("rope_offsets needs one entry per row")
     a = _capi.AspirePrologueArgs()

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from aspire_b200 import _capi
-from aspire_b200.kv_ops import build_step_tables
+from aspire_b200.kv_ops import build_step_tables, qkv_prologue
 from aspire_b200.logits import adjust_logits, pick_tokens
 from aspire_b200.tree import accept_tree
 
@@ -187,3 +187,21 @@ def test_prologue_at_abi(built_library):
     lib = built_library
     a = _capi.AspirePrologueArgs()
     _refused(lib, lib.aspire_qkv_prologue_at(ctypes.byref(a), None, None), "positions")
+
+
+def test_the_prologue_of_trees_refuses_gradients_and_overlaps():
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    q, k, v = (torch.zeros(4, h, 128, dtype=torch.bfloat16) for h in (2, 1, 1))
+    cache = torch.zeros(2, 2, 16, 1, 128, dtype=torch.bfloat16)
+    w = torch.ones(128, dtype=torch.bfloat16)
+    rows = (i32(0, 4), None), (cache, i32(0), i32(0, 1), i32(4))
+
+    def call(q=q, k=k, v=v, cache=cache, w=w, positions=i32(0, 1, 1, 2), **kw):
+        return qkv_prologue(q, k, v, *rows[0], cache, *rows[1][1:], q_norm_weight=w, k_norm_weight=w, positions=positions, **kw)
+
+    for name, t in (("q", q), ("k", k), ("v", v), ("cache", cache), ("w", w), ("q_out", q)):
+        with pytest.raises(ValueError, match="gradient"):
+            call(**{name: t.clone().requires_grad_()})
+    for name, t in (("q_out", torch.zeros_like(q)), ("cache", torch.zeros_like(cache))):
+        with pytest.raises(ValueError, match="overlap"):
+            call(positions=t.view(-1).view(torch.int32)[100:104], **{name: t})
