@@ -54,6 +54,11 @@ def _ptr_i32(t: torch.Tensor):
     return ctypes.cast(ctypes.c_void_p(t.data_ptr()), _capi.c_int32_p)
 
 
+def _bytes_i32(t: torch.Tensor, n: int) -> bytes:
+    """The first ``n`` values of a contiguous int32 host tensor."""
+    return ctypes.string_at(t.data_ptr(), 4 * n) if n else b""
+
+
 def _unpack_paged_kv_cache(
     paged_kv_cache: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], kv_layout: str
 ) -> torch.Tensor:
@@ -132,7 +137,7 @@ class HolisticAttentionWrapper:
         self._has_jit = jit_args is not None
 
         self._plan_info: Optional[_capi.AspirePlanInfo] = None
-        self._plan_host_arrays: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None
+        self._plan_host_arrays: Optional[Tuple[bytes, bytes, bytes]] = None
         self._plan_trees = False
         self._tree_args: Optional[_capi.AspireAttnArgs] = None
         self._kv_indices: Optional[torch.Tensor] = None
@@ -232,8 +237,9 @@ class HolisticAttentionWrapper:
         self._plan_arrays(qo, kvp, kvl, (int(num_qo_heads), int(num_kv_heads), int(head_dim_qk), int(page_size)),
                           _capi.PLAN_TREE if trees else 1 if causal else 0)
         # What a plan that is not causal is made from, should its rows turn out to be trees (the caller may
-        # write the next step into its arrays before that).
-        self._plan_host_arrays = None if causal or trees else (qo[:batch + 1].clone(), kvp[:batch + 1].clone(), kvl.clone())
+        # write the next step into its arrays before that): as bytes, a third of what three tensors' copies take.
+        self._plan_host_arrays = None if causal or trees else (
+            _bytes_i32(qo, batch + 1), _bytes_i32(kvp, batch + 1), _bytes_i32(kvl, batch))
         self._kv_indices = paged_kv_indices
         self._page_size = int(page_size)
         self._sm_scale = sm_scale
@@ -276,7 +282,9 @@ class HolisticAttentionWrapper:
         False where there is none or a graph is being captured."""
         if self._plan_host_arrays is None or torch.cuda.is_current_stream_capturing():
             return False
-        self._plan_arrays(*self._plan_host_arrays, (self._num_qo_heads, self._num_kv_heads, 128, self._page_size), mode)
+        arrays = (torch.frombuffer(bytearray(b), dtype=torch.int32) if b else torch.empty(0, dtype=torch.int32)
+                  for b in self._plan_host_arrays)
+        self._plan_arrays(*arrays, (self._num_qo_heads, self._num_kv_heads, 128, self._page_size), mode)
         return True
 
     def plan_device(
