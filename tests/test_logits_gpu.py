@@ -294,3 +294,28 @@ def test_lists_are_bounded_by_the_vocabulary(cuda_device):
     a.logits, a.type, a.tokens, a.rows, a.vocab, a.logits_stride, a.out, a.out_stride = 256, 0, 64, 64, 151936, 151936, 256, 151936
     a.history, a.history_len, a.history_cols, a.history_stride, a.frequency = 256, 256, 131072, 131072, 256
     assert 64 * 151936 * 8 <= _capi.load_library().aspire_logits_workspace(a) <= 1.1 * 64 * 151936 * 8
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("negative", [False, True])
+def test_nan_and_infinities_under_penalties(cuda_device, dtype, negative):
+    """On listed entries too; with terms below their neutral values an infinity may turn."""
+    c = Case(31, [3, 9, 1], 3001, dtype, hist=400, bias=20, allowed=True)
+    g = torch.Generator().manual_seed(31)
+    kind = torch.rand(c.base.shape, generator=g)
+    for value, lo in ((math.nan, 0.0), (math.inf, 0.02), (-math.inf, 0.04)):
+        c.base[(kind >= lo) & (kind < lo + 0.02)] = value
+    c.base[3] = -math.inf  # nothing but listed entries could rise
+    c.base[4] = math.nan
+    if negative:
+        c.terms = {k: -v for k, v in c.terms.items()}
+    for b, lists in enumerate(c.bias_lists):
+        if lists:
+            lists[0] = (lists[0][0], math.inf)
+            c.bias[b] = dict(lists)
+    x32, _, _ = ref.adjust(c.logits, c.row_of, c.history, c.prompts, c.paths, *(
+        c.terms[k] for k in ("repetition", "frequency", "presence")), c.bias, c.allowed)
+    x, kw = c.logits.to(cuda_device), c.args(cuda_device)
+    got, want = adjust_logits(x, **kw).cpu(), x32.to(dtype)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.5), want.nan_to_num(0.5))
+    assert pick_tokens(x, **kw).tolist() == ref.pick(x32, c.row_of)

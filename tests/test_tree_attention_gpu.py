@@ -145,6 +145,28 @@ def test_page_tables_and_device_plans(cuda_device, rows):
         c.check(out, lse)
 
 
+@pytest.mark.parametrize("device_plan", [False, True])
+def test_draft_rows_beside_trees(cuda_device, device_plan):
+    """Rows of one token that read a draft table's pages in a batch with trees that read the block table's."""
+    c = Case(cuda_device, [(500, 12), (95, 1), (30, 40), (0, 1), (2000, 1)], 8, 2, seed=27)
+    draft = [False, True, False, True, True]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    cols = max(len(r) for r in c.pages)
+    own = [r + [10 ** 6] * (cols - len(r)) for r in c.pages]
+    none = [10 ** 6] * cols
+    w = HolisticAttentionWrapper(torch.empty(1, device=cuda_device))
+    w.set_page_tables(i32([0 if d else 1 for d in draft]).to(cuda_device),
+                      i32([r if d else none for r, d in zip(own, draft)]).to(cuda_device),
+                      i32([none if d else r for r, d in zip(own, draft)]).to(cuda_device))
+    if device_plan:
+        w.plan_device(i32(c.starts).to(cuda_device), i32(c.kv_indptr).to(cuda_device),
+                      i32([(e - 1) % 16 + 1 for e in c.ends]).to(cuda_device), 8, 2, 128, 16, trees=True)
+    else:
+        w.plan_host(i32(c.starts), i32(c.kv_indptr), i32(c.ends), None, 8, 2, 128, 16, trees=True)
+    c.check(*w.run(c.q.to(cuda_device), c.cache.to(cuda_device), tree_mask=c.mask, return_lse=True))
+    assert w.device_status() == 0
+
+
 @pytest.mark.parametrize("heads,kv_heads", [(4, 1), (16, 2), (10, 2)])
 @pytest.mark.parametrize("rows", ["ragged", "wide", "split", "tile_edges"])
 def test_device_plans_for_trees_hold_the_host_plans_items(cuda_device, rows, heads, kv_heads):
