@@ -100,7 +100,7 @@ struct TcShared {
   uint64_t v_full[kVStages], v_empty[kVStages];
   uint64_t s_full[2], s_empty[2], p_full[2], p_empty[2];
   uint64_t o_free, q_full, q_empty, done, done_pv, grp[2];
-  uint64_t stage_free;  // (kStageInP) both groups' rows of an item have left the P buffers, where the next is of another width
+  uint64_t stage_free;  // (kStageInP) both groups' rows have left the P buffers, before an item of another width
   pf::Barriers pf;  // prefill phase
   uint64_t seq_full[kSeqDepth], seq_empty[kSeqDepth];
   int seq[kSeqDepth];
@@ -396,8 +396,9 @@ __device__ __noinline__ void dump_columns(const AttnParams& p, int lo, int hi, i
 // The item's N packed columns are split between the two softmax warpgroups:
 // warpgroup wg owns columns [c0, c0 + NH) with c0 = wg * NH, NH = N / 2.  A
 // column's running statistics (reference max, sum, rescale factor) live with
-// its owner, so the two groups never wait for each other; they meet only on
-// the S / P / O barriers shared with the MMA warp.
+// its owner, so the two groups do not wait for each other: they meet on the
+// S / P / O barriers shared with the MMA warp and, in the tree kernel, before
+// an item of another width than the last one's (stage_free).
 // Bits [lo, hi) of a word, 0 <= lo < hi <= 32, without a shift by 32, which the language leaves undefined.
 __host__ __device__ constexpr uint32_t bits_between(int lo, int hi) {
   return (0xffffffffu >> (32 - hi)) & (0xffffffffu << lo);
@@ -482,9 +483,20 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
   bool failed = false;
   // kStageInP: the previous item's rows lie in the group's part of the P buffers,
   // which its width gives it.  An item of another width writes its P over the
-  // other group's rows too, which that group may still be storing.
-  const bool other_width = Sh::kStageInP && staged_cols != 0 && staged_cols != N;
-  staged_cols = N;
+  // other group's rows too, so both groups' rows leave before it begins (a wait
+  // where the P is written would cost items of one width 7 %: 89 us for 82, 16
+  // rows of 6k keys with 16 nodes of a group of 4).
+  if constexpr (Sh::kStageInP) {
+    if (staged_cols != N && staged_cols != 0) {
+      if (ctid == 0) {
+        ptx::bulk_wait_read();
+        ptx::mbar_arrive(ptx::smem_addr(&sm.stage_free));
+      }
+      failed |= !wait_bar(sm, sm.stage_free, width_changes & 1, p.status);
+      ++width_changes;
+    }
+    staged_cols = N;
+  }
   int flag = 0;  // the first tile sets its flags whatever they hold
 
   for (int t = 0; t < nt; ++t) {
@@ -558,10 +570,7 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
     // last barrier: it is free to be cleared.)
     const int next_flag = flag == 2 ? 0 : flag + 1;
     // The previous item's rows have left the P buffers before this item's P is written.
-    if (Sh::kStageInP && t == 0 && ctid == 0) {
-      ptx::bulk_wait_read();
-      if (other_width) ptx::mbar_arrive(ptx::smem_addr(&sm.stage_free));
-    }
+    if (Sh::kStageInP && t == 0 && ctid == 0) ptx::bulk_wait_read();
     if (exceed) flags[flag][wq] = 1;
     if (lane == 0) flags[next_flag][wq] = 0;
     failed |= !group_sync(sm, grp, grp_uses, p.status);
@@ -633,10 +642,6 @@ __device__ bool consume_item(const AttnParams& p, Sh& sm, const WorkItem& it, bo
     }
     // P^T as bf16, MN-major without swizzle: 8 queries x 16 B per token, token-major.
     failed |= !wait_bar(sm, sm.p_empty[b], ph ^ 1, p.status);
-    if (Sh::kStageInP && t == 0 && other_width) {
-      failed |= !wait_bar(sm, sm.stage_free, width_changes & 1, p.status);
-      ++width_changes;
-    }
     uint8_t* pbuf = sm.p[b] + (c0 / 8) * (kTile * 16);
 #pragma unroll
     for (int c = 0; c < NH / 8; ++c) {
