@@ -8,6 +8,7 @@ import random
 import pytest
 import torch
 
+from aspire_b200 import _capi
 from aspire_b200.attention import HolisticAttentionWrapper, first_last_dump_jit_args
 import tree_reference as ref
 
@@ -233,6 +234,36 @@ def test_consecutive_items_of_other_widths(cuda_device, rows, sms):
         o, l = w.run(q, kv, tree_mask=c.mask, return_lse=True)
         assert torch.equal(o, out) and torch.equal(l, lse)
     assert w.device_status() == 0
+
+
+@pytest.mark.parametrize("rows,sms", [(_short_rows_of_four_widths(), 3), (_long_rows_of_four_widths(), 11),
+                                      ([(4200, 17), (1432, 30), (50, 32), (300, 5)], 6)])
+def test_waits_that_expire_at_different_places(cuda_device, built_library, rows, sms):
+    c = Case(cuda_device, rows, 8, 2, seed=28)
+    w = HolisticAttentionWrapper(torch.empty(1, device=cuda_device), num_sms=sms)
+    q, kv = c.q.to(cuda_device), c.cache.to(cuda_device)
+
+    def run():
+        c.plan(wrapper=w, trees=True)
+        w.clear_device_status()
+        out, lse = w.run(q, kv, tree_mask=c.mask, return_lse=True)
+        return out, lse, w.device_status()
+
+    want = run()
+    c.check(*want[:2])
+    expired = 0
+    for limit in (1, 500, 2000, 4000, 8000, 16000):
+        for _ in range(5):
+            _capi.check(built_library.aspire_set_wait_limit_ns(limit), "aspire_set_wait_limit_ns")
+            try:
+                first = run()
+            finally:
+                _capi.check(built_library.aspire_set_wait_limit_ns(0), "aspire_set_wait_limit_ns")
+            assert first[2] in (0, _capi.STATUS_TIMEOUT)
+            expired += first[2] != 0
+            for got in ((first, run()) if first[2] == 0 else (run(),)):
+                assert got[2] == 0 and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert expired
 
 
 def test_a_plain_plan_is_made_again_for_trees_outside_captures(cuda_device):
