@@ -15,9 +15,11 @@
 // vocabulary, count in shared memory (integer atomics: the order does not
 // matter) and write a bitmap and the list of the touched entries in order.
 // aspire_logits_kernel or aspire_logits_pick_kernel then streams the logits,
-// which bound the call, its first loads on their way before the marks are
-// done: listed entries are adjusted, all others go by the bitmap and the
-// grammar's bits as they came.
+// which bound the call: listed entries are adjusted, all others go by the
+// bitmap and the grammar's bits as they came.  Its first loads are on their way
+// before the marks are done, but on SMs without a marking CTA only: the 1024
+// threads of one have a whole register file, so none of the streaming CTAs fits
+// beside it (64 rows of 151936 entries: 128 of 148 SMs).
 #include "tree.cuh"
 
 namespace aspire {
@@ -103,7 +105,8 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {
 // that are its, flags the prompt's, the step's and the biased ones, sums the
 // flags up, a warp 1024 entries at a time, and writes the list.  Counts have
 // 16 bits where the history allows (kWide: 32): two CTAs then hold 152000
-// entries, and 64 rows are one wave.  Bound by the latency of its few steps
+// entries.  An SM has one of these CTAs at a time, so rows times CTAs past the
+// SMs are another wave (with two a row, from 75 rows on).  Bound by the latency of its few steps
 // and by its instructions, so what it reads is requested before anything
 // waits.  64 rows with histories of up to 16384 over 151936 entries: 19.6 us
 // with cold caches; one row with 900 over eight CTAs: 8.7.

@@ -19,7 +19,7 @@
 // same 16 bytes of up to kBatch tokens at a time, all read before the first is
 // written.  node_d grows with d and is at least d, so no place is written
 // before it is read.  Bound by latency (the tree, the walk, the pages, the
-// move); 64 rows of 36 layers with 8 heads move 17 MB: 16.3 us, one row of 28
+// move); 64 rows of 36 layers with 8 heads move 17 MB: 14.4 us, one row of 28
 // layers 6.3.
 #include "tree.cuh"
 
